@@ -19,8 +19,10 @@ PKG = HERE.parent
 REPO = PKG.parent
 LIB = PKG / "libflyguy_b200.so"
 TRAIN = PKG / "fg_train"                             # the trainer executable (a main() over fg_train_main)
-SOURCES = [HERE / "fg_core.cu", HERE / "fg_noalloc.cu", HERE / "fg_hopop.cu", HERE / "fg_train.cu", HERE / "fg_fly.cu"]
-DEPS = SOURCES + [HERE / "fg_kernels.cuh", HERE / "fg_tcgen05.cuh", HERE / "fg_outtc.cuh", REPO / "include" / "flyguy_b200.h"]
+SOURCES = [HERE / "fg_core.cu", HERE / "fg_noalloc.cu", HERE / "fg_hopop.cu", HERE / "fg_train.cu", HERE / "fg_fly.cu",
+           HERE / "fg_rotate.cu", HERE / "fg_decay.cu"]
+DEPS = SOURCES + [HERE / "fg_kernels.cuh", HERE / "fg_tcgen05.cuh", HERE / "fg_outtc.cuh", HERE / "fg_memory.cuh",
+                  REPO / "include" / "flyguy_b200.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,80 @@
+// Shared pieces of the memory-over-ticks kernels (fg_rotate.cu, fg_decay.cu): values of the three types as fp32, and the
+// entry points' error handling. No counterpart in the reference, whose fly actor has no memory (flyguy/fly.py:76).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <string>
+
+#include "flyguy_b200.h"
+
+namespace fgm {
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+template <class T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+
+__device__ __forceinline__ float warp_sum(float s) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+struct MemErr {
+    std::string msg;
+};
+std::string& last_error();
+
+#define MCK(call)                                                                                         \
+    do {                                                                                                  \
+        cudaError_t e_ = (call);                                                                          \
+        if (e_ != cudaSuccess) throw ::fgm::MemErr{std::string(#call) + ": " + cudaGetErrorString(e_)};  \
+    } while (0)
+
+// runs f; whatever it throws becomes -1 and the calling thread's message
+template <class F>
+long long mem_guard(F&& f) {
+    try {
+        const long long r = f();
+        last_error().clear();
+        return r;
+    } catch (const MemErr& e) {
+        last_error() = e.msg;
+    } catch (const std::exception& e) {
+        last_error() = e.what();
+    }
+    return -1;
+}
+
+inline void need(bool ok, const char* what) {
+    if (!ok) throw MemErr{what};
+}
+
+// f with a value of the type that FG_F32 / FG_BF16 / FG_F16 names
+template <class F>
+void by_type(long long type, F&& f) {
+    if (type == FG_F32) f(float());
+    else if (type == FG_BF16) f(__nv_bfloat16());
+    else if (type == FG_F16) f(__half());
+    else throw MemErr{"unknown type"};
+}
+
+inline int sm_count() {
+    static thread_local int dev = -1, n = 0;
+    int d = 0;
+    MCK(cudaGetDevice(&d));
+    if (d != dev) {
+        MCK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d));
+        dev = d;
+    }
+    return n;
+}
+
+}  // namespace fgm

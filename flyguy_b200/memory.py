@@ -1,0 +1,393 @@
+"""A memory over ticks beside the fly actor. The reference's actor answers each tick from that tick's observation alone
+(FlyActor.memory = 0, flyguy/fly.py:76); the operators here carry what earlier ticks showed, learned on whole recordings
+at once and played a tick at a time with a state of fixed size:
+
+  rotary_turns      the rotation's plan: a tick's angle of each pair of a head's values
+  rotate            queries or keys turned by their position
+  norm_rotate       the norms of queries and keys for each head and the rotation in one pass
+  decay_attention   linear attention with a decay for each head over whole recordings (also packed end to end)
+  decay_step        the same for one tick, the states updated in place
+
+They run in the library (fg_norm_rotate, fg_decay_attn, fg_decay_step of include/flyguy_b200.h) on CUDA tensors, on
+torch's current stream; rotate, norm_rotate and decay_attention have gradients. TickMemory puts them together.
+
+Queries, keys and values are float32, bfloat16 or float16 of one type, [batch, ticks, heads, dim] or, for recordings packed
+end to end, [ticks, heads, dim]; any strides with a head's values adjacent (others are copied first). Norms, sums,
+states and decays are float32; results are rounded to the type once.
+"""
+from __future__ import annotations
+
+import math
+import struct
+from decimal import Decimal, localcontext
+
+import torch
+from torch import nn
+
+from .native import FlyguyError, lib
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LAYOUTS = {"half": 0, "interleaved": 1}
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510")
+
+
+# ---- argument checks and the library's argument structures ----------------------------------------------------------
+
+def _values(name: str, t, dims: tuple[int, ...], like=None) -> torch.Tensor:
+    """t as the library takes it; its last dimension made adjacent if it is not."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise FlyguyError(f"{name} must be a CUDA tensor (flyguy_b200 has no CPU path)")
+    if t.dtype not in TYPES:
+        raise FlyguyError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    if t.dim() not in dims:
+        raise FlyguyError(f"{name} must have {' or '.join(map(str, dims))} dimensions, not {t.dim()}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.dim() != like.dim()):
+        raise FlyguyError(f"{name} must have the type, device and number of dimensions of the first tensor")
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _float32(name: str, t, like: torch.Tensor, *shapes) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != torch.float32:
+        raise FlyguyError(f"{name} must be a float32 tensor on {like.device}")
+    if tuple(t.shape) not in shapes:
+        raise FlyguyError(f"{name} must be {' or '.join(map(str, shapes))}, not {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _ticks(t: torch.Tensor | None) -> tuple[int, int, int, int]:
+    """fg_ticks of [batch, ticks, heads, dim] or [ticks, heads, dim]."""
+    if t is None:
+        return 0, 0, 0, 0
+    st = t.stride()
+    return (t.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (t.data_ptr(), 0, st[0], st[1])
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _call(fn, packed: bytes, device: torch.device) -> None:
+    """fn(arguments, the current stream) on the tensors' device."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            rc = fn(packed, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        rc = fn(packed, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        raise FlyguyError(lib().fg_mem_last_error().decode())
+
+
+def _work(size: int, device: torch.device) -> tuple[torch.Tensor | None, int, int]:
+    if size < 0:
+        raise FlyguyError(lib().fg_mem_last_error().decode())
+    if not size:
+        return None, 0, 0
+    t = torch.empty(size, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), size
+
+
+# ---- rotation ------------------------------------------------------------------------------------------------------
+
+def rotary_turns(turned: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                 original: int = 1024, device=None) -> torch.Tensor:
+    """[turned / 2] int64: pair i's angle a tick, base^(-2i / turned) radians, as a fraction of a turn times 2^64.
+
+    For recordings longer than those learned from (`original` ticks), by `factor`:
+      "linear"  every angle divided by factor
+      "base"    the base raised so that the slowest pair's angle is divided by factor, the fastest's kept
+      "parts"   kept where a pair turns over 32 times in `original` ticks, divided by factor where it turns less than
+                once, in proportion between (to be used with rotate's amplitude 0.1 ln(factor) + 1)"""
+    if turned < 0 or turned % 2:
+        raise FlyguyError(f"turned must be even and not negative, not {turned}")
+    if not (base > 1 and math.isfinite(base) and factor >= 1 and original >= 1):
+        raise FlyguyError("base must be over 1, factor and original at least 1")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise FlyguyError(f"scaling must be None, 'linear', 'base' or 'parts', not {scaling!r}")
+    n = turned // 2
+    with localcontext() as c:                              # (doubles would be off by some units at 2^64)
+        c.prec = 40
+        pace, by, two_pi = Decimal(base), Decimal(factor), 2 * _PI
+        if scaling == "base" and n > 1:
+            pace *= by ** (Decimal(n) / (n - 1))
+        f = [pace ** (Decimal(-i) / n) for i in range(n)]
+        if scaling == "linear":
+            f = [x / by for x in f]
+        elif scaling == "parts":
+            keep = [min(Decimal(1), max(Decimal(0), (original * x / two_pi - 1) / 31)) for x in f]
+            f = [x * a + x / by * (1 - a) for x, a in zip(f, keep)]
+        return torch.tensor([int((x / two_pi * 2 ** 64).to_integral_value()) for x in f], dtype=torch.int64, device=device)
+
+
+# fg_rotate_args: x, y, gy, gx (two fg_ticks each), w, w_head, gw, heads (two each), batch, ticks, dim, turned, turns,
+# positions, pos_batch, pos_tick, pos_bytes, type, interleaved, norm, eps, amplitude, work, work_bytes
+_ROTATE = struct.Struct("=32q8q12q2d2q")
+_NONE = (0, 0, 0, 0)
+
+
+class _Rotation:
+    """The checked arguments of one call: what forward and backward share."""
+
+    def __init__(self, q, k, turns, positions, layout, amplitude, eps):
+        self.q, self.k = q, k
+        *lead, heads, dim = q.shape
+        if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != dim):
+            raise FlyguyError(f"k must be {(*lead, 'key heads', dim)}, not {tuple(k.shape)}")
+        batch, ticks = lead if len(lead) == 2 else (1, lead[0])
+        if layout not in LAYOUTS:
+            raise FlyguyError(f"layout must be one of {list(LAYOUTS)}, not {layout!r}")
+        turned = 0
+        if turns is not None:
+            if not isinstance(turns, torch.Tensor) or turns.dtype != torch.int64 or turns.device != q.device or turns.dim() != 1:
+                raise FlyguyError(f"turns must be an int64 vector on {q.device} (rotary_turns)")
+            turned = 2 * turns.numel()
+            if turned > dim:
+                raise FlyguyError(f"turns are of {turned} values, a head has {dim}")
+            turns = turns.contiguous()
+        pos = (0, 0, 0, 8)
+        if positions is not None:
+            if not isinstance(positions, torch.Tensor) or positions.device != q.device or positions.dtype not in (torch.int64, torch.int32):
+                raise FlyguyError(f"positions must be int64 or int32 on {q.device}")
+            try:
+                p = positions.expand(batch, ticks)
+            except RuntimeError:
+                raise FlyguyError(f"positions {tuple(positions.shape)} do not fit {batch} x {ticks} ticks") from None
+            pos = (p.data_ptr(), p.stride(0), p.stride(1), p.element_size())
+        self.keep = (turns, positions)
+        self.dims = (heads, 0 if k is None else k.shape[-2], batch, ticks, dim, turned, _ptr(turns), *pos, TYPES[q.dtype],
+                     LAYOUTS[layout])
+        self.floats = (float(eps or 1.0), float(amplitude))
+        self.norm = int(eps is not None)
+
+    def pack(self, y=_NONE, z=_NONE, gy=_NONE, gz=_NONE, gx=_NONE, gk=_NONE, wq=None, wk=None, gwq=None, gwk=None,
+             work=(0, 0)) -> bytes:
+        dim = self.dims[4]
+        return _ROTATE.pack(*_ticks(self.q), *_ticks(self.k), *y, *z, *gy, *gz, *gx, *gk, _ptr(wq), _ptr(wk),
+                            dim if wq is not None and wq.dim() == 2 else 0, dim if wk is not None and wk.dim() == 2 else 0,
+                            _ptr(gwq), _ptr(gwk), *self.dims, self.norm, *self.floats, *work)
+
+    def forward(self, wq=None, wk=None):
+        q, k = self.q, self.k
+        y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        z = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _call(lib().fg_norm_rotate, self.pack(_ticks(y), _ticks(z), wq=wq, wk=wk), q.device)
+        return y, z
+
+    def backward(self, gy, gz, wq=None, wk=None, want_w=(False, False)):
+        q, k = self.q, self.k
+        gy = _grad("the gradient of the queries", gy, q)
+        gz = None if k is None else _grad("the gradient of the keys", gz, k)
+        gx = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        gk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        gwq = torch.empty_like(wq) if wq is not None and want_w[0] else None
+        gwk = torch.empty_like(wk) if wk is not None and want_w[1] else None
+        kw = dict(gy=_ticks(gy), gz=_ticks(gz), gx=_ticks(gx), gk=_ticks(gk), wq=wq, wk=wk, gwq=gwq, gwk=gwk)
+        work = (None, 0, 0)
+        if gwq is not None or gwk is not None:
+            work = _work(lib().fg_norm_rotate_work(self.pack(**kw)), q.device)
+        _call(lib().fg_norm_rotate_bwd, self.pack(**kw, work=work[1:]), q.device)
+        return gx, gk, gwq, gwk
+
+
+def _grad(name: str, g, like: torch.Tensor) -> torch.Tensor:
+    """An incoming gradient as the library takes it (None: zeros)."""
+    if g is None:
+        return torch.zeros(like.shape, dtype=like.dtype, device=like.device)
+    return _values(name, g.to(like.dtype), (like.dim(),))
+
+
+class _RotateFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, rotation):
+        ctx.rotation = rotation
+        return rotation.forward()[0]
+
+    @staticmethod
+    def backward(ctx, gy):
+        return ctx.rotation.backward(gy, None)[0], None
+
+
+class _NormRotateFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, rotation):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, wq, wk)
+        ctx.rotation = rotation
+        return rotation.forward(wq, wk)
+
+    @staticmethod
+    def backward(ctx, gy, gz):
+        q, k, wq, wk = ctx.saved_tensors
+        r = ctx.rotation
+        r.q, r.k = _values("q", q.detach(), (3, 4)), _values("k", k.detach(), (3, 4))
+        return *r.backward(gy, gz, wq, wk, ctx.needs_input_grad[2:4]), None
+
+
+def rotate(x, turns, positions=None, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:
+    """x [batch, ticks, heads, dim] or [ticks, heads, dim] with the first 2 * len(turns) values of each head turned pair by
+    pair: (a, b) -> amplitude (a cos - b sin, b cos + a sin) at the angle position * turns (rotary_turns).
+
+    positions: int64 / int32 that expand to [batch, ticks] (None: 0, 1, ..). layout "half": pairs (i, i + turned / 2);
+    "interleaved": (2i, 2i + 1). The gradient is the rotation back."""
+    x0 = _values("x", x, (3, 4))
+    r = _Rotation(x0.detach(), None, turns, positions, layout, amplitude, None)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _RotateFn.apply(x, r)
+    return r.forward()[0]
+
+
+def norm_rotate(q, k, turns=None, q_weight=None, k_weight=None, positions=None, layout: str = "half",
+                amplitude: float = 1.0, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """rotate(x / sqrt(mean(x^2) + eps) * weight) over each head of queries [.., heads, dim] and keys [.., key heads, dim],
+    in one pass over both. Weights: float32 [dim] (one for all heads) or [heads, dim], or None; turns None: the
+    norms alone. Gradients of q, k and the weights; the weights' are the same bits on every run."""
+    q0 = _values("q", q, (3, 4))
+    k0 = _values("k", k, (3, 4), q)
+    if not eps > 0:
+        raise FlyguyError(f"eps must be positive, not {eps}")
+    if q_weight is not None:
+        q_weight = _float32("q_weight", q_weight, q, tuple(q.shape[-1:]), tuple(q.shape[-2:]))
+    if k_weight is not None:
+        k_weight = _float32("k_weight", k_weight, k, tuple(k.shape[-1:]), tuple(k.shape[-2:]))
+    r = _Rotation(q0.detach(), k0.detach(), turns, positions, layout, amplitude, eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _NormRotateFn.apply(q, k, q_weight, k_weight, r)
+    return r.forward(None if q_weight is None else q_weight.detach(), None if k_weight is None else k_weight.detach())
+
+
+# ---- attention whose state decays -----------------------------------------------------------------------------------
+
+# fg_decay_args: q, k, v, o, go, gq, gk, gv (fg_ticks), log_decay, state, state_out, gstate_out, gstate, offsets, batch, ticks,
+# heads, key_heads, dim, value_dim, type, scale, work, work_bytes
+_DECAY = struct.Struct("=32q6q7qd2q")
+# fg_step_args: q, k, v, o (fg_ticks), log_decay, state, slots, n_slots, batch, heads, key_heads, dim, value_dim, type, scale
+_STEP = struct.Struct("=16q10qd")
+
+
+class _Decay:
+    """The checked arguments of one decay_attention call."""
+
+    def __init__(self, q, k, v, log_decay, state, scale, offsets):
+        heads, dim = q.shape[-2:]
+        key_heads, value_dim = v.shape[-2:]
+        lead = q.shape[:-2]
+        if k.shape != (*lead, key_heads, dim) or v.shape[:-2] != lead:
+            raise FlyguyError(f"k and v must be {(*lead, 'key heads', dim)} and {(*lead, 'key heads', 'value dim')}, not "
+                              f"{tuple(k.shape)} and {tuple(v.shape)}")
+        if not key_heads or heads % key_heads:
+            raise FlyguyError(f"{heads} query heads cannot share {key_heads} key heads")
+        if offsets is None:
+            batch, ticks = lead if len(lead) == 2 else (1, lead[0])
+        else:
+            if len(lead) != 1:
+                raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
+            if (not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int64 or offsets.device != q.device
+                    or offsets.dim() != 1 or not offsets.numel()):
+                raise FlyguyError(f"offsets must be an int64 vector [recordings + 1] on {q.device}")
+            offsets = offsets.contiguous()
+            batch, ticks = offsets.numel() - 1, lead[0]
+        if log_decay.requires_grad:
+            raise FlyguyError("log_decay is a constant of each head: it has no gradient")
+        self.log_decay = _float32("log_decay", log_decay, q, (heads,))
+        self.states = (batch, heads, dim, value_dim)
+        if state is not None:
+            state = _float32("state", state, q, self.states)
+        self.q, self.k, self.v, self.state, self.offsets = q, k, v, state, offsets
+        self.sizes = (batch, ticks, heads, key_heads, dim, value_dim, TYPES[q.dtype])
+        self.scale = float(dim ** -0.5 if scale is None else scale)
+
+    def pack(self, o=_NONE, go=_NONE, gq=_NONE, gk=_NONE, gv=_NONE, state_out=None, gstate_out=None, gstate=None,
+             work=(0, 0)) -> bytes:
+        return _DECAY.pack(*_ticks(self.q), *_ticks(self.k), *_ticks(self.v), *o, *go, *gq, *gk, *gv,
+                           self.log_decay.data_ptr(), _ptr(self.state), _ptr(state_out), _ptr(gstate_out), _ptr(gstate),
+                           _ptr(self.offsets), *self.sizes, self.scale, *work)
+
+    def forward(self):
+        q, v = self.q, self.v
+        o = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
+        end = torch.empty(self.states, dtype=torch.float32, device=q.device)
+        kw = dict(o=_ticks(o), state_out=end)
+        work = _work(lib().fg_decay_work(self.pack(**kw), 0), q.device)
+        _call(lib().fg_decay_attn, self.pack(**kw, work=work[1:]), q.device)
+        return o, end
+
+    def backward(self, go, gend, want_state: bool):
+        q, k, v = self.q, self.k, self.v
+        if go is None:
+            go = torch.zeros((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
+        go = _values("the gradient of o", go.to(q.dtype), (q.dim(),))
+        if gend is not None:
+            gend = gend.float().contiguous()
+        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        gstate = torch.empty(self.states, dtype=torch.float32, device=q.device) if want_state else None
+        kw = dict(go=_ticks(go), gq=_ticks(gq), gk=_ticks(gk), gv=_ticks(gv), gstate_out=gend, gstate=gstate)
+        work = _work(lib().fg_decay_work(self.pack(**kw), 1), q.device)
+        _call(lib().fg_decay_attn_bwd, self.pack(**kw, work=work[1:]), q.device)
+        return gq, gk, gv, gstate
+
+
+class _DecayFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, state, job):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, state)
+        ctx.job = job
+        return job.forward()
+
+    @staticmethod
+    def backward(ctx, go, gend):
+        q, k, v, state = ctx.saved_tensors
+        job = ctx.job
+        job.q, job.k, job.v = (_values("q", t.detach(), (3, 4)) for t in (q, k, v))
+        job.state = None if state is None else state.detach().contiguous()
+        return *job.backward(go, gend, ctx.needs_input_grad[3]), None
+
+
+def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,
+                    offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t for every recording and head.
+
+    q [batch, ticks, heads, dim], k [.., key heads, dim], v [.., key heads, value dim], each key head serving heads / key
+    heads query heads; or [ticks, ..] with recordings packed end to end and offsets int64 [recordings + 1] (recordings may
+    be empty). log_decay float32 [heads], at most 0, a constant. state float32 [recordings, heads, dim, value dim] before
+    the first ticks (None: zeros). scale: dim^-0.5 when None. dim and value dim at most 256.
+    Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v and state."""
+    q0 = _values("q", q, (3, 4))
+    k0, v0 = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
+    job = _Decay(q0.detach(), k0.detach(), v0.detach(), log_decay, None if state is None else state.detach(), scale, offsets)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+        return _DecayFn.apply(q, k, v, state, job)
+    return job.forward()
+
+
+def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None) -> torch.Tensor:
+    """One tick of decay_attention for a batch: q [batch, heads, dim], k [batch, key heads, dim], v [batch, key heads, value
+    dim]. state float32 [slots, heads, dim, value dim], contiguous, is updated in place at each row's slot (slots int64
+    [batch], no two alike; None: row b's is b); a row whose slot is outside answers 0 and changes nothing. Returns o
+    [batch, heads, value dim]. No gradient: for learning, decay_attention."""
+    q, k, v = _values("q", q, (3,)), _values("k", k, (3,), q), _values("v", v, (3,), q)
+    batch, heads, dim = q.shape
+    key_heads, value_dim = v.shape[1:]
+    if k.shape != (batch, key_heads, dim) or v.shape[0] != batch:
+        raise FlyguyError(f"k and v must be {(batch, 'key heads', dim)} and {(batch, 'key heads', 'value dim')}, not "
+                          f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if not key_heads or heads % key_heads:
+        raise FlyguyError(f"{heads} query heads cannot share {key_heads} key heads")
+    log_decay = _float32("log_decay", log_decay, q, (heads,))
+    if (not isinstance(state, torch.Tensor) or state.dtype != torch.float32 or state.device != q.device
+            or state.dim() != 4 or state.shape[1:] != (heads, dim, value_dim) or not state.is_contiguous()):
+        raise FlyguyError(f"state must be contiguous float32 {('slots', heads, dim, value_dim)} on {q.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        raise FlyguyError("decay_step has no gradient (decay_attention has): call it under torch.no_grad()")
+    if slots is not None:
+        if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int64 or slots.device != q.device or slots.shape != (batch,):
+            raise FlyguyError(f"slots must be int64 [{batch}] on {q.device}")
+        slots = slots.contiguous()
+    elif state.shape[0] < batch:
+        raise FlyguyError(f"{batch} rows need as many states, not {state.shape[0]}")
+    o = torch.empty((batch, heads, value_dim), dtype=q.dtype, device=q.device)
+    rows = lambda t: (t.data_ptr(), t.stride(0), 0, t.stride(1))    # noqa: E731
+    packed = _STEP.pack(*rows(q), *rows(k), *rows(v), *rows(o), log_decay.data_ptr(), state.data_ptr(), _ptr(slots),
+                        state.shape[0], batch, heads, key_heads, dim, value_dim, TYPES[q.dtype],
+                        float(dim ** -0.5 if scale is None else scale))
+    _call(lib().fg_decay_step, packed, q.device)
+    return o

@@ -58,6 +58,14 @@ SIGNATURES = {
     "fg_hop_fwd": (_ci, [_vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, _vp]),
     "fg_hop_bwd": (_ci, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, _vp, _vp]),
     "fg_hop_last_error": (ctypes.c_char_p, []),
+    "fg_norm_rotate": (_ci, [_vp, _vp]),
+    "fg_norm_rotate_bwd": (_ci, [_vp, _vp]),
+    "fg_norm_rotate_work": (_cll, [_vp]),
+    "fg_decay_attn": (_ci, [_vp, _vp]),
+    "fg_decay_attn_bwd": (_ci, [_vp, _vp]),
+    "fg_decay_work": (_cll, [_vp, _ci]),
+    "fg_decay_step": (_ci, [_vp, _vp]),
+    "fg_mem_last_error": (ctypes.c_char_p, []),
     "fg_train_main": (_ci, [_ci, ctypes.POINTER(ctypes.c_char_p)]),
     "fg_survey": (_ci, [_vp, _vp, _vp, _ci, _ci, _vp, _vp, ctypes.POINTER(ctypes.c_double)]),
     "fly_create": (_vp, [_ci, _ci, _ci]),

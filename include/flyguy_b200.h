@@ -208,6 +208,90 @@ void fly_free(void* p);
 /* Why the calling thread's last fly_* call failed ("" after a success). */
 const char* fg_fly_last_error(void);
 
+/* ---- a memory over ticks ------------------------------------------------------------------------------------------
+ * The fly actor answers each tick from that tick alone (FlyActor.memory = 0, flyguy/fly.py:76). These operators are the
+ * parts of a memory that runs beside it: the norms of queries and keys with the position rotation, and a linear
+ * attention whose state decays by a constant a tick for each head. Handle-free, on the caller's device buffers and
+ * stream (NULL = the legacy default stream); nothing is allocated: what needs room takes it from `work`. Return 0, or
+ * -1 with the reason in fg_mem_last_error(). Every field of the argument structures is 8 bytes wide. */
+
+/* Values [batch, ticks, heads, dim]: a head's values are adjacent, the other strides (in values) are the caller's and
+ * may be 0. Recordings packed end to end: batch stride unused, the tick runs over all of them. */
+typedef struct fg_ticks {
+    void* p;
+    long long batch, tick, head;
+} fg_ticks;
+
+#define FG_F32 0      /* types of queries, keys, values and outputs */
+#define FG_BF16 1
+#define FG_F16 2
+
+typedef struct fg_rotate_args {
+    fg_ticks x[2], y[2];              /* queries, keys (heads[1] = 0: none) and what comes out */
+    fg_ticks gy[2], gx[2];            /* backward: the outputs' gradients, the inputs' */
+    const float* w[2];                /* the norms' weights, or NULL */
+    long long w_head[2];              /* from one head's weights to the next (0: one set for all heads) */
+    float* gw[2];                     /* backward: the weights' gradients (written), as w; NULL: not wanted */
+    long long heads[2], batch, ticks, dim;
+    long long turned;                 /* the first `turned` values of a head rotate (even, 0: none) */
+    const long long* turns;           /* [turned / 2]: a tick's angle as a fraction of a turn, times 2^64 */
+    const void* positions;            /* a tick's position: [batch, ticks] with the strides below; NULL: the tick */
+    long long pos_batch, pos_tick, pos_bytes;   /* strides in positions; 4 or 8 bytes each */
+    long long type, interleaved;      /* FG_F32..; pairs (2i, 2i+1), else (i, i + turned / 2) */
+    long long norm;                   /* 0: the rotation alone */
+    double eps, amplitude;            /* under the norm's root; factor of the rotated pairs */
+    void* work;                       /* backward with gw: fg_norm_rotate_work bytes, 16-byte aligned */
+    long long work_bytes;
+} fg_rotate_args;
+
+/* y = rotate(x / sqrt(mean(x^2) + eps) * w): per head the norm, then each pair (a, b) turned by
+ * position * turns[i] / 2^64 of a turn and scaled by amplitude; sums and products in fp32, rounded once. */
+int fg_norm_rotate(const fg_rotate_args* args, void* stream);
+/* gx and gw from x and gy (x unused without the norm). The sums of gw run in a fixed order. */
+int fg_norm_rotate_bwd(const fg_rotate_args* args, void* stream);
+long long fg_norm_rotate_work(const fg_rotate_args* args);
+
+typedef struct fg_decay_args {
+    fg_ticks q, k, v, o;              /* [.., heads, dim], [.., key_heads, dim], [.., key_heads, value_dim], [.., heads, value_dim] */
+    fg_ticks go, gq, gk, gv;          /* backward */
+    const float* log_decay;           /* [heads], at most 0; a constant, without a gradient */
+    const float* state;               /* [batch, heads, dim, value_dim] before the first tick, or NULL: zeros */
+    float* state_out;                 /* after the last tick (may not overlap state) */
+    const float* gstate_out;          /* backward: gradient of state_out, or NULL: zeros */
+    float* gstate;                    /* backward: gradient of state, or NULL: not wanted */
+    const long long* offsets;         /* [batch + 1] first ticks of recordings packed end to end, or NULL: all of `ticks` */
+    long long batch, ticks;           /* with offsets: ticks of all recordings together */
+    long long heads, key_heads, dim, value_dim, type;
+    double scale;
+    void* work;                       /* fg_decay_work bytes, 16-byte aligned */
+    long long work_bytes;
+} fg_decay_args;
+
+/* For every recording and head h (keys and values of head h / (heads / key_heads)):
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t.
+ * States are fp32. Offsets outside 0..ticks or falling are clamped to it, never followed out of the buffers. */
+int fg_decay_attn(const fg_decay_args* args, void* stream);
+/* With R_t = exp(log_decay) R_{t+1} + scale q_t go_t^T (the last also + gstate_out):
+ *   gq_t = scale S_t go_t, gk_t = R_t v_t, gv_t = R_t^T k_t (summed over the query heads that share them), gstate =
+ * exp(log_decay) R_0. o and state_out are unused. */
+int fg_decay_attn_bwd(const fg_decay_args* args, void* stream);
+long long fg_decay_work(const fg_decay_args* args, int backward);
+
+typedef struct fg_step_args {
+    fg_ticks q, k, v, o;              /* one tick: the tick stride is unused */
+    const float* log_decay;
+    float* state;                     /* [slots, heads, dim, value_dim], updated in place */
+    const long long* slots;           /* [batch], each row's state (no two alike), or NULL: its own number; a row whose */
+    long long n_slots;                /* slot is not in 0..n_slots-1 answers 0 and changes nothing */
+    long long batch, heads, key_heads, dim, value_dim, type;
+    double scale;
+} fg_step_args;
+
+/* One tick of fg_decay_attn for each row, its state updated in place. */
+int fg_decay_step(const fg_step_args* args, void* stream);
+/* Why the calling thread's last call of these failed ("" after a success). */
+const char* fg_mem_last_error(void);
+
 /* ---- the standalone teaching trainer (replaces the reference's flyguy_train executable, flyguy/native/
  * flyguy_train.cu main() at 631-788): argv as the command line "fg_train NET.bin PARAMS.bin DATA_DIR OUT_PREFIX
  * [options]" (options and file formats in csrc/fg_train.cu). Returns the process exit status (0: done or stopped). */
