@@ -10,6 +10,8 @@
 //
 // Few long recordings: the ticks of each are split into parts; a first launch leaves every part's own state (from
 // zero) in the workspace, the second starts each part from the decayed sum of the states before it.
+#include <type_traits>
+
 #include "fg_memory.cuh"
 
 namespace {
@@ -56,6 +58,10 @@ __device__ __forceinline__ long long part_ticks(long long n, int parts) {
     const long long per = (n + parts - 1) / parts;
     return (per + kAlign - 1) / kAlign * kAlign;
 }
+
+}  // namespace
+#include "fg_decay_tc.cuh"
+namespace {
 
 // The recurrence itself, in fp32, for any type, size and stride: a block of 8 warps owns 32 columns of one head's
 // state; lane = column, warp w holds rows w R .. w R + R - 1 in registers. 16 ticks of a and b are staged in shared
@@ -292,6 +298,7 @@ Scan scan_of(const fg_decay_args* g) {
 
 template <class T>
 void launch(const Scan& s, cudaStream_t st) {
+    if (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value && tc_fits(s)) return tc_launch(s, st);
     const long long blocks = s.batch * s.heads * ((s.E + kRecCols - 1) / kRecCols);
     if (s.parts > 1) k_decay_rec<T><<<dim3((unsigned)blocks, s.parts - 1), 32 * kRecWarps, 0, st>>>(s, 1);
     k_decay_rec<T><<<dim3((unsigned)blocks, s.parts), 32 * kRecWarps, 0, st>>>(s, 0);
@@ -395,6 +402,17 @@ int fg_decay_step(const fg_step_args* g, void* stream) {
                 g->slots, g->n_slots, (int)g->heads, (int)g->dim, (int)g->value_dim, (float)g->scale);
         });
         MCK(cudaGetLastError());
+        return 0;
+    });
+}
+
+int fg_mem_sync(void* stream) {
+    return (int)mem_guard([&]() -> long long {
+        int bad = 0;
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        MCK(cudaMemcpyFromSymbolAsync(&bad, g_tc_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+        MCK(cudaStreamSynchronize(st));
+        need(!bad, "fg_decay_attn: a wait on the tensor cores ran out; its results are not to be used");
         return 0;
     });
 }

@@ -65,6 +65,7 @@ SIGNATURES = {
     "fg_decay_attn_bwd": (_ci, [_vp, _vp]),
     "fg_decay_work": (_cll, [_vp, _ci]),
     "fg_decay_step": (_ci, [_vp, _vp]),
+    "fg_mem_sync": (_ci, [_vp]),
     "fg_mem_last_error": (ctypes.c_char_p, []),
     "fg_train_main": (_ci, [_ci, ctypes.POINTER(ctypes.c_char_p)]),
     "fg_survey": (_ci, [_vp, _vp, _vp, _ci, _ci, _vp, _vp, ctypes.POINTER(ctypes.c_double)]),
