@@ -188,11 +188,12 @@ class _Rotation:
         return gx, gk, gwq, gwk
 
 
-def _grad(name: str, g, like: torch.Tensor) -> torch.Tensor:
+def _grad(name: str, g, like: torch.Tensor, shape=None) -> torch.Tensor:
     """An incoming gradient as the library takes it (None: zeros)."""
     if g is None:
-        return torch.zeros(like.shape, dtype=like.dtype, device=like.device)
-    return _values(name, g.to(like.dtype), (like.dim(),))
+        return torch.zeros(like.shape if shape is None else shape, dtype=like.dtype, device=like.device)
+    g = _values(name, g.to(like.dtype), (like.dim(),))
+    return g if 0 not in g.stride() else g.contiguous()   # (an expanded sum)
 
 
 class _RotateFn(torch.autograd.Function):
@@ -312,9 +313,7 @@ class _Decay:
 
     def backward(self, go, gend, want_state: bool):
         q, k, v = self.q, self.k, self.v
-        if go is None:
-            go = torch.zeros((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
-        go = _values("the gradient of o", go.to(q.dtype), (q.dim(),))
+        go = _grad("the gradient of o", go, q, (*q.shape[:-1], v.shape[-1]))
         if gend is not None:
             gend = gend.float().contiguous()
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
