@@ -247,11 +247,14 @@ void check_sizes(const Sizes& z, const char* who) {
     if (z.batch * z.heads > (1ll << 27)) throw MemErr{w + ": batch * heads is over 2^27"};
 }
 
-// Parts a recording: enough blocks for the machine, none under 256 ticks on average.
+// Parts a recording. On the tensor cores a block takes a SM to itself and a part costs its b and c read twice: as many parts
+// as keep blocks within the SMs, of at least four chunks. The recurrence's blocks share a SM and are slow: more of them.
 int parts_of(const fg_decay_args* g) {
     const long long rows = std::max<long long>(1, g->batch * g->heads);
     const long long mean = g->offsets ? g->ticks / std::max<long long>(1, g->batch) : g->ticks;
-    const long long want = (2 * 148 + rows - 1) / rows, most = std::max<long long>(1, mean / 256);
+    const bool tc = g->type == FG_BF16 && g->dim % 16 == 0 && g->value_dim % 16 == 0 && g->dim <= 128 && g->value_dim <= 128;
+    const long long blocks = tc ? rows : rows * ((std::min(g->dim, g->value_dim) + kRecCols - 1) / kRecCols);
+    const long long want = (tc ? 148 : 4 * 148) / blocks, most = mean / (tc ? 512 : 256);
     return (int)std::min<long long>(64, std::max<long long>(1, std::min(want, most)));
 }
 long long partial_floats(const fg_decay_args* g) {

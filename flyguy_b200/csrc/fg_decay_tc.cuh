@@ -14,7 +14,7 @@
 // Tiles lie in shared memory as TMA writes them, 64 values (128 bytes, swizzled) of a tick in a row: read along the values
 // or along the ticks that is the K-major or the MN-major form of the same bytes, so nothing is transposed.
 //
-// 17 warps: 0-7 the ticks (A to W, O1 and O2 to out; warps w and w + 4 share TMEM lanes 32 (w % 4) .. and take alternate
+// 20 warps: 0-7 the ticks (A to W, O1 and O2 to out; warps w and w + 4 share TMEM lanes 32 (w % 4) .. and take alternate
 // blocks of 32 columns), 8-15 the state (b to b', S), 16 the copies and the MMAs. The roles meet at mbarriers only, so a
 // chunk's elementwise work runs beside its MMAs and the next chunk's copies.
 #pragma once
@@ -26,7 +26,7 @@
 namespace {
 using namespace fgm;
 
-constexpr int kTcTicks = 128, kTcThreads = 17 * 32;
+constexpr int kTcTicks = 128, kTcThreads = 20 * 32;
 __device__ int g_tc_error;                                   // a wait ran out (fg_mem_sync)
 
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -61,13 +61,10 @@ __device__ __forceinline__ void tmem_ready(uint32_t (&r)[16]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
@@ -92,19 +89,53 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// Bounded wait for a barrier's phase. A try suspends the thread until the phase or about 0.1 ms are over, so that waiting
+// warps leave shared memory to the MMAs' operands.
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    const long long t0 = clock64();
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (*gave_up) return false;
+        if (clock64() - t0 > fg::kTcWaitCycles) {
+            *gave_up = 1;
+            atomicExch(&g_tc_error, 1);
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int head, int tick, int batch) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map),
+                 "r"(x), "r"(head), "r"(tick), "r"(batch), "r"(src)
+                 : "memory");
+}
+// the stores that this thread has issued have left shared memory
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 struct TcMaps {
-    CUtensorMap a, b, c;
+    CUtensorMap a, b, c, out;
 };
 // DP, EP: dim and value_dim up to 64 or 128
 template <int DP, int EP>
 struct TcLayout {
     static constexpr uint32_t a = 0, b = kTcTicks * DP * 2, c = 2 * b, stage = c + kTcTicks * EP * 2;
     static constexpr uint32_t state = 2 * stage;             // the copy of S, then the third term of b'
-    static constexpr uint32_t table = state + (DP * EP * 2 > kTcTicks * DP * 2 ? DP * EP * 2 : kTcTicks * DP * 2);
-    static constexpr uint32_t bars = table + (132 + 32) * 4;
+    static constexpr uint32_t after = state + (DP * EP * 2 > kTcTicks * DP * 2 ? DP * EP * 2 : kTcTicks * DP * 2);
+    // where a chunk of out is put together: room for fp32, or (no room left) where its c was, fp32 in two halves
+    static constexpr bool own_out = DP + EP < 256;
+    static constexpr uint32_t table = after + (own_out ? kTcTicks * EP * 4 : 0);
+    static constexpr uint32_t bars = table + (32 + 132 + 16) * 4;
     static constexpr uint32_t bytes = bars + 128;
 };
-enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kWReady, kBReady, kSReady, kOutRead, kBars };
+enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kCFree, kWReady, kBReady, kSReady, kOutRead, kMeet, kBars };
 
 // PARTS: the states of the parts alone
 template <int DP, int EP, bool BACK, bool PARTS>
@@ -115,8 +146,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     constexpr uint32_t kBox = kTcTicks * 128, kStateBox = DP * 128;
     constexpr int kTmem = 512;
     constexpr uint32_t tA = 0, tO1 = 128, tO2 = tO1 + EP, tS = tO2 + EP;
-    float* pw = reinterpret_cast<float*>(smem + L::table);   // gamma^0 .. gamma^128
-    float* ramp = pw + 132;                                  // gamma^{31-j}, from the back gamma^j
+    float* pw = reinterpret_cast<float*>(smem + L::table) + 32;   // gamma^0 .. gamma^128, before them zeros
+    float* ramp = pw + 132;                                  // gamma^{15-j}, from the back gamma^j
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -145,7 +176,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     for (int i = tid; i <= kTcTicks; i += kTcThreads) pw[i] = power(ld, (float)i);
-    if (tid < 32) ramp[tid] = power(ld, (float)(BACK ? tid : 31 - tid));
+    if (tid < 32) pw[-1 - tid] = 0.f;
+    if (tid < 16) ramp[tid] = power(ld, (float)(BACK ? tid : 15 - tid));
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
@@ -156,7 +188,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
         const long long t = t0 + (long long)i * kTcTicks;
         return sp.start + (BACK ? sp.n - t - ticks_of(i) : t);
     };
-    auto wait = [&](int i, int chunk) { return fg::mbar_wait(bar(i), (uint32_t)chunk & 1, gave_up, &g_tc_error, 1); };
+    auto wait = [&](int i, int chunk) { return tc_wait(bar(i), (uint32_t)chunk & 1, gave_up); };
     auto wait_warp = [&](int i, int chunk) {
         const bool ok = wait(i, chunk);
         const bool all = __all_sync(0xffffffffu, ok);
@@ -171,52 +203,75 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     const int lead0 = BACK && s.first && part == 0 && !PARTS ? 0 : 1;
     bool ok = true;
 
-    if (warp == 16) {
+    // 20 warps start with 96 registers a thread: 640 x 96 = 61,440. The copies and MMAs (and the three warps beside them, there
+    // because registers change hands by four warps) keep 48, the ticks 88, so that the state has 128 (S alone is 64):
+    // 128 x 48 + 256 x 88 + 256 x 128 = 61,440
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         // ---- copies and MMAs -----------------------------------------------------------------------------------
-        if (lane == 0) {
-            auto copy = [&](int i) {
+        if (warp == 16 && lane == 0) {
+            const int da = (D + 63) / 64, ec = (E + 63) / 64, batch = s.offsets ? 0 : (int)b;
+            auto copy = [&](int i) {                         // a and b (and the bytes that c will add)
                 const uint32_t stage = sm + (i & 1) * L::stage, full = bar(kFull0 + (i & 1));
-                const int tick = (int)first_of(i), batch = s.offsets ? 0 : (int)b;
-                const int da = (D + 63) / 64, ec = (E + 63) / 64;
+                const int tick = (int)first_of(i);
                 fg::mbar_expect_tx(full, (uint32_t)((PARTS ? 1 : 2) * da + ec) * kBox);
                 for (int x = 0; x < da; ++x) {
                     if (!PARTS) tma_tile(stage + L::a + x * kBox, &maps.a, x * 64, h / s.a.share, tick, batch, full);
                     tma_tile(stage + L::b + x * kBox, &maps.b, x * 64, h / s.b.share, tick, batch, full);
                 }
-                for (int x = 0; x < ec; ++x)
-                    tma_tile(stage + L::c + x * kBox, &maps.c, x * 64, h / s.c.share, tick, batch, full);
             };
-            const int kd = D / 16;
-            // 16 values of a K-major tile; 16 ticks of an MN-major one
-            auto along = [&](uint32_t at, int k) { return swizzled(at + (k >> 2) * kBox + (k & 3) * 32, 0); };
-            auto down = [&](uint32_t at, int k, uint32_t next) { return swizzled(at + k * 2048, next); };
-            int copied = 0;
-            if (chunks) { copy(0); copied = 1; }
+            auto copy_c = [&](int i) {
+                const uint32_t stage = sm + (i & 1) * L::stage, full = bar(kFull0 + (i & 1));
+                for (int x = 0; x < ec; ++x)
+                    tma_tile(stage + L::c + x * kBox, &maps.c, x * 64, h / s.c.share, (int)first_of(i), batch, full);
+            };
+            // 16 values of a K-major tile; 16 ticks (rows) of an MN-major one; descriptors count in 16 bytes
+            constexpr auto along = [](int k) { return (uint64_t)((k >> 2) * kBox + (k & 3) * 32) >> 4; };
+            constexpr auto down = [](int k) { return (uint64_t)(k * 2048) >> 4; };
+            const uint32_t id_a = bf16_idesc(128, 0, 0), id_o = bf16_idesc(E, 0, 1), id_s = bf16_idesc(E, 1, 1);
+            const uint64_t state_rows = swizzled(sm + L::state, kStateBox);
+            constexpr uint32_t next_b = DP == 128 ? kBox : 0;     // (an M = 128 operand of 64 values: twice the same)
+            int started = 0, copied = 0;                     // chunks whose a and b, and whose c too, are on their way
+            if (chunks) { copy(0); copy_c(0); started = copied = 1; }
             for (int i = 0; i < chunks && ok; ++i) {
                 const uint32_t stage = sm + (i & 1) * L::stage;
+                const uint64_t a_ticks = swizzled(stage + L::a, 0), b_ticks = swizzled(stage + L::b, 0),
+                               c_rows = swizzled(stage + L::c, kBox);
+                const uint64_t terms[3] = {swizzled(stage + L::b, next_b), swizzled(stage + L::a, next_b), swizzled(sm + L::state, next_b)};
                 if (i > 0) ok = wait(kKv, i - 1) && (PARTS || wait(kPv, i - 1));   // the other stage is free, and A
                 if (!ok) break;
-                if (i + 1 < chunks) { copy(i + 1); ++copied; }
-                ok = fg::mbar_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up, &g_tc_error, 1);
+                const bool more = i + 1 < chunks, wait_c = !PARTS && !L::own_out && i > 0;
+                if (more) { copy(i + 1); ++started; }
+                if (more && !wait_c) { copy_c(i + 1); ++copied; }
+                ok = tc_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up);
                 if (!ok) break;
                 fg::tc_fence_after();
                 if (!PARTS) {
-                    for (int k = 0; k < kd; ++k)
-                        mma_bf16(tmem + tA, along(stage + L::a, k), along(stage + L::b, k), bf16_idesc(128, 0, 0), k > 0);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        mma_bf16(tmem + tA, a_ticks + along(k), b_ticks + along(k), id_a, k > 0);
                     fg::mma_commit(bar(kQk));
+                    if (more && wait_c) {                    // out of the chunk before has left c's place
+                        ok = wait(kCFree, i - 1);
+                        if (!ok) break;
+                        copy_c(i + 1);
+                        ++copied;
+                    }
                     ok = wait(kSReady, i) && (i == 0 || wait(kOutRead, i - 1));
                     if (!ok) break;
                     fg::tc_fence_after();
-                    for (int k = 0; k < kd; ++k)
-                        mma_bf16(tmem + tO1, along(stage + L::a, k), down(sm + L::state, k, kStateBox), bf16_idesc(E, 0, 1), k > 0);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        mma_bf16(tmem + tO1, a_ticks + along(k), state_rows + down(k), id_o, k > 0);
                     fg::mma_commit(bar(kQs));
                     ok = wait(kWReady, i) && (ticks_of(i) == kTcTicks || wait(kBReady, i));   // (c's end is cleared there)
                     if (!ok) break;
                     fg::tc_fence_after();
+#pragma unroll
                     for (int term = 0; term < 2; ++term)
+#pragma unroll
                         for (int k = 0; k < kTcTicks / 16; ++k)
-                            mma_bf16_tmem(tmem + tO2, tmem + tA + (k >> 1) * 32 + term * 16 + (k & 1) * 8,
-                                          down(stage + L::c, k, kBox), bf16_idesc(E, 0, 1), term + k > 0);
+                            mma_bf16_tmem(tmem + tO2, tmem + tA + k * 16 + term * 8, c_rows + down(k), id_o, term + k > 0);
                     fg::mma_commit(bar(kPv));
                 } else {
                     fg::mma_commit(bar(kQk));                // (nothing before it: the tile has arrived)
@@ -226,12 +281,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 ok = wait(kBReady, i);
                 if (!ok) break;
                 fg::tc_fence_after();
+#pragma unroll
                 for (int term = 0; term < 3; ++term)
+#pragma unroll
                     for (int k = 0; k < kTcTicks / 16; ++k)
-                        mma_bf16(tmem + tS, down(term == 0 ? stage + L::b : term == 1 ? stage + L::a : sm + L::state, k, DP == 128 ? kBox : 0),
-                                 down(stage + L::c, k, kBox), bf16_idesc(E, 1, 1), term + k > 0);
+                        mma_bf16(tmem + tS, terms[term] + down(k), c_rows + down(k), id_s, term + k > 0);
                 fg::mma_commit(bar(kKv));
             }
+            if (!ok && copied < started) copy_c(copied++);
             if (!ok)                                         // let the copies in flight land before the block ends
                 for (int i = max(0, copied - 2); i < copied; ++i) {
                     const long long c0 = clock64();
@@ -239,105 +296,164 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 }
         }
     } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- ticks ---------------------------------------------------------------------------------------------
         const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const bool pairs = reinterpret_cast<uintptr_t>(s.out.p) % 32 == 0 &&
-                           ((s.offsets ? 0 : s.out.batch) | s.out.tick | s.out.head) % 16 == 0;
+        int meetings = 0;
+        auto meet = [&]() {                                  // the eight warps wait for one another
+            arrive(kMeet);
+            return wait_warp(kMeet, meetings++);
+        };
         for (int i = 0; !PARTS && i < chunks && ok; ++i) {
             const int n = ticks_of(i);
             ok = wait_warp(kQk, i);
             if (!ok) break;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int blk = 2 * j + half, s0 = blk * 32;  // blocks on one side of the diagonal are 0
-                uint32_t v[16], w[16], hi[16], lo[16];
+                const int blk = 2 * j + half;                 // blocks of 32 on one side of the diagonal are 0
+                uint32_t v[2][16], hi[8], lo[8];
                 if (BACK ? blk < quarter : blk > quarter) {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) hi[k] = 0;
-                    tmem_st16(lanes + tA + s0, hi);
-                    tmem_st16(lanes + tA + s0 + 16, hi);
+                    for (int k = 0; k < 8; ++k) hi[k] = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tmem_st8(lanes + tA + blk * 32 + k * 8, hi);
                     continue;
                 }
-                tmem_ld16(lanes + tA + s0, v);
-                tmem_ld16(lanes + tA + s0 + 16, w);
-                tmem_ready(v);
-                tmem_ready(w);
-                if (blk != quarter && (!BACK || n == kTcTicks)) {   // gamma^{t-s} as two factors, both at most 1
-                    const float f = pw[BACK ? s0 - row : row - s0 - 31];
-                    const float4* r4 = reinterpret_cast<const float4*>(ramp);
+                tmem_ld16(lanes + tA + blk * 32, v[0]);
+                tmem_ld16(lanes + tA + blk * 32 + 16, v[1]);
+                tmem_ready(v[0]);
+                tmem_ready(v[1]);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float4 g = r4[k];
-                        const uint32_t* src = k < 4 ? &v[4 * k] : &w[4 * (k - 4)];
-                        float x0 = __uint_as_float(src[0]) * (f * g.x), x1 = __uint_as_float(src[1]) * (f * g.y);
-                        float x2 = __uint_as_float(src[2]) * (f * g.z), x3 = __uint_as_float(src[3]) * (f * g.w);
-                        hi[2 * k] = take_bf16(x0, x1);
-                        lo[2 * k] = pack_bf16(x0, x1);
-                        hi[2 * k + 1] = take_bf16(x2, x3);
-                        lo[2 * k + 1] = pack_bf16(x2, x3);
-                    }
-                } else {
+                for (int q = 0; q < 2; ++q) {
+                    const int s0 = blk * 32 + q * 16;
+                    if (BACK && n < kTcTicks) {               // the last ticks are not the chunk's
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const uint32_t* src = k < 8 ? &v[2 * k] : &w[2 * (k - 8)];
-                        const int d0 = BACK ? s0 + 2 * k - row : row - s0 - 2 * k, d1 = BACK ? d0 + 1 : d0 - 1;
-                        const bool in0 = d0 >= 0 && (!BACK || s0 + 2 * k < n), in1 = d1 >= 0 && (!BACK || s0 + 2 * k + 1 < n);
-                        float x = in0 ? __uint_as_float(src[0]) * pw[max(d0, 0)] : 0.f;
-                        float y = in1 ? __uint_as_float(src[1]) * pw[max(d1, 0)] : 0.f;
-                        hi[k] = take_bf16(x, y);
-                        lo[k] = pack_bf16(x, y);
+                        for (int k = 0; k < 16; ++k)
+                            if (s0 + k >= n) v[q][k] = 0;
                     }
+                    if (blk != quarter) {                    // gamma^{t-s} as two factors, both at most 1
+                        const float f = pw[BACK ? s0 - row : row - s0 - 15];
+                        const float4* r4 = reinterpret_cast<const float4*>(ramp);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float4 g = r4[k];
+                            float x0 = __uint_as_float(v[q][4 * k]) * (f * g.x), x1 = __uint_as_float(v[q][4 * k + 1]) * (f * g.y);
+                            float x2 = __uint_as_float(v[q][4 * k + 2]) * (f * g.z), x3 = __uint_as_float(v[q][4 * k + 3]) * (f * g.w);
+                            hi[2 * k] = take_bf16(x0, x1);
+                            lo[2 * k] = pack_bf16(x0, x1);
+                            hi[2 * k + 1] = take_bf16(x2, x3);
+                            lo[2 * k + 1] = pack_bf16(x2, x3);
+                        }
+                    } else {
+                        const float* g = pw + (BACK ? s0 - row : row - s0);   // gamma^{t-s} in turn; 0 past the diagonal
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            float x = __uint_as_float(v[q][2 * k]) * g[BACK ? 2 * k : -2 * k];
+                            float y = __uint_as_float(v[q][2 * k + 1]) * g[BACK ? 2 * k + 1 : -2 * k - 1];
+                            hi[k] = take_bf16(x, y);
+                            lo[k] = pack_bf16(x, y);
+                        }
+                    }
+                    tmem_st8(lanes + tA + s0, hi);
+                    tmem_st8(lanes + tA + s0 + 8, lo);
                 }
-                tmem_st16(lanes + tA + s0, hi);
-                tmem_st16(lanes + tA + s0 + 16, lo);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             fg::tc_fence_before();
             arrive(kWReady);
             const float f = pw[max(BACK ? n - 1 - row : row, 0) + (i ? 1 : lead0)] * s.scale_out;
             const float g = s.scale_in * s.scale_out;
-            const long long at = (s.offsets ? 0 : b * s.out.batch) + (first_of(i) + row) * s.out.tick + h * s.out.head;
             ok = wait_warp(kQs, i) && wait_warp(kPv, i);
             if (!ok) break;
-#pragma unroll
-            for (int j = 0; j < EP / 32; ++j) {
-                const int e0 = (2 * j + half) * 16;
-                if (e0 >= E) continue;
+            auto out16 = [&](int e0, float (&o)[16]) {
                 uint32_t x[16], y[16];
                 tmem_ld16(lanes + tO1 + e0, x);
                 tmem_ld16(lanes + tO2 + e0, y);
                 tmem_ready(x);
                 tmem_ready(y);
-                float o[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[k] = fmaf(__uint_as_float(x[k]), f, __uint_as_float(y[k]) * g);
-                if (row < n) {
-                    if (s.out_f32) {
+            };
+            if (n == kTcTicks) {
+                // put together in shared memory, stored as one tile (a thread's own stores, 32 lines at a time, held up the
+                // MMAs' operands: 4,000 instead of 1,900 clocks for dS)
+                const uint32_t tile = L::own_out ? L::after : (i & 1) * L::stage + L::c;
+                if (!L::own_out) {
+                    ok = wait_warp(kKv, i);
+                    if (!ok) break;
+                }
+                if (tid == 0) stores_read();
+                ok = meet();
+                if (!ok) break;
+                const int halves = !L::own_out && s.out_f32 ? 2 : 1;
+                for (int r = 0; r < halves && ok; ++r) {
+#pragma unroll 1
+                    for (int e0 = (halves == 2 ? r * 64 : 0) + half * 16; e0 < (halves == 2 ? min(E, r * 64 + 64) : E); e0 += 32) {
+                        float o[16];
+                        out16(e0, o);
+                        const int x0 = halves == 2 ? e0 - r * 64 : e0;
+                        if (s.out_f32) {
+                            unsigned char* at = smem + tile + (x0 >> 5) * kBox + row * 128;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                *reinterpret_cast<float4*>(at + (((((x0 & 31) >> 2) + k) ^ (row & 7)) << 4)) =
+                                    make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        } else {
+                            unsigned char* at = smem + tile + (x0 >> 6) * kBox + row * 128;
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                *reinterpret_cast<uint4*>(at + (((((x0 & 63) >> 3) + k) ^ (row & 7)) << 4)) =
+                                    make_uint4(pack_bf16(o[8 * k], o[8 * k + 1]), pack_bf16(o[8 * k + 2], o[8 * k + 3]),
+                                               pack_bf16(o[8 * k + 4], o[8 * k + 5]), pack_bf16(o[8 * k + 6], o[8 * k + 7]));
+                        }
+                    }
+                    if (r + 1 == halves) {
+                        fg::tc_fence_before();
+                        arrive(kOutRead);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    ok = meet();
+                    if (ok && tid == 0) {
+                        const int values = s.out_f32 ? 32 : 64, e1 = halves == 2 ? min(E, r * 64 + 64) : E;
+                        for (int e0 = halves == 2 ? r * 64 : 0, x = 0; e0 < e1; e0 += values, ++x)
+                            tma_store(&maps.out, sm + tile + x * kBox, e0, h, (int)first_of(i), s.offsets ? 0 : (int)b);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        if (!L::own_out) {
+                            stores_read();
+                            if (r + 1 == halves) fg::mbar_arrive(bar(kCFree));
+                        }
+                    }
+                    __syncwarp();
+                    if (r + 1 < halves) ok = ok && meet();
+                }
+            } else {                                          // a recording's last ticks: what follows them is another's
+                const long long at = (s.offsets ? 0 : b * s.out.batch) + (first_of(i) + row) * s.out.tick + h * s.out.head;
+#pragma unroll 1
+                for (int e0 = half * 16; e0 < E; e0 += 32) {
+                    float o[16];
+                    out16(e0, o);
+                    if (row < n && s.out_f32) {
                         float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(s.out.p) + at + e0);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) p[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                    } else {
-                        __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(s.out.p) + at + e0;
-                        uint32_t r[8];
+                    } else if (row < n) {
+                        uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(s.out.p) + at + e0);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) r[k] = pack_bf16(o[2 * k], o[2 * k + 1]);
-                        if (pairs) {                          // one whole 32-byte sector a thread
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]),
-                                         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                                         : "memory");
-                        } else {
-                            reinterpret_cast<uint4*>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
-                            reinterpret_cast<uint4*>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
-                        }
+                        for (int k = 0; k < 2; ++k)
+                            p[k] = make_uint4(pack_bf16(o[8 * k], o[8 * k + 1]), pack_bf16(o[8 * k + 2], o[8 * k + 3]),
+                                              pack_bf16(o[8 * k + 4], o[8 * k + 5]), pack_bf16(o[8 * k + 6], o[8 * k + 7]));
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
+                fg::tc_fence_before();
+                arrive(kOutRead);
+                if (!L::own_out && tid == 0) fg::mbar_arrive(bar(kCFree));
             }
-            fg::tc_fence_before();
-            arrive(kOutRead);
         }
+        if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ---- state ---------------------------------------------------------------------------------------------
         const int quarter = warp & 3, half = (warp >> 2) & 1, row = quarter * 32 + lane, st = tid - 256;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -375,7 +491,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 #pragma unroll
                 for (int j = 0; j < EP / 32; ++j) {
                     const int e0 = (2 * j + half) * 16, unit = (e0 & 63) >> 3;
-                    if (mine && e0 < E) {
+                    if (row < DP && e0 < E) {                // (rows past D: zeros, for the k-steps of 16 up to DP)
                         unsigned char* at = smem + L::state + (e0 >> 6) * kStateBox + row * 128;
                         const float* x = S[j];
                         *reinterpret_cast<uint4*>(at + ((unit ^ (row & 7)) << 4)) =
@@ -395,7 +511,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             unsigned char* stage = smem + (i & 1) * L::stage;
             ok = wait_warp(kQk, i) && (PARTS || wait_warp(kQs, i));
             // (the tile itself: TMA's writes are seen through its own barrier)
-            ok = ok && __all_sync(0xffffffffu, fg::mbar_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up, &g_tc_error, 1));
+            ok = ok && __all_sync(0xffffffffu, tc_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up));
             if (!ok) break;
             // b' in three terms, over b, a and the copy of S; ticks past the chunk's end (another recording's) become 0 in
             // b' and c, whatever they hold
@@ -403,23 +519,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 #pragma unroll
                 for (int x = 0; x < EP / 64; ++x) *reinterpret_cast<uint4*>(stage + L::c + x * kBox + u * 16) = make_uint4(0, 0, 0, 0);
             }
-            for (int u = st; u < kTcTicks * DP / 8; u += 256) {
-                const int r = (u >> 3) & 127;
-                const float f = pw[BACK ? r : max(n - 1 - r, 0)];
-                uint4 v = *reinterpret_cast<uint4*>(stage + L::b + u * 16), m, l;
-                uint32_t* pv = &v.x;
-                uint32_t* pm = &m.x;
-                uint32_t* pl = &l.x;
+            float f[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = pw[BACK ? (st >> 3) + 32 * k : max(n - 1 - (st >> 3) - 32 * k, 0)];
+#pragma unroll 1
+            for (int x = 0; x < DP / 64; ++x) {
+                unsigned char* at = stage + L::b + x * kBox + st * 16;
+                unsigned char* at_lo = smem + L::state + x * kBox + st * 16;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float x = r < n ? bf16_lo(pv[k]) * f : 0.f, y = r < n ? bf16_hi(pv[k]) * f : 0.f;
-                    pv[k] = take_bf16(x, y);
-                    pm[k] = take_bf16(x, y);
-                    pl[k] = pack_bf16(x, y);
+                    uint4 v = *reinterpret_cast<uint4*>(at + k * 4096), m, l;
+                    if ((st >> 3) + 32 * k >= n) v = make_uint4(0, 0, 0, 0);
+                    uint32_t* pv = &v.x;
+                    uint32_t* pm = &m.x;
+                    uint32_t* pl = &l.x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float y = bf16_lo(pv[j]) * f[k], z = bf16_hi(pv[j]) * f[k];
+                        pv[j] = take_bf16(y, z);
+                        pm[j] = take_bf16(y, z);
+                        pl[j] = pack_bf16(y, z);
+                    }
+                    *reinterpret_cast<uint4*>(at + k * 4096) = v;
+                    *reinterpret_cast<uint4*>(at - L::b + L::a + k * 4096) = m;
+                    *reinterpret_cast<uint4*>(at_lo + k * 4096) = l;
                 }
-                *reinterpret_cast<uint4*>(stage + L::b + u * 16) = v;
-                *reinterpret_cast<uint4*>(stage + L::a + u * 16) = m;
-                *reinterpret_cast<uint4*>(smem + L::state + u * 16) = l;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             arrive(kBReady);
@@ -470,18 +594,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 }
 
 // what 16-byte copies and tensor maps take: strides of dimensions that there is more than one of
-inline bool whole_units(const Scan& s, const Operand& o, bool read) {
-    const auto fits = [&](long long st, long long n) { return n <= 1 || (st % 8 == 0 && (!read || (st > 0 && st < (1ll << 36)))); };
+inline bool whole_units(const Scan& s, const Operand& o) {
+    const auto fits = [&](long long st, long long n) { return n <= 1 || (st % 8 == 0 && st > 0 && st < (1ll << 36)); };
     return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && fits(o.batch, s.offsets ? 1 : s.batch) && fits(o.tick, s.ticks) &&
            fits(o.head, s.heads / o.share);
 }
 inline bool tc_fits(const Scan& s) {
     return s.D % 16 == 0 && s.E % 16 == 0 && s.D <= 128 && s.E <= 128 && s.ticks < (1ll << 31) && s.ticks > 0 &&
-           s.batch < (1ll << 31) && whole_units(s, s.a, true) && whole_units(s, s.b, true) && whole_units(s, s.c, true) &&
-           whole_units(s, s.out, false) && reinterpret_cast<uintptr_t>(s.last) % 16 == 0;
+           s.batch < (1ll << 31) && whole_units(s, s.a) && whole_units(s, s.b) && whole_units(s, s.c) &&
+           whole_units(s, s.out) && reinterpret_cast<uintptr_t>(s.last) % 16 == 0;
 }
-// [batch][ticks][heads][dim] as 64 values x 128 ticks tiles, zeros outside
-inline CUtensorMap tile_map(const Scan& s, const Operand& o, int dim) {
+// [batch][ticks][heads][dim] as tiles of 128 bytes x 128 ticks, zeros outside
+inline CUtensorMap tile_map(const Scan& s, const Operand& o, int dim, bool f32 = false) {
+    const cuuint64_t size = f32 ? 4 : 2;
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -495,10 +620,10 @@ inline CUtensorMap tile_map(const Scan& s, const Operand& o, int dim) {
     CUtensorMap m;
     const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)(s.heads / o.share), (cuuint64_t)s.ticks,
                                 (cuuint64_t)(s.offsets ? 1 : s.batch)};
-    const cuuint64_t st[3] = {dims[1] > 1 ? (cuuint64_t)o.head * 2 : 16, dims[2] > 1 ? (cuuint64_t)o.tick * 2 : 16,
-                              dims[3] > 1 ? (cuuint64_t)o.batch * 2 : 16};
-    const cuuint32_t box[4] = {64, 1, kTcTicks, 1}, step[4] = {1, 1, 1, 1};
-    need(encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, o.p, dims, st, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t st[3] = {dims[1] > 1 ? o.head * size : 16, dims[2] > 1 ? o.tick * size : 16,
+                              dims[3] > 1 ? o.batch * size : 16};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, kTcTicks, 1}, step[4] = {1, 1, 1, 1};
+    need(encode(&m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, o.p, dims, st, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
          "fg_decay_attn: no tensor map for these strides");
     return m;
@@ -512,7 +637,8 @@ void tc_launch_as(const Scan& s, cudaStream_t st) {
         return true;
     }();
     (void)once;
-    const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E)};
+    const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E),
+                      tile_map(s, s.out, s.E, s.out_f32)};
     const unsigned rows = (unsigned)(s.batch * s.heads);
     if (s.parts > 1) k_decay_tc<DP, EP, BACK, true><<<dim3(rows, s.parts - 1), kTcThreads, bytes, st>>>(s, maps);
     k_decay_tc<DP, EP, BACK, false><<<dim3(rows, s.parts), kTcThreads, bytes, st>>>(s, maps);
