@@ -6,16 +6,19 @@
 // (run from the back: s >= t, gamma^{s-t}, exponents mirrored). Four products a chunk:
 //   A  [128 x 128] = a b^T                operands as they arrive, exact products
 //   O1 [128 x E]   = a S                  S rounded to bf16
-//   O2 [128 x E]   = W c                  W = A . gamma^{t-s} as two bf16 terms (2^-17), over A in TMEM
-//   dS [D x E]     = b'^T c               b' = gamma^{n-1-s} b as three bf16 terms (2^-25), over b, a and the copy of S
-// S itself stays in fp32 registers for the whole recording, thread = row, so states are as good as fp32 sums. The one
-// rounding to bf16, of S in O1, is of the size of the rounding of out itself.
+//   O2 [128 x E]   = W c                  W = A . gamma^{t-s} rounded to bf16, over A in TMEM
+//   dS [D x E]     = b'^T c               b' = gamma^{n-1-s} b as three bf16 terms (2^-25)
+// S itself stays in fp32 registers for the whole recording, thread = row, so states are as good as fp32 sums. The roundings
+// of S in O1 and of W in O2 are of the size of the rounding of out itself, and apart from one another: the three together
+// leave out sqrt(2) as far from exact as its own rounding alone.
 //
 // Tiles lie in shared memory as TMA writes them, 64 values (128 bytes, swizzled) of a tick in a row: read along the values
-// or along the ticks that is the K-major or the MN-major form of the same bytes, so nothing is transposed.
+// or along the ticks that is the K-major or the MN-major form of the same bytes, so nothing is transposed. 227 KB hold two
+// stages of a, b, c and a bf16 copy of S. At dim 64 the second and third terms of b' and out have places of their own; at
+// 128 the terms go over a and the copy of S once O1 is done with both, and out (with a value_dim of 128, too) over c.
 //
 // 20 warps: 0-7 the ticks (A to W, O1 and O2 to out; warps w and w + 4 share TMEM lanes 32 (w % 4) .. and take alternate
-// blocks of 32 columns), 8-15 the state (b to b', S), 16 the copies and the MMAs. The roles meet at mbarriers only, so a
+// blocks of columns), 8-15 the state (S), both b to b', 16 and 18 the MMAs, 17 the copies. The roles meet at mbarriers only, so a
 // chunk's elementwise work runs beside its MMAs and the next chunk's copies.
 #pragma once
 #include <cuda.h>
@@ -73,11 +76,32 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
-// (x, y) rounded to a bf16 pair, and what is left of them
-__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
-    const uint32_t r = pack_bf16(x, y);
-    x -= bf16_lo(r);
-    y -= bf16_hi(r);
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(uint64_t x) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+    return pack_bf16(a, b);
+}
+__device__ __forceinline__ uint64_t unpack2(uint32_t v) { return two(bf16_lo(v), bf16_hi(v)); }
+// a pair rounded to bf16, and what is left of it
+__device__ __forceinline__ uint32_t take2(uint64_t& x) {
+    const uint32_t r = pack2(x);
+    x = fma2(unpack2(r), two(-1.f, -1.f), x);
     return r;
 }
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int x, int head, int tick, int batch,
@@ -89,11 +113,9 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// Bounded wait for a barrier's phase. A try suspends the thread until the phase or about 0.1 ms are over, so that waiting
-// warps leave shared memory to the MMAs' operands.
+// Bounded wait for a barrier's phase: a try suspends the thread until the phase or about 0.1 ms are over.
 __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    const long long t0 = clock64();
-    for (;;) {
+    for (int tries = 0;; ++tries) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -104,14 +126,13 @@ __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile 
             : "memory");
         if (done) return true;
         if (*gave_up) return false;
-        if (clock64() - t0 > fg::kTcWaitCycles) {
+        if (tries > 20000) {                                 // (2 s)
             *gave_up = 1;
             atomicExch(&g_tc_error, 1);
             return false;
         }
     }
 }
-
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int head, int tick, int batch) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(map),
                  "r"(x), "r"(head), "r"(tick), "r"(batch), "r"(src)
@@ -126,428 +147,399 @@ struct TcMaps {
 // DP, EP: dim and value_dim up to 64 or 128
 template <int DP, int EP>
 struct TcLayout {
+    static constexpr bool own_terms = DP == 64, own_out = DP + EP < 256;
     static constexpr uint32_t a = 0, b = kTcTicks * DP * 2, c = 2 * b, stage = c + kTcTicks * EP * 2;
-    static constexpr uint32_t state = 2 * stage;             // the copy of S, then the third term of b'
-    static constexpr uint32_t after = state + (DP * EP * 2 > kTcTicks * DP * 2 ? DP * EP * 2 : kTcTicks * DP * 2);
-    // where a chunk of out is put together: room for fp32, or (no room left) where its c was, fp32 in two halves
-    static constexpr bool own_out = DP + EP < 256;
-    static constexpr uint32_t table = after + (own_out ? kTcTicks * EP * 4 : 0);
-    static constexpr uint32_t bars = table + (32 + 132 + 16) * 4;
-    static constexpr uint32_t bytes = bars + 128;
+    static constexpr uint32_t state = 2 * stage;
+    static constexpr uint32_t third = own_terms ? state + DP * EP * 2 : state, second = third + kTcTicks * DP * 2;   // (or over a)
+    static constexpr uint32_t out = own_terms ? second + kTcTicks * DP * 2 : second, out_bytes = 32768;              // (or over c)
+    static constexpr uint32_t table = out + (own_out ? out_bytes : 0);
+    static constexpr uint32_t bars = table + (32 + 132) * 4;
+    static constexpr uint32_t bytes = bars + 8 * 16 + 16;
+    static_assert(own_terms || DP * EP * 2 <= kTcTicks * DP * 2, "the copy of S fits the third term's place");
 };
-enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kCFree, kWReady, kBReady, kSReady, kOutRead, kMeet, kBars };
+enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kOutStored, kWReady, kBReady, kSReady, kOutRead, kMeet, kBars };
+static_assert(kBars <= 16, "room for the barriers");
 
-// PARTS: the states of the parts alone
-template <int DP, int EP, bool BACK, bool PARTS>
+// BACK: from the last tick to the first; F32: out in fp32; PARTS: the states of the parts alone
+template <int DP, int EP, bool BACK, bool F32, bool PARTS>
 __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constant__ Scan s,
                                                             const __grid_constant__ TcMaps maps) {
     extern __shared__ __align__(1024) unsigned char smem[];
     using L = TcLayout<DP, EP>;
     constexpr uint32_t kBox = kTcTicks * 128, kStateBox = DP * 128;
-    constexpr int kTmem = 512;
     constexpr uint32_t tA = 0, tO1 = 128, tO2 = tO1 + EP, tS = tO2 + EP;
     float* pw = reinterpret_cast<float*>(smem + L::table) + 32;   // gamma^0 .. gamma^128, before them zeros
-    float* ramp = pw + 132;                                  // gamma^{15-j}, from the back gamma^j
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
     volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const uint32_t sm = fg::smem_u32(smem), bar0 = fg::smem_u32(bars);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = s.D, E = s.E;
-    const int h = blockIdx.x % s.heads, part = blockIdx.y;
-    const long long b = blockIdx.x / s.heads;
+    const int h = blockIdx.x % s.heads, part = blockIdx.y, b = blockIdx.x / s.heads;
     const Span sp = span_of(s, b);
     const long long per = part_ticks(sp.n, s.parts), t0 = min(sp.n, part * per), t1 = min(sp.n, t0 + per);
     const bool hand_on = !PARTS && s.last && (sp.n ? t1 == sp.n && t1 > t0 : part == 0);
     if (t1 == t0 && !hand_on && !PARTS) return;
-    const int chunks = (int)((t1 - t0 + kTcTicks - 1) / kTcTicks);
+    const int total = (int)(t1 - t0), chunks = (total + kTcTicks - 1) / kTcTicks;
     const float ld = s.log_decay[h];
 
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     if (tid == 0) {
-        for (int i = 0; i < kBars; ++i) fg::mbar_init(bar(i), i >= kWReady ? 8 : 1);
+        for (int i = 0; i < kBars; ++i) fg::mbar_init(bar(i), i == kBReady && !PARTS ? 16 : i >= kWReady ? 8 : 1);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fg::smem_u32(tmem_slot)),
-                     "r"(kTmem)
+                     "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    for (int i = tid; i <= kTcTicks; i += kTcThreads) pw[i] = power(ld, (float)i);
-    if (tid < 32) pw[-1 - tid] = 0.f;
-    if (tid < 16) ramp[tid] = power(ld, (float)(BACK ? tid : 15 - tid));
+    if (tid <= kTcTicks) pw[tid] = power(ld, (float)tid);
+    else if (tid <= kTcTicks + 32) pw[kTcTicks - tid] = 0.f;
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // chunk i: its ticks, and the recording's tick of its first row (rows in recording order)
-    auto ticks_of = [&](int i) { return (int)min((long long)kTcTicks, t1 - t0 - (long long)i * kTcTicks); };
-    auto first_of = [&](int i) {
-        const long long t = t0 + (long long)i * kTcTicks;
-        return sp.start + (BACK ? sp.n - t - ticks_of(i) : t);
-    };
+    const int begin = (int)(sp.start + (BACK ? sp.n - t0 : t0));
+    auto ticks_of = [&](int i) { return min(kTcTicks, total - i * kTcTicks); };
+    auto first_of = [&](int i) { return BACK ? begin - i * kTcTicks - ticks_of(i) : begin + i * kTcTicks; };
+    const int batch = s.offsets ? 0 : b;
     auto wait = [&](int i, int chunk) { return tc_wait(bar(i), (uint32_t)chunk & 1, gave_up); };
-    auto wait_warp = [&](int i, int chunk) {
-        const bool ok = wait(i, chunk);
-        const bool all = __all_sync(0xffffffffu, ok);
+    auto wait_full = [&](int i) { return tc_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up); };
+    auto together = [&](bool ok) {                           // a warp goes on, or not, as one
+        ok = __all_sync(0xffffffffu, ok);
         fg::tc_fence_after();
-        return all;
+        return ok;
     };
     auto arrive = [&](int i) {                               // a warp's threads are all done
         __syncwarp();
         if (lane == 0) fg::mbar_arrive(bar(i));
     };
+    // b' = scale_in gamma^{..} b of chunk i (n ticks); ticks past its end (another recording's) become 0 in b' and c, whatever they hold.
+    // Worker w of 512 (256 without the ticks' warps).
+    auto fade_b = [&](int i, int n, int w) {
+        constexpr int kWorkers = PARTS ? 256 : 512;
+        unsigned char* stage = smem + (i & 1) * L::stage;
+        unsigned char* second = L::own_terms ? smem + L::second : stage + L::a;
+        if (n < kTcTicks)
+            for (int u = n * 8 + w; u < kTcTicks * 8; u += kWorkers)
+#pragma unroll
+                for (int x = 0; x < EP / 64; ++x) *reinterpret_cast<uint4*>(stage + L::c + x * kBox + u * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (int u = w; u < kTcTicks * DP / 8; u += kWorkers) {
+            const int r = (u >> 3) & 127;
+            const float f = pw[BACK ? r : max(n - 1 - r, 0)] * s.scale_in;
+            uint4 v = *reinterpret_cast<uint4*>(stage + L::b + u * 16), m, l;
+            if (r >= n) v = make_uint4(0, 0, 0, 0);
+            uint32_t* pv = &v.x;
+            uint32_t* pm = &m.x;
+            uint32_t* pl = &l.x;
+            const uint64_t f2 = two(f, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint64_t x = mul2(unpack2(pv[j]), f2);
+                pv[j] = take2(x);
+                pm[j] = take2(x);
+                pl[j] = pack2(x);
+            }
+            *reinterpret_cast<uint4*>(stage + L::b + u * 16) = v;
+            *reinterpret_cast<uint4*>(second + u * 16) = m;
+            *reinterpret_cast<uint4*>(smem + L::third + u * 16) = l;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        arrive(kBReady);
+    };
+    // when b' may be made: b is no longer A's operand, the terms' places are free, and the tile has arrived (TMA's writes are
+    // seen through its own barrier)
+    auto b_free = [&](int i) {
+        return (PARTS || wait(L::own_terms ? kQk : kQs, i)) && (i == 0 || wait(kKv, i - 1)) && wait_full(i);
+    };
     // with `first`, run from the back, S counts undecayed at the first tick
     const int lead0 = BACK && s.first && part == 0 && !PARTS ? 0 : 1;
     bool ok = true;
 
-    // 20 warps start with 96 registers a thread: 640 x 96 = 61,440. The copies and MMAs (and the three warps beside them, there
+    // 20 warps start with 96 registers a thread: 640 x 96 = 61,440. The MMAs and copies (and the warp beside them, there
     // because registers change hands by four warps) keep 48, the ticks 88, so that the state has 128 (S alone is 64):
     // 128 x 48 + 256 x 88 + 256 x 128 = 61,440
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         // ---- copies and MMAs -----------------------------------------------------------------------------------
-        if (warp == 16 && lane == 0) {
-            const int da = (D + 63) / 64, ec = (E + 63) / 64, batch = s.offsets ? 0 : (int)b;
-            auto copy = [&](int i) {                         // a and b (and the bytes that c will add)
+        if (warp == 17 && lane == 0) {
+            // a chunk goes into the stage that the one before the last has left: its products are done, and its out, where it
+            // is put together over c, is stored
+            const int da = (D + 63) / 64, ec = (E + 63) / 64;
+            const int head_a = h / s.a.share, head_b = h / s.b.share, head_c = h / s.c.share;
+            int copied = 0;
+#pragma unroll 1
+            for (int i = 0; i < chunks && ok; ++i) {
                 const uint32_t stage = sm + (i & 1) * L::stage, full = bar(kFull0 + (i & 1));
-                const int tick = (int)first_of(i);
+                const int tick = first_of(i);
+                if (i >= 2) ok = wait(kKv, i - 2) && (PARTS || (wait(kPv, i - 2) && (L::own_out || wait(kOutStored, i - 2))));
+                if (!ok) break;
                 fg::mbar_expect_tx(full, (uint32_t)((PARTS ? 1 : 2) * da + ec) * kBox);
+#pragma unroll 1
                 for (int x = 0; x < da; ++x) {
-                    if (!PARTS) tma_tile(stage + L::a + x * kBox, &maps.a, x * 64, h / s.a.share, tick, batch, full);
-                    tma_tile(stage + L::b + x * kBox, &maps.b, x * 64, h / s.b.share, tick, batch, full);
+                    if (!PARTS) tma_tile(stage + L::a + x * kBox, &maps.a, x * 64, head_a, tick, batch, full);
+                    tma_tile(stage + L::b + x * kBox, &maps.b, x * 64, head_b, tick, batch, full);
                 }
-            };
-            auto copy_c = [&](int i) {
-                const uint32_t stage = sm + (i & 1) * L::stage, full = bar(kFull0 + (i & 1));
-                for (int x = 0; x < ec; ++x)
-                    tma_tile(stage + L::c + x * kBox, &maps.c, x * 64, h / s.c.share, (int)first_of(i), batch, full);
-            };
-            // 16 values of a K-major tile; 16 ticks (rows) of an MN-major one; descriptors count in 16 bytes
-            constexpr auto along = [](int k) { return (uint64_t)((k >> 2) * kBox + (k & 3) * 32) >> 4; };
-            constexpr auto down = [](int k) { return (uint64_t)(k * 2048) >> 4; };
-            const uint32_t id_a = bf16_idesc(128, 0, 0), id_o = bf16_idesc(E, 0, 1), id_s = bf16_idesc(E, 1, 1);
+#pragma unroll 1
+                for (int x = 0; x < ec; ++x) tma_tile(stage + L::c + x * kBox, &maps.c, x * 64, head_c, tick, batch, full);
+                ++copied;
+            }
+            // (after a wait ran out, too) the copies land before the block ends
+            for (int i = max(0, copied - 2); i < copied; ++i)
+                for (int tries = 0; !fg::mbar_try(bar(kFull0 + (i & 1)), (i >> 1) & 1) && tries < 10000000; ++tries) {}
+        } else if (warp == 16 && lane == 0 && !PARTS) {
+            // A, O1 and O2. Unrolled: issued one by one in a loop they took longer than the tensor cores
+            const uint32_t id_a = bf16_idesc(128, 0, 0), id_o = bf16_idesc(E, 0, 1);
+            // descriptors count in 16 bytes: 16 values of a K-major tile, 16 ticks (rows) of an MN-major one
+            constexpr auto along = [](int k) { return (uint64_t)((k >> 2) * (kBox >> 4) + (k & 3) * 2); };
             const uint64_t state_rows = swizzled(sm + L::state, kStateBox);
-            constexpr uint32_t next_b = DP == 128 ? kBox : 0;     // (an M = 128 operand of 64 values: twice the same)
-            int started = 0, copied = 0;                     // chunks whose a and b, and whose c too, are on their way
-            if (chunks) { copy(0); copy_c(0); started = copied = 1; }
+#pragma unroll 1
             for (int i = 0; i < chunks && ok; ++i) {
                 const uint32_t stage = sm + (i & 1) * L::stage;
-                const uint64_t a_ticks = swizzled(stage + L::a, 0), b_ticks = swizzled(stage + L::b, 0),
-                               c_rows = swizzled(stage + L::c, kBox);
-                const uint64_t terms[3] = {swizzled(stage + L::b, next_b), swizzled(stage + L::a, next_b), swizzled(sm + L::state, next_b)};
-                if (i > 0) ok = wait(kKv, i - 1) && (PARTS || wait(kPv, i - 1));   // the other stage is free, and A
-                if (!ok) break;
-                const bool more = i + 1 < chunks, wait_c = !PARTS && !L::own_out && i > 0;
-                if (more) { copy(i + 1); ++started; }
-                if (more && !wait_c) { copy_c(i + 1); ++copied; }
-                ok = tc_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up);
-                if (!ok) break;
-                fg::tc_fence_after();
-                if (!PARTS) {
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k)
-                        mma_bf16(tmem + tA, a_ticks + along(k), b_ticks + along(k), id_a, k > 0);
-                    fg::mma_commit(bar(kQk));
-                    if (more && wait_c) {                    // out of the chunk before has left c's place
-                        ok = wait(kCFree, i - 1);
-                        if (!ok) break;
-                        copy_c(i + 1);
-                        ++copied;
-                    }
-                    ok = wait(kSReady, i) && (i == 0 || wait(kOutRead, i - 1));
-                    if (!ok) break;
-                    fg::tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k)
-                        mma_bf16(tmem + tO1, a_ticks + along(k), state_rows + down(k), id_o, k > 0);
-                    fg::mma_commit(bar(kQs));
-                    ok = wait(kWReady, i) && (ticks_of(i) == kTcTicks || wait(kBReady, i));   // (c's end is cleared there)
-                    if (!ok) break;
-                    fg::tc_fence_after();
-#pragma unroll
-                    for (int term = 0; term < 2; ++term)
-#pragma unroll
-                        for (int k = 0; k < kTcTicks / 16; ++k)
-                            mma_bf16_tmem(tmem + tO2, tmem + tA + k * 16 + term * 8, c_rows + down(k), id_o, term + k > 0);
-                    fg::mma_commit(bar(kPv));
-                } else {
-                    fg::mma_commit(bar(kQk));                // (nothing before it: the tile has arrived)
-                    ok = wait(kSReady, i);                   // dS has been read
-                    if (!ok) break;
-                }
-                ok = wait(kBReady, i);
+                const uint64_t a_ticks = swizzled(stage + L::a, 0), b_ticks = swizzled(stage + L::b, 0), c_rows = swizzled(stage + L::c, kBox);
+                ok = wait_full(i) && (i == 0 || wait(kPv, i - 1));   // W is read
                 if (!ok) break;
                 fg::tc_fence_after();
 #pragma unroll
-                for (int term = 0; term < 3; ++term)
+                for (int k = 0; k < DP / 16; ++k) mma_bf16(tmem + tA, a_ticks + along(k), b_ticks + along(k), id_a, k > 0);
+                fg::mma_commit(bar(kQk));
+                ok = wait(kSReady, i) && (i == 0 || wait(kOutRead, i - 1));
+                if (!ok) break;
+                fg::tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < kTcTicks / 16; ++k)
-                        mma_bf16(tmem + tS, terms[term] + down(k), c_rows + down(k), id_s, term + k > 0);
+                for (int k = 0; k < DP / 16; ++k) mma_bf16(tmem + tO1, a_ticks + along(k), state_rows + 128 * k, id_o, k > 0);
+                fg::mma_commit(bar(kQs));
+                ok = wait(kWReady, i) && (ticks_of(i) == kTcTicks || wait(kBReady, i));   // (c's end is cleared there)
+                if (!ok) break;
+                fg::tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kTcTicks / 16; ++k) mma_bf16_tmem(tmem + tO2, tmem + tA + k * 16, c_rows + 128 * k, id_o, k > 0);
+                fg::mma_commit(bar(kPv));
+            }
+        } else if (warp == 18 && lane == 0) {
+            // dS
+            const uint32_t id_s = bf16_idesc(E, 1, 1);
+            constexpr uint32_t next_b = DP == 128 ? kBox : 0;     // (an M = 128 operand of 64 values: twice the same)
+            const uint64_t third = swizzled(sm + L::third, next_b);
+#pragma unroll 1
+            for (int i = 0; i < chunks && ok; ++i) {
+                const uint32_t stage = sm + (i & 1) * L::stage;
+                const uint64_t first = swizzled(stage + L::b, next_b), c_rows = swizzled(stage + L::c, kBox),
+                               second = swizzled(L::own_terms ? sm + L::second : stage + L::a, next_b);
+                ok = wait(kBReady, i) && wait(kSReady, i);   // dS of the chunk before has been read
+                if (!ok) break;
+                fg::tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mma_bf16(tmem + tS, first + 128 * k, c_rows + 128 * k, id_s, k > 0);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mma_bf16(tmem + tS, second + 128 * k, c_rows + 128 * k, id_s, true);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mma_bf16(tmem + tS, third + 128 * k, c_rows + 128 * k, id_s, true);
                 fg::mma_commit(bar(kKv));
             }
-            if (!ok && copied < started) copy_c(copied++);
-            if (!ok)                                         // let the copies in flight land before the block ends
-                for (int i = max(0, copied - 2); i < copied; ++i) {
-                    const long long c0 = clock64();
-                    while (!fg::mbar_try(bar(kFull0 + (i & 1)), (i >> 1) & 1) && clock64() - c0 < fg::kTcWaitCycles) {}
-                }
         }
     } else if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- ticks ---------------------------------------------------------------------------------------------
         const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+        // gamma^{t-s} of a block of 16 columns s0 .. is gamma^{t-s0-15} gamma^{15-j} (from the back gamma^{s0-t} gamma^j). Off the
+        // diagonal both are at most 1; on it the first may be over 1, and where it could overflow the weights are looked up.
+        uint64_t near[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) near[k] = BACK ? two(pw[2 * k], pw[2 * k + 1]) : two(pw[15 - 2 * k], pw[14 - 2 * k]);
+        const float scale = s.scale_in * s.scale_out;
+        const bool in_range = ld > -2.f;                     // (e^(2 * 31) is finite by far)
         int meetings = 0;
         auto meet = [&]() {                                  // the eight warps wait for one another
             arrive(kMeet);
-            return wait_warp(kMeet, meetings++);
+            return together(wait(kMeet, meetings++));
         };
+#pragma unroll 1
         for (int i = 0; !PARTS && i < chunks && ok; ++i) {
             const int n = ticks_of(i);
-            ok = wait_warp(kQk, i);
+            ok = together(wait(kQk, i));
             if (!ok) break;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int blk = 2 * j + half;                 // blocks of 32 on one side of the diagonal are 0
-                uint32_t v[2][16], hi[8], lo[8];
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                const int blk = (j & 2) + half, s0 = blk * 32 + (j & 1) * 16;   // blocks of 32 on one side of the diagonal are 0
+                uint32_t v[16], x[8];
                 if (BACK ? blk < quarter : blk > quarter) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) hi[k] = 0;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tmem_st8(lanes + tA + blk * 32 + k * 8, hi);
+                    for (int k = 0; k < 8; ++k) x[k] = 0;
+                    tmem_st8(lanes + tA + s0, x);
                     continue;
                 }
-                tmem_ld16(lanes + tA + blk * 32, v[0]);
-                tmem_ld16(lanes + tA + blk * 32 + 16, v[1]);
-                tmem_ready(v[0]);
-                tmem_ready(v[1]);
+                tmem_ld16(lanes + tA + s0, v);
+                const int away = BACK ? s0 - row : row - s0 - 15;   // exponent of the first factor
+                const float e = (in_range ? expf(ld * (float)away) : power(ld, (float)away)) * scale;
+                tmem_ready(v);
+                if (blk != quarter || in_range) {
+                    const uint64_t e2 = two(e, e);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int s0 = blk * 32 + q * 16;
-                    if (BACK && n < kTcTicks) {               // the last ticks are not the chunk's
+                    for (int k = 0; k < 8; ++k)
+                        x[k] = pack2(mul2(two(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), mul2(e2, near[k])));
+                } else {                                      // (rare: one pair at a time, to keep it short)
+#pragma unroll 1
+                    for (int k = 0; k < 16; k += 2) {
+                        const float* g = pw + (BACK ? s0 + k - row : row - s0 - k);   // gamma^{t-s}; 0 past the diagonal
+                        const uint32_t y = pack_bf16(__uint_as_float(v[0]) * g[0] * scale, __uint_as_float(v[1]) * g[BACK ? 1 : -1] * scale);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (s0 + k >= n) v[q][k] = 0;
+                        for (int m = 0; m < 14; ++m) v[m] = v[m + 2];
+#pragma unroll
+                        for (int m = 0; m < 7; ++m) x[m] = x[m + 1];
+                        x[7] = y;
                     }
-                    if (blk != quarter) {                    // gamma^{t-s} as two factors, both at most 1
-                        const float f = pw[BACK ? s0 - row : row - s0 - 15];
-                        const float4* r4 = reinterpret_cast<const float4*>(ramp);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float4 g = r4[k];
-                            float x0 = __uint_as_float(v[q][4 * k]) * (f * g.x), x1 = __uint_as_float(v[q][4 * k + 1]) * (f * g.y);
-                            float x2 = __uint_as_float(v[q][4 * k + 2]) * (f * g.z), x3 = __uint_as_float(v[q][4 * k + 3]) * (f * g.w);
-                            hi[2 * k] = take_bf16(x0, x1);
-                            lo[2 * k] = pack_bf16(x0, x1);
-                            hi[2 * k + 1] = take_bf16(x2, x3);
-                            lo[2 * k + 1] = pack_bf16(x2, x3);
-                        }
-                    } else {
-                        const float* g = pw + (BACK ? s0 - row : row - s0);   // gamma^{t-s} in turn; 0 past the diagonal
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            float x = __uint_as_float(v[q][2 * k]) * g[BACK ? 2 * k : -2 * k];
-                            float y = __uint_as_float(v[q][2 * k + 1]) * g[BACK ? 2 * k + 1 : -2 * k - 1];
-                            hi[k] = take_bf16(x, y);
-                            lo[k] = pack_bf16(x, y);
-                        }
-                    }
-                    tmem_st8(lanes + tA + s0, hi);
-                    tmem_st8(lanes + tA + s0 + 8, lo);
                 }
+                if (blk == quarter || (BACK && n < kTcTicks)) {
+                    // only columns up to the diagonal (from it on), and only the chunk's own
+                    const int lo = BACK ? row - s0 : 0, up = BACK ? n - s0 : row - s0 + 1;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t keep = (2 * k >= lo && 2 * k < up ? 0xffffu : 0u) | (2 * k + 1 >= lo && 2 * k + 1 < up ? 0xffff0000u : 0u);
+                        x[k] &= keep;
+                    }
+                }
+                tmem_st8(lanes + tA + s0, x);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             fg::tc_fence_before();
             arrive(kWReady);
-            const float f = pw[max(BACK ? n - 1 - row : row, 0) + (i ? 1 : lead0)] * s.scale_out;
-            const float g = s.scale_in * s.scale_out;
-            ok = wait_warp(kQs, i) && wait_warp(kPv, i);
+            ok = together(b_free(i));
             if (!ok) break;
-            auto out16 = [&](int e0, float (&o)[16]) {
-                uint32_t x[16], y[16];
-                tmem_ld16(lanes + tO1 + e0, x);
-                tmem_ld16(lanes + tO2 + e0, y);
-                tmem_ready(x);
-                tmem_ready(y);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = fmaf(__uint_as_float(x[k]), f, __uint_as_float(y[k]) * g);
-            };
-            if (n == kTcTicks) {
-                // put together in shared memory, stored as one tile (a thread's own stores, 32 lines at a time, held up the
-                // MMAs' operands: 4,000 instead of 1,900 clocks for dS)
-                const uint32_t tile = L::own_out ? L::after : (i & 1) * L::stage + L::c;
-                if (!L::own_out) {
-                    ok = wait_warp(kKv, i);
-                    if (!ok) break;
-                }
-                if (tid == 0) stores_read();
-                ok = meet();
-                if (!ok) break;
-                const int halves = !L::own_out && s.out_f32 ? 2 : 1;
-                for (int r = 0; r < halves && ok; ++r) {
+            fade_b(i, n, tid);
+            ok = together(wait(kQs, i) && wait(kPv, i) && (L::own_out || wait(kKv, i)));
+            if (!ok) break;
+            // out of whole chunks is put together in shared memory and stored as tiles (a thread's own stores, 32 lines at a
+            // time, held up the MMAs' operands); a recording's last ticks go by themselves: what follows them is another's
+            const bool whole = n == kTcTicks;
+            const float f = pw[max(BACK ? n - 1 - row : row, 0) + (i ? 1 : lead0)] * s.scale_out;
+            const uint64_t f2 = two(f, f);
+            const long long at = batch * s.out.batch + (long long)(first_of(i) + row) * s.out.tick + h * s.out.head;
+            unsigned char* tile = smem + (L::own_out ? L::out : (i & 1) * L::stage + L::c);
+            constexpr int width = F32 ? 64 : 128, units = F32 ? 4 : 2;   // columns that fit; 16-byte units of 16
 #pragma unroll 1
-                    for (int e0 = (halves == 2 ? r * 64 : 0) + half * 16; e0 < (halves == 2 ? min(E, r * 64 + 64) : E); e0 += 32) {
-                        float o[16];
-                        out16(e0, o);
-                        const int x0 = halves == 2 ? e0 - r * 64 : e0;
-                        if (s.out_f32) {
-                            unsigned char* at = smem + tile + (x0 >> 5) * kBox + row * 128;
+            for (int first = 0; first < E && ok; first += width) {
+                const int end = min(E, first + width);
+#pragma unroll 1
+                for (int e0 = first + half * 16; e0 < end; e0 += 32) {
+                    uint32_t x[16], y[16];
+                    tmem_ld16(lanes + tO1 + e0, x);
+                    tmem_ld16(lanes + tO2 + e0, y);
+                    tmem_ready(x);
+                    tmem_ready(y);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                *reinterpret_cast<float4*>(at + (((((x0 & 31) >> 2) + k) ^ (row & 7)) << 4)) =
-                                    make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    for (int k = 0; k < 8; ++k) {
+                        const uint64_t o = fma2(two(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), f2,
+                                                two(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])));
+                        if (F32) {
+                            asm("mov.b64 {%0, %1}, %2;" : "=r"(x[2 * k]), "=r"(x[2 * k + 1]) : "l"(o));
                         } else {
-                            unsigned char* at = smem + tile + (x0 >> 6) * kBox + row * 128;
-#pragma unroll
-                            for (int k = 0; k < 2; ++k)
-                                *reinterpret_cast<uint4*>(at + (((((x0 & 63) >> 3) + k) ^ (row & 7)) << 4)) =
-                                    make_uint4(pack_bf16(o[8 * k], o[8 * k + 1]), pack_bf16(o[8 * k + 2], o[8 * k + 3]),
-                                               pack_bf16(o[8 * k + 4], o[8 * k + 5]), pack_bf16(o[8 * k + 6], o[8 * k + 7]));
+                            x[k] = pack2(o);
                         }
                     }
-                    if (r + 1 == halves) {
-                        fg::tc_fence_before();
-                        arrive(kOutRead);
+                    const int u0 = (e0 - first) * units / 16;        // 16-byte units, 8 to a box's row
+                    unsigned char* to = whole ? tile + (u0 >> 3) * kBox + row * 128
+                                              : reinterpret_cast<unsigned char*>(s.out.p) + (at + e0) * (F32 ? 4 : 2);
+                    if (whole || row < n) {
+#pragma unroll
+                        for (int k = 0; k < units; ++k)
+                                *reinterpret_cast<uint4*>(to + (whole ? (((u0 & 7) + k) ^ (row & 7)) << 4 : k * 16)) =
+                                    make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
                     }
+                    __syncwarp();
+                }
+                if (end == E) {
+                    fg::tc_fence_before();
+                    arrive(kOutRead);
+                }
+                if (whole) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     ok = meet();
                     if (ok && tid == 0) {
-                        const int values = s.out_f32 ? 32 : 64, e1 = halves == 2 ? min(E, r * 64 + 64) : E;
-                        for (int e0 = halves == 2 ? r * 64 : 0, x = 0; e0 < e1; e0 += values, ++x)
-                            tma_store(&maps.out, sm + tile + x * kBox, e0, h, (int)first_of(i), s.offsets ? 0 : (int)b);
+                        constexpr int values = F32 ? 32 : 64;
+                        for (int e0 = first; e0 < end; e0 += values)
+                            tma_store(&maps.out, fg::smem_u32(tile) + (e0 - first) / values * kBox, e0, h, first_of(i), batch);
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                        if (!L::own_out) {
-                            stores_read();
-                            if (r + 1 == halves) fg::mbar_arrive(bar(kCFree));
-                        }
+                        stores_read();
                     }
                     __syncwarp();
-                    if (r + 1 < halves) ok = ok && meet();
+                    if (end < E || L::own_out) ok = ok && meet();    // (then the place is free again)
                 }
-            } else {                                          // a recording's last ticks: what follows them is another's
-                const long long at = (s.offsets ? 0 : b * s.out.batch) + (first_of(i) + row) * s.out.tick + h * s.out.head;
-#pragma unroll 1
-                for (int e0 = half * 16; e0 < E; e0 += 32) {
-                    float o[16];
-                    out16(e0, o);
-                    if (row < n && s.out_f32) {
-                        float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(s.out.p) + at + e0);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) p[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                    } else if (row < n) {
-                        uint4* p = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(s.out.p) + at + e0);
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            p[k] = make_uint4(pack_bf16(o[8 * k], o[8 * k + 1]), pack_bf16(o[8 * k + 2], o[8 * k + 3]),
-                                              pack_bf16(o[8 * k + 4], o[8 * k + 5]), pack_bf16(o[8 * k + 6], o[8 * k + 7]));
-                    }
-                    __syncwarp();
-                }
-                fg::tc_fence_before();
-                arrive(kOutRead);
-                if (!L::own_out && tid == 0) fg::mbar_arrive(bar(kCFree));
             }
+            if (!L::own_out && tid == 0) fg::mbar_arrive(bar(kOutStored));
         }
         if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ---- state ---------------------------------------------------------------------------------------------
-        const int quarter = warp & 3, half = (warp >> 2) & 1, row = quarter * 32 + lane, st = tid - 256;
+        const int quarter = warp & 3, half = (warp >> 2) & 1, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const bool mine = row < D;
         float S[EP / 32][16];
-        const long long state0 = (b * s.heads + h) * D * E;
 #pragma unroll
-        for (int j = 0; j < EP / 32; ++j) {
-            const int e0 = (2 * j + half) * 16;
+        for (int j = 0; j < EP / 32; ++j)
 #pragma unroll
             for (int i = 0; i < 16; ++i) S[j][i] = 0.f;
-            if (PARTS || !mine || e0 >= E) continue;
-            if (s.first) {
-                const float f = power(ld, (float)(BACK ? max(t0 - 1, 0ll) : t0));
+        const long long state0 = ((long long)b * s.heads + h) * D * E;
+        // S += f * the state at p, which may lie [E][D]
+        auto add = [&](const float* p, float f, bool across) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    S[j][i] = f * s.first[state0 + (s.first_t ? (long long)(e0 + i) * D + row : (long long)row * E + e0 + i)];
-            }
-            for (int p = 0; p < part; ++p) {
-                const float f = power(ld, (float)(t0 - min(sp.n, (p + 1) * per)));
-                const float4* q = reinterpret_cast<const float4*>(
-                    s.partial + ((b * s.heads + h) * s.parts + p) * D * E + (long long)row * E + e0);
+            for (int j = 0; j < EP / 32; ++j) {
+                const int e0 = (2 * j + half) * 16;
+                if (!mine || e0 >= E) continue;
+                if (across) {
+                    const float* q = p + (long long)e0 * D + row;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 v = q[i];
-                    S[j][4 * i] = fmaf(f, v.x, S[j][4 * i]);
-                    S[j][4 * i + 1] = fmaf(f, v.y, S[j][4 * i + 1]);
-                    S[j][4 * i + 2] = fmaf(f, v.z, S[j][4 * i + 2]);
-                    S[j][4 * i + 3] = fmaf(f, v.w, S[j][4 * i + 3]);
+                    for (int i = 0; i < 16; ++i, q += D) S[j][i] = fmaf(f, *q, S[j][i]);
+                } else {
+                    const float4* q = reinterpret_cast<const float4*>(p + row * E + e0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 v = q[i];
+                        S[j][4 * i] = fmaf(f, v.x, S[j][4 * i]);
+                        S[j][4 * i + 1] = fmaf(f, v.y, S[j][4 * i + 1]);
+                        S[j][4 * i + 2] = fmaf(f, v.z, S[j][4 * i + 2]);
+                        S[j][4 * i + 3] = fmaf(f, v.w, S[j][4 * i + 3]);
+                    }
                 }
             }
+        };
+        if (!PARTS) {
+            const float* parts = s.partial + ((long long)b * s.heads + h) * s.parts * D * E;
+#pragma unroll 1
+            for (int p = s.first ? -1 : 0; p < part; ++p)
+                add(p < 0 ? s.first + state0 : parts + (long long)p * D * E,
+                    power(ld, (float)(p < 0 ? (BACK ? max(t0 - 1, 0ll) : t0) : t0 - min(sp.n, (p + 1) * per))), p < 0 && s.first_t);
         }
-        auto put_state = [&]() {                             // S as the operand of O1: rows d, columns e, swizzled
-            if (!PARTS) {
+#pragma unroll 1
+        for (int i = 0; i < chunks && ok; ++i) {
+            // S as the operand of O1: rows d, columns e, swizzled (rows past D: zeros, for the k-steps of 16 up to DP)
+            if (!PARTS && row < DP) {
+                unsigned char* at = smem + L::state + row * 128;
 #pragma unroll
                 for (int j = 0; j < EP / 32; ++j) {
-                    const int e0 = (2 * j + half) * 16, unit = (e0 & 63) >> 3;
-                    if (row < DP && e0 < E) {                // (rows past D: zeros, for the k-steps of 16 up to DP)
-                        unsigned char* at = smem + L::state + (e0 >> 6) * kStateBox + row * 128;
-                        const float* x = S[j];
-                        *reinterpret_cast<uint4*>(at + ((unit ^ (row & 7)) << 4)) =
+                    const int e0 = (2 * j + half) * 16;
+                    if (e0 >= E) continue;
+                    const float* x = S[j];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k, x += 8)
+                        *reinterpret_cast<uint4*>(at + (e0 >> 6) * kStateBox + (((((e0 & 63) >> 3) + k) ^ (row & 7)) << 4)) =
                             make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-                        *reinterpret_cast<uint4*>(at + (((unit + 1) ^ (row & 7)) << 4)) = make_uint4(
-                            pack_bf16(x[8], x[9]), pack_bf16(x[10], x[11]), pack_bf16(x[12], x[13]), pack_bf16(x[14], x[15]));
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
-            fg::tc_fence_before();
-            arrive(kSReady);
-        };
-        put_state();
-        for (int i = 0; i < chunks && ok; ++i) {
-            const int n = ticks_of(i);
-            unsigned char* stage = smem + (i & 1) * L::stage;
-            ok = wait_warp(kQk, i) && (PARTS || wait_warp(kQs, i));
-            // (the tile itself: TMA's writes are seen through its own barrier)
-            ok = ok && __all_sync(0xffffffffu, tc_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up));
-            if (!ok) break;
-            // b' in three terms, over b, a and the copy of S; ticks past the chunk's end (another recording's) become 0 in
-            // b' and c, whatever they hold
-            for (int u = n * 8 + st; n < kTcTicks && u < kTcTicks * 8; u += 256) {
-#pragma unroll
-                for (int x = 0; x < EP / 64; ++x) *reinterpret_cast<uint4*>(stage + L::c + x * kBox + u * 16) = make_uint4(0, 0, 0, 0);
-            }
-            float f[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = pw[BACK ? (st >> 3) + 32 * k : max(n - 1 - (st >> 3) - 32 * k, 0)];
-#pragma unroll 1
-            for (int x = 0; x < DP / 64; ++x) {
-                unsigned char* at = stage + L::b + x * kBox + st * 16;
-                unsigned char* at_lo = smem + L::state + x * kBox + st * 16;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint4 v = *reinterpret_cast<uint4*>(at + k * 4096), m, l;
-                    if ((st >> 3) + 32 * k >= n) v = make_uint4(0, 0, 0, 0);
-                    uint32_t* pv = &v.x;
-                    uint32_t* pm = &m.x;
-                    uint32_t* pl = &l.x;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float y = bf16_lo(pv[j]) * f[k], z = bf16_hi(pv[j]) * f[k];
-                        pv[j] = take_bf16(y, z);
-                        pm[j] = take_bf16(y, z);
-                        pl[j] = pack_bf16(y, z);
-                    }
-                    *reinterpret_cast<uint4*>(at + k * 4096) = v;
-                    *reinterpret_cast<uint4*>(at - L::b + L::a + k * 4096) = m;
-                    *reinterpret_cast<uint4*>(at_lo + k * 4096) = l;
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(kBReady);
-            ok = wait_warp(kKv, i);
+            fg::tc_fence_before();
+            arrive(kSReady);
+            const int n = ticks_of(i);
+            ok = together(b_free(i));
+            if (!ok) break;
+            fade_b(i, n, PARTS ? tid - 256 : tid);
+            ok = together(wait(kKv, i));
             if (!ok) break;
             const float fade = pw[n - 1 + (i ? 1 : lead0)];
 #pragma unroll
@@ -557,28 +549,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 tmem_ld16(lanes + tS + (2 * j + half) * 16, v);
                 tmem_ready(v);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) S[j][k] = fmaf(S[j][k], fade, s.scale_in * __uint_as_float(v[k]));
+                for (int k = 0; k < 16; ++k) S[j][k] = fmaf(S[j][k], fade, __uint_as_float(v[k]));
             }
-            if (i + 1 < chunks) put_state();
         }
-        if (*gave_up) {                                      // say so in what is handed on, too
-#pragma unroll
-            for (int j = 0; j < EP / 32; ++j)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) S[j][k] = __int_as_float(0x7fc00000);
-        }
-        float* to = PARTS ? s.partial + ((b * s.heads + h) * s.parts + part) * D * E : hand_on ? s.last + state0 : nullptr;
+        float* to = PARTS ? s.partial + (((long long)b * s.heads + h) * s.parts + part) * D * E : hand_on ? s.last + state0 : nullptr;
         if (to && mine) {
-            const float f = !PARTS && BACK && sp.n ? pw[1] : 1.f;
+            const bool across = !PARTS && s.last_t;
+            // (a wait that ran out says so in what is handed on, too)
+            const float f = *gave_up ? __int_as_float(0x7fc00000) : !PARTS && BACK && sp.n ? pw[1] : 1.f;
 #pragma unroll
             for (int j = 0; j < EP / 32; ++j) {
                 const int e0 = (2 * j + half) * 16;
                 if (e0 >= E) continue;
-                if (!PARTS && s.last_t) {
+                if (across) {
+                    float* p = to + (long long)e0 * D + row;
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) to[(long long)(e0 + k) * D + row] = f * S[j][k];
+                    for (int k = 0; k < 16; ++k, p += D) *p = f * S[j][k];
                 } else {
-                    float4* p = reinterpret_cast<float4*>(to + (long long)row * E + e0);
+                    float4* p = reinterpret_cast<float4*>(to + row * E + e0);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         p[k] = make_float4(f * S[j][4 * k], f * S[j][4 * k + 1], f * S[j][4 * k + 2], f * S[j][4 * k + 3]);
@@ -589,8 +577,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
-    if (warp == 16)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // what 16-byte copies and tensor maps take: strides of dimensions that there is more than one of
@@ -628,29 +615,29 @@ inline CUtensorMap tile_map(const Scan& s, const Operand& o, int dim, bool f32 =
          "fg_decay_attn: no tensor map for these strides");
     return m;
 }
-template <int DP, int EP, bool BACK>
+template <int DP, int EP, bool BACK, bool F32>
 void tc_launch_as(const Scan& s, cudaStream_t st) {
     constexpr int bytes = TcLayout<DP, EP>::bytes;
     static const bool once = [] {
-        MCK(cudaFuncSetAttribute(k_decay_tc<DP, EP, BACK, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        MCK(cudaFuncSetAttribute(k_decay_tc<DP, EP, BACK, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        MCK(cudaFuncSetAttribute(k_decay_tc<DP, EP, BACK, F32, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        MCK(cudaFuncSetAttribute(k_decay_tc<DP, EP, BACK, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         return true;
     }();
     (void)once;
-    const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E),
-                      tile_map(s, s.out, s.E, s.out_f32)};
+    const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E), tile_map(s, s.out, s.E, F32)};
     const unsigned rows = (unsigned)(s.batch * s.heads);
-    if (s.parts > 1) k_decay_tc<DP, EP, BACK, true><<<dim3(rows, s.parts - 1), kTcThreads, bytes, st>>>(s, maps);
-    k_decay_tc<DP, EP, BACK, false><<<dim3(rows, s.parts), kTcThreads, bytes, st>>>(s, maps);
+    if (s.parts > 1) k_decay_tc<DP, EP, BACK, false, true><<<dim3(rows, s.parts - 1), kTcThreads, bytes, st>>>(s, maps);
+    k_decay_tc<DP, EP, BACK, F32, false><<<dim3(rows, s.parts), kTcThreads, bytes, st>>>(s, maps);
     MCK(cudaGetLastError());
 }
-template <bool BACK>
+template <bool BACK, bool F32>
 void tc_launch_dims(const Scan& s, cudaStream_t st) {
-    if (s.D > 64) s.E > 64 ? tc_launch_as<128, 128, BACK>(s, st) : tc_launch_as<128, 64, BACK>(s, st);
-    else s.E > 64 ? tc_launch_as<64, 128, BACK>(s, st) : tc_launch_as<64, 64, BACK>(s, st);
+    if (s.D > 64) s.E > 64 ? tc_launch_as<128, 128, BACK, F32>(s, st) : tc_launch_as<128, 64, BACK, F32>(s, st);
+    else s.E > 64 ? tc_launch_as<64, 128, BACK, F32>(s, st) : tc_launch_as<64, 64, BACK, F32>(s, st);
 }
 inline void tc_launch(const Scan& s, cudaStream_t st) {
-    s.backward ? tc_launch_dims<true>(s, st) : tc_launch_dims<false>(s, st);
+    if (!s.backward) tc_launch_dims<false, false>(s, st);
+    else s.out_f32 ? tc_launch_dims<true, true>(s, st) : tc_launch_dims<true, false>(s, st);
 }
 
 }  // namespace
