@@ -18,7 +18,8 @@
 // 128 the terms go over a and the copy of S once O1 is done with both, and out (with a value_dim of 128, too) over c.
 //
 // 20 warps: 0-7 the ticks (A to W, O1 and O2 to out; warps w and w + 4 share TMEM lanes 32 (w % 4) .. and take alternate
-// blocks of columns), 8-15 the state (S), both b to b', 16 and 18 the MMAs, 17 the copies. The roles meet at mbarriers only, so a
+// blocks of columns), 8-15 the state (S, b to b'), 16 and 18 the MMAs, 17 and 19 the copies in and
+// out. The roles meet at mbarriers only, so a
 // chunk's elementwise work runs beside its MMAs and the next chunk's copies.
 #pragma once
 #include <cuda.h>
@@ -157,7 +158,7 @@ struct TcLayout {
     static constexpr uint32_t bytes = bars + 8 * 16 + 16;
     static_assert(own_terms || DP * EP * 2 <= kTcTicks * DP * 2, "the copy of S fits the third term's place");
 };
-enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kOutStored, kWReady, kBReady, kSReady, kOutRead, kMeet, kBars };
+enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kOutStored, kWReady, kBReady, kSReady, kOutRead, kOutReady, kBars };
 static_assert(kBars <= 16, "room for the barriers");
 
 // BACK: from the last tick to the first; F32: out in fp32; PARTS: the states of the parts alone
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     if (tid == 0) {
-        for (int i = 0; i < kBars; ++i) fg::mbar_init(bar(i), i == kBReady && !PARTS ? 16 : i >= kWReady ? 8 : 1);
+        for (int i = 0; i < kBars; ++i) fg::mbar_init(bar(i), i >= kWReady ? 8 : 1);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -218,9 +219,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
         if (lane == 0) fg::mbar_arrive(bar(i));
     };
     // b' = scale_in gamma^{..} b of chunk i (n ticks); ticks past its end (another recording's) become 0 in b' and c, whatever they hold.
-    // Worker w of 512 (256 without the ticks' warps).
+    // Worker w of 256.
     auto fade_b = [&](int i, int n, int w) {
-        constexpr int kWorkers = PARTS ? 256 : 512;
+        constexpr int kWorkers = 256;
         unsigned char* stage = smem + (i & 1) * L::stage;
         unsigned char* second = L::own_terms ? smem + L::second : stage + L::a;
         if (n < kTcTicks)
@@ -256,12 +257,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     auto b_free = [&](int i) {
         return (PARTS || wait(L::own_terms ? kQk : kQs, i)) && (i == 0 || wait(kKv, i - 1)) && wait_full(i);
     };
+    // where a chunk of out is put together, and how many columns at a time
+    auto out_at = [&](int i) { return L::own_out ? L::out : (i & 1) * L::stage + L::c; };
+    constexpr int kRound = F32 ? 64 : 128;
     // with `first`, run from the back, S counts undecayed at the first tick
     const int lead0 = BACK && s.first && part == 0 && !PARTS ? 0 : 1;
     bool ok = true;
 
-    // 20 warps start with 96 registers a thread: 640 x 96 = 61,440. The MMAs and copies (and the warp beside them, there
-    // because registers change hands by four warps) keep 48, the ticks 88, so that the state has 128 (S alone is 64):
+    // 20 warps start with 96 registers a thread: 640 x 96 = 61,440. The MMAs and copies keep 48, the ticks 88, so that the state has 128 (S alone is 64):
     // 128 x 48 + 256 x 88 + 256 x 128 = 61,440
     if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
@@ -271,12 +274,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             // is put together over c, is stored
             const int da = (D + 63) / 64, ec = (E + 63) / 64;
             const int head_a = h / s.a.share, head_b = h / s.b.share, head_c = h / s.c.share;
-            int copied = 0;
+            int copied = 0, stored = 0;
 #pragma unroll 1
             for (int i = 0; i < chunks && ok; ++i) {
                 const uint32_t stage = sm + (i & 1) * L::stage, full = bar(kFull0 + (i & 1));
                 const int tick = first_of(i);
-                if (i >= 2) ok = wait(kKv, i - 2) && (PARTS || (wait(kPv, i - 2) && (L::own_out || wait(kOutStored, i - 2))));
+                if (i >= 2) ok = wait(kKv, i - 2) && (PARTS || wait(kPv, i - 2));
+                if (i >= 2 && !PARTS && !L::own_out)         // (every phase in turn: a wait tells odd from even only)
+                    for (int e0 = 0; e0 < E; e0 += kRound) ok = ok && wait(kOutStored, stored++);
                 if (!ok) break;
                 fg::mbar_expect_tx(full, (uint32_t)((PARTS ? 1 : 2) * da + ec) * kBox);
 #pragma unroll 1
@@ -320,6 +325,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 for (int k = 0; k < kTcTicks / 16; ++k) mma_bf16_tmem(tmem + tO2, tmem + tA + k * 16, c_rows + 128 * k, id_o, k > 0);
                 fg::mma_commit(bar(kPv));
             }
+        } else if (warp == 19 && lane == 0 && !PARTS) {
+            // out of whole chunks, round by round
+            constexpr int values = F32 ? 32 : 64;
+            int round = 0;
+#pragma unroll 1
+            for (int i = 0; i < chunks && ok; ++i) {
+                if (ticks_of(i) < kTcTicks) break;
+#pragma unroll 1
+                for (int e0 = 0; e0 < E && ok; e0 += kRound) {
+                    ok = wait(kOutReady, round++);
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int e = e0; e < min(E, e0 + kRound); e += values)
+                        tma_store(&maps.out, sm + out_at(i) + (e - e0) / values * kBox, e, h, first_of(i), batch);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    stores_read();
+                    fg::mbar_arrive(bar(kOutStored));
+                }
+            }
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         } else if (warp == 18 && lane == 0) {
             // dS
             const uint32_t id_s = bf16_idesc(E, 1, 1);
@@ -330,7 +355,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 const uint32_t stage = sm + (i & 1) * L::stage;
                 const uint64_t first = swizzled(stage + L::b, next_b), c_rows = swizzled(stage + L::c, kBox),
                                second = swizzled(L::own_terms ? sm + L::second : stage + L::a, next_b);
-                ok = wait(kBReady, i) && wait(kSReady, i);   // dS of the chunk before has been read
+                ok = wait_full(i) && wait(kBReady, i) && wait(kSReady, i);   // dS of the chunk before has been read
                 if (!ok) break;
                 fg::tc_fence_after();
 #pragma unroll
@@ -354,11 +379,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
         for (int k = 0; k < 8; ++k) near[k] = BACK ? two(pw[2 * k], pw[2 * k + 1]) : two(pw[15 - 2 * k], pw[14 - 2 * k]);
         const float scale = s.scale_in * s.scale_out;
         const bool in_range = ld > -2.f;                     // (e^(2 * 31) is finite by far)
-        int meetings = 0;
-        auto meet = [&]() {                                  // the eight warps wait for one another
-            arrive(kMeet);
-            return together(wait(kMeet, meetings++));
-        };
+        int round = 0;
 #pragma unroll 1
         for (int i = 0; !PARTS && i < chunks && ok; ++i) {
             const int n = ticks_of(i);
@@ -409,71 +430,92 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             fg::tc_fence_before();
             arrive(kWReady);
-            ok = together(b_free(i));
-            if (!ok) break;
-            fade_b(i, n, tid);
-            ok = together(wait(kQs, i) && wait(kPv, i) && (L::own_out || wait(kKv, i)));
+            ok = together(wait(kQs, i) && wait(kPv, i));
             if (!ok) break;
             // out of whole chunks is put together in shared memory and stored as tiles (a thread's own stores, 32 lines at a
             // time, held up the MMAs' operands); a recording's last ticks go by themselves: what follows them is another's
-            const bool whole = n == kTcTicks;
             const float f = pw[max(BACK ? n - 1 - row : row, 0) + (i ? 1 : lead0)] * s.scale_out;
             const uint64_t f2 = two(f, f);
-            const long long at = batch * s.out.batch + (long long)(first_of(i) + row) * s.out.tick + h * s.out.head;
-            unsigned char* tile = smem + (L::own_out ? L::out : (i & 1) * L::stage + L::c);
-            constexpr int width = F32 ? 64 : 128, units = F32 ? 4 : 2;   // columns that fit; 16-byte units of 16
-#pragma unroll 1
-            for (int first = 0; first < E && ok; first += width) {
-                const int end = min(E, first + width);
-#pragma unroll 1
-                for (int e0 = first + half * 16; e0 < end; e0 += 32) {
-                    uint32_t x[16], y[16];
-                    tmem_ld16(lanes + tO1 + e0, x);
-                    tmem_ld16(lanes + tO2 + e0, y);
-                    tmem_ready(x);
-                    tmem_ready(y);
+            constexpr int units = F32 ? 4 : 2;                // 16-byte units of 16 columns
+            auto out16 = [&](int e0, uint32_t (&x)[16]) {
+                uint32_t y[16];
+                tmem_ld16(lanes + tO1 + e0, x);
+                tmem_ld16(lanes + tO2 + e0, y);
+                tmem_ready(x);
+                tmem_ready(y);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint64_t o = fma2(two(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), f2,
-                                                two(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])));
-                        if (F32) {
-                            asm("mov.b64 {%0, %1}, %2;" : "=r"(x[2 * k]), "=r"(x[2 * k + 1]) : "l"(o));
-                        } else {
-                            x[k] = pack2(o);
-                        }
-                    }
-                    const int u0 = (e0 - first) * units / 16;        // 16-byte units, 8 to a box's row
-                    unsigned char* to = whole ? tile + (u0 >> 3) * kBox + row * 128
-                                              : reinterpret_cast<unsigned char*>(s.out.p) + (at + e0) * (F32 ? 4 : 2);
-                    if (whole || row < n) {
+                for (int k = 0; k < 8; ++k) {
+                    const uint64_t o = fma2(two(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), f2,
+                                            two(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1])));
+                    if (F32) asm("mov.b64 {%0, %1}, %2;" : "=r"(x[2 * k]), "=r"(x[2 * k + 1]) : "l"(o));
+                    else x[k] = pack2(o);
+                }
+            };
+            auto put = [&](int e0, const uint32_t* x) {       // e0: column of the round
+                const int u0 = e0 * units / 16;
+                unsigned char* to = smem + out_at(i) + (u0 >> 3) * kBox + row * 128;
 #pragma unroll
-                        for (int k = 0; k < units; ++k)
-                                *reinterpret_cast<uint4*>(to + (whole ? (((u0 & 7) + k) ^ (row & 7)) << 4 : k * 16)) =
-                                    make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+                for (int k = 0; k < units; ++k)
+                    *reinterpret_cast<uint4*>(to + ((((u0 & 7) + k) ^ (row & 7)) << 4)) =
+                        make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+            };
+            auto done = [&]() {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(kOutReady);
+            };
+            if (n < kTcTicks) {
+                const long long at = batch * s.out.batch + (long long)(first_of(i) + row) * s.out.tick + h * s.out.head;
+#pragma unroll 1
+                for (int e0 = half * 16; e0 < E; e0 += 32) {
+                    uint32_t x[16];
+                    out16(e0, x);
+                    uint4* to = reinterpret_cast<uint4*>(s.out.p + (at + e0) * (F32 ? 4 : 2));
+                    if (row < n) {
+#pragma unroll
+                        for (int k = 0; k < units; ++k) to[k] = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
                     }
                     __syncwarp();
                 }
-                if (end == E) {
-                    fg::tc_fence_before();
-                    arrive(kOutRead);
-                }
-                if (whole) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    ok = meet();
-                    if (ok && tid == 0) {
-                        constexpr int values = F32 ? 32 : 64;
-                        for (int e0 = first; e0 < end; e0 += values)
-                            tma_store(&maps.out, fg::smem_u32(tile) + (e0 - first) / values * kBox, e0, h, first_of(i), batch);
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                        stores_read();
+                fg::tc_fence_before();
+                arrive(kOutRead);
+            } else if (L::own_out || F32) {
+#pragma unroll 1
+                for (int e0 = 0; e0 < E && ok; e0 += kRound, ++round) {
+                    // the place is free: over c, once dS is done with it; the round before is stored
+                    ok = together((L::own_out || e0 || wait(kKv, i)) && (!round || wait(kOutStored, round - 1)));
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int e = half * 16; e < min(E - e0, kRound); e += 32) {
+                        uint32_t x[16];
+                        out16(e0 + e, x);
+                        put(e, x);
                     }
-                    __syncwarp();
-                    if (end < E || L::own_out) ok = ok && meet();    // (then the place is free again)
+                    if (e0 + kRound >= E) {
+                        fg::tc_fence_before();
+                        arrive(kOutRead);
+                    }
+                    done();
                 }
+            } else {                                          // (read at once, so that the next chunk's O1 can come)
+                uint32_t held[EP / 32][8];
+#pragma unroll
+                for (int j = 0; j < EP / 32; ++j) {
+                    if ((2 * j + half) * 16 >= E) continue;
+                    uint32_t x[16];
+                    out16((2 * j + half) * 16, x);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) held[j][k] = x[k];
+                }
+                fg::tc_fence_before();
+                arrive(kOutRead);
+                ok = together(wait(kKv, i));
+                if (!ok) break;
+#pragma unroll
+                for (int j = 0; j < EP / 32; ++j)
+                    if ((2 * j + half) * 16 < E) put((2 * j + half) * 16, held[j]);
+                done();
             }
-            if (!L::own_out && tid == 0) fg::mbar_arrive(bar(kOutStored));
         }
-        if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ---- state ---------------------------------------------------------------------------------------------
@@ -538,7 +580,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             const int n = ticks_of(i);
             ok = together(b_free(i));
             if (!ok) break;
-            fade_b(i, n, PARTS ? tid - 256 : tid);
+            fade_b(i, n, tid - 256);
             ok = together(wait(kKv, i));
             if (!ok) break;
             const float fade = pw[n - 1 + (i ? 1 : lead0)];
