@@ -172,16 +172,249 @@ __global__ void __launch_bounds__(128) k_rotate_gw_any(const __grid_constant__ R
     }
     part[((long long)split * sets + set) * a.dim + i] = sum;
 }
-// gw = the splits' sums added in order
-__global__ void k_rotate_gw_sum(const float* __restrict__ part, float* __restrict__ gw, int n, int splits) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n) return;
+// gw = the splits' sums added in a fixed order: 8 warps each take every 8th split of 32 values, then their sums in turn
+__global__ void __launch_bounds__(256) k_rotate_gw_sum(const float* __restrict__ part, float* __restrict__ gw, int n,
+                                                       int stride, int splits) {
+    __shared__ float sums[8][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part[(long long)k * n + i];
+    if (i < n) {
+#pragma unroll 8
+        for (int k = w; k < splits; k += 8) s += part[(long long)k * stride + i];
+    }
+    sums[w][lane] = s;
+    __syncthreads();
+    if (w || i >= n) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sums[k][lane];
     gw[i] = s;
 }
 
-constexpr int kSplits = 256;
+// ---- rows of whole 16-byte units ------------------------------------------------------------------------------------
+//
+// A block takes a few ticks at a time: 256 threads form the ticks' angles once into shared memory (as many as one each),
+// then every group of 2^k lanes takes one head of one tick, each lane two 16-byte units of it: the partners of the "half"
+// layout (unit u and u + turned / 2), or two neighbours. A lane's pairs of values are its own, so the rotation needs no
+// exchange, the norm a few shuffles, and every value is read and written once, 16 bytes a load.
+
+template <class T>
+struct Unit {                                                // 16 bytes of T as floats
+    static constexpr int n = 16 / sizeof(T);
+};
+template <class T>
+__device__ __forceinline__ void load_unit(const T* p, float (&v)[Unit<T>::n]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+    } else {
+        const T* t = reinterpret_cast<const T*>(r);
+#pragma unroll
+        for (int i = 0; i < Unit<T>::n; ++i) v[i] = to_f(t[i]);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store_unit(T* p, const float (&v)[Unit<T>::n]) {
+    uint32_t r[4];
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[i]);
+    } else {
+        T* t = reinterpret_cast<T*>(r);
+#pragma unroll
+        for (int i = 0; i < Unit<T>::n; ++i) t[i] = from_f<T>(v[i]);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
+}
+// (p[i], q[i]) turned by (c, s); INTER: the pairs are neighbours within p, then within q
+template <bool INTER, int N>
+__device__ __forceinline__ void turn(float (&p)[N], float (&q)[N], const float (&c)[N], const float (&s)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float& a = INTER ? (i < N / 2 ? p[2 * i] : q[2 * i - N]) : p[i];
+        float& b = INTER ? (i < N / 2 ? p[2 * i + 1] : q[2 * i + 1 - N]) : q[i];
+        const float u = a, v = b;
+        a = u * c[i] - v * s[i];
+        b = v * c[i] + u * s[i];
+    }
+}
+
+constexpr int kTicksMost = 8;
+
+enum { kForward, kBackward, kBackwardW, kBackwardEach };     // the last two with gw: one set of weights, one for each head
+
+template <class T, bool INTER, bool NORM, int MODE>
+__global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_units(const __grid_constant__ Rotate a, int per_batch,
+                                                                 int lanes, float* __restrict__ part) {
+    constexpr int N = Unit<T>::n;
+    extern __shared__ __align__(16) float shared[];
+    __shared__ long long base[4][2][kTicksMost];             // where a tick of x, y, gy, gx starts, for queries and keys
+    const int half_turn = a.turned / 2, heads = a.s[0].heads, rows = heads + a.s[1].heads;
+    float2* angles = reinterpret_cast<float2*>(shared);      // [per_batch][turned / 2]
+    float* sums = shared + per_batch * half_turn * 2;        // kBackwardEach: [rows][dim]
+    const int tid = threadIdx.x, lane = tid & (lanes - 1), group = tid / lanes, groups = 256 / lanes;
+    const int items = a.dim / (2 * N);
+    const bool busy = lane < items;
+    // the lane's two units of a row, and its first pair
+    const bool turns = busy && lane * N < half_turn;
+    const int rest = lane - half_turn / N;
+    const int u0 = !INTER && turns ? lane * N : !INTER ? a.turned + rest * 2 * N : lane * 2 * N;
+    const int u1 = !INTER && turns ? u0 + half_turn : u0 + N;
+    const int total = (int)(a.batch * a.ticks);
+    float gw[2][2][N];                                       // side, unit
+    if (MODE == kBackwardW) {
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) gw[i / (2 * N)][i / N % 2][i % N] = 0.f;
+    }
+    if (MODE == kBackwardEach) {
+        for (int i = tid; i < rows * a.dim; i += 256) sums[i] = 0.f;
+    }
+    for (int tick0 = blockIdx.x * per_batch; tick0 < total; tick0 += gridDim.x * per_batch) {
+        const int n = min(per_batch, total - tick0);
+        __syncthreads();
+        for (int i = tid; i < n * half_turn; i += 256) {
+            const int j = i / half_turn, pair = i - j * half_turn, tick = tick0 + j;
+            const int b = tick / (int)a.ticks;
+            float2 cs;
+            angle(a, position(a, b, tick - b * (int)a.ticks), pair, cs.x, cs.y);
+            angles[i] = cs;
+        }
+        if (tid < 8 * n) {
+            const int j = tid >> 3, what = tid & 3, side = (tid >> 2) & 1, tick = tick0 + j;
+            const int b = tick / (int)a.ticks, t = tick - b * (int)a.ticks;
+            const Side& s = a.s[side];
+            const long long(&st)[3] = what == 0 ? s.xs : what == 1 ? s.ys : what == 2 ? s.gys : s.gxs;
+            base[what][side][j] = b * st[0] + t * st[1];
+        }
+        __syncthreads();
+        // with sums for each head a row stays with its group
+        const int count = MODE == kBackwardEach ? (rows + groups - 1) / groups * groups * n : n * rows;
+        for (int i = group; i < (count + groups - 1) / groups * groups; i += groups) {
+            int j, row;
+            if (MODE == kBackwardEach) {
+                const int each = (rows + groups - 1) / groups * groups;
+                j = i / each;
+                row = i - j * each;
+            } else {
+                j = i / rows;
+                row = i - j * rows;
+            }
+            const bool here = busy && j < n && row < rows;
+            const int side = row >= heads, h = side ? row - heads : row;
+            const Side& s = a.s[side];
+            float p[N], q[N], x[N], y[N], c[N], sn[N], w0[N], w1[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) p[k] = q[k] = x[k] = y[k] = 0.f, w0[k] = w1[k] = 1.f;
+            if (here) {
+                if (MODE == kForward || NORM) {
+                    const T* at = reinterpret_cast<const T*>(s.x) + base[0][side][j] + h * s.xs[2];
+                    load_unit(at + u0, x);
+                    load_unit(at + u1, y);
+                }
+                if (MODE != kForward) {
+                    const T* at = reinterpret_cast<const T*>(s.gy) + base[2][side][j] + h * s.gys[2];
+                    load_unit(at + u0, p);
+                    load_unit(at + u1, q);
+                }
+                if (NORM && s.w) {
+                    const float4* w = reinterpret_cast<const float4*>(s.w + h * s.w_head);
+#pragma unroll
+                    for (int k = 0; k < N / 4; ++k) {
+                        const float4 f = __ldg(w + u0 / 4 + k), g = __ldg(w + u1 / 4 + k);
+                        w0[4 * k] = f.x; w0[4 * k + 1] = f.y; w0[4 * k + 2] = f.z; w0[4 * k + 3] = f.w;
+                        w1[4 * k] = g.x; w1[4 * k + 1] = g.y; w1[4 * k + 2] = g.z; w1[4 * k + 3] = g.w;
+                    }
+                }
+            }
+            if (turns && here) {
+                const float4* cs = reinterpret_cast<const float4*>(angles + j * half_turn + lane * N);
+#pragma unroll
+                for (int k = 0; k < N / 2; ++k) {
+                    const float4 f = cs[k];
+                    c[2 * k] = f.x; sn[2 * k] = f.y; c[2 * k + 1] = f.z; sn[2 * k + 1] = f.w;
+                }
+                if (MODE != kForward) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) sn[k] = -sn[k];
+                    turn<INTER, N>(p, q, c, sn);
+                }
+            }
+            float norm = 1.f;
+            if (NORM) {
+                float sq = 0.f, m = 0.f;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    sq = fmaf(x[k], x[k], fmaf(y[k], y[k], sq));
+                    if (MODE != kForward) m = fmaf(p[k] * w0[k], x[k], fmaf(q[k] * w1[k], y[k], m));
+                }
+                for (int o = lanes >> 1; o; o >>= 1) {
+                    sq += __shfl_xor_sync(0xffffffffu, sq, o);
+                    if (MODE != kForward) m += __shfl_xor_sync(0xffffffffu, m, o);
+                }
+                norm = 1.f / sqrtf(sq / (float)a.dim + a.eps);
+                if (MODE != kForward) {
+                    const float mean = m * norm * norm / (float)a.dim;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const float f = p[k] * (x[k] * norm), g = q[k] * (y[k] * norm);
+                        if (MODE == kBackwardW) {
+                            gw[0][0][k] += side ? 0.f : f;
+                            gw[0][1][k] += side ? 0.f : g;
+                            gw[1][0][k] += side ? f : 0.f;
+                            gw[1][1][k] += side ? g : 0.f;
+                        }
+                        if (MODE == kBackwardEach && here) {
+                            sums[row * a.dim + u0 + k] += f;
+                            sums[row * a.dim + u1 + k] += g;
+                        }
+                        p[k] = norm * (p[k] * w0[k] - x[k] * mean);
+                        q[k] = norm * (q[k] * w1[k] - y[k] * mean);
+                    }
+                }
+            }
+            if (!here) continue;
+            if (MODE == kForward) {
+                if (NORM) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) x[k] *= norm * w0[k], y[k] *= norm * w1[k];
+                }
+                if (turns) turn<INTER, N>(x, y, c, sn);
+                T* to = reinterpret_cast<T*>(s.y) + base[1][side][j] + h * s.ys[2];
+                store_unit(to + u0, x);
+                store_unit(to + u1, y);
+            } else {
+                T* to = reinterpret_cast<T*>(s.gx) + base[3][side][j] + h * s.gxs[2];
+                store_unit(to + u0, p);
+                store_unit(to + u1, q);
+            }
+        }
+    }
+    if (MODE == kBackwardW) {
+        // the groups' sums in turn: [side][dim] of this block
+        float* all = shared;                                  // [groups][2][dim]
+        __syncthreads();
+        if (busy) {
+#pragma unroll
+            for (int i = 0; i < 4 * N; ++i) {
+                const int side = i / (2 * N), unit = i / N % 2, k = i % N;
+                all[(group * 2 + side) * a.dim + (unit ? u1 : u0) + k] = gw[side][unit][k];
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < 2 * a.dim; i += 256) {
+            float t = 0.f;
+            for (int g = 0; g < groups; ++g) t += all[g * 2 * a.dim + i];
+            part[(long long)blockIdx.x * 2 * a.dim + i] = t;
+        }
+    }
+    if (MODE == kBackwardEach) {
+        __syncthreads();
+        for (int i = tid; i < rows * a.dim; i += 256) part[(long long)blockIdx.x * rows * a.dim + i] = sums[i];
+    }
+}
+
+constexpr int kSplits = 148 * 4;                             // blocks with sums of their own, at most
 
 void strides(long long (&to)[3], const fg_ticks& t) {
     to[0] = t.batch;
@@ -240,12 +473,54 @@ long long sets_of(const fg_rotate_args* g, int i) { return g->w_head[i] ? g->hea
 
 long long work_bytes(const fg_rotate_args* g) {
     if (!g->norm || (!g->gw[0] && !g->gw[1])) return 0;
-    const long long sets = std::max(sets_of(g, 0), sets_of(g, 1));
-    return (rows_of(g) + 3) / 4 * 16 + sets * g->dim * kSplits * 4;
+    const long long sets = std::max<long long>(2, g->w_head[0] || g->w_head[1] ? g->heads[0] + g->heads[1] : 2);
+    const long long blocks = std::max<long long>(1, std::min<long long>(kSplits, g->batch * g->ticks));
+    return (rows_of(g) + 3) / 4 * 16 + sets * g->dim * blocks * 4;
 }
 
 unsigned blocks_for(long long rows) {
     return (unsigned)std::max<long long>(1, std::min<long long>((rows + kWarps - 1) / kWarps, 1 << 20));
+}
+
+bool aligned(const void* p, const long long (&st)[3], long long unit) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st[0] % unit == 0 && st[1] % unit == 0 && st[2] % unit == 0;
+}
+// whether rows are whole pairs of 16-byte units
+bool has_units(const Rotate& a, int size, bool backward) {
+    const int unit = 16 / size;
+    if (a.dim % (2 * unit) || a.turned % (2 * unit) || a.dim / (2 * unit) > 32 || a.batch * a.ticks >= (1ll << 30)) return false;
+    for (const Side& s : a.s) {
+        if (!s.heads) continue;
+        if ((!backward || a.norm) && !aligned(s.x, s.xs, unit)) return false;
+        if (backward ? !aligned(s.gy, s.gys, unit) || !aligned(s.gx, s.gxs, unit) : !aligned(s.y, s.ys, unit)) return false;
+        if (s.w && (reinterpret_cast<uintptr_t>(s.w) % 16 || s.w_head % 4)) return false;
+    }
+    return true;
+}
+template <class T, bool INTER, bool NORM, int MODE>
+void launch_units(const Rotate& a, float* part, int& blocks, cudaStream_t st) {
+    const int items = a.dim / (2 * Unit<T>::n), half = a.turned / 2, rows = a.s[0].heads + a.s[1].heads;
+    int lanes = 1;
+    while (lanes < items) lanes *= 2;
+    const int total = (int)(a.batch * a.ticks);
+    // a few ticks at a time give every thread an angle, unless there are not enough to go round
+    int per = std::max(1, std::min(kTicksMost, half ? 256 / half : kTicksMost));
+    while (per > 1 && (total + per - 1) / per < 148 * 4) per /= 2;
+    const int groups = 256 / lanes;
+    size_t bytes = (size_t)per * half * 8;
+    if (MODE == kBackwardW) bytes = std::max(bytes, (size_t)groups * 2 * a.dim * 4);
+    if (MODE == kBackwardEach) bytes += (size_t)rows * a.dim * 4;
+    auto* k = k_rotate_units<T, INTER, NORM, MODE>;
+    if (bytes > 48 * 1024) MCK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    blocks = std::min((total + per - 1) / per, MODE >= kBackwardW ? kSplits : 148 * 32);
+    k<<<blocks, 256, bytes, st>>>(a, per, lanes, part);
+    MCK(cudaGetLastError());
+}
+template <class T, int MODE>
+void launch_units(const Rotate& a, float* part, int& blocks, cudaStream_t st) {
+    constexpr bool with_norm = MODE >= kBackwardW;            // (sums of gw are the norm's)
+    if (a.norm) a.interleaved ? launch_units<T, true, true, MODE>(a, part, blocks, st) : launch_units<T, false, true, MODE>(a, part, blocks, st);
+    else if constexpr (!with_norm) a.interleaved ? launch_units<T, true, false, MODE>(a, part, blocks, st) : launch_units<T, false, false, MODE>(a, part, blocks, st);
 }
 
 }  // namespace
@@ -258,7 +533,11 @@ int fg_norm_rotate(const fg_rotate_args* g, void* stream) {
         const long long rows = rows_of(g);
         if (!rows) return 0;
         by_type(g->type, [&](auto t) {
-            k_rotate_any<decltype(t)><<<blocks_for(rows), 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(a, rows);
+            using T = decltype(t);
+            cudaStream_t st = static_cast<cudaStream_t>(stream);
+            int blocks = 0;
+            if (has_units(a, sizeof(T), false)) launch_units<T, kForward>(a, nullptr, blocks, st);
+            else k_rotate_any<T><<<blocks_for(rows), 32 * kWarps, 0, st>>>(a, rows);
         });
         MCK(cudaGetLastError());
         return 0;
@@ -282,17 +561,36 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
         float* norms = need_bytes ? static_cast<float*>(g->work) : nullptr;
         by_type(g->type, [&](auto t) {
             using T = decltype(t);
+            float* part = norms ? norms + (rows + 3) / 4 * 4 : nullptr;
+            // (the sums of one set of weights for some heads and sets of their own for others go the general way)
+            const bool each = g->w_head[0] || g->w_head[1];
+            const bool all_each = (!a.s[0].gw || !a.s[0].heads || g->w_head[0]) && (!a.s[1].gw || !a.s[1].heads || g->w_head[1]);
+            const bool fits = !each || (all_each && (g->heads[0] + g->heads[1]) * g->dim * 4 <= 64 * 1024);
+            if (rows && has_units(a, sizeof(T), true) && (!norms || fits)) {
+                int blocks = 0;
+                if (!norms) launch_units<T, kBackward>(a, nullptr, blocks, st);
+                else if (each) launch_units<T, kBackwardEach>(a, part, blocks, st);
+                else launch_units<T, kBackwardW>(a, part, blocks, st);
+                for (int i = 0; norms && i < 2; ++i) {
+                    if (!a.s[i].gw || !a.s[i].heads) continue;
+                    const int n = (int)sets_of(g, i) * a.dim;
+                    const int stride = each ? (a.s[0].heads + a.s[1].heads) * a.dim : 2 * a.dim;
+                    const int at = i ? (each ? a.s[0].heads * a.dim : a.dim) : 0;
+                    k_rotate_gw_sum<<<(n + 31) / 32, 256, 0, st>>>(part + at, a.s[i].gw, n, stride, blocks);
+                    MCK(cudaGetLastError());
+                }
+                return;
+            }
             if (rows) k_rotate_bwd_any<T><<<blocks_for(rows), 32 * kWarps, 0, st>>>(a, rows, norms);
             MCK(cudaGetLastError());
             for (int i = 0; i < 2; ++i) {
                 if (!a.s[i].gw || !a.s[i].heads) continue;
                 const int sets = (int)sets_of(g, i), n = sets * a.dim;
                 need(sets <= 65535, "fg_norm_rotate_bwd: too many heads with weights of their own");
-                float* part = norms + (rows + 3) / 4 * 4;
-                const int splits = (int)std::max<long long>(1, std::min<long long>(kSplits, g->batch * g->ticks));
+                const int splits = (int)std::max<long long>(1, std::min<long long>(256, g->batch * g->ticks));
                 const dim3 grid((a.dim + 127) / 128, sets, splits);
                 k_rotate_gw_any<T><<<grid, 128, 0, st>>>(a, i, norms, part, sets, splits);
-                k_rotate_gw_sum<<<(n + 127) / 128, 128, 0, st>>>(part, a.s[i].gw, n, splits);
+                k_rotate_gw_sum<<<(n + 31) / 32, 256, 0, st>>>(part, a.s[i].gw, n, n, splits);
                 MCK(cudaGetLastError());
             }
         });
