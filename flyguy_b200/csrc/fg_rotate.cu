@@ -172,38 +172,44 @@ __global__ void __launch_bounds__(128) k_rotate_gw_any(const __grid_constant__ R
     }
     part[((long long)split * sets + set) * a.dim + i] = sum;
 }
-// gw = the splits' sums added in a fixed order: 8 warps each take every 8th split of 32 values, then their sums in turn
-__global__ void __launch_bounds__(256) k_rotate_gw_sum(const float* __restrict__ part, float* __restrict__ gw, int n,
-                                                       int stride, int splits) {
-    __shared__ float sums[8][32];
+// gw = the splits' sums added in a fixed order: 32 warps each take every 32nd split of 32 values, then their sums in turn.
+// Values 0 .. n0 - 1 of a split go to gw0, those from `second` on to gw1.
+__global__ void __launch_bounds__(1024) k_rotate_gw_sum(const float* __restrict__ part, float* __restrict__ gw0, int n0,
+                                                        float* __restrict__ gw1, int second, int n1, int stride,
+                                                        int splits) {
+    __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+    const bool one = gw0 && i < n0, two = gw1 && i >= second && i < second + n1;
     float s = 0.f;
-    if (i < n) {
-#pragma unroll 8
-        for (int k = w; k < splits; k += 8) s += part[(long long)k * stride + i];
+    if (one || two) {
+#pragma unroll 4
+        for (int k = w; k < splits; k += 32) s += part[(long long)k * stride + i];
     }
     sums[w][lane] = s;
     __syncthreads();
-    if (w || i >= n) return;
+    if (w) return;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][lane];
-    gw[i] = s;
+    for (int k = 1; k < 32; ++k) s += sums[k][lane];
+    if (one) gw0[i] = s;
+    if (two) gw1[i - second] = s;
 }
 
 // ---- rows of whole 16-byte units ------------------------------------------------------------------------------------
 //
 // A block takes a few ticks at a time: 256 threads form the ticks' angles once into shared memory (as many as one each),
-// then every group of 2^k lanes takes one head of one tick, each lane two 16-byte units of it: the partners of the "half"
-// layout (unit u and u + turned / 2), or two neighbours. A lane's pairs of values are its own, so the rotation needs no
-// exchange, the norm a few shuffles, and every value is read and written once, 16 bytes a load.
+// then every group of 2^k lanes takes some heads of one tick, each lane two 16-byte units of a head: the partners of the
+// "half" layout (unit u and u + turned / 2), or two neighbours. A lane's pairs of values are its own, so the rotation needs
+// no exchange, the norm a few shuffles, and every value is read and written once, 16 bytes a load. The lane's angles and
+// weights stay in registers over its heads: fetched for each head they are three times the bytes of the values, and L1
+// was the limit (128 recordings of 128 ticks, 16 + 4 heads of 128 in bf16: @@ us forward, @@ us back). The next head's
+// values are asked for before the present one's are used.
 
 template <class T>
 struct Unit {                                                // 16 bytes of T as floats
     static constexpr int n = 16 / sizeof(T);
 };
 template <class T>
-__device__ __forceinline__ void load_unit(const T* p, float (&v)[Unit<T>::n]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void from_unit(const uint4& u, float (&v)[Unit<T>::n]) {
     const uint32_t r[4] = {u.x, u.y, u.z, u.w};
     if (sizeof(T) == 4) {
 #pragma unroll
@@ -244,103 +250,107 @@ constexpr int kTicksMost = 8;
 
 enum { kForward, kBackward, kBackwardW, kBackwardEach };     // the last two with gw: one set of weights, one for each head
 
+struct UnitPlan {
+    int per[2];                                              // ticks at a time, for queries and keys (powers of 2)
+    int lanes;                                               // of a group
+};
+
 template <class T, bool INTER, bool NORM, int MODE>
-__global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_units(const __grid_constant__ Rotate a, int per_batch,
-                                                                 int lanes, float* __restrict__ part) {
+__global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_units(const __grid_constant__ Rotate a,
+                                                                                 const UnitPlan plan,
+                                                                                 float* __restrict__ part) {
     constexpr int N = Unit<T>::n;
     extern __shared__ __align__(16) float shared[];
-    __shared__ long long base[4][2][kTicksMost];             // where a tick of x, y, gy, gx starts, for queries and keys
-    const int half_turn = a.turned / 2, heads = a.s[0].heads, rows = heads + a.s[1].heads;
-    float2* angles = reinterpret_cast<float2*>(shared);      // [per_batch][turned / 2]
-    float* sums = shared + per_batch * half_turn * 2;        // kBackwardEach: [rows][dim]
-    const int tid = threadIdx.x, lane = tid & (lanes - 1), group = tid / lanes, groups = 256 / lanes;
-    const int items = a.dim / (2 * N);
-    const bool busy = lane < items;
-    // the lane's two units of a row, and its first pair
+    const Side& s = a.s[blockIdx.y];
+    const int heads = s.heads, per = plan.per[blockIdx.y], half_turn = a.turned / 2;
+    float2* angles = reinterpret_cast<float2*>(shared);      // [2][per][turned / 2]
+    float* sums = shared + 4 * per * half_turn;              // kBackwardEach: [heads][dim]
+    const int tid = threadIdx.x, lane = tid & (plan.lanes - 1), group = tid / plan.lanes, groups = 256 / plan.lanes;
+    const bool busy = lane < a.dim / (2 * N);
+    // the lane's two units of a head, and its first pair
     const bool turns = busy && lane * N < half_turn;
     const int rest = lane - half_turn / N;
     const int u0 = !INTER && turns ? lane * N : !INTER ? a.turned + rest * 2 * N : lane * 2 * N;
     const int u1 = !INTER && turns ? u0 + half_turn : u0 + N;
-    const int total = (int)(a.batch * a.ticks);
-    float gw[2][2][N];                                       // side, unit
-    if (MODE == kBackwardW) {
+    // groups of one tick share its heads; with sums for each head there is one tick, so that a head stays with its group
+    const int share = groups / per, j = group / share, first = group - j * share;
+    const int total = (int)(a.batch * a.ticks), ticks = (int)a.ticks;
+    const float inverse = 1.f / (float)a.dim;
+    float w0[N], w1[N], gw0[N], gw1[N];
 #pragma unroll
-        for (int i = 0; i < 4 * N; ++i) gw[i / (2 * N)][i / N % 2][i % N] = 0.f;
-    }
+    for (int k = 0; k < N; ++k) w0[k] = w1[k] = 1.f, gw0[k] = gw1[k] = 0.f;
+    auto weights = [&](int h) {
+        const float4* w = reinterpret_cast<const float4*>(s.w + h * s.w_head);
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+            const float4 f = __ldg(w + u0 / 4 + k), g = __ldg(w + u1 / 4 + k);
+            w0[4 * k] = f.x; w0[4 * k + 1] = f.y; w0[4 * k + 2] = f.z; w0[4 * k + 3] = f.w;
+            w1[4 * k] = g.x; w1[4 * k + 1] = g.y; w1[4 * k + 2] = g.z; w1[4 * k + 3] = g.w;
+        }
+    };
+    if (NORM && s.w && !s.w_head && busy) weights(0);
     if (MODE == kBackwardEach) {
-        for (int i = tid; i < rows * a.dim; i += 256) sums[i] = 0.f;
+        for (int i = tid; i < heads * a.dim; i += 256) sums[i] = 0.f;
+        __syncthreads();
     }
-    for (int tick0 = blockIdx.x * per_batch; tick0 < total; tick0 += gridDim.x * per_batch) {
-        const int n = min(per_batch, total - tick0);
-        __syncthreads();
-        for (int i = tid; i < n * half_turn; i += 256) {
-            const int j = i / half_turn, pair = i - j * half_turn, tick = tick0 + j;
-            const int b = tick / (int)a.ticks;
-            float2 cs;
-            angle(a, position(a, b, tick - b * (int)a.ticks), pair, cs.x, cs.y);
-            angles[i] = cs;
-        }
-        if (tid < 8 * n) {
-            const int j = tid >> 3, what = tid & 3, side = (tid >> 2) & 1, tick = tick0 + j;
-            const int b = tick / (int)a.ticks, t = tick - b * (int)a.ticks;
-            const Side& s = a.s[side];
-            const long long(&st)[3] = what == 0 ? s.xs : what == 1 ? s.ys : what == 2 ? s.gys : s.gxs;
-            base[what][side][j] = b * st[0] + t * st[1];
-        }
-        __syncthreads();
-        // with sums for each head a row stays with its group
-        const int count = MODE == kBackwardEach ? (rows + groups - 1) / groups * groups * n : n * rows;
-        for (int i = group; i < (count + groups - 1) / groups * groups; i += groups) {
-            int j, row;
-            if (MODE == kBackwardEach) {
-                const int each = (rows + groups - 1) / groups * groups;
-                j = i / each;
-                row = i - j * each;
-            } else {
-                j = i / rows;
-                row = i - j * rows;
+    for (int tick0 = blockIdx.x * per, turn_no = 0; tick0 < total; tick0 += gridDim.x * per, ++turn_no) {
+        const int n = min(per, total - tick0);
+        const bool there = busy && j < n;
+        const int mine = tick0 + (there ? j : 0), b = mine / ticks, t = mine - b * ticks;
+        const T* x_at = reinterpret_cast<const T*>(s.x) + b * s.xs[0] + t * s.xs[1];
+        const T* gy_at = reinterpret_cast<const T*>(s.gy) + b * s.gys[0] + t * s.gys[1];
+        T* to = MODE == kForward ? reinterpret_cast<T*>(s.y) + b * s.ys[0] + t * s.ys[1]
+                                 : reinterpret_cast<T*>(s.gx) + b * s.gxs[0] + t * s.gxs[1];
+        const long long to_head = MODE == kForward ? s.ys[2] : s.gxs[2];
+        uint4 next[4];
+        auto fetch = [&](int h) {
+            if (!there || h >= heads) return;
+            if (MODE == kForward || NORM) {
+                next[0] = *reinterpret_cast<const uint4*>(x_at + h * s.xs[2] + u0);
+                next[1] = *reinterpret_cast<const uint4*>(x_at + h * s.xs[2] + u1);
             }
-            const bool here = busy && j < n && row < rows;
-            const int side = row >= heads, h = side ? row - heads : row;
-            const Side& s = a.s[side];
-            float p[N], q[N], x[N], y[N], c[N], sn[N], w0[N], w1[N];
+            if (MODE != kForward) {
+                next[2] = *reinterpret_cast<const uint4*>(gy_at + h * s.gys[2] + u0);
+                next[3] = *reinterpret_cast<const uint4*>(gy_at + h * s.gys[2] + u1);
+            }
+        };
+        fetch(first);                                         // (on its way while the angles are formed)
+        float2* here_angles = angles + (turn_no & 1) * per * half_turn;
+        for (int i = tid; i < n * half_turn; i += 256) {
+            const int q = i / half_turn, pair = i - q * half_turn, tick = tick0 + q, tb = tick / ticks;
+            float2 cs;
+            angle(a, position(a, tb, tick - tb * ticks), pair, cs.x, cs.y);
+            here_angles[i] = cs;
+        }
+        __syncthreads();                                      // (two sets of angles: nobody is a whole turn ahead)
+        float c[N], sn[N];
+        if (turns && there) {
+            const float4* cs = reinterpret_cast<const float4*>(here_angles + j * half_turn + lane * N);
 #pragma unroll
-            for (int k = 0; k < N; ++k) p[k] = q[k] = x[k] = y[k] = 0.f, w0[k] = w1[k] = 1.f;
+            for (int k = 0; k < N / 2; ++k) {
+                const float4 f = cs[k];
+                c[2 * k] = f.x; sn[2 * k] = MODE == kForward ? f.y : -f.y;
+                c[2 * k + 1] = f.z; sn[2 * k + 1] = MODE == kForward ? f.w : -f.w;
+            }
+        }
+        for (int h = first; h < (heads + share - 1) / share * share; h += share) {
+            const bool here = there && h < heads;
+            float p[N], q[N], x[N], y[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) p[k] = q[k] = x[k] = y[k] = 0.f;
             if (here) {
                 if (MODE == kForward || NORM) {
-                    const T* at = reinterpret_cast<const T*>(s.x) + base[0][side][j] + h * s.xs[2];
-                    load_unit(at + u0, x);
-                    load_unit(at + u1, y);
+                    from_unit<T>(next[0], x);
+                    from_unit<T>(next[1], y);
                 }
                 if (MODE != kForward) {
-                    const T* at = reinterpret_cast<const T*>(s.gy) + base[2][side][j] + h * s.gys[2];
-                    load_unit(at + u0, p);
-                    load_unit(at + u1, q);
+                    from_unit<T>(next[2], p);
+                    from_unit<T>(next[3], q);
                 }
-                if (NORM && s.w) {
-                    const float4* w = reinterpret_cast<const float4*>(s.w + h * s.w_head);
-#pragma unroll
-                    for (int k = 0; k < N / 4; ++k) {
-                        const float4 f = __ldg(w + u0 / 4 + k), g = __ldg(w + u1 / 4 + k);
-                        w0[4 * k] = f.x; w0[4 * k + 1] = f.y; w0[4 * k + 2] = f.z; w0[4 * k + 3] = f.w;
-                        w1[4 * k] = g.x; w1[4 * k + 1] = g.y; w1[4 * k + 2] = g.z; w1[4 * k + 3] = g.w;
-                    }
-                }
+                fetch(h + share);
+                if (NORM && s.w && s.w_head) weights(h);
+                if (turns && MODE != kForward) turn<INTER, N>(p, q, c, sn);
             }
-            if (turns && here) {
-                const float4* cs = reinterpret_cast<const float4*>(angles + j * half_turn + lane * N);
-#pragma unroll
-                for (int k = 0; k < N / 2; ++k) {
-                    const float4 f = cs[k];
-                    c[2 * k] = f.x; sn[2 * k] = f.y; c[2 * k + 1] = f.z; sn[2 * k + 1] = f.w;
-                }
-                if (MODE != kForward) {
-#pragma unroll
-                    for (int k = 0; k < N; ++k) sn[k] = -sn[k];
-                    turn<INTER, N>(p, q, c, sn);
-                }
-            }
-            float norm = 1.f;
             if (NORM) {
                 float sq = 0.f, m = 0.f;
 #pragma unroll
@@ -348,25 +358,25 @@ __global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_unit
                     sq = fmaf(x[k], x[k], fmaf(y[k], y[k], sq));
                     if (MODE != kForward) m = fmaf(p[k] * w0[k], x[k], fmaf(q[k] * w1[k], y[k], m));
                 }
-                for (int o = lanes >> 1; o; o >>= 1) {
+                for (int o = plan.lanes >> 1; o; o >>= 1) {
                     sq += __shfl_xor_sync(0xffffffffu, sq, o);
                     if (MODE != kForward) m += __shfl_xor_sync(0xffffffffu, m, o);
                 }
-                norm = 1.f / sqrtf(sq / (float)a.dim + a.eps);
-                if (MODE != kForward) {
-                    const float mean = m * norm * norm / (float)a.dim;
+                const float norm = rsqrtf(fmaf(sq, inverse, a.eps));
+                if (MODE == kForward) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) x[k] *= norm * w0[k], y[k] *= norm * w1[k];
+                } else {
+                    const float mean = m * norm * norm * inverse;
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        const float f = p[k] * (x[k] * norm), g = q[k] * (y[k] * norm);
                         if (MODE == kBackwardW) {
-                            gw[0][0][k] += side ? 0.f : f;
-                            gw[0][1][k] += side ? 0.f : g;
-                            gw[1][0][k] += side ? f : 0.f;
-                            gw[1][1][k] += side ? g : 0.f;
+                            gw0[k] = fmaf(p[k], x[k] * norm, gw0[k]);
+                            gw1[k] = fmaf(q[k], y[k] * norm, gw1[k]);
                         }
                         if (MODE == kBackwardEach && here) {
-                            sums[row * a.dim + u0 + k] += f;
-                            sums[row * a.dim + u1 + k] += g;
+                            sums[h * a.dim + u0 + k] += p[k] * (x[k] * norm);
+                            sums[h * a.dim + u1 + k] += q[k] * (y[k] * norm);
                         }
                         p[k] = norm * (p[k] * w0[k] - x[k] * mean);
                         q[k] = norm * (q[k] * w1[k] - y[k] * mean);
@@ -375,46 +385,41 @@ __global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_unit
             }
             if (!here) continue;
             if (MODE == kForward) {
-                if (NORM) {
-#pragma unroll
-                    for (int k = 0; k < N; ++k) x[k] *= norm * w0[k], y[k] *= norm * w1[k];
-                }
                 if (turns) turn<INTER, N>(x, y, c, sn);
-                T* to = reinterpret_cast<T*>(s.y) + base[1][side][j] + h * s.ys[2];
-                store_unit(to + u0, x);
-                store_unit(to + u1, y);
+                store_unit(to + h * to_head + u0, x);
+                store_unit(to + h * to_head + u1, y);
             } else {
-                T* to = reinterpret_cast<T*>(s.gx) + base[3][side][j] + h * s.gxs[2];
-                store_unit(to + u0, p);
-                store_unit(to + u1, q);
+                store_unit(to + h * to_head + u0, p);
+                store_unit(to + h * to_head + u1, q);
             }
         }
     }
     if (MODE == kBackwardW) {
-        // the groups' sums in turn: [side][dim] of this block
-        float* all = shared;                                  // [groups][2][dim]
+        // the groups' sums in turn: part [block][side][dim]
+        float* all = shared;                                  // [groups][dim]
         __syncthreads();
         if (busy) {
 #pragma unroll
-            for (int i = 0; i < 4 * N; ++i) {
-                const int side = i / (2 * N), unit = i / N % 2, k = i % N;
-                all[(group * 2 + side) * a.dim + (unit ? u1 : u0) + k] = gw[side][unit][k];
+            for (int k = 0; k < N; ++k) {
+                all[group * a.dim + u0 + k] = gw0[k];
+                all[group * a.dim + u1 + k] = gw1[k];
             }
         }
         __syncthreads();
-        for (int i = tid; i < 2 * a.dim; i += 256) {
-            float t = 0.f;
-            for (int g = 0; g < groups; ++g) t += all[g * 2 * a.dim + i];
-            part[(long long)blockIdx.x * 2 * a.dim + i] = t;
+        for (int i = tid; i < a.dim; i += 256) {
+            float sum = 0.f;
+            for (int g = 0; g < groups; ++g) sum += all[g * a.dim + i];
+            part[((long long)blockIdx.x * 2 + blockIdx.y) * a.dim + i] = sum;
         }
     }
-    if (MODE == kBackwardEach) {
+    if (MODE == kBackwardEach) {                              // part [block][queries' heads, keys' heads][dim]
         __syncthreads();
-        for (int i = tid; i < rows * a.dim; i += 256) part[(long long)blockIdx.x * rows * a.dim + i] = sums[i];
+        float* to = part + ((long long)blockIdx.x * (a.s[0].heads + a.s[1].heads) + (blockIdx.y ? a.s[0].heads : 0)) * a.dim;
+        for (int i = tid; i < heads * a.dim; i += 256) to[i] = sums[i];
     }
 }
 
-constexpr int kSplits = 148 * 4;                             // blocks with sums of their own, at most
+constexpr int kSplits = 148 * 2;                             // blocks with sums of their own, at most
 
 void strides(long long (&to)[3], const fg_ticks& t) {
     to[0] = t.batch;
@@ -499,21 +504,27 @@ bool has_units(const Rotate& a, int size, bool backward) {
 }
 template <class T, bool INTER, bool NORM, int MODE>
 void launch_units(const Rotate& a, float* part, int& blocks, cudaStream_t st) {
-    const int items = a.dim / (2 * Unit<T>::n), half = a.turned / 2, rows = a.s[0].heads + a.s[1].heads;
-    int lanes = 1;
-    while (lanes < items) lanes *= 2;
-    const int total = (int)(a.batch * a.ticks);
-    // a few ticks at a time give every thread an angle, unless there are not enough to go round
-    int per = std::max(1, std::min(kTicksMost, half ? 256 / half : kTicksMost));
-    while (per > 1 && (total + per - 1) / per < 148 * 4) per /= 2;
-    const int groups = 256 / lanes;
-    size_t bytes = (size_t)per * half * 8;
-    if (MODE == kBackwardW) bytes = std::max(bytes, (size_t)groups * 2 * a.dim * 4);
-    if (MODE == kBackwardEach) bytes += (size_t)rows * a.dim * 4;
+    const int items = a.dim / (2 * Unit<T>::n), half = a.turned / 2, total = (int)(a.batch * a.ticks);
+    UnitPlan plan{{1, 1}, 1};
+    while (plan.lanes < items) plan.lanes *= 2;
+    const int groups = 256 / plan.lanes;
+    size_t bytes = 0;
+    blocks = 1;
+    for (int i = 0; i < 2; ++i) {
+        const int heads = a.s[i].heads;
+        // as many ticks as leave a group a head or two of one, unless there are too few to go round
+        int per = 1;
+        while (MODE != kBackwardEach && per < kTicksMost && per * 2 <= groups && groups / per > std::max(1, heads / 2)) per *= 2;
+        while (per > 1 && (total + per - 1) / per < 148 * 4) per /= 2;
+        plan.per[i] = per;
+        bytes = std::max(bytes, (size_t)per * half * 16 + (MODE == kBackwardEach ? (size_t)heads * a.dim * 4 : 0));
+        if (heads) blocks = std::max(blocks, (total + per - 1) / per);
+    }
+    if (MODE == kBackwardW) bytes = std::max(bytes, (size_t)groups * a.dim * 4);
     auto* k = k_rotate_units<T, INTER, NORM, MODE>;
     if (bytes > 48 * 1024) MCK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    blocks = std::min((total + per - 1) / per, MODE >= kBackwardW ? kSplits : 148 * 32);
-    k<<<blocks, 256, bytes, st>>>(a, per, lanes, part);
+    blocks = std::min(blocks, MODE >= kBackwardW ? kSplits : 148 * 32);
+    k<<<dim3(blocks, a.s[1].heads ? 2 : 1), 256, bytes, st>>>(a, plan, part);
     MCK(cudaGetLastError());
 }
 template <class T, int MODE>
@@ -571,12 +582,12 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
                 if (!norms) launch_units<T, kBackward>(a, nullptr, blocks, st);
                 else if (each) launch_units<T, kBackwardEach>(a, part, blocks, st);
                 else launch_units<T, kBackwardW>(a, part, blocks, st);
-                for (int i = 0; norms && i < 2; ++i) {
-                    if (!a.s[i].gw || !a.s[i].heads) continue;
-                    const int n = (int)sets_of(g, i) * a.dim;
+                if (norms) {
+                    const int n[2] = {(int)sets_of(g, 0) * a.dim, (int)sets_of(g, 1) * a.dim};
                     const int stride = each ? (a.s[0].heads + a.s[1].heads) * a.dim : 2 * a.dim;
-                    const int at = i ? (each ? a.s[0].heads * a.dim : a.dim) : 0;
-                    k_rotate_gw_sum<<<(n + 31) / 32, 256, 0, st>>>(part + at, a.s[i].gw, n, stride, blocks);
+                    k_rotate_gw_sum<<<(stride + 31) / 32, 1024, 0, st>>>(part, a.s[0].heads ? a.s[0].gw : nullptr, n[0],
+                                                                         a.s[1].heads ? a.s[1].gw : nullptr,
+                                                                         each ? a.s[0].heads * a.dim : a.dim, n[1], stride, blocks);
                     MCK(cudaGetLastError());
                 }
                 return;
@@ -590,7 +601,7 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
                 const int splits = (int)std::max<long long>(1, std::min<long long>(256, g->batch * g->ticks));
                 const dim3 grid((a.dim + 127) / 128, sets, splits);
                 k_rotate_gw_any<T><<<grid, 128, 0, st>>>(a, i, norms, part, sets, splits);
-                k_rotate_gw_sum<<<(n + 31) / 32, 256, 0, st>>>(part, a.s[i].gw, n, n, splits);
+                k_rotate_gw_sum<<<(n + 31) / 32, 1024, 0, st>>>(part, a.s[i].gw, n, nullptr, 0, 0, n, splits);
                 MCK(cudaGetLastError());
             }
         });
