@@ -22,6 +22,7 @@ TRAIN = PKG / "fg_train"                             # the trainer executable (a
 SOURCES = [HERE / "fg_core.cu", HERE / "fg_noalloc.cu", HERE / "fg_hopop.cu", HERE / "fg_train.cu", HERE / "fg_fly.cu",
            HERE / "fg_rotate.cu", HERE / "fg_decay.cu"]
 DEPS = SOURCES + [HERE / "fg_kernels.cuh", HERE / "fg_tcgen05.cuh", HERE / "fg_outtc.cuh", HERE / "fg_memory.cuh", HERE / "fg_decay_tc.cuh",
+                  HERE / "fg_decay_mma.cuh",
                   REPO / "include" / "flyguy_b200.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

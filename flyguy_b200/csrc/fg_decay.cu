@@ -60,6 +60,7 @@ __device__ __forceinline__ long long part_ticks(long long n, int parts) {
 }
 
 }  // namespace
+#include "fg_decay_mma.cuh"
 #include "fg_decay_tc.cuh"
 namespace {
 
@@ -316,14 +317,16 @@ void check_sizes(const Sizes& z, const char* who) {
     if (z.batch * z.heads > (1ll << 27)) throw MemErr{w + ": batch * heads is over 2^27"};
 }
 
-// Parts a recording. On the tensor cores a block takes a SM to itself and a part costs its b and c read twice: as many parts
-// as keep blocks within the SMs, of at least four chunks. The recurrence's blocks share a SM and are slow: more of them.
+// Parts a recording. A part costs its b and c read twice, so: as many as keep the blocks within one round of the SMs (the
+// tcgen05 kernel takes a SM to itself, two blocks of the mma.sync kernel share one), of at least four chunks. The
+// recurrence's blocks are slow and share a SM: more of them.
 int parts_of(const fg_decay_args* g) {
     const long long rows = std::max<long long>(1, g->batch * g->heads);
     const long long mean = g->offsets ? g->ticks / std::max<long long>(1, g->batch) : g->ticks;
-    const bool tc = g->type == FG_BF16 && g->dim % 16 == 0 && g->value_dim % 16 == 0 && g->dim <= 128 && g->value_dim <= 128;
-    const long long blocks = tc ? rows : rows * ((std::min(g->dim, g->value_dim) + kRecCols - 1) / kRecCols);
-    const long long want = (tc ? 148 : 4 * 148) / blocks, most = mean / (tc ? 512 : 256);
+    const bool mma = g->dim <= 128 && g->value_dim <= 128;
+    const bool tc = mma && g->type == FG_BF16 && g->dim % 16 == 0 && g->value_dim % 16 == 0;
+    const long long blocks = mma ? rows : rows * ((std::min(g->dim, g->value_dim) + kRecCols - 1) / kRecCols);
+    const long long want = (tc ? 148 : mma ? 2 * 148 : 4 * 148) / blocks, most = mean / (tc ? 512 : 256);
     return (int)std::min<long long>(64, std::max<long long>(1, std::min(want, most)));
 }
 long long partial_floats(const fg_decay_args* g) {
@@ -370,7 +373,8 @@ Scan scan_of(const fg_decay_args* g) {
 
 template <class T>
 void launch(const Scan& s, cudaStream_t st) {
-    if (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value && tc_fits(s)) return tc_launch(s, st);
+    if (std::is_same<T, __nv_bfloat16>::value && tc_fits(s)) return tc_launch(s, st);
+    if (s.D <= 128 && s.E <= 128) return s.backward ? mma_launch_dims<T, true>(s, st) : mma_launch_dims<T, false>(s, st);
     const long long blocks = s.batch * s.heads * ((s.E + kRecCols - 1) / kRecCols);
     if (s.parts > 1) k_decay_rec<T><<<dim3((unsigned)blocks, s.parts - 1), 32 * kRecWarps, 0, st>>>(s, 1);
     k_decay_rec<T><<<dim3((unsigned)blocks, s.parts), 32 * kRecWarps, 0, st>>>(s, 0);
