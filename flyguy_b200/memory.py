@@ -20,6 +20,7 @@ from __future__ import annotations
 import math
 import struct
 from decimal import Decimal, localcontext
+from functools import lru_cache
 
 import torch
 from torch import nn
@@ -41,49 +42,60 @@ def _values(name: str, t, dims: tuple[int, ...], like=None) -> torch.Tensor:
         raise FlyguyError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     if t.dim() not in dims:
         raise FlyguyError(f"{name} must have {' or '.join(map(str, dims))} dimensions, not {t.dim()}")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.dim() != like.dim()):
+    if like is not None and (t.dtype is not like.dtype or t.dim() != like.dim() or t.get_device() != like.get_device()):
         raise FlyguyError(f"{name} must have the type, device and number of dimensions of the first tensor")
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _float32(name: str, t, like: torch.Tensor, *shapes) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != torch.float32:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != like.get_device():
         raise FlyguyError(f"{name} must be a float32 tensor on {like.device}")
-    if tuple(t.shape) not in shapes:
-        raise FlyguyError(f"{name} must be {' or '.join(map(str, shapes))}, not {tuple(t.shape)}")
-    return t.contiguous()
+    if t.shape not in shapes:
+        raise FlyguyError(f"{name} must be {' or '.join(map(str, map(tuple, shapes)))}, not {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _ticks(t: torch.Tensor | None) -> tuple[int, int, int, int]:
+def _ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
     """fg_ticks of [batch, ticks, heads, dim] or [ticks, heads, dim]."""
-    if t is None:
-        return 0, 0, 0, 0
     st = t.stride()
     return (t.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (t.data_ptr(), 0, st[0], st[1])
+
+
+_NONE = (0, 0, 0, 0)
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice   # (torch.cuda's own, without its objects)
 
 
 def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _call(fn, packed: bytes, device: torch.device) -> None:
+def _call(fn, packed: bytes, device: int) -> None:
     """fn(arguments, the current stream) on the tensors' device."""
-    if torch.cuda.current_device() != device.index:
+    if _device() != device:
         with torch.cuda.device(device):
-            rc = fn(packed, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(packed, _raw_stream(device))
     else:
-        rc = fn(packed, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(packed, _raw_stream(device))
     if rc:
         raise FlyguyError(lib().fg_mem_last_error().decode())
 
 
-def _work(size: int, device: torch.device) -> tuple[torch.Tensor | None, int, int]:
+def _room(size: int, device) -> tuple[torch.Tensor | None, tuple[int, int]]:
+    """A workspace of so many bytes, and its fields in an argument structure."""
     if size < 0:
         raise FlyguyError(lib().fg_mem_last_error().decode())
     if not size:
-        return None, 0, 0
+        return None, (0, 0)
     t = torch.empty(size, dtype=torch.uint8, device=device)
-    return t, t.data_ptr(), size
+    return t, (t.data_ptr(), size)
+
+
+def _grad(name: str, g, like: torch.Tensor, shape=None) -> torch.Tensor:
+    """An incoming gradient as the library takes it (None: zeros)."""
+    if g is None:
+        return torch.zeros(like.shape if shape is None else shape, dtype=like.dtype, device=like.device)
+    g = _values(name, g if g.dtype is like.dtype else g.to(like.dtype), (like.dim(),))
+    return g if 0 not in g.stride() else g.contiguous()   # (an expanded sum)
 
 
 # ---- rotation ------------------------------------------------------------------------------------------------------
@@ -121,106 +133,101 @@ def rotary_turns(turned: int, base: float = 10000.0, scaling: str | None = None,
 # fg_rotate_args: x, y, gy, gx (two fg_ticks each), w, w_head, gw, heads (two each), batch, ticks, dim, turned, turns,
 # positions, pos_batch, pos_tick, pos_bytes, type, interleaved, norm, eps, amplitude, work, work_bytes
 _ROTATE = struct.Struct("=32q8q12q2d2q")
-_NONE = (0, 0, 0, 0)
 
 
 class _Rotation:
-    """The checked arguments of one call: what forward and backward share."""
+    """What forward and backward of one call share: the sizes and settings as the argument structure has them."""
 
     def __init__(self, q, k, turns, positions, layout, amplitude, eps):
-        self.q, self.k = q, k
-        *lead, heads, dim = q.shape
-        if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != dim):
-            raise FlyguyError(f"k must be {(*lead, 'key heads', dim)}, not {tuple(k.shape)}")
-        batch, ticks = lead if len(lead) == 2 else (1, lead[0])
+        shape = q.shape
+        dim = shape[-1]
+        if k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != dim):
+            raise FlyguyError(f"k must be {(*shape[:-2], 'key heads', dim)}, not {tuple(k.shape)}")
+        batch, ticks = (shape[0], shape[1]) if len(shape) == 4 else (1, shape[0])
         if layout not in LAYOUTS:
             raise FlyguyError(f"layout must be one of {list(LAYOUTS)}, not {layout!r}")
-        turned = 0
+        turned = at = 0
         if turns is not None:
-            if not isinstance(turns, torch.Tensor) or turns.dtype != torch.int64 or turns.device != q.device or turns.dim() != 1:
+            if not isinstance(turns, torch.Tensor) or turns.dtype is not torch.int64 or turns.get_device() != q.get_device() or turns.dim() != 1:
                 raise FlyguyError(f"turns must be an int64 vector on {q.device} (rotary_turns)")
-            turned = 2 * turns.numel()
+            turned = 2 * turns.shape[0]
             if turned > dim:
                 raise FlyguyError(f"turns are of {turned} values, a head has {dim}")
-            turns = turns.contiguous()
+            if not turns.is_contiguous():
+                turns = turns.contiguous()
+            at = turns.data_ptr()
         pos = (0, 0, 0, 8)
         if positions is not None:
-            if not isinstance(positions, torch.Tensor) or positions.device != q.device or positions.dtype not in (torch.int64, torch.int32):
+            if not isinstance(positions, torch.Tensor) or positions.get_device() != q.get_device() or positions.dtype not in (torch.int64, torch.int32):
                 raise FlyguyError(f"positions must be int64 or int32 on {q.device}")
-            try:
-                p = positions.expand(batch, ticks)
-            except RuntimeError:
-                raise FlyguyError(f"positions {tuple(positions.shape)} do not fit {batch} x {ticks} ticks") from None
+            p = positions
+            if p.shape != (batch, ticks):
+                try:
+                    p = p.expand(batch, ticks)
+                except RuntimeError:
+                    raise FlyguyError(f"positions {tuple(positions.shape)} do not fit {batch} x {ticks} ticks") from None
             pos = (p.data_ptr(), p.stride(0), p.stride(1), p.element_size())
-        self.keep = (turns, positions)
-        self.dims = (heads, 0 if k is None else k.shape[-2], batch, ticks, dim, turned, _ptr(turns), *pos, TYPES[q.dtype],
-                     LAYOUTS[layout])
-        self.floats = (float(eps or 1.0), float(amplitude))
-        self.norm = int(eps is not None)
+        self.keep = (turns, positions)                        # (their memory, until the backward has run)
+        self.dim, self.device = dim, q.get_device()
+        self.fields = (shape[-2], 0 if k is None else k.shape[-2], batch, ticks, dim, turned, at, *pos, TYPES[q.dtype],
+                       LAYOUTS[layout], int(eps is not None), float(eps or 1.0), float(amplitude))
 
-    def pack(self, y=_NONE, z=_NONE, gy=_NONE, gz=_NONE, gx=_NONE, gk=_NONE, wq=None, wk=None, gwq=None, gwk=None,
+    def pack(self, x, z=_NONE, y=_NONE, yk=_NONE, gy=_NONE, gz=_NONE, gx=_NONE, gk=_NONE, wq=None, wk=None, gwq=None, gwk=None,
              work=(0, 0)) -> bytes:
-        dim = self.dims[4]
-        return _ROTATE.pack(*_ticks(self.q), *_ticks(self.k), *y, *z, *gy, *gz, *gx, *gk, _ptr(wq), _ptr(wk),
-                            dim if wq is not None and wq.dim() == 2 else 0, dim if wk is not None and wk.dim() == 2 else 0,
-                            _ptr(gwq), _ptr(gwk), *self.dims, self.norm, *self.floats, *work)
+        return _ROTATE.pack(*x, *z, *y, *yk, *gy, *gz, *gx, *gk, _ptr(wq), _ptr(wk),
+                            self.dim if wq is not None and wq.dim() == 2 else 0, self.dim if wk is not None and wk.dim() == 2 else 0,
+                            _ptr(gwq), _ptr(gwk), *self.fields, *work)
 
-    def forward(self, wq=None, wk=None):
-        q, k = self.q, self.k
+    def forward(self, q, k=None, wq=None, wk=None):
         y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        z = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _call(lib().fg_norm_rotate, self.pack(_ticks(y), _ticks(z), wq=wq, wk=wk), q.device)
+        if k is None:
+            _call(lib().fg_norm_rotate, self.pack(_ticks(q), y=_ticks(y)), self.device)
+            return y
+        z = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _call(lib().fg_norm_rotate, self.pack(_ticks(q), _ticks(k), _ticks(y), _ticks(z), wq=wq, wk=wk), self.device)
         return y, z
 
-    def backward(self, gy, gz, wq=None, wk=None, want_w=(False, False)):
-        q, k = self.q, self.k
-        gy = _grad("the gradient of the queries", gy, q)
-        gz = None if k is None else _grad("the gradient of the keys", gz, k)
-        gx = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        gk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    def backward(self, gy, gz=None, q=None, k=None, wq=None, wk=None, want_w=(False, False)):
+        gx = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device)
+        if q is None:                                         # the rotation alone
+            _call(lib().fg_norm_rotate_bwd, self.pack(_NONE, gy=_ticks(gy), gx=_ticks(gx)), self.device)
+            return gx
+        gk = torch.empty(gz.shape, dtype=gz.dtype, device=gz.device)
         gwq = torch.empty_like(wq) if wq is not None and want_w[0] else None
         gwk = torch.empty_like(wk) if wk is not None and want_w[1] else None
-        kw = dict(gy=_ticks(gy), gz=_ticks(gz), gx=_ticks(gx), gk=_ticks(gk), wq=wq, wk=wk, gwq=gwq, gwk=gwk)
-        work = (None, 0, 0)
+        a = (_ticks(q), _ticks(k), _NONE, _NONE, _ticks(gy), _ticks(gz), _ticks(gx), _ticks(gk), wq, wk, gwq, gwk)
+        room, work = None, (0, 0)
         if gwq is not None or gwk is not None:
-            work = _work(lib().fg_norm_rotate_work(self.pack(**kw)), q.device)
-        _call(lib().fg_norm_rotate_bwd, self.pack(**kw, work=work[1:]), q.device)
+            room, work = _room(lib().fg_norm_rotate_work(self.pack(*a)), q.device)
+        _call(lib().fg_norm_rotate_bwd, self.pack(*a, work), self.device)
         return gx, gk, gwq, gwk
-
-
-def _grad(name: str, g, like: torch.Tensor, shape=None) -> torch.Tensor:
-    """An incoming gradient as the library takes it (None: zeros)."""
-    if g is None:
-        return torch.zeros(like.shape if shape is None else shape, dtype=like.dtype, device=like.device)
-    g = _values(name, g.to(like.dtype), (like.dim(),))
-    return g if 0 not in g.stride() else g.contiguous()   # (an expanded sum)
 
 
 class _RotateFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rotation):
         ctx.rotation = rotation
-        return rotation.forward()[0]
+        return rotation.forward(x)
 
     @staticmethod
     def backward(ctx, gy):
-        return ctx.rotation.backward(gy, None)[0], None
+        return ctx.rotation.backward(_grad("the gradient", gy, gy)), None
 
 
 class _NormRotateFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, rotation):
         ctx.set_materialize_grads(False)
+        q, k = _values("q", q, (3, 4)), _values("k", k, (3, 4))
         ctx.save_for_backward(q, k, wq, wk)
         ctx.rotation = rotation
-        return rotation.forward(wq, wk)
+        return rotation.forward(q, k, wq, wk)
 
     @staticmethod
     def backward(ctx, gy, gz):
         q, k, wq, wk = ctx.saved_tensors
-        r = ctx.rotation
-        r.q, r.k = _values("q", q.detach(), (3, 4)), _values("k", k.detach(), (3, 4))
-        return *r.backward(gy, gz, wq, wk, ctx.needs_input_grad[2:4]), None
+        gy, gz = _grad("the gradient of the queries", gy, q), _grad("the gradient of the keys", gz, k)
+        return *ctx.rotation.backward(gy, gz, q, k, wq, wk, ctx.needs_input_grad[2:4]), None
 
 
 def rotate(x, turns, positions=None, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:
@@ -229,11 +236,11 @@ def rotate(x, turns, positions=None, layout: str = "half", amplitude: float = 1.
 
     positions: int64 / int32 that expand to [batch, ticks] (None: 0, 1, ..). layout "half": pairs (i, i + turned / 2);
     "interleaved": (2i, 2i + 1). The gradient is the rotation back."""
-    x0 = _values("x", x, (3, 4))
-    r = _Rotation(x0.detach(), None, turns, positions, layout, amplitude, None)
-    if torch.is_grad_enabled() and x.requires_grad:
+    x = _values("x", x, (3, 4))
+    r = _Rotation(x, None, turns, positions, layout, amplitude, None)
+    if x.requires_grad and torch.is_grad_enabled():
         return _RotateFn.apply(x, r)
-    return r.forward()[0]
+    return r.forward(x)
 
 
 def norm_rotate(q, k, turns=None, q_weight=None, k_weight=None, positions=None, layout: str = "half",
@@ -241,18 +248,19 @@ def norm_rotate(q, k, turns=None, q_weight=None, k_weight=None, positions=None, 
     """rotate(x / sqrt(mean(x^2) + eps) * weight) over each head of queries [.., heads, dim] and keys [.., key heads, dim],
     in one pass over both. Weights: float32 [dim] (one for all heads) or [heads, dim], or None; turns None: the
     norms alone. Gradients of q, k and the weights; the weights' are the same bits on every run."""
-    q0 = _values("q", q, (3, 4))
-    k0 = _values("k", k, (3, 4), q)
+    q = _values("q", q, (3, 4))
+    k = _values("k", k, (3, 4), q)
     if not eps > 0:
         raise FlyguyError(f"eps must be positive, not {eps}")
     if q_weight is not None:
-        q_weight = _float32("q_weight", q_weight, q, tuple(q.shape[-1:]), tuple(q.shape[-2:]))
+        q_weight = _float32("q_weight", q_weight, q, q.shape[-1:], q.shape[-2:])
     if k_weight is not None:
-        k_weight = _float32("k_weight", k_weight, k, tuple(k.shape[-1:]), tuple(k.shape[-2:]))
-    r = _Rotation(q0.detach(), k0.detach(), turns, positions, layout, amplitude, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        k_weight = _float32("k_weight", k_weight, k, k.shape[-1:], k.shape[-2:])
+    r = _Rotation(q, k, turns, positions, layout, amplitude, eps)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         return _NormRotateFn.apply(q, k, q_weight, k_weight, r)
-    return r.forward(None if q_weight is None else q_weight.detach(), None if k_weight is None else k_weight.detach())
+    return r.forward(q, k, q_weight, k_weight)
 
 
 # ---- attention whose state decays -----------------------------------------------------------------------------------
@@ -264,13 +272,18 @@ _DECAY = struct.Struct("=32q6q7qd2q")
 _STEP = struct.Struct("=16q10qd")
 
 
+@lru_cache(maxsize=256)
+def _decay_room(sizes: tuple, packed: bool, backward: bool) -> int:
+    """Bytes of workspace that a call of these sizes needs (fg_decay_work)."""
+    return lib().fg_decay_work(_DECAY.pack(*(0,) * 37, int(packed), *sizes, 1.0, 0, 0), int(backward))
+
+
 class _Decay:
-    """The checked arguments of one decay_attention call."""
+    """What forward and backward of one call share."""
 
     def __init__(self, q, k, v, log_decay, state, scale, offsets):
-        heads, dim = q.shape[-2:]
-        key_heads, value_dim = v.shape[-2:]
-        lead = q.shape[:-2]
+        lead, heads, dim = q.shape[:-2], q.shape[-2], q.shape[-1]
+        key_heads, value_dim = v.shape[-2], v.shape[-1]
         if k.shape != (*lead, key_heads, dim) or v.shape[:-2] != lead:
             raise FlyguyError(f"k and v must be {(*lead, 'key heads', dim)} and {(*lead, 'key heads', 'value dim')}, not "
                               f"{tuple(k.shape)} and {tuple(v.shape)}")
@@ -281,46 +294,40 @@ class _Decay:
         else:
             if len(lead) != 1:
                 raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
-            if (not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int64 or offsets.device != q.device
+            if (not isinstance(offsets, torch.Tensor) or offsets.dtype is not torch.int64 or offsets.get_device() != q.get_device()
                     or offsets.dim() != 1 or not offsets.numel()):
                 raise FlyguyError(f"offsets must be an int64 vector [recordings + 1] on {q.device}")
             offsets = offsets.contiguous()
-            batch, ticks = offsets.numel() - 1, lead[0]
+            batch, ticks = offsets.shape[0] - 1, lead[0]
         if log_decay.requires_grad:
             raise FlyguyError("log_decay is a constant of each head: it has no gradient")
         self.log_decay = _float32("log_decay", log_decay, q, (heads,))
-        self.states = (batch, heads, dim, value_dim)
+        self.states, self.device, self.offsets = (batch, heads, dim, value_dim), q.get_device(), offsets
         if state is not None:
-            state = _float32("state", state, q, self.states)
-        self.q, self.k, self.v, self.state, self.offsets = q, k, v, state, offsets
+            _float32("state", state, q, self.states)
         self.sizes = (batch, ticks, heads, key_heads, dim, value_dim, TYPES[q.dtype])
         self.scale = float(dim ** -0.5 if scale is None else scale)
 
-    def pack(self, o=_NONE, go=_NONE, gq=_NONE, gk=_NONE, gv=_NONE, state_out=None, gstate_out=None, gstate=None,
-             work=(0, 0)) -> bytes:
-        return _DECAY.pack(*_ticks(self.q), *_ticks(self.k), *_ticks(self.v), *o, *go, *gq, *gk, *gv,
-                           self.log_decay.data_ptr(), _ptr(self.state), _ptr(state_out), _ptr(gstate_out), _ptr(gstate),
-                           _ptr(self.offsets), *self.sizes, self.scale, *work)
+    def run(self, fn, backward: bool, tensors, state=None, state_out=None, gstate_out=None, gstate=None) -> None:
+        room, work = _room(_decay_room(self.sizes, self.offsets is not None, backward), tensors[0].device)
+        packed = _DECAY.pack(*(f for t in tensors for f in (_NONE if t is None else _ticks(t))), self.log_decay.data_ptr(),
+                             _ptr(state), _ptr(state_out), _ptr(gstate_out), _ptr(gstate), _ptr(self.offsets), *self.sizes,
+                             self.scale, *work)
+        _call(fn, packed, self.device)
 
-    def forward(self):
-        q, v = self.q, self.v
+    def forward(self, q, k, v, state):
         o = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
         end = torch.empty(self.states, dtype=torch.float32, device=q.device)
-        kw = dict(o=_ticks(o), state_out=end)
-        work = _work(lib().fg_decay_work(self.pack(**kw), 0), q.device)
-        _call(lib().fg_decay_attn, self.pack(**kw, work=work[1:]), q.device)
+        self.run(lib().fg_decay_attn, False, (q, k, v, o, None, None, None, None), state, end)
         return o, end
 
-    def backward(self, go, gend, want_state: bool):
-        q, k, v = self.q, self.k, self.v
+    def backward(self, q, k, v, state, go, gend, want_state: bool):
         go = _grad("the gradient of o", go, q, (*q.shape[:-1], v.shape[-1]))
         if gend is not None:
             gend = gend.float().contiguous()
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         gstate = torch.empty(self.states, dtype=torch.float32, device=q.device) if want_state else None
-        kw = dict(go=_ticks(go), gq=_ticks(gq), gk=_ticks(gk), gv=_ticks(gv), gstate_out=gend, gstate=gstate)
-        work = _work(lib().fg_decay_work(self.pack(**kw), 1), q.device)
-        _call(lib().fg_decay_attn_bwd, self.pack(**kw, work=work[1:]), q.device)
+        self.run(lib().fg_decay_attn_bwd, True, (q, k, v, None, go, gq, gk, gv), state, None, gend, gstate)
         return gq, gk, gv, gstate
 
 
@@ -328,17 +335,15 @@ class _DecayFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, state, job):
         ctx.set_materialize_grads(False)
+        q, k, v = (_values("q", t, (3, 4)) for t in (q, k, v))
+        state = None if state is None else state.contiguous()
         ctx.save_for_backward(q, k, v, state)
         ctx.job = job
-        return job.forward()
+        return job.forward(q, k, v, state)
 
     @staticmethod
     def backward(ctx, go, gend):
-        q, k, v, state = ctx.saved_tensors
-        job = ctx.job
-        job.q, job.k, job.v = (_values("q", t.detach(), (3, 4)) for t in (q, k, v))
-        job.state = None if state is None else state.detach().contiguous()
-        return *job.backward(go, gend, ctx.needs_input_grad[3]), None
+        return *ctx.job.backward(*ctx.saved_tensors, go, gend, ctx.needs_input_grad[3]), None
 
 
 def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,
@@ -350,12 +355,13 @@ def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,
     be empty). log_decay float32 [heads], at most 0, a constant. state float32 [recordings, heads, dim, value dim] before
     the first ticks (None: zeros). scale: dim^-0.5 when None. dim and value dim at most 256.
     Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v and state."""
-    q0 = _values("q", q, (3, 4))
-    k0, v0 = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
-    job = _Decay(q0.detach(), k0.detach(), v0.detach(), log_decay, None if state is None else state.detach(), scale, offsets)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+    q = _values("q", q, (3, 4))
+    k, v = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
+    job = _Decay(q, k, v, log_decay, state, scale, offsets)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (state is not None and state.requires_grad)):
         return _DecayFn.apply(q, k, v, state, job)
-    return job.forward()
+    return job.forward(q, k, v, None if state is None else state.contiguous())
 
 
 def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None) -> torch.Tensor:
@@ -372,21 +378,25 @@ def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None
     if not key_heads or heads % key_heads:
         raise FlyguyError(f"{heads} query heads cannot share {key_heads} key heads")
     log_decay = _float32("log_decay", log_decay, q, (heads,))
-    if (not isinstance(state, torch.Tensor) or state.dtype != torch.float32 or state.device != q.device
+    if (not isinstance(state, torch.Tensor) or state.dtype is not torch.float32 or state.get_device() != q.get_device()
             or state.dim() != 4 or state.shape[1:] != (heads, dim, value_dim) or not state.is_contiguous()):
         raise FlyguyError(f"state must be contiguous float32 {('slots', heads, dim, value_dim)} on {q.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise FlyguyError("decay_step has no gradient (decay_attention has): call it under torch.no_grad()")
     if slots is not None:
-        if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int64 or slots.device != q.device or slots.shape != (batch,):
+        if (not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.get_device() != q.get_device()
+                or slots.shape != (batch,)):
             raise FlyguyError(f"slots must be int64 [{batch}] on {q.device}")
-        slots = slots.contiguous()
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
     elif state.shape[0] < batch:
         raise FlyguyError(f"{batch} rows need as many states, not {state.shape[0]}")
     o = torch.empty((batch, heads, value_dim), dtype=q.dtype, device=q.device)
-    rows = lambda t: (t.data_ptr(), t.stride(0), 0, t.stride(1))    # noqa: E731
-    packed = _STEP.pack(*rows(q), *rows(k), *rows(v), *rows(o), log_decay.data_ptr(), state.data_ptr(), _ptr(slots),
-                        state.shape[0], batch, heads, key_heads, dim, value_dim, TYPES[q.dtype],
-                        float(dim ** -0.5 if scale is None else scale))
-    _call(lib().fg_decay_step, packed, q.device)
+    f = []
+    for t in (q, k, v, o):
+        st = t.stride()
+        f += (t.data_ptr(), st[0], 0, st[1])
+    packed = _STEP.pack(*f, log_decay.data_ptr(), state.data_ptr(), _ptr(slots), state.shape[0], batch, heads, key_heads, dim,
+                        value_dim, TYPES[q.dtype], float(dim ** -0.5 if scale is None else scale))
+    _call(lib().fg_decay_step, packed, q.get_device())
     return o
