@@ -400,3 +400,60 @@ def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None
                         value_dim, TYPES[q.dtype], float(dim ** -0.5 if scale is None else scale))
     _call(lib().fg_decay_step, packed, q.get_device())
     return o
+
+
+# ---- the operators together ---------------------------------------------------------------------------------------
+
+class TickMemory(nn.Module):
+    """What earlier ticks add to an actor's logits: logits = actor(obs) + memory(obs).
+
+    Queries, keys and values are projections of the observations in `dtype`; norm_rotate turns queries and keys,
+    decay_attention carries the states (the heads' memories spread from ticks[0] to ticks[1] ticks), a last projection
+    gives the logits. That one starts at zero, so that a fresh memory changes nothing. Learning sees whole recordings
+    (forward), playing one tick of every car at a time (step); both give the same answers, to the rounding of `dtype`."""
+
+    def __init__(self, obs_dim: int, n_actions: int, heads: int = 8, key_heads: int = 2, dim: int = 64,
+                 ticks: tuple[float, float] = (16.0, 4096.0), base: float = 10000.0, dtype: torch.dtype = torch.bfloat16):
+        super().__init__()
+        if key_heads < 1 or heads % key_heads:
+            raise FlyguyError(f"{heads} query heads cannot share {key_heads} key heads")
+        if not 1 < ticks[0] <= ticks[1]:
+            raise FlyguyError(f"memories of {ticks} ticks: over 1, the shorter first")
+        self.heads, self.key_heads, self.dim, self.dtype = heads, key_heads, dim, dtype
+        self.qkv = nn.Linear(obs_dim, (heads + 2 * key_heads) * dim, bias=False)
+        self.out = nn.Linear(heads * dim, n_actions, bias=False)
+        nn.init.zeros_(self.out.weight)
+        self.q_weight, self.k_weight = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.ones(dim))
+        span = torch.logspace(math.log10(ticks[0]), math.log10(ticks[1]), heads, dtype=torch.float64)
+        self.register_buffer("log_decay", torch.log1p(-1 / span).float(), persistent=False)
+        self.register_buffer("turns", rotary_turns(dim // 2 * 2, base), persistent=False)
+
+    def states(self, cars: int) -> torch.Tensor:
+        """The states of so many cars that remember nothing: float32 [cars, heads, dim, dim]."""
+        return torch.zeros(cars, self.heads, self.dim, self.dim, device=self.log_decay.device)
+
+    def _qkv(self, obs: torch.Tensor, positions):
+        x = nn.functional.linear(obs.to(self.dtype), self.qkv.weight.to(self.dtype))
+        x = x.unflatten(-1, (self.heads + 2 * self.key_heads, self.dim))
+        q, k, v = x.split((self.heads, self.key_heads, self.key_heads), -2)
+        return *norm_rotate(q, k, self.turns, self.q_weight, self.k_weight, positions), v
+
+    def _logits(self, o: torch.Tensor) -> torch.Tensor:
+        return nn.functional.linear(o.flatten(-2), self.out.weight.to(self.dtype)).float()
+
+    def forward(self, obs: torch.Tensor, state=None, positions=None, offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """obs [recordings, ticks, obs_dim], or [ticks, obs_dim] packed end to end with offsets: logits of every tick and
+        the states after the last. A recording carried on needs its states and positions (a rotation depends on them)."""
+        if state is not None and positions is None:
+            raise FlyguyError("a recording carried on from a state needs its ticks' positions")
+        q, k, v = self._qkv(obs, positions)
+        o, end = decay_attention(q, k, v, self.log_decay, state, offsets=offsets)
+        return self._logits(o), end
+
+    @torch.no_grad()
+    def step(self, obs: torch.Tensor, state: torch.Tensor, positions: torch.Tensor, slots=None) -> torch.Tensor:
+        """One tick of every car: obs [cars, obs_dim], positions [cars] the tick of each car's recording; the states are updated
+        in place (at `slots`, see decay_step)."""
+        q, k, v = self._qkv(obs.unsqueeze(1), positions.unsqueeze(1))
+        o = decay_step(q.squeeze(1), k.squeeze(1), v.squeeze(1), self.log_decay, state, slots=slots)
+        return self._logits(o)
