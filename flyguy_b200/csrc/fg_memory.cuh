@@ -27,6 +27,32 @@ __device__ __forceinline__ float warp_sum(float s) {
     return s;
 }
 
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ void halves(uint64_t x, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+// the two halves' sum
+__device__ __forceinline__ float sum2(uint64_t x) {
+    float a, b;
+    halves(x, a, b);
+    return a + b;
+}
+
 struct MemErr {
     std::string msg;
 };

@@ -5,7 +5,8 @@
 //
 // A tick's angle is position * turns[i] / 2^64 of a turn: the 64-bit product wraps, which drops whole turns exactly, so
 // the angle is as good at position 2^40 as at 0 (an fp32 product of position and frequency is off by 0.06 rad at 10^6).
-// Its upper 32 bits, as a signed fraction of half a turn, go to sincospif.
+// Its upper 32 bits give the nearest quarter turn and what is left, at most pi / 4 either way, for which the Taylor series
+// of sine and cosine up to x^9 and x^8 are good to 2.5e-8.
 #include "fg_memory.cuh"
 
 namespace {
@@ -40,11 +41,27 @@ __device__ __forceinline__ long long position(const Rotate& a, long long b, long
     const long long i = b * a.pos_batch + t * a.pos_tick;
     return a.pos8 ? static_cast<const long long*>(a.positions)[i] : static_cast<const int*>(a.positions)[i];
 }
+// cosine and sine of u / 2^32 of a turn, times `amplitude`
+__device__ __forceinline__ void turned(uint32_t u, float amplitude, float& c, float& s) {
+    const uint32_t quarter = (u + 0x20000000u) >> 30;
+    const float x = (float)(int)(u - (quarter << 30)) * 1.46291807926715968e-9f, y = x * x;   // 2 pi / 2^32
+    float sine = fmaf(y, 1.f / 362880, -1.f / 5040);
+    sine = fmaf(y, sine, 1.f / 120);
+    sine = fmaf(y, sine, -1.f / 6);
+    sine = fmaf(y * x, sine, x);
+    float cosine = fmaf(y, 1.f / 40320, -1.f / 720);
+    cosine = fmaf(y, cosine, 1.f / 24);
+    cosine = fmaf(y, cosine, -0.5f);
+    cosine = fmaf(y, cosine, 1.f);
+    const float p = quarter & 1 ? sine : cosine, q = quarter & 1 ? cosine : sine;
+    c = (quarter + 1) & 2 ? -amplitude * p : amplitude * p;
+    s = quarter & 2 ? -amplitude * q : amplitude * q;
+}
+__device__ __forceinline__ uint32_t upper(long long pos, unsigned long long turns) {
+    return (uint32_t)(((unsigned long long)pos * turns) >> 32);
+}
 __device__ __forceinline__ void angle(const Rotate& a, long long pos, int i, float& c, float& s) {
-    const unsigned long long u = (unsigned long long)pos * (unsigned long long)__ldg(&a.turns[i]);
-    sincospif((float)(int)(u >> 32) * 4.656612873077393e-10f, &s, &c);   // 2^-31: a full turn is 2
-    c *= a.amplitude;
-    s *= a.amplitude;
+    turned(upper(pos, (unsigned long long)__ldg(&a.turns[i])), a.amplitude, c, s);
 }
 __device__ __forceinline__ void pair_of(const Rotate& a, int i, int& p, int& q) {
     p = a.interleaved ? 2 * i : i;
@@ -172,120 +189,181 @@ __global__ void __launch_bounds__(128) k_rotate_gw_any(const __grid_constant__ R
     }
     part[((long long)split * sets + set) * a.dim + i] = sum;
 }
-// gw = the splits' sums added in a fixed order: 32 warps each take every 32nd split of 32 values, then their sums in turn.
-// Values 0 .. n0 - 1 of a split go to gw0, those from `second` on to gw1.
-__global__ void __launch_bounds__(1024) k_rotate_gw_sum(const float* __restrict__ part, float* __restrict__ gw0, int n0,
-                                                        float* __restrict__ gw1, int second, int n1, int stride,
-                                                        int splits) {
+// gw = the splits' sums added in a fixed order: 32 warps each take every 32nd split of 32 values, then their sums in turn
+struct SumSide {
+    const float* part;
+    float* gw;
+    int n, splits;
+};
+__global__ void __launch_bounds__(1024) k_rotate_gw_sum(const SumSide queries, const SumSide keys) {
     __shared__ float sums[32][33];
+    const SumSide a = blockIdx.y ? keys : queries;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
-    const bool one = gw0 && i < n0, two = gw1 && i >= second && i < second + n1;
     float s = 0.f;
-    if (one || two) {
+    if (i < a.n) {
 #pragma unroll 4
-        for (int k = w; k < splits; k += 32) s += part[(long long)k * stride + i];
+        for (int k = w; k < a.splits; k += 32) s += a.part[(long long)k * a.n + i];
     }
     sums[w][lane] = s;
     __syncthreads();
-    if (w) return;
+    if (w || i >= a.n) return;
 #pragma unroll
     for (int k = 1; k < 32; ++k) s += sums[k][lane];
-    if (one) gw0[i] = s;
-    if (two) gw1[i - second] = s;
+    a.gw[i] = s;
 }
 
 // ---- rows of whole 16-byte units ------------------------------------------------------------------------------------
 //
-// A block takes a few ticks at a time: 256 threads form the ticks' angles once into shared memory (as many as one each),
-// then every group of 2^k lanes takes some heads of one tick, each lane two 16-byte units of a head: the partners of the
-// "half" layout (unit u and u + turned / 2), or two neighbours. A lane's pairs of values are its own, so the rotation needs
-// no exchange, the norm a few shuffles, and every value is read and written once, 16 bytes a load. The lane's angles and
-// weights stay in registers over its heads: fetched for each head they are three times the bytes of the values, and L1
-// was the limit (128 recordings of 128 ticks, 16 + 4 heads of 128 in bf16: @@ us forward, @@ us back). The next head's
-// values are asked for before the present one's are used.
+// A block takes a few ticks of the queries, or of the keys, at a time. Its 256 threads form the ticks' angles once into
+// shared memory; then every group of 2^k lanes takes heads of one tick, each lane two 16-byte units of a head: partners of
+// the "half" layout, or any two. A lane's pairs are its own, so the rotation needs no exchange, the norm a few shuffles, and
+// every value is read and written once. The lane's angles and weights stay in registers over its heads: fetched for each
+// head they are three times the bytes of the values.
+//
+// The bound is the memory: 2 passes over the values forward (read, write), 3 back. What it takes to get near it: kAhead
+// heads of each lane are on their way into shared memory at any time (a lane reads only what it asked for itself, so no
+// barrier is needed), and the arithmetic is done on pairs of floats, for the kernel is half bound by its instructions. In
+// bf16, half layout, 128 recordings of 128 ticks, 16 + 4 heads of 128, forward and back with the sums of gw: 41 and 74 us,
+// where one head ahead in registers takes 49 and 99, and a row for each group, with its angles and weights fetched anew,
+// 73 and 95; the bytes alone are 26 and 39 us. In fp16, 32 recordings of 2,048 ticks, 8 + 8 heads of 128, the first 96
+// values turned as neighbours: 115 us (bytes: 82); where the lane's two units are neighbours too, 182.
 
+// 16 bytes of T as pairs of floats, n values in all
 template <class T>
-struct Unit {                                                // 16 bytes of T as floats
-    static constexpr int n = 16 / sizeof(T);
+struct Unit {
+    static constexpr int n = 16 / sizeof(T), pairs = n / 2;
 };
+__device__ __forceinline__ uint64_t pair_of_bits(uint32_t v, __nv_bfloat16) {
+    return two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ uint64_t pair_of_bits(uint32_t v, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return two(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t bits_of_pair(uint64_t x, __nv_bfloat16) {
+    float a, b;
+    halves(x, a, b);
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t bits_of_pair(uint64_t x, __half) {
+    float a, b;
+    halves(x, a, b);
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
 template <class T>
-__device__ __forceinline__ void from_unit(const uint4& u, float (&v)[Unit<T>::n]) {
+__device__ __forceinline__ void from_unit(const uint4& u, uint64_t (&v)[Unit<T>::pairs]) {
     const uint32_t r[4] = {u.x, u.y, u.z, u.w};
-    if (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+    if constexpr (sizeof(T) == 4) {
+        v[0] = two(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        v[1] = two(__uint_as_float(r[2]), __uint_as_float(r[3]));
     } else {
-        const T* t = reinterpret_cast<const T*>(r);
 #pragma unroll
-        for (int i = 0; i < Unit<T>::n; ++i) v[i] = to_f(t[i]);
+        for (int i = 0; i < 4; ++i) v[i] = pair_of_bits(r[i], T());
     }
 }
 template <class T>
-__device__ __forceinline__ void store_unit(T* p, const float (&v)[Unit<T>::n]) {
+__device__ __forceinline__ void store_unit(T* p, const uint64_t (&v)[Unit<T>::pairs]) {
     uint32_t r[4];
-    if (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[i]);
+    if constexpr (sizeof(T) == 4) {
+        float a, b, c, d;
+        halves(v[0], a, b);
+        halves(v[1], c, d);
+        r[0] = __float_as_uint(a); r[1] = __float_as_uint(b); r[2] = __float_as_uint(c); r[3] = __float_as_uint(d);
     } else {
-        T* t = reinterpret_cast<T*>(r);
 #pragma unroll
-        for (int i = 0; i < Unit<T>::n; ++i) t[i] = from_f<T>(v[i]);
+        for (int i = 0; i < 4; ++i) r[i] = bits_of_pair(v[i], T());
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
 }
-// (p[i], q[i]) turned by (c, s); INTER: the pairs are neighbours within p, then within q
-template <bool INTER, int N>
-__device__ __forceinline__ void turn(float (&p)[N], float (&q)[N], const float (&c)[N], const float (&s)[N]) {
+// values of p and of q turned by the angles c, s (with `minus` = -s), value i of p with value i of q
+template <int P>
+__device__ __forceinline__ void turn_apart(uint64_t (&p)[P], uint64_t (&q)[P], const uint64_t (&c)[P], const uint64_t (&s)[P],
+                                           const uint64_t (&minus)[P]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float& a = INTER ? (i < N / 2 ? p[2 * i] : q[2 * i - N]) : p[i];
-        float& b = INTER ? (i < N / 2 ? p[2 * i + 1] : q[2 * i + 1 - N]) : q[i];
-        const float u = a, v = b;
-        a = u * c[i] - v * s[i];
-        b = v * c[i] + u * s[i];
+    for (int i = 0; i < P; ++i) {
+        const uint64_t u = p[i], v = q[i];
+        p[i] = fma2(u, c[i], mul2(v, minus[i]));
+        q[i] = fma2(v, c[i], mul2(u, s[i]));
     }
 }
-
-constexpr int kTicksMost = 8;
+// neighbours of one unit, by its half of the angles
+template <int HALF, int P>
+__device__ __forceinline__ void turn_neighbours(uint64_t (&p)[P], const uint64_t (&c)[P], const uint64_t (&s)[P]) {
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+        float c0, c1, s0, s1, a, b;
+        halves(c[HALF * P / 2 + i], c0, c1);
+        halves(s[HALF * P / 2 + i], s0, s1);
+        halves(p[2 * i], a, b);
+        p[2 * i] = two(a * c0 - b * s0, b * c0 + a * s0);
+        halves(p[2 * i + 1], a, b);
+        p[2 * i + 1] = two(a * c1 - b * s1, b * c1 + a * s1);
+    }
+}
 
 enum { kForward, kBackward, kBackwardW, kBackwardEach };     // the last two with gw: one set of weights, one for each head
 
 struct UnitPlan {
-    int per[2];                                              // ticks at a time, for queries and keys (powers of 2)
+    int per[2], blocks[2];                                   // ticks at a time (powers of 2) and blocks, for queries and keys
     int lanes;                                               // of a group
+    uint32_t by_ticks;                                       // 2^32 / ticks, rounded up
 };
+constexpr int kAhead = 4;                                    // heads whose values are on their way into shared memory
+template <bool NORM, int MODE>
+constexpr int kUnits = MODE != kForward && NORM ? 4 : 2;     // 16-byte units that a lane reads of a head
+// 16 bytes, or zeros: nothing is read then
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+// n / d with r = 2^32 / d rounded up, n < 2^30: at most one too many
+__device__ __forceinline__ int divided(int n, int d, uint32_t r) {
+    if (d == 1) return n;
+    const int q = (int)__umulhi((uint32_t)n, r);
+    return q * d > n ? q - 1 : q;
+}
 
 template <class T, bool INTER, bool NORM, int MODE>
-__global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_units(const __grid_constant__ Rotate a,
+__global__ void __launch_bounds__(256, MODE != kForward && NORM ? 2 : 3) k_rotate_units(const __grid_constant__ Rotate a,
                                                                                  const UnitPlan plan,
                                                                                  float* __restrict__ part) {
-    constexpr int N = Unit<T>::n;
-    extern __shared__ __align__(16) float shared[];
-    const Side& s = a.s[blockIdx.y];
-    const int heads = s.heads, per = plan.per[blockIdx.y], half_turn = a.turned / 2;
+    constexpr int N = Unit<T>::n, P = Unit<T>::pairs, U = kUnits<NORM, MODE>;
+    extern __shared__ __align__(16) float all_shared[];      // [kAhead][U][256] units, then what follows
+    float* shared = all_shared + kAhead * U * 256 * 4;
+    const int side = (int)blockIdx.x >= plan.blocks[0], block = side ? (int)blockIdx.x - plan.blocks[0] : (int)blockIdx.x;
+    const Side s = side ? a.s[1] : a.s[0];                   // (by selection: an index into the arguments is a load each time)
+    const int heads = s.heads, per = side ? plan.per[1] : plan.per[0], half_turn = a.turned / 2;
     float2* angles = reinterpret_cast<float2*>(shared);      // [2][per][turned / 2]
     float* sums = shared + 4 * per * half_turn;              // kBackwardEach: [heads][dim]
     const int tid = threadIdx.x, lane = tid & (plan.lanes - 1), group = tid / plan.lanes, groups = 256 / plan.lanes;
     const bool busy = lane < a.dim / (2 * N);
-    // the lane's two units of a head, and its first pair
-    const bool turns = busy && lane * N < half_turn;
-    const int rest = lane - half_turn / N;
-    const int u0 = !INTER && turns ? lane * N : !INTER ? a.turned + rest * 2 * N : lane * 2 * N;
-    const int u1 = !INTER && turns ? u0 + half_turn : u0 + N;
+    // the lane's two units of a head: partners, or, where pairs are neighbours or not turned at all, any two. Lanes side by
+    // side take units side by side: 32-byte sectors that two loads or stores take a half of each cost twice.
+    const bool partners = !INTER && busy && lane * N < half_turn;
+    const int rest = lane - half_turn / N, left = (a.dim - a.turned) / 2;
+    const int u0 = INTER || partners ? lane * N : a.turned + rest * N;
+    const int u1 = INTER ? u0 + a.dim / 2 : partners ? u0 + half_turn : u0 + left;
+    const bool turns0 = INTER ? busy && u0 < a.turned : partners, turns1 = INTER ? busy && u1 < a.turned : partners;
     // groups of one tick share its heads; with sums for each head there is one tick, so that a head stays with its group
     const int share = groups / per, j = group / share, first = group - j * share;
     const int total = (int)(a.batch * a.ticks), ticks = (int)a.ticks;
     const float inverse = 1.f / (float)a.dim;
-    float w0[N], w1[N], gw0[N], gw1[N];
+    uint64_t w0[P], w1[P], gw0[P], gw1[P];
 #pragma unroll
-    for (int k = 0; k < N; ++k) w0[k] = w1[k] = 1.f, gw0[k] = gw1[k] = 0.f;
+    for (int k = 0; k < P; ++k) w0[k] = w1[k] = two(1.f, 1.f), gw0[k] = gw1[k] = 0;
     auto weights = [&](int h) {
         const float4* w = reinterpret_cast<const float4*>(s.w + h * s.w_head);
 #pragma unroll
         for (int k = 0; k < N / 4; ++k) {
             const float4 f = __ldg(w + u0 / 4 + k), g = __ldg(w + u1 / 4 + k);
-            w0[4 * k] = f.x; w0[4 * k + 1] = f.y; w0[4 * k + 2] = f.z; w0[4 * k + 3] = f.w;
-            w1[4 * k] = g.x; w1[4 * k + 1] = g.y; w1[4 * k + 2] = g.z; w1[4 * k + 3] = g.w;
+            w0[2 * k] = two(f.x, f.y); w0[2 * k + 1] = two(f.z, f.w);
+            w1[2 * k] = two(g.x, g.y); w1[2 * k + 1] = two(g.z, g.w);
         }
     };
     if (NORM && s.w && !s.w_head && busy) weights(0);
@@ -293,133 +371,184 @@ __global__ void __launch_bounds__(256, MODE >= kBackwardW ? 2 : 3) k_rotate_unit
         for (int i = tid; i < heads * a.dim; i += 256) sums[i] = 0.f;
         __syncthreads();
     }
-    for (int tick0 = blockIdx.x * per, turn_no = 0; tick0 < total; tick0 += gridDim.x * per, ++turn_no) {
+    // the thread's first angle of the block's ticks, and how far on its next is
+    const int my_tick = half_turn ? tid / half_turn : 0, my_pair = tid - my_tick * half_turn;
+    const int more_ticks = half_turn ? 256 / half_turn : 0, more_pairs = 256 - more_ticks * half_turn;
+    const long long x_head = s.xs[2], gy_head = s.gys[2], to_head = MODE == kForward ? s.ys[2] : s.gxs[2];
+    constexpr uint32_t kSlot = U * 256 * 16;
+    const T *x_base = reinterpret_cast<const T*>(s.x), *gy_base = reinterpret_cast<const T*>(s.gy);
+    const uint32_t my_slot = (uint32_t)__cvta_generic_to_shared(all_shared) + tid * 16;
+    const int step = (side ? plan.blocks[1] : plan.blocks[0]) * per;
+    for (int tick0 = block * per, turn_no = 0; tick0 < total; tick0 += step, ++turn_no) {
         const int n = min(per, total - tick0);
         const bool there = busy && j < n;
-        const int mine = tick0 + (there ? j : 0), b = mine / ticks, t = mine - b * ticks;
-        const T* x_at = reinterpret_cast<const T*>(s.x) + b * s.xs[0] + t * s.xs[1];
-        const T* gy_at = reinterpret_cast<const T*>(s.gy) + b * s.gys[0] + t * s.gys[1];
-        T* to = MODE == kForward ? reinterpret_cast<T*>(s.y) + b * s.ys[0] + t * s.ys[1]
-                                 : reinterpret_cast<T*>(s.gx) + b * s.gxs[0] + t * s.gxs[1];
-        const long long to_head = MODE == kForward ? s.ys[2] : s.gxs[2];
-        uint4 next[4];
-        auto fetch = [&](int h) {
-            if (!there || h >= heads) return;
+        const int mine = tick0 + (there ? j : 0), b = divided(mine, ticks, plan.by_ticks), t = mine - b * ticks;
+        const T* x_at = reinterpret_cast<const T*>(s.x) + b * s.xs[0] + t * s.xs[1] + first * x_head;
+        const T* gy_at = reinterpret_cast<const T*>(s.gy) + b * s.gys[0] + t * s.gys[1] + first * gy_head;
+        T* to = MODE == kForward ? reinterpret_cast<T*>(s.y) + b * s.ys[0] + t * s.ys[1] + first * to_head
+                                 : reinterpret_cast<T*>(s.gx) + b * s.gxs[0] + t * s.gxs[1] + first * to_head;
+        const int mine_heads = there ? heads : 0;
+        int ask = first;                                      // the head that is asked for next, and its place
+        uint32_t ask_slot = my_slot;
+        auto fetch = [&]() {                                  // (zeros where there is none)
+            const bool some = ask < mine_heads;
             if (MODE == kForward || NORM) {
-                next[0] = *reinterpret_cast<const uint4*>(x_at + h * s.xs[2] + u0);
-                next[1] = *reinterpret_cast<const uint4*>(x_at + h * s.xs[2] + u1);
+                copy16(ask_slot, some ? x_at + u0 : x_base, some);
+                copy16(ask_slot + 256 * 16, some ? x_at + u1 : x_base, some);
             }
             if (MODE != kForward) {
-                next[2] = *reinterpret_cast<const uint4*>(gy_at + h * s.gys[2] + u0);
-                next[3] = *reinterpret_cast<const uint4*>(gy_at + h * s.gys[2] + u1);
+                copy16(ask_slot + (U - 2) * 256 * 16, some ? gy_at + u0 : gy_base, some);
+                copy16(ask_slot + (U - 1) * 256 * 16, some ? gy_at + u1 : gy_base, some);
             }
+            copies_end();
+            x_at += share * x_head;
+            gy_at += share * gy_head;
+            ask += share;
+            ask_slot = ask_slot == my_slot + (kAhead - 1) * kSlot ? my_slot : ask_slot + kSlot;
         };
-        fetch(first);                                         // (on its way while the angles are formed)
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; ++i) fetch();         // (on their way while the angles are formed)
         float2* here_angles = angles + (turn_no & 1) * per * half_turn;
-        for (int i = tid; i < n * half_turn; i += 256) {
-            const int q = i / half_turn, pair = i - q * half_turn, tick = tick0 + q, tb = tick / ticks;
+        for (int i = tid, at = my_tick, pair = my_pair; i < n * half_turn; i += 256) {
+            const int tick = tick0 + at, tb = divided(tick, ticks, plan.by_ticks);
             float2 cs;
             angle(a, position(a, tb, tick - tb * ticks), pair, cs.x, cs.y);
             here_angles[i] = cs;
+            at += more_ticks;
+            pair += more_pairs;
+            if (pair >= half_turn) pair -= half_turn, ++at;
         }
         __syncthreads();                                      // (two sets of angles: nobody is a whole turn ahead)
-        float c[N], sn[N];
-        if (turns && there) {
-            const float4* cs = reinterpret_cast<const float4*>(here_angles + j * half_turn + lane * N);
+        uint64_t c[P], sn[P], minus[P];                       // the lane's N angles (back: turned the other way)
 #pragma unroll
-            for (int k = 0; k < N / 2; ++k) {
-                const float4 f = cs[k];
-                c[2 * k] = f.x; sn[2 * k] = MODE == kForward ? f.y : -f.y;
-                c[2 * k + 1] = f.z; sn[2 * k + 1] = MODE == kForward ? f.w : -f.w;
+        for (int k = 0; k < P; ++k) c[k] = sn[k] = minus[k] = 0;   // (a group without a tick adds zeros to gw)
+        if (turns0 && there) {                                // (partners have one set, of N pairs; neighbours two of N / 2)
+            const float4* of0 = reinterpret_cast<const float4*>(here_angles + j * half_turn + (INTER ? u0 / 2 : u0));
+            const float4* of1 = reinterpret_cast<const float4*>(here_angles + j * half_turn + u1 / 2) - P / 2;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                if (INTER && k >= P / 2 && !turns1) break;
+                const float4 f = INTER && k >= P / 2 ? of1[k] : of0[k];
+                c[k] = two(f.x, f.z);
+                sn[k] = MODE == kForward ? two(f.y, f.w) : two(-f.y, -f.w);
+                minus[k] = MODE == kForward ? two(-f.y, -f.w) : two(f.y, f.w);
             }
         }
-        for (int h = first; h < (heads + share - 1) / share * share; h += share) {
-            const bool here = there && h < heads;
-            float p[N], q[N], x[N], y[N];
-#pragma unroll
-            for (int k = 0; k < N; ++k) p[k] = q[k] = x[k] = y[k] = 0.f;
-            if (here) {
-                if (MODE == kForward || NORM) {
-                    from_unit<T>(next[0], x);
-                    from_unit<T>(next[1], y);
-                }
-                if (MODE != kForward) {
-                    from_unit<T>(next[2], p);
-                    from_unit<T>(next[3], q);
-                }
-                fetch(h + share);
-                if (NORM && s.w && s.w_head) weights(h);
-                if (turns && MODE != kForward) turn<INTER, N>(p, q, c, sn);
+        auto turn = [&](uint64_t (&p)[P], uint64_t (&q)[P]) {
+            if (INTER) {
+                if (turns0) turn_neighbours<0, P>(p, c, sn);
+                if (turns1) turn_neighbours<1, P>(q, c, sn);
+            } else if (partners) {
+                turn_apart<P>(p, q, c, sn, minus);
             }
+        };
+        int slot = 0;
+        for (int h = first; h < (heads + share - 1) / share * share; h += share) {
+            fetch();                                          // (into the slot of the head before, which is used up)
+            copies_wait<kAhead - 1>();
+            const uint4* got = reinterpret_cast<const uint4*>(all_shared) + tid + slot;
+            slot = slot == (kAhead - 1) * U * 256 ? 0 : slot + U * 256;
+            const bool here = h < mine_heads;
+            uint64_t p[P], q[P], x[P], y[P];
+            if (MODE == kForward || NORM) {
+                from_unit<T>(got[0], x);
+                from_unit<T>(got[256], y);
+            }
+            if (MODE != kForward) {
+                from_unit<T>(got[(U - 2) * 256], p);
+                from_unit<T>(got[(U - 1) * 256], q);
+                turn(p, q);
+            }
+            if (NORM && s.w && s.w_head && here) weights(h);
             if (NORM) {
-                float sq = 0.f, m = 0.f;
+                uint64_t sq2 = 0, m2 = 0;
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    sq = fmaf(x[k], x[k], fmaf(y[k], y[k], sq));
-                    if (MODE != kForward) m = fmaf(p[k] * w0[k], x[k], fmaf(q[k] * w1[k], y[k], m));
+                for (int k = 0; k < P; ++k) {
+                    sq2 = fma2(x[k], x[k], fma2(y[k], y[k], sq2));
+                    if (MODE != kForward) {
+                        m2 = fma2(mul2(p[k], w0[k]), x[k], fma2(mul2(q[k], w1[k]), y[k], m2));
+                    }
                 }
-                for (int o = plan.lanes >> 1; o; o >>= 1) {
+                float sq = sum2(sq2), m = MODE != kForward ? sum2(m2) : 0.f;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    if (o >= plan.lanes) break;
                     sq += __shfl_xor_sync(0xffffffffu, sq, o);
                     if (MODE != kForward) m += __shfl_xor_sync(0xffffffffu, m, o);
                 }
                 const float norm = rsqrtf(fmaf(sq, inverse, a.eps));
+                const uint64_t norm2 = two(norm, norm);
                 if (MODE == kForward) {
 #pragma unroll
-                    for (int k = 0; k < N; ++k) x[k] *= norm * w0[k], y[k] *= norm * w1[k];
+                    for (int k = 0; k < P; ++k) {
+                        x[k] = mul2(x[k], mul2(norm2, w0[k]));
+                        y[k] = mul2(y[k], mul2(norm2, w1[k]));
+                    }
                 } else {
-                    const float mean = m * norm * norm * inverse;
+                    // gx = norm (g w - x norm^2 mean(g w x))
+                    const float mean = -m * norm * norm * inverse;
+                    const uint64_t mean2 = two(mean, mean);
 #pragma unroll
-                    for (int k = 0; k < N; ++k) {
+                    for (int k = 0; k < P; ++k) {
                         if (MODE == kBackwardW) {
-                            gw0[k] = fmaf(p[k], x[k] * norm, gw0[k]);
-                            gw1[k] = fmaf(q[k], y[k] * norm, gw1[k]);
+                            gw0[k] = fma2(p[k], mul2(x[k], norm2), gw0[k]);
+                            gw1[k] = fma2(q[k], mul2(y[k], norm2), gw1[k]);
                         }
                         if (MODE == kBackwardEach && here) {
-                            sums[h * a.dim + u0 + k] += p[k] * (x[k] * norm);
-                            sums[h * a.dim + u1 + k] += q[k] * (y[k] * norm);
+                            float2* at0 = reinterpret_cast<float2*>(sums + h * a.dim + u0 + 2 * k);
+                            float2* at1 = reinterpret_cast<float2*>(sums + h * a.dim + u1 + 2 * k);
+                            float f, g;
+                            halves(fma2(p[k], mul2(x[k], norm2), two(at0->x, at0->y)), f, g);
+                            *at0 = make_float2(f, g);
+                            halves(fma2(q[k], mul2(y[k], norm2), two(at1->x, at1->y)), f, g);
+                            *at1 = make_float2(f, g);
                         }
-                        p[k] = norm * (p[k] * w0[k] - x[k] * mean);
-                        q[k] = norm * (q[k] * w1[k] - y[k] * mean);
+                        p[k] = mul2(norm2, fma2(x[k], mean2, mul2(p[k], w0[k])));
+                        q[k] = mul2(norm2, fma2(y[k], mean2, mul2(q[k], w1[k])));
                     }
                 }
             }
             if (!here) continue;
             if (MODE == kForward) {
-                if (turns) turn<INTER, N>(x, y, c, sn);
-                store_unit(to + h * to_head + u0, x);
-                store_unit(to + h * to_head + u1, y);
+                turn(x, y);
+                store_unit(to + u0, x);
+                store_unit(to + u1, y);
             } else {
-                store_unit(to + h * to_head + u0, p);
-                store_unit(to + h * to_head + u1, q);
+                store_unit(to + u0, p);
+                store_unit(to + u1, q);
             }
+            to += share * to_head;
         }
     }
     if (MODE == kBackwardW) {
-        // the groups' sums in turn: part [block][side][dim]
+        // the groups' sums in turn: part [block][dim], the queries' blocks first
         float* all = shared;                                  // [groups][dim]
         __syncthreads();
         if (busy) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                all[group * a.dim + u0 + k] = gw0[k];
-                all[group * a.dim + u1 + k] = gw1[k];
+            for (int k = 0; k < P; ++k) {
+                float f, g;
+                halves(gw0[k], f, g);
+                *reinterpret_cast<float2*>(all + group * a.dim + u0 + 2 * k) = make_float2(f, g);
+                halves(gw1[k], f, g);
+                *reinterpret_cast<float2*>(all + group * a.dim + u1 + 2 * k) = make_float2(f, g);
             }
         }
         __syncthreads();
         for (int i = tid; i < a.dim; i += 256) {
             float sum = 0.f;
             for (int g = 0; g < groups; ++g) sum += all[g * a.dim + i];
-            part[((long long)blockIdx.x * 2 + blockIdx.y) * a.dim + i] = sum;
+            part[(long long)blockIdx.x * a.dim + i] = sum;
         }
     }
-    if (MODE == kBackwardEach) {                              // part [block][queries' heads, keys' heads][dim]
+    if (MODE == kBackwardEach) {                              // part [block][heads][dim], the queries' blocks first
         __syncthreads();
-        float* to = part + ((long long)blockIdx.x * (a.s[0].heads + a.s[1].heads) + (blockIdx.y ? a.s[0].heads : 0)) * a.dim;
+        float* to = part + ((long long)block * heads + (side ? (long long)plan.blocks[0] * a.s[0].heads : 0)) * a.dim;
         for (int i = tid; i < heads * a.dim; i += 256) to[i] = sums[i];
     }
 }
 
-constexpr int kSplits = 148 * 2;                             // blocks with sums of their own, at most
+constexpr int kSplits = 148 * 4;                             // blocks with sums of their own, at most
 
 void strides(long long (&to)[3], const fg_ticks& t) {
     to[0] = t.batch;
@@ -435,7 +564,7 @@ Rotate checked(const fg_rotate_args* g, bool backward) {
          "fg_norm_rotate: turned must be even and at most dim");
     need(!g->turned || g->turns, "fg_norm_rotate: turned values need turns");
     need(!g->positions || g->pos_bytes == 4 || g->pos_bytes == 8, "fg_norm_rotate: positions are of 4 or 8 bytes");
-    need(!g->norm || g->eps > 0, "fg_norm_rotate: eps must be positive");
+    need(!g->norm || (float)g->eps > 0, "fg_norm_rotate: eps must be positive");
     need(g->type >= FG_F32 && g->type <= FG_F16, "fg_norm_rotate: unknown type");
     Rotate a{};
     for (int i = 0; i < 2; ++i) {
@@ -478,8 +607,8 @@ long long sets_of(const fg_rotate_args* g, int i) { return g->w_head[i] ? g->hea
 
 long long work_bytes(const fg_rotate_args* g) {
     if (!g->norm || (!g->gw[0] && !g->gw[1])) return 0;
-    const long long sets = std::max<long long>(2, g->w_head[0] || g->w_head[1] ? g->heads[0] + g->heads[1] : 2);
-    const long long blocks = std::max<long long>(1, std::min<long long>(kSplits, g->batch * g->ticks));
+    const long long sets = std::max<long long>(1, std::max(g->w_head[0] ? g->heads[0] : 1, g->w_head[1] ? g->heads[1] : 1));
+    const long long blocks = std::min<long long>(kSplits, 2 * g->batch * g->ticks) + 2;
     return (rows_of(g) + 3) / 4 * 16 + sets * g->dim * blocks * 4;
 }
 
@@ -503,35 +632,37 @@ bool has_units(const Rotate& a, int size, bool backward) {
     return true;
 }
 template <class T, bool INTER, bool NORM, int MODE>
-void launch_units(const Rotate& a, float* part, int& blocks, cudaStream_t st) {
+void launch_units(const Rotate& a, float* part, UnitPlan& plan, cudaStream_t st) {
     const int items = a.dim / (2 * Unit<T>::n), half = a.turned / 2, total = (int)(a.batch * a.ticks);
-    UnitPlan plan{{1, 1}, 1};
+    const int rows = a.s[0].heads + a.s[1].heads;
+    plan = UnitPlan{{1, 1}, {0, 0}, 1, (uint32_t)(((1ull << 32) + a.ticks - 1) / a.ticks)};
     while (plan.lanes < items) plan.lanes *= 2;
-    const int groups = 256 / plan.lanes;
+    const int groups = 256 / plan.lanes, most = MODE >= kBackwardW ? kSplits : 148 * 12;
     size_t bytes = 0;
-    blocks = 1;
     for (int i = 0; i < 2; ++i) {
         const int heads = a.s[i].heads;
-        // as many ticks as leave a group a head or two of one, unless there are too few to go round
-        int per = 1;
-        while (MODE != kBackwardEach && per < kTicksMost && per * 2 <= groups && groups / per > std::max(1, heads / 2)) per *= 2;
-        while (per > 1 && (total + per - 1) / per < 148 * 4) per /= 2;
+        if (!heads) continue;
+        // a group takes a tick's heads one after another, unless the ticks are too few to give each SM two blocks: what a
+        // tick costs by itself (its place, its angles) is spread over its heads. With the sizes above 2 blocks an SM take
+        // 41 and 74 us, 8 take 57 and 87; 2,048 angles twice are 32 KB of an SM's shared memory a block.
+        int per = MODE == kBackwardEach ? 1 : groups;
+        while (per > 1 && ((total + per - 1) / per < 148 * 2 || (size_t)per * half > 2048)) per /= 2;
         plan.per[i] = per;
         bytes = std::max(bytes, (size_t)per * half * 16 + (MODE == kBackwardEach ? (size_t)heads * a.dim * 4 : 0));
-        if (heads) blocks = std::max(blocks, (total + per - 1) / per);
+        plan.blocks[i] = std::max(1, std::min((total + per - 1) / per, (int)((long long)most * heads / rows)));
     }
     if (MODE == kBackwardW) bytes = std::max(bytes, (size_t)groups * a.dim * 4);
+    bytes += kAhead * kUnits<NORM, MODE> * 256 * 16;
     auto* k = k_rotate_units<T, INTER, NORM, MODE>;
     if (bytes > 48 * 1024) MCK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    blocks = std::min(blocks, MODE >= kBackwardW ? kSplits : 148 * 32);
-    k<<<dim3(blocks, a.s[1].heads ? 2 : 1), 256, bytes, st>>>(a, plan, part);
+    k<<<plan.blocks[0] + plan.blocks[1], 256, bytes, st>>>(a, plan, part);
     MCK(cudaGetLastError());
 }
 template <class T, int MODE>
-void launch_units(const Rotate& a, float* part, int& blocks, cudaStream_t st) {
+void launch_units(const Rotate& a, float* part, UnitPlan& plan, cudaStream_t st) {
     constexpr bool with_norm = MODE >= kBackwardW;            // (sums of gw are the norm's)
-    if (a.norm) a.interleaved ? launch_units<T, true, true, MODE>(a, part, blocks, st) : launch_units<T, false, true, MODE>(a, part, blocks, st);
-    else if constexpr (!with_norm) a.interleaved ? launch_units<T, true, false, MODE>(a, part, blocks, st) : launch_units<T, false, false, MODE>(a, part, blocks, st);
+    if (a.norm) a.interleaved ? launch_units<T, true, true, MODE>(a, part, plan, st) : launch_units<T, false, true, MODE>(a, part, plan, st);
+    else if constexpr (!with_norm) a.interleaved ? launch_units<T, true, false, MODE>(a, part, plan, st) : launch_units<T, false, false, MODE>(a, part, plan, st);
 }
 
 }  // namespace
@@ -546,8 +677,8 @@ int fg_norm_rotate(const fg_rotate_args* g, void* stream) {
         by_type(g->type, [&](auto t) {
             using T = decltype(t);
             cudaStream_t st = static_cast<cudaStream_t>(stream);
-            int blocks = 0;
-            if (has_units(a, sizeof(T), false)) launch_units<T, kForward>(a, nullptr, blocks, st);
+            UnitPlan plan;
+            if (has_units(a, sizeof(T), false)) launch_units<T, kForward>(a, nullptr, plan, st);
             else k_rotate_any<T><<<blocks_for(rows), 32 * kWarps, 0, st>>>(a, rows);
         });
         MCK(cudaGetLastError());
@@ -578,16 +709,20 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
             const bool all_each = (!a.s[0].gw || !a.s[0].heads || g->w_head[0]) && (!a.s[1].gw || !a.s[1].heads || g->w_head[1]);
             const bool fits = !each || (all_each && (g->heads[0] + g->heads[1]) * g->dim * 4 <= 64 * 1024);
             if (rows && has_units(a, sizeof(T), true) && (!norms || fits)) {
-                int blocks = 0;
-                if (!norms) launch_units<T, kBackward>(a, nullptr, blocks, st);
-                else if (each) launch_units<T, kBackwardEach>(a, part, blocks, st);
-                else launch_units<T, kBackwardW>(a, part, blocks, st);
+                UnitPlan plan;
+                if (!norms) launch_units<T, kBackward>(a, nullptr, plan, st);
+                else if (each) launch_units<T, kBackwardEach>(a, part, plan, st);
+                else launch_units<T, kBackwardW>(a, part, plan, st);
                 if (norms) {
-                    const int n[2] = {(int)sets_of(g, 0) * a.dim, (int)sets_of(g, 1) * a.dim};
-                    const int stride = each ? (a.s[0].heads + a.s[1].heads) * a.dim : 2 * a.dim;
-                    k_rotate_gw_sum<<<(stride + 31) / 32, 1024, 0, st>>>(part, a.s[0].heads ? a.s[0].gw : nullptr, n[0],
-                                                                         a.s[1].heads ? a.s[1].gw : nullptr,
-                                                                         each ? a.s[0].heads * a.dim : a.dim, n[1], stride, blocks);
+                    SumSide sums[2];
+                    for (int i = 0; i < 2; ++i) {
+                        const int n = (int)(each ? g->heads[i] : 1) * a.dim;
+                        sums[i] = {i ? sums[0].part + (long long)plan.blocks[0] * sums[0].n : part, a.s[i].gw, n, plan.blocks[i]};
+                    }
+                    const int n0 = a.s[0].gw && a.s[0].heads ? sums[0].n : 0, n1 = a.s[1].gw && a.s[1].heads ? sums[1].n : 0;
+                    sums[0].n = n0;
+                    sums[1].n = n1;
+                    k_rotate_gw_sum<<<dim3((std::max(n0, n1) + 31) / 32, 2), 1024, 0, st>>>(sums[0], sums[1]);
                     MCK(cudaGetLastError());
                 }
                 return;
@@ -601,7 +736,7 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
                 const int splits = (int)std::max<long long>(1, std::min<long long>(256, g->batch * g->ticks));
                 const dim3 grid((a.dim + 127) / 128, sets, splits);
                 k_rotate_gw_any<T><<<grid, 128, 0, st>>>(a, i, norms, part, sets, splits);
-                k_rotate_gw_sum<<<(n + 31) / 32, 1024, 0, st>>>(part, a.s[i].gw, n, nullptr, 0, 0, n, splits);
+                k_rotate_gw_sum<<<dim3((n + 31) / 32, 1), 1024, 0, st>>>(SumSide{part, a.s[i].gw, n, splits}, SumSide{});
                 MCK(cudaGetLastError());
             }
         });
