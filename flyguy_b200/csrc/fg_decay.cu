@@ -28,6 +28,7 @@ struct Operand {
 struct Scan {
     Operand a, b, c, out;
     int out_f32;             // out is fp32 (a partial result per query head)
+    int beside;              // may run beside the launch before it: it reads nothing that one writes, and writes nothing that one touches
     const float* log_decay;
     const float* first;      // the state before the scan's first tick, or NULL
     float* last;             // the state after its last, or NULL
@@ -171,23 +172,41 @@ __global__ void __launch_bounds__(32 * kRecWarps) k_decay_rec(const __grid_const
     }
 }
 
-// out[tick][key head][:] = the fp32 results of the query heads that share it, added in order
-template <class T>
-__global__ void k_share_sum(const float* __restrict__ in, Operand out, long long batch, long long ticks, int heads,
-                            int key_heads, int dim) {
-    const int share = heads / key_heads;
-    const long long n = batch * ticks * key_heads * dim;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const int d = (int)(i % dim);
-        const long long row = i / dim;
-        const int h = (int)(row % key_heads);
-        const long long tick = row / key_heads;
-        const float* p = in + (tick * heads + (long long)h * share) * dim + d;
-        float s = 0.f;
-        for (int k = 0; k < share; ++k) s += p[(long long)k * dim];
-        const long long b = tick / ticks;
-        reinterpret_cast<T*>(out.p)[b * out.batch + (tick - b * ticks) * out.tick + h * out.head + d] = from_f<T>(s);
+// out[tick][key head][:] = the fp32 results of the query heads that share it, added in order; V values a thread
+template <class T, int V, class Index>
+__global__ void __launch_bounds__(256) k_share_sum(const float* __restrict__ in, Operand out, Index ticks, int heads,
+                                                   int key_heads, int dim, Index units) {
+    const int share = heads / key_heads, of_row = dim / V;
+    using Load = std::conditional_t<V == 4, float4, float>;
+    for (Index i = blockIdx.x * (Index)blockDim.x + threadIdx.x; i < units; i += gridDim.x * (Index)blockDim.x) {
+        const Index row = i / of_row;
+        const int d = (int)(i - row * of_row) * V;
+        const Index tick = row / key_heads, b = tick / ticks;
+        const int h = (int)(row - tick * key_heads);
+        const float* p = in + ((long long)tick * heads + h * share) * dim + d;
+        float s[V] = {};
+#pragma unroll 4
+        for (int k = 0; k < share; ++k) {
+            const Load v = *reinterpret_cast<const Load*>(p + (long long)k * dim);
+            const float* x = reinterpret_cast<const float*>(&v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] += x[j];
+        }
+        T* to = reinterpret_cast<T*>(out.p) + (long long)b * out.batch + (long long)(tick - b * ticks) * out.tick + h * out.head + d;
+#pragma unroll
+        for (int j = 0; j < V; ++j) to[j] = from_f<T>(s[j]);
     }
+}
+template <class T>
+void share_sum(const float* in, const Operand& out, long long batch, long long ticks, int heads, int key_heads, int dim, cudaStream_t st) {
+    const bool four = dim % 4 == 0;                          // (`in` is the workspace's: aligned)
+    const long long units = batch * ticks * key_heads * dim / (four ? 4 : 1);
+    const unsigned blocks = (unsigned)std::min<long long>((units + 255) / 256, 148 * 32);
+    const bool small = units < (1ll << 31) - 148 * 32 * 256;  // 32-bit divisions: a third of the time
+    if (small && four) k_share_sum<T, 4, uint32_t><<<blocks, 256, 0, st>>>(in, out, (uint32_t)ticks, heads, key_heads, dim, (uint32_t)units);
+    else if (small) k_share_sum<T, 1, uint32_t><<<blocks, 256, 0, st>>>(in, out, (uint32_t)ticks, heads, key_heads, dim, (uint32_t)units);
+    else k_share_sum<T, 1, long long><<<blocks, 256, 0, st>>>(in, out, ticks, heads, key_heads, dim, batch * ticks * key_heads * dim);
+    MCK(cudaGetLastError());
 }
 
 // A single tick: a block per (row, head). A warp takes every 8th row of the state, its lanes the columns; state in and
@@ -335,9 +354,10 @@ long long partial_floats(const fg_decay_args* g) {
 }
 long long all_ticks(const fg_decay_args* g) { return g->offsets ? g->ticks : g->batch * g->ticks; }
 long long work_floats(const fg_decay_args* g, bool backward) {
-    long long n = partial_floats(g);
-    if (backward && g->heads != g->key_heads) n += all_ticks(g) * g->heads * std::max(g->dim, g->value_dim);
-    return (n + 3) / 4 * 4;
+    const auto whole = [](long long n) { return (n + 3) / 4 * 4; };   // (each part begins at 16 bytes)
+    long long n = whole(partial_floats(g));
+    if (backward && g->heads != g->key_heads) n += whole(all_ticks(g) * g->heads * g->dim) + whole(all_ticks(g) * g->heads * g->value_dim);
+    return n;
 }
 
 void check(const fg_decay_args* g, bool backward) {
@@ -408,7 +428,8 @@ int fg_decay_attn_bwd(const fg_decay_args* g, void* stream) {
         if (!g->batch) return 0;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         const long long share = g->heads / g->key_heads;
-        float* wide = static_cast<float*>(g->work) + (partial_floats(g) + 3) / 4 * 4;
+        float* for_gv = static_cast<float*>(g->work) + (partial_floats(g) + 3) / 4 * 4;
+        float* for_gk = for_gv + (all_ticks(g) * g->heads * g->value_dim + 3) / 4 * 4;
         by_type(g->type, [&](auto t) {
             using T = decltype(t);
             Scan s = scan_of(g);
@@ -421,19 +442,15 @@ int fg_decay_attn_bwd(const fg_decay_args* g, void* stream) {
             s.first_t = 1;
             launch<T>(s, st);
             // the gradients of shared heads: per query head in fp32, then added
-            auto shared = [&](Scan x, const fg_ticks& to, long long dim) {
-                x.out = operand(to, 1);
-                if (share > 1) {
-                    x.out = {reinterpret_cast<char*>(wide), g->ticks * g->heads * dim, g->heads * dim, dim, 1};
-                    x.out_f32 = 1;
-                }
+            auto shared = [&](Scan x, const fg_ticks& to, long long dim, float* wide) {
+                x.out = share > 1 ? Operand{reinterpret_cast<char*>(wide), g->ticks * g->heads * dim, g->heads * dim, dim, 1} : operand(to, 1);
+                x.out_f32 = share > 1;
+                x.beside = 1;
                 launch<T>(x, st);
-                if (share > 1 && all_ticks(g)) {
-                    const long long n = all_ticks(g) * g->key_heads * dim;
-                    k_share_sum<T><<<(unsigned)std::min<long long>((n + 255) / 256, 148 * 32), 256, 0, st>>>(
-                        wide, operand(to, 1), g->offsets ? 1 : g->batch, g->ticks, (int)g->heads, (int)g->key_heads, (int)dim);
-                    MCK(cudaGetLastError());
-                }
+            };
+            auto add = [&](const fg_ticks& to, long long dim, const float* wide) {
+                if (share > 1 && all_ticks(g))
+                    share_sum<T>(wide, operand(to, 1), g->offsets ? 1 : g->batch, g->ticks, (int)g->heads, (int)g->key_heads, (int)dim, st);
             };
             s = scan_of(g);                                   // gv = scan'(k, q, go)
             s.backward = 1;
@@ -443,13 +460,15 @@ int fg_decay_attn_bwd(const fg_decay_args* g, void* stream) {
             s.c = operand(g->go, 1);
             s.first = g->gstate_out;
             s.last = g->gstate;
-            shared(s, g->gv, g->value_dim);
+            shared(s, g->gv, g->value_dim, for_gv);
             std::swap(s.D, s.E);                              // gk = scan'(v, go, q), its states transposed
             s.a = operand(g->v, share);
             std::swap(s.b, s.c);
             s.first_t = 1;
             s.last = nullptr;
-            shared(s, g->gk, g->dim);
+            shared(s, g->gk, g->dim, for_gk);
+            add(g->gv, g->value_dim, for_gv);
+            add(g->gk, g->dim, for_gk);
         });
         return 0;
     });

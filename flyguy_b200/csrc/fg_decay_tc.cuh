@@ -161,10 +161,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = s.D, E = s.E;
     const int h = blockIdx.x % s.heads, part = blockIdx.y, b = blockIdx.x / s.heads;
+    const bool last_block = s.beside && blockIdx.x == gridDim.x - 1;
     const Span sp = span_of(s, b);
     const long long per = part_ticks(sp.n, s.parts), t0 = min(sp.n, part * per), t1 = min(sp.n, t0 + per);
     const bool hand_on = !PARTS && s.last && (sp.n ? t1 == sp.n && t1 > t0 : part == 0);
-    if (t1 == t0 && !hand_on && !PARTS) return;
+    // the next launch, where it may run beside this one, begins as soon as all of this one's blocks have
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (t1 == t0 && !hand_on && !PARTS && !last_block) return;
     const int total = (int)(t1 - t0), chunks = (total + kTcTicks - 1) / kTcTicks;
     const float ld = s.log_decay[h];
 
@@ -544,7 +547,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
         }
 #pragma unroll 1
         for (int i = 0; i < chunks && ok; ++i) {
-            // S as the operand of O1: rows d, columns e, swizzled (rows past D: zeros, for the k-steps of 16 up to DP)
+            // S as the operand of O1: rows d, columns e, swizzled (rows past D: zeros, for the k-steps of 16 up to DP), once
+            // O1 of the chunk before is done with it (at 128, kQs is waited for below)
+            if (!PARTS && L::own_terms && i) ok = together(wait(kQs, i - 1));
+            if (!ok) break;
             if (!PARTS && row < DP) {
                 unsigned char* at = smem + L::state + row * 128;
 #pragma unroll
@@ -603,6 +609,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
+    // what follows this launch follows the one before it, too
+    if (last_block) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
@@ -653,8 +661,22 @@ void tc_launch_as(const Scan& s, cudaStream_t st) {
     const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E), tile_map(s, s.out, s.E, F32)};
     const unsigned rows = (unsigned)(s.batch * s.heads);
     if (s.parts > 1) k_decay_tc<DP, EP, BACK, false, true><<<dim3(rows, s.parts - 1), kTcThreads, bytes, st>>>(s, maps);
-    k_decay_tc<DP, EP, BACK, F32, false><<<dim3(rows, s.parts), kTcThreads, bytes, st>>>(s, maps);
-    MCK(cudaGetLastError());
+    // Beside the launch before it: its blocks take the SMs that the other's last ones leave free, 512 blocks on 148 SMs
+    // being 3.5 rounds (64 recordings of 1,024 ticks, 8 heads of 128, forward and the three scans back: 698 -> 631 us). With
+    // parts that launch is theirs, and their states are read here.
+    Scan now = s;
+    now.beside = s.beside && s.parts == 1;
+    cudaLaunchAttribute beside{};
+    beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    beside.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t how{};
+    how.gridDim = dim3(rows, s.parts);
+    how.blockDim = dim3(kTcThreads);
+    how.dynamicSmemBytes = bytes;
+    how.stream = st;
+    how.attrs = &beside;
+    how.numAttrs = now.beside ? 1 : 0;
+    MCK(cudaLaunchKernelEx(&how, k_decay_tc<DP, EP, BACK, F32, false>, now, maps));
 }
 template <bool BACK, bool F32>
 void tc_launch_dims(const Scan& s, cudaStream_t st) {
