@@ -53,6 +53,29 @@ __device__ __forceinline__ Span span_of(const Scan& s, long long b) {
 // no room for its last digits in fp32 (off by 1e-4 over the 3,000 ticks that it remembers), gamma - 1 has.
 __device__ __forceinline__ float power(float log_decay, float n) { return n > 0.f ? expf(log_decay * n) : 1.f; }
 
+// Scans that need nothing of one another overlap: a launch that may run beside the one before it begins once all of that
+// one's blocks have begun, and takes the SMs that its last blocks leave free. 512 blocks on 148 SMs are 3.5 rounds: 64
+// recordings of 1,024 ticks, 8 heads of 128 in bf16, forward and the three scans back take 631 us, in turn 698. What follows
+// must follow both, so one block of the later launch ends after the earlier one has. (With parts the launch before is the
+// parts', whose states are read.)
+__device__ __forceinline__ void next_may_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... Rest>
+void launch_beside(void (*kernel)(Scan, Rest...), dim3 grid, int threads, int bytes, cudaStream_t st, Scan s, const Rest&... rest) {
+    s.beside = s.beside && s.parts == 1;
+    cudaLaunchAttribute beside{};
+    beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    beside.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t how{};
+    how.gridDim = grid;
+    how.blockDim = dim3(threads);
+    how.dynamicSmemBytes = bytes;
+    how.stream = st;
+    how.attrs = &beside;
+    how.numAttrs = s.beside ? 1 : 0;
+    MCK(cudaLaunchKernelEx(&how, kernel, s, rest...));
+}
+
 // ticks of a recording in one part: whole blocks of kAlign
 constexpr int kAlign = 128;
 __device__ __forceinline__ long long part_ticks(long long n, int parts) {
@@ -67,7 +90,10 @@ namespace {
 
 // The recurrence itself, in fp32, for any type, size and stride: a block of 8 warps owns 32 columns of one head's
 // state; lane = column, warp w holds rows w R .. w R + R - 1 in registers. 16 ticks of a and b are staged in shared
-// memory as fp32 and read as broadcasts; the warps' shares of out meet in shared memory once per 16 ticks.
+// memory as fp32 and read as broadcasts; the warps' shares of out meet in shared memory once per 16 ticks. It is what runs
+// for a dim or value_dim over 128, where neither of the other kernels has room for the state. Bound by the multiply-adds,
+// two a value of S and tick on the fp32 units, and the barriers between 16 ticks: 32 recordings of 509 ticks, 8 heads of 64 in
+// fp32 with gradients take 2,825 us here and 379 as products of chunks (bf16, 64 of 1,024, 8 heads of 128: 49,100 and 706).
 constexpr int kRecTicks = 16, kRecWarps = 8, kRecCols = 32;
 constexpr int kRecRows = kMaxDim / kRecWarps;
 
@@ -172,7 +198,8 @@ __global__ void __launch_bounds__(32 * kRecWarps) k_decay_rec(const __grid_const
     }
 }
 
-// out[tick][key head][:] = the fp32 results of the query heads that share it, added in order; V values a thread
+// out[tick][key head][:] = the fp32 results of the query heads that share it, added in order; V values a thread. Bound by
+// the memory: 97,500 ticks, 8 heads of 64 to 2 take 35 us, 6.1 TB/s (a value a thread with 64-bit divisions: 99 us).
 template <class T, int V, class Index>
 __global__ void __launch_bounds__(256) k_share_sum(const float* __restrict__ in, Operand out, Index ticks, int heads,
                                                    int key_heads, int dim, Index units) {
@@ -210,7 +237,7 @@ void share_sum(const float* in, const Operand& out, long long batch, long long t
 }
 
 // A single tick: a block per (row, head). A warp takes every 8th row of the state, its lanes the columns; state in and
-// out are the whole cost.
+// out are the whole cost. For value_dims that are no multiple of 4 (2,048 rows, 8 heads of 128 x 128: 744 us, below 333).
 template <class T>
 __global__ void __launch_bounds__(256) k_decay_step(Operand q, Operand k, Operand v, Operand out,
                                                     const float* __restrict__ log_decay, float* __restrict__ state,
@@ -252,7 +279,9 @@ __global__ void __launch_bounds__(256) k_decay_step(Operand q, Operand k, Operan
 }
 
 // The same with value_dim a multiple of 4 and 16-byte aligned: a thread owns 4 columns of every R-th row, and asks for 8 rows
-// before it uses the first: state in and out is all there is to a tick, 16 bytes a load.
+// before it uses the first: state in and out is all there is to a tick, 16 bytes a load. 2,048 rows, 8 heads of 128 x 128:
+// 333 us, 6.5 TB/s, 99% of a plain copy's rate. One tick of 8 rows is one wait for the memory; the call costs 14 us, most of
+// it on the host.
 template <class T>
 __global__ void __launch_bounds__(256, 3) k_decay_step4(Operand q, Operand k, Operand v, Operand out,
                                                         const float* __restrict__ log_decay, float* __restrict__ state,
@@ -338,7 +367,8 @@ void check_sizes(const Sizes& z, const char* who) {
 
 // Parts a recording. A part costs its b and c read twice, so: as many as keep the blocks within one round of the SMs (the
 // tcgen05 kernel takes a SM to itself, two blocks of the mma.sync kernel share one), of at least four chunks. The
-// recurrence's blocks are slow and share a SM: more of them.
+// recurrence's blocks are slow and share a SM: more of them. (1 recording of 65,536 ticks, 8 heads of 128 in bf16: 287 us in 18
+// parts a head; unsplit, 512 chunks of 4.7 us follow one another.)
 int parts_of(const fg_decay_args* g) {
     const long long rows = std::max<long long>(1, g->batch * g->heads);
     const long long mean = g->offsets ? g->ticks / std::max<long long>(1, g->batch) : g->ticks;
@@ -370,6 +400,8 @@ void check(const fg_decay_args* g, bool backward) {
     need(!used || (g->q.p && g->k.p && g->v.p && (backward ? g->go.p && g->gq.p && g->gk.p && g->gv.p : g->o.p != nullptr)),
          "fg_decay_attn: null pointer");
     need(backward || !g->state || g->state != g->state_out, "fg_decay_attn: state and state_out are the same");
+    need(!backward || !g->gstate || (g->gstate != g->state && g->gstate != g->gstate_out),
+         "fg_decay_attn_bwd: gstate is state or gstate_out");
     const long long bytes = work_floats(g, backward) * 4;
     need(!bytes || (g->work && g->work_bytes >= bytes), "fg_decay_attn: the workspace is too small");
     need(reinterpret_cast<uintptr_t>(g->work) % 16 == 0, "fg_decay_attn: the workspace is not 16-byte aligned");
@@ -391,6 +423,8 @@ Scan scan_of(const fg_decay_args* g) {
     return s;
 }
 
+// By what fits: bf16 tiles that TMA takes go to the tcgen05 kernel, other types and strides up to 128 to mma.sync (fp32
+// needs its terms; 64 recordings of 1,024 ticks, 8 heads of 128 with gradients: 706 us and, in fp16, 5.4 ms), the rest to the recurrence.
 template <class T>
 void launch(const Scan& s, cudaStream_t st) {
     if (std::is_same<T, __nv_bfloat16>::value && tc_fits(s)) return tc_launch(s, st);

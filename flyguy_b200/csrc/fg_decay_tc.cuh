@@ -21,6 +21,13 @@
 // blocks of columns), 8-15 the state (S, b to b'), 16 and 18 the MMAs, 17 and 19 the copies in and
 // out. The roles meet at mbarriers only, so a
 // chunk's elementwise work runs beside its MMAs and the next chunk's copies.
+//
+// 64 recordings of 1,024 ticks, 8 heads of 128, forward: 185 us (403 MB in, 137 MB out; at the rate of a plain copy 82 us), 8
+// chunks of 4.7 us a block and some 8 us around them, four rounds of blocks. What bounds it is the chain from one state to the
+// next: S copied, O1, b' made (b is read and three terms written, 128 KB of shared memory at 128), 24 MMAs of dS (64 clocks
+// each, for both operands come from shared memory), S read back. The tensor pipe is 26% busy, DRAM 36%, issue slots 31%. At dim
+// 64 b' is made while O1 runs: 97,500 ticks, 8 heads, 180 us (250 MB). Blocks that took over one recording after another
+// instead of ending (with the next one's first tiles on their way) lost more a chunk than they saved: forward and back 713 us, 698 without.
 #pragma once
 #include <cuda.h>
 
@@ -165,8 +172,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     const Span sp = span_of(s, b);
     const long long per = part_ticks(sp.n, s.parts), t0 = min(sp.n, part * per), t1 = min(sp.n, t0 + per);
     const bool hand_on = !PARTS && s.last && (sp.n ? t1 == sp.n && t1 > t0 : part == 0);
-    // the next launch, where it may run beside this one, begins as soon as all of this one's blocks have
-    asm volatile("griddepcontrol.launch_dependents;");
+    next_may_begin();
     if (t1 == t0 && !hand_on && !PARTS && !last_block) return;
     const int total = (int)(t1 - t0), chunks = (total + kTcTicks - 1) / kTcTicks;
     const float ld = s.log_decay[h];
@@ -609,8 +615,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
-    // what follows this launch follows the one before it, too
-    if (last_block) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (last_block) wait_for_previous();
     if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
@@ -661,22 +666,7 @@ void tc_launch_as(const Scan& s, cudaStream_t st) {
     const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E), tile_map(s, s.out, s.E, F32)};
     const unsigned rows = (unsigned)(s.batch * s.heads);
     if (s.parts > 1) k_decay_tc<DP, EP, BACK, false, true><<<dim3(rows, s.parts - 1), kTcThreads, bytes, st>>>(s, maps);
-    // Beside the launch before it: its blocks take the SMs that the other's last ones leave free, 512 blocks on 148 SMs
-    // being 3.5 rounds (64 recordings of 1,024 ticks, 8 heads of 128, forward and the three scans back: 698 -> 631 us). With
-    // parts that launch is theirs, and their states are read here.
-    Scan now = s;
-    now.beside = s.beside && s.parts == 1;
-    cudaLaunchAttribute beside{};
-    beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    beside.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t how{};
-    how.gridDim = dim3(rows, s.parts);
-    how.blockDim = dim3(kTcThreads);
-    how.dynamicSmemBytes = bytes;
-    how.stream = st;
-    how.attrs = &beside;
-    how.numAttrs = now.beside ? 1 : 0;
-    MCK(cudaLaunchKernelEx(&how, k_decay_tc<DP, EP, BACK, F32, false>, now, maps));
+    launch_beside(k_decay_tc<DP, EP, BACK, F32, false>, dim3(rows, s.parts), kTcThreads, bytes, st, s, maps);
 }
 template <bool BACK, bool F32>
 void tc_launch_dims(const Scan& s, cudaStream_t st) {

@@ -258,7 +258,7 @@ typedef struct fg_decay_args {
     const float* state;               /* [batch, heads, dim, value_dim] before the first tick, or NULL: zeros */
     float* state_out;                 /* after the last tick (may not overlap state) */
     const float* gstate_out;          /* backward: gradient of state_out, or NULL: zeros */
-    float* gstate;                    /* backward: gradient of state, or NULL: not wanted */
+    float* gstate;                    /* backward: gradient of state, or NULL: not wanted; neither state nor gstate_out */
     const long long* offsets;         /* [batch + 1] first ticks of recordings packed end to end, or NULL: all of `ticks` */
     long long batch, ticks;           /* with offsets: ticks of all recordings together */
     long long heads, key_heads, dim, value_dim, type;
