@@ -621,10 +621,10 @@ unsigned blocks_for(long long rows) {
 bool aligned(const void* p, const long long (&st)[3], long long unit) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st[0] % unit == 0 && st[1] % unit == 0 && st[2] % unit == 0;
 }
-// whether rows are whole pairs of 16-byte units
+// whether rows are whole pairs of 16-byte units, each turned as a whole or not at all, partners in units of their own
 bool has_units(const Rotate& a, int size, bool backward) {
     const int unit = 16 / size;
-    if (a.dim % (2 * unit) || a.turned % (2 * unit) || a.dim / (2 * unit) > 32 || a.batch * a.ticks >= (1ll << 30)) return false;
+    if (a.dim % (2 * unit) || a.turned % (a.interleaved ? unit : 2 * unit) || a.dim / (2 * unit) > 32 || a.batch * a.ticks >= (1ll << 30)) return false;
     for (const Side& s : a.s) {
         if (!s.heads) continue;
         if ((!backward || a.norm) && !aligned(s.x, s.xs, unit)) return false;

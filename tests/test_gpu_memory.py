@@ -129,6 +129,20 @@ def test_norm_rotate(shape, layout, each, typ, cuda):
     assert not grads[:, :, H + K:].any()
 
 
+# heads of whole 16-byte units: lanes without one, part of a head turned, groups of lanes without a tick, ticks that go round
+# the blocks several times
+UNITS = [(2, 3, 5, 96, 48), (1, 1, 3, 80, 40), (3, 33, 4, 160, 160), (2, 301, 3, 48, 16), (1, 5, 2, 512, 96), (1, 8000, 1, 512, 512),
+         (7, 1, 2, 16, 16), (1, 129, 1, 224, 0)]
+
+
+@pytest.mark.parametrize("typ", TYPES, ids=names)
+@pytest.mark.parametrize("each", [False, True], ids=["one", "each"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", UNITS)
+def test_norm_rotate_in_units(shape, layout, each, typ, cuda):
+    test_norm_rotate(shape, layout, each, typ, cuda)
+
+
 def test_norm_rotate_plain_forms(cuda):
     """Without turns, weights or positions; packed ticks; a transposed input; the batch's positions from one row."""
     g = _gen(3)
@@ -181,6 +195,17 @@ def test_norm_rotate_gradient_against_differences(cuda):
         plus[i], minus[i] = ins[i] + step * d, ins[i] - step * d
         slope = (loss(*plus) - loss(*minus)).item() / (2 * step.item())
         assert abs(slope - t.grad.norm().item()) <= 1e-3 * t.grad.norm().item(), i
+
+
+def test_infinities_stay_in_what_is_turned(cuda):
+    """An infinite value turns its partner into infinity or not-a-number, and nothing else: not the values left alone."""
+    for layout, partner in (("half", 24), ("interleaved", 9)):
+        x = _rand(_gen(5), 1, 3, 2, 128, typ=torch.bfloat16)
+        x[0, 1, 0, 8] = x[0, 1, 0, 100] = float("inf")
+        y = memory.rotate(x, memory.rotary_turns(32, device="cuda"), layout=layout).float()
+        bad = ~torch.isfinite(y)
+        assert bad[0, 1, 0, 100] and bad[0, 1, 0, 8] and bad[0, 1, 0, partner]
+        assert bad.sum().item() == 3, layout
 
 
 # ---- attention whose state decays ----------------------------------------------------------------------------------

@@ -67,6 +67,30 @@ def test_argument_errors_are_statuses():
     assert L.fg_norm_rotate(memory._ROTATE.pack(*rot), None) == -1 and "turns" in L.fg_mem_last_error().decode()
 
 
+def test_outputs_that_inputs_still_need_are_refused():
+    """gstate is written while another of the gradients' scans still reads the states; an eps that is 0 in fp32 is none."""
+    L = native.lib()
+    for other in (33, 35):                                                   # state, gstate_out
+        fields = [0] * 32 + [0] * 6 + [0, 0, 4, 4, 64, 64, 0] + [1.0, 0, 0]
+        fields[32], fields[36], fields[other] = 16, 256, 256
+        assert L.fg_decay_attn_bwd(memory._DECAY.pack(*fields), None) == -1
+        assert "gstate" in L.fg_mem_last_error().decode()
+    rot = [0] * 32 + [0] * 6 + [1, 0] + [0, 0, 64, 0, 0, 0, 0, 0, 8, 0, 0, 1] + [1e-60, 1.0, 0, 0]
+    assert L.fg_norm_rotate(memory._ROTATE.pack(*rot), None) == -1 and "eps" in L.fg_mem_last_error().decode()
+
+
+def test_the_workspace_holds_its_parts():
+    """Heads' states of 9 floats in parts, then the shared heads' results: each begins at 16 bytes and all of it fits."""
+    L = native.lib()
+    sizes = [1, 4096, 2, 1, 3, 3, 0]                                         # few long recordings are split
+    pack = lambda heads, keys: memory._DECAY.pack(*[0] * 38, *sizes[:2], heads, keys, *sizes[4:], 1.0, 0, 0)  # noqa: E731
+    for heads in (1, 2, 3, 5):
+        states = L.fg_decay_work(pack(heads, heads), 1)
+        assert states > 0 and states % 16 == 0
+        one = -(-4096 * heads * 3 * 4 // 16) * 16
+        assert L.fg_decay_work(pack(heads, 1), 1) == states + (2 * one if heads > 1 else 0)
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(1, 2, 2, 8)
     for fn, args in ((memory.rotate, (x, memory.rotary_turns(8))), (memory.norm_rotate, (x, x)),
