@@ -521,6 +521,9 @@ __global__ void __launch_bounds__(256, MODE != kForward && NORM ? 2 : 3) k_rotat
             }
             to += share * to_head;
         }
+        // what was asked for past the last head (zeros) lands before the next ticks' copies go to the same places: copies are
+        // in no order among themselves
+        copies_wait<0>();
     }
     if (MODE == kBackwardW) {
         // the groups' sums in turn: part [block][dim], the queries' blocks first

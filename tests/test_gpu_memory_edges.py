@@ -1,0 +1,65 @@
+"""The memory-over-ticks operators (flyguy_b200.memory) at their edges: what a caller may pass that the operators' own cases do
+not reach. Tolerances as in test_gpu_memory.py: 2^-8 of the norm for bfloat16, 5e-6 for float32."""
+import numpy as np
+import pytest
+import torch
+
+from flyguy_b200 import memory
+
+pytestmark = pytest.mark.gpu
+TOL = {torch.float32: 5e-6, torch.bfloat16: 4e-3, torch.float16: 5e-4}
+
+
+def _rand(g, *shape, typ=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(typ).cuda()
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _off(got, want):
+    """||got - want|| / ||want||"""
+    return ((got.double() - want).norm() / want.norm().clamp(min=1e-30)).item()
+
+
+def _turn64(x, turns, positions, layout="half", sign=1):
+    """x [B, T, H, D] in float64, its first pairs turned."""
+    n = len(turns)
+    part = (positions.unsqueeze(-1) * turns) >> 32
+    unit = torch.polar(torch.ones_like(part, dtype=torch.float64), sign * part.double() * (2 * np.pi / 2.0 ** 32)).unsqueeze(2)
+    a, b = (x[..., :n], x[..., n:2 * n]) if layout == "half" else (x[..., 0:2 * n:2], x[..., 1:2 * n:2])
+    z = torch.complex(a, b) * unit
+    y = x.clone()
+    if layout == "half":
+        y[..., :n], y[..., n:2 * n] = z.real, z.imag
+    else:
+        y[..., 0:2 * n:2], y[..., 1:2 * n:2] = z.real, z.imag
+    return y
+
+
+@pytest.mark.parametrize("typ", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", [(1, 20011, 1, 128), (3, 7001, 2, 256), (1, 16384, 5, 64)])
+def test_heads_of_ticks_that_a_block_takes_in_turn(shape, layout, typ, cuda):
+    """Few heads and many ticks: a block goes from one set of ticks to the next with copies of the set before still asked for.
+    Every head of every tick, the last ones of a set and the first of the next among them."""
+    B, T, H, D = shape
+    g = _gen(1)
+    x, gy = _rand(g, B, T, H, D, typ=typ), _rand(g, B, T, H, D, typ=typ)
+    w = (1 + 0.2 * _rand(g, H, D)).requires_grad_()
+    turns = memory.rotary_turns(D, device="cuda")
+    positions = torch.arange(T, device="cuda").expand(B, T)
+    q = x.clone().requires_grad_()
+    y, _ = memory.norm_rotate(q, x[:, :, :0], turns, w, None, positions, layout, eps=1e-3)
+    y.backward(gy)
+    x64 = x.double()
+    r = (x64.square().mean(-1, keepdim=True) + 1e-3).rsqrt()
+    back = _turn64(gy.double(), turns, positions, layout, -1)
+    gw = back * w.detach().double()
+    want = _turn64(x64 * r * w.detach().double(), turns, positions, layout)
+    want_x = r * (gw - x64 * r * (gw * x64 * r).mean(-1, keepdim=True))
+    for got, ref in ((y, want), (q.grad, want_x)):
+        rows = (got.double() - ref).norm(dim=-1) / ref.norm(dim=-1)
+        assert rows.max().item() <= 2 * TOL[typ]
+    assert _off(w.grad, (back * x64 * r).sum((0, 1))) <= TOL[torch.float32]
