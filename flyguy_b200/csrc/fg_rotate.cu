@@ -610,9 +610,23 @@ Rotate checked(const fg_rotate_args* g, bool backward) {
 long long rows_of(const fg_rotate_args* g) { return g->batch * g->ticks * (g->heads[0] + g->heads[1]); }
 long long sets_of(const fg_rotate_args* g, int i) { return g->w_head[i] ? g->heads[i] : 1; }
 
+// Whether heads have weights of their own, and whether k_rotate_units forms their sums: those of one set of weights for some
+// heads and sets of their own for others go the general way.
+bool each_head(const fg_rotate_args* g) { return g->w_head[0] || g->w_head[1]; }
+bool sums_of_each(const fg_rotate_args* g) {
+    for (int i = 0; i < 2; ++i)
+        if (g->gw[i] && g->heads[i] && !g->w_head[i]) return false;
+    return each_head(g) && (g->heads[0] + g->heads[1]) * g->dim * 4 <= 64 * 1024;
+}
+
+// The rows' norms, then every block's sums. In sums_of_each calls a block leaves sums for each head of its side, also of a
+// side whose weights are shared, frozen or absent.
 long long work_bytes(const fg_rotate_args* g) {
     if (!g->norm || (!g->gw[0] && !g->gw[1])) return 0;
-    const long long sets = std::max<long long>(1, std::max(g->w_head[0] ? g->heads[0] : 1, g->w_head[1] ? g->heads[1] : 1));
+    const bool all = sums_of_each(g);
+    long long sets = 1;
+    for (int i = 0; i < 2; ++i)
+        if (all || (g->gw[i] && g->w_head[i])) sets = std::max(sets, g->heads[i]);
     const long long blocks = std::min<long long>(kSplits, 2 * g->batch * g->ticks) + 2;
     return (rows_of(g) + 3) / 4 * 16 + sets * g->dim * blocks * 4;
 }
@@ -709,10 +723,7 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
         by_type(g->type, [&](auto t) {
             using T = decltype(t);
             float* part = norms ? norms + (rows + 3) / 4 * 4 : nullptr;
-            // (the sums of one set of weights for some heads and sets of their own for others go the general way)
-            const bool each = g->w_head[0] || g->w_head[1];
-            const bool all_each = (!a.s[0].gw || !a.s[0].heads || g->w_head[0]) && (!a.s[1].gw || !a.s[1].heads || g->w_head[1]);
-            const bool fits = !each || (all_each && (g->heads[0] + g->heads[1]) * g->dim * 4 <= 64 * 1024);
+            const bool each = each_head(g), fits = !each || sums_of_each(g);
             if (rows && has_units(a, sizeof(T), true) && (!norms || fits)) {
                 UnitPlan plan;
                 if (!norms) launch_units<T, kBackward>(a, nullptr, plan, st);

@@ -63,3 +63,46 @@ def test_heads_of_ticks_that_a_block_takes_in_turn(shape, layout, typ, cuda):
         rows = (got.double() - ref).norm(dim=-1) / ref.norm(dim=-1)
         assert rows.max().item() <= 2 * TOL[typ]
     assert _off(w.grad, (back * x64 * r).sum((0, 1))) <= TOL[torch.float32]
+
+
+@pytest.mark.parametrize("each_of", ["keys", "queries"])
+@pytest.mark.parametrize("other", ["none", "frozen", "frozen each"])
+@pytest.mark.parametrize("size", [(2, 8, 16, 4, 128), (3, 300, 2, 8, 64), (4, 200, 8, 2, 96)])
+def test_weights_of_each_head_beside_weights_that_do_not_learn(size, other, each_of, cuda, monkeypatch):
+    """One side learns a weight for each head, the other has none, or one that is held: the gradients, and not a byte behind
+    the workspace."""
+    B, T, H, K, D = size
+    guard, rooms = 1 << 22, []
+
+    def room(n, device):
+        if not n:
+            return None, (0, 0)
+        t = torch.full((n + guard,), 0xa5, dtype=torch.uint8, device=device)
+        rooms.append((t, n))
+        return t, (t.data_ptr(), n)
+
+    monkeypatch.setattr(memory, "_room", room)
+    g = _gen(2)
+    ins = [_rand(g, B, T, h, D, typ=torch.bfloat16).requires_grad_() for h in (H, K)]
+    outs = [_rand(g, B, T, h, D, typ=torch.bfloat16) for h in (H, K)]
+    learns = 1 if each_of == "keys" else 0
+    w = [None, None]
+    w[learns] = (1 + 0.2 * _rand(g, (H, K)[learns], D)).requires_grad_()
+    if other != "none":
+        w[1 - learns] = 1 + 0.2 * _rand(g, *(((H, K)[1 - learns], D) if other == "frozen each" else (D,)))
+    turns = memory.rotary_turns(D, device="cuda")
+    y = memory.norm_rotate(*ins, turns, *w, eps=1e-3)
+    got = torch.autograd.grad(y, [*ins, w[learns]], outs)
+    positions = torch.arange(T, device="cuda").expand(B, T)
+    for i in range(2):
+        x, w64 = ins[i].detach().double(), 1.0 if w[i] is None else w[i].detach().double()
+        r = (x.square().mean(-1, keepdim=True) + 1e-3).rsqrt()
+        back = _turn64(outs[i].double(), turns, positions, sign=-1)
+        gw = back * w64
+        assert _off(y[i].detach(), _turn64(x * r * w64, turns, positions)) <= TOL[torch.bfloat16]
+        assert _off(got[i], r * (gw - x * r * (gw * x * r).mean(-1, keepdim=True))) <= TOL[torch.bfloat16]
+        if i == learns:
+            assert _off(got[2], (back * x * r).sum((0, 1))) <= TOL[torch.float32]
+    assert len(rooms) == 1
+    for t, n in rooms:
+        assert (t[n:] == 0xa5).all()
