@@ -149,7 +149,9 @@ struct TcLayout {
     static constexpr uint32_t bytes = bars + 8 * 16 + 16;
     static_assert(own_terms || DP * EP * 2 <= kTcTicks * DP * 2, "the copy of S fits the third term's place");
 };
-enum { kFull0, kFull1, kQk, kQs, kPv, kKv, kOutStored, kWReady, kBReady, kSReady, kOutRead, kOutReady, kBars };
+// A wait tells odd phases from even ones only, so no phase may end before all that wait for the one before have seen it. kFull, kPv,
+// kKv and kOutLeft are one barrier a stage: their next phase needs the copies into the stage, which come after those waits.
+enum { kFull0, kFull1, kQk, kQs, kPv0, kPv1, kKv0, kKv1, kOutStored, kOutLeft0, kOutLeft1, kWReady, kBReady, kSReady, kOutRead, kOutReady, kBars };
 static_assert(kBars <= 16, "room for the barriers");
 
 // BACK: from the last tick to the first; F32: out in fp32; PARTS: the states of the parts alone
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     auto first_of = [&](int i) { return BACK ? begin - i * kTcTicks - ticks_of(i) : begin + i * kTcTicks; };
     const int batch = s.offsets ? 0 : b;
     auto wait = [&](int i, int chunk) { return tc_wait(bar(i), (uint32_t)chunk & 1, gave_up); };
-    auto wait_full = [&](int i) { return tc_wait(bar(kFull0 + (i & 1)), (i >> 1) & 1, gave_up); };
+    auto wait_stage = [&](int first, int chunk) { return tc_wait(bar(first + (chunk & 1)), (chunk >> 1) & 1, gave_up); };
+    auto wait_full = [&](int i) { return wait_stage(kFull0, i); };
     auto together = [&](bool ok) {                           // a warp goes on, or not, as one
         ok = __all_sync(0xffffffffu, ok);
         fg::tc_fence_after();
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     // when b' may be made: b is no longer A's operand, the terms' places are free, and the tile has arrived (TMA's writes are
     // seen through its own barrier)
     auto b_free = [&](int i) {
-        return (PARTS || wait(L::own_terms ? kQk : kQs, i)) && (i == 0 || wait(kKv, i - 1)) && wait_full(i);
+        return (PARTS || wait(L::own_terms ? kQk : kQs, i)) && (i == 0 || wait_stage(kKv0, i - 1)) && wait_full(i);
     };
     // where a chunk of out is put together, and how many columns at a time
     auto out_at = [&](int i) { return L::own_out ? L::out : (i & 1) * L::stage + L::c; };
@@ -267,14 +270,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             // is put together over c, is stored
             const int da = (D + 63) / 64, ec = (E + 63) / 64;
             const int head_a = h / s.a.share, head_b = h / s.b.share, head_c = h / s.c.share;
-            int copied = 0, stored = 0;
+            int copied = 0;
 #pragma unroll 1
             for (int i = 0; i < chunks && ok; ++i) {
                 const uint32_t stage = sm + (i & 1) * L::stage, full = bar(kFull0 + (i & 1));
                 const int tick = first_of(i);
-                if (i >= 2) ok = wait(kKv, i - 2) && (PARTS || wait(kPv, i - 2));
-                if (i >= 2 && !PARTS && !L::own_out)         // (every phase in turn: a wait tells odd from even only)
-                    for (int e0 = 0; e0 < E; e0 += kRound) ok = ok && wait(kOutStored, stored++);
+                if (i >= 2)
+                    ok = wait_stage(kKv0, i - 2) && (PARTS || (wait_stage(kPv0, i - 2) && (L::own_out || wait_stage(kOutLeft0, i - 2))));
                 if (!ok) break;
                 fg::mbar_expect_tx(full, (uint32_t)((PARTS ? 1 : 2) * da + ec) * kBox);
 #pragma unroll 1
@@ -299,7 +301,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             for (int i = 0; i < chunks && ok; ++i) {
                 const uint32_t stage = sm + (i & 1) * L::stage;
                 const uint64_t a_ticks = swizzled(stage + L::a, 0), b_ticks = swizzled(stage + L::b, 0), c_rows = swizzled(stage + L::c, kBox);
-                ok = wait_full(i) && (i == 0 || wait(kPv, i - 1));   // W is read
+                // W of the chunk before is read; and b' of it made, so that those who make it have seen its A
+                ok = wait_full(i) && (i == 0 || (wait_stage(kPv0, i - 1) && (!L::own_terms || wait(kBReady, i - 1))));
                 if (!ok) break;
                 fg::tc_fence_after();
 #pragma unroll
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 fg::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < kTcTicks / 16; ++k) mma_bf16_tmem(tmem + tO2, tmem + tA + k * 16, c_rows + 128 * k, id_o, k > 0);
-                fg::mma_commit(bar(kPv));
+                fg::mma_commit(bar(kPv0 + (i & 1)));
             }
         } else if (warp == 19 && lane == 0 && !PARTS) {
             // out of whole chunks, round by round
@@ -336,6 +339,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                     stores_read();
                     fg::mbar_arrive(bar(kOutStored));
                 }
+                if (!L::own_out && ok) fg::mbar_arrive(bar(kOutLeft0 + (i & 1)));
             }
             asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         } else if (warp == 18 && lane == 0) {
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 for (int k = 0; k < 8; ++k) mma_bf16(tmem + tS, second + 128 * k, c_rows + 128 * k, id_s, true);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) mma_bf16(tmem + tS, third + 128 * k, c_rows + 128 * k, id_s, true);
-                fg::mma_commit(bar(kKv));
+                fg::mma_commit(bar(kKv0 + (i & 1)));
             }
         }
     } else if (warp < 8) {
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             fg::tc_fence_before();
             arrive(kWReady);
-            ok = together(wait(kQs, i) && wait(kPv, i));
+            ok = together(wait(kQs, i) && wait_stage(kPv0, i));
             if (!ok) break;
             // out of whole chunks is put together in shared memory and stored as tiles (a thread's own stores, 32 lines at a
             // time, held up the MMAs' operands); a recording's last ticks go by themselves: what follows them is another's
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 #pragma unroll 1
                 for (int e0 = 0; e0 < E && ok; e0 += kRound, ++round) {
                     // the place is free: over c, once dS is done with it; the round before is stored
-                    ok = together((L::own_out || e0 || wait(kKv, i)) && (!round || wait(kOutStored, round - 1)));
+                    ok = together((L::own_out || e0 || wait_stage(kKv0, i)) && (!round || wait(kOutStored, round - 1)));
                     if (!ok) break;
 #pragma unroll 1
                     for (int e = half * 16; e < min(E - e0, kRound); e += 32) {
@@ -501,7 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
                 }
                 fg::tc_fence_before();
                 arrive(kOutRead);
-                ok = together(wait(kKv, i));
+                ok = together(wait_stage(kKv0, i) && (!i || wait(kOutStored, i - 1)));   // (a round a chunk)
                 if (!ok) break;
 #pragma unroll
                 for (int j = 0; j < EP / 32; ++j)
@@ -577,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
             ok = together(b_free(i));
             if (!ok) break;
             fade_b(i, n, tid - 256);
-            ok = together(wait(kKv, i));
+            ok = together(wait_stage(kKv0, i));
             if (!ok) break;
             const float fade = pw[n - 1 + (i ? 1 : lead0)];
 #pragma unroll
