@@ -525,18 +525,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 #pragma unroll
             for (int i = 0; i < 16; ++i) S[j][i] = 0.f;
         const long long state0 = ((long long)b * s.heads + h) * D * E;
-        // S += f * the state at p, which may lie [E][D]
+        // S += f * the state at p, which may lie [E][D] or, a caller's, begin at any float: then value by value
         auto add = [&](const float* p, float f, bool across) {
+            const bool single = across || reinterpret_cast<uintptr_t>(p) % 16;
+            const int step = across ? D : 1;
 #pragma unroll
             for (int j = 0; j < EP / 32; ++j) {
                 const int e0 = (2 * j + half) * 16;
                 if (!mine || e0 >= E) continue;
-                if (across) {
-                    const float* q = p + (long long)e0 * D + row;
+                const float* at = p + (across ? e0 * D + row : row * E + e0);
+                if (single) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i, q += D) S[j][i] = fmaf(f, *q, S[j][i]);
+                    for (int i = 0; i < 16; ++i, at += step) S[j][i] = fmaf(f, *at, S[j][i]);
                 } else {
-                    const float4* q = reinterpret_cast<const float4*>(p + row * E + e0);
+                    const float4* q = reinterpret_cast<const float4*>(at);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float4 v = q[i];

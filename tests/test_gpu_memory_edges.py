@@ -106,3 +106,30 @@ def test_weights_of_each_head_beside_weights_that_do_not_learn(size, other, each
     assert len(rooms) == 1
     for t, n in rooms:
         assert (t[n:] == 0xa5).all()
+
+
+def _at_float(t, offset):
+    """t's values in a contiguous view that begins `offset` floats after a 16-byte boundary."""
+    return torch.empty(t.numel() + offset, dtype=t.dtype, device=t.device)[offset:].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("typ", [torch.float32, torch.bfloat16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("dims", [(2, 1, 64, 64), (2, 2, 128, 128), (1, 1, 96, 80)])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_states_that_begin_at_any_float(offset, dims, typ, cuda):
+    """States, and gradients of states, cut from a longer buffer: the bits of aligned ones. One recording is long enough to be
+    split, so that its parts begin from such a state too."""
+    H, K, D, E = dims
+    for T in (70, 1500):
+        g = _gen(3)
+        ins = [_rand(g, 1, T, h, n, typ=typ).requires_grad_() for h, n in ((H, D), (K, D), (K, E))]
+        state, go, gend = _rand(g, 1, H, D, E), _rand(g, 1, T, H, E, typ=typ), _rand(g, 1, H, D, E, scale=0.3)
+        ld = torch.log1p(-torch.exp2(-4.0 - torch.arange(H, device="cuda")))
+        runs = []
+        for move in (lambda t: t, lambda t: _at_float(t, offset)):
+            s = move(state).requires_grad_()
+            assert s.data_ptr() % 16 == (0 if not runs else 4 * offset)
+            o, end = memory.decay_attention(*ins, ld, s)
+            runs.append((o, end, *torch.autograd.grad((o, end), (*ins, s), (go, move(gend)))))
+        for a, b in zip(*runs):
+            assert torch.equal(a, b)
