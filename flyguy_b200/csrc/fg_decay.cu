@@ -236,6 +236,54 @@ void share_sum(const float* in, const Operand& out, long long batch, long long t
     MCK(cudaGetLastError());
 }
 
+// Zeros for the ticks that no recording covers, before the first and after the last (a packed buffer with room to spare): the
+// scans write recordings only, and what reads these outputs, the gradient of a projection's weights say, sums over all ticks.
+// Rows of `units` pieces of U of each head; up to three outputs, one a grid row.
+struct Outside {
+    struct {
+        char* p;
+        long long tick, head;        // strides in pieces
+        int heads, units;
+    } out[3];
+    const long long* offsets;
+    long long batch, ticks;
+};
+template <class U>
+__global__ void __launch_bounds__(256) k_clear_outside(const __grid_constant__ Outside a) {
+    const auto& o = a.out[blockIdx.y];
+    const long long lo = min(max(a.offsets[0], 0ll), a.ticks), hi = min(max(a.offsets[a.batch], lo), a.ticks);
+    const long long row = (long long)o.heads * o.units, n = (lo + a.ticks - hi) * row;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        const long long t = i / row;
+        const int r = (int)(i - t * row), h = r / o.units;
+        reinterpret_cast<U*>(o.p)[(t < lo ? t : hi + t - lo) * o.tick + h * o.head + r - h * o.units] = U{};
+    }
+}
+// `n` outputs of heads[i] x dims[i] values of `size` bytes
+void clear_outside(const fg_decay_args* g, const fg_ticks* const (&to)[3], const long long (&heads)[3], const long long (&dims)[3], int n, int size,
+                   cudaStream_t st) {
+    if (!g->offsets || !g->ticks) return;
+    bool wide = true;                                        // pieces of 16 bytes
+    for (int i = 0; i < n; ++i) {
+        if (!to[i]->p) return;                               // (no recordings, and no outputs)
+        wide = wide && reinterpret_cast<uintptr_t>(to[i]->p) % 16 == 0 && to[i]->tick * size % 16 == 0 && to[i]->head * size % 16 == 0 &&
+               dims[i] * size % 16 == 0;
+    }
+    const int piece = wide ? 16 : size, values = piece / size;
+    Outside a{};
+    long long most = 1;
+    for (int i = 0; i < n; ++i) {
+        a.out[i] = {static_cast<char*>(to[i]->p), to[i]->tick / values, to[i]->head / values, (int)heads[i], (int)(dims[i] / values)};
+        most = std::max(most, g->ticks * heads[i] * (dims[i] / values));
+    }
+    a.offsets = g->offsets;
+    a.batch = g->batch;
+    a.ticks = g->ticks;
+    auto* kernel = piece == 16 ? k_clear_outside<uint4> : piece == 4 ? k_clear_outside<uint32_t> : k_clear_outside<uint16_t>;
+    kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 4), n), 256, 0, st>>>(a);
+    MCK(cudaGetLastError());
+}
+
 // A single tick: a block per (row, head). A warp takes every 8th row of the state, its lanes the columns; state in and
 // out are the whole cost. For value_dims that are no multiple of 4 (2,048 rows, 8 heads of 128 x 128: 744 us, below 333).
 template <class T>
@@ -442,6 +490,7 @@ extern "C" {
 int fg_decay_attn(const fg_decay_args* g, void* stream) {
     return (int)mem_guard([&]() -> long long {
         check(g, false);
+        clear_outside(g, {&g->o}, {g->heads}, {g->value_dim}, 1, g->type == FG_F32 ? 4 : 2, static_cast<cudaStream_t>(stream));
         if (!g->batch) return 0;
         const long long share = g->heads / g->key_heads;
         Scan s = scan_of(g);
@@ -459,8 +508,15 @@ int fg_decay_attn(const fg_decay_args* g, void* stream) {
 int fg_decay_attn_bwd(const fg_decay_args* g, void* stream) {
     return (int)mem_guard([&]() -> long long {
         check(g, true);
-        if (!g->batch) return 0;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const auto clear = [&] {                              // (last: sums of shared heads go over all ticks)
+            clear_outside(g, {&g->gq, &g->gk, &g->gv}, {g->heads, g->key_heads, g->key_heads}, {g->dim, g->dim, g->value_dim}, 3,
+                          g->type == FG_F32 ? 4 : 2, st);
+        };
+        if (!g->batch) {
+            clear();
+            return 0;
+        }
         const long long share = g->heads / g->key_heads;
         float* for_gv = static_cast<float*>(g->work) + (partial_floats(g) + 3) / 4 * 4;
         float* for_gk = for_gv + (all_ticks(g) * g->heads * g->value_dim + 3) / 4 * 4;
@@ -504,6 +560,7 @@ int fg_decay_attn_bwd(const fg_decay_args* g, void* stream) {
             add(g->gv, g->value_dim, for_gv);
             add(g->gk, g->dim, for_gk);
         });
+        clear();
         return 0;
     });
 }

@@ -351,9 +351,10 @@ def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,
     """S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t for every recording and head.
 
     q [batch, ticks, heads, dim], k [.., key heads, dim], v [.., key heads, value dim], each key head serving heads / key
-    heads query heads; or [ticks, ..] with recordings packed end to end and offsets int64 [recordings + 1] (recordings may
-    be empty). log_decay float32 [heads], at most 0, a constant. state float32 [recordings, heads, dim, value dim] before
-    the first ticks (None: zeros). scale: dim^-0.5 when None. dim and value dim at most 256.
+    heads query heads; or [ticks, ..] with recordings packed end to end and offsets int64 [recordings + 1], not falling
+    (recordings may be empty; ticks before the first and after the last get zeros, in o and in the gradients). log_decay
+    float32 [heads], at most 0, a constant. state float32 [recordings, heads, dim, value dim] before the first ticks (None:
+    zeros). scale: dim^-0.5 when None. dim and value dim at most 256.
     Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v and state."""
     q = _values("q", q, (3, 4))
     k, v = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)

@@ -133,3 +133,32 @@ def test_states_that_begin_at_any_float(offset, dims, typ, cuda):
             runs.append((o, end, *torch.autograd.grad((o, end), (*ins, s), (go, move(gend)))))
         for a, b in zip(*runs):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("typ", [torch.float32, torch.bfloat16, torch.float16], ids=["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("dims", [(4, 2, 64, 64), (2, 2, 128, 128), (3, 1, 20, 7), (2, 1, 200, 130)])
+@pytest.mark.parametrize("offsets", [[40, 170, 170, 300], [0, 130, 260], [7, 400], [400, 400], [0], [0, 0]])
+def test_ticks_of_no_recording_are_zero(offsets, dims, typ, cuda):
+    """A packed buffer of 400 ticks with room before and behind its recordings, NaN in what is there: zeros in the output and in
+    the gradients, and the recordings' own as if packed without it. (What was in the outputs' memory before is made NaN, too.)"""
+    H, K, D, E = dims
+    n, N = 400, len(offsets) - 1
+    g = _gen(4)
+    ins = [_rand(g, n, h, d, typ=typ) for h, d in ((H, D), (K, D), (K, E))]
+    state, go, gend = _rand(g, N, H, D, E), _rand(g, n, H, E, typ=typ), _rand(g, N, H, D, E, scale=0.3)
+    a, z = offsets[0], offsets[-1]
+    for t in (*ins, go):
+        t[:a] = t[z:] = float("nan")
+    ld = torch.log1p(-torch.exp2(-4.0 - torch.arange(H, device="cuda")))
+
+    def run(parts, off):
+        torch.full((1 << 24,), float("nan"), device="cuda")                 # (freed at once: what the outputs may be made from)
+        leaves = [t.clone().requires_grad_() for t in (*parts[:3], state)]
+        o, end = memory.decay_attention(*leaves[:3], ld, leaves[3], offsets=torch.tensor(off, device="cuda"))
+        return (o, end), torch.autograd.grad((o, end), leaves, (parts[3], gend))
+
+    (o, end), grads = run((*ins, go), offsets)
+    (o1, end1), grads1 = run([t[a:z] for t in (*ins, go)], [x - a for x in offsets])
+    for got, want in ((o, o1), *zip(grads[:3], grads1[:3])):
+        assert torch.equal(got[a:z], want) and not got[:a].any() and not got[z:].any()
+    assert torch.equal(end, end1) and torch.equal(grads[3], grads1[3])
