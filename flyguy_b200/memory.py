@@ -90,6 +90,13 @@ def _room(size: int, device) -> tuple[torch.Tensor | None, tuple[int, int]]:
     return t, (t.data_ptr(), size)
 
 
+def _offsets(t, like: torch.Tensor) -> torch.Tensor:
+    """The first ticks of recordings packed end to end, as the library takes them."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int64 or t.get_device() != like.get_device() or t.dim() != 1 or not t.numel():
+        raise FlyguyError(f"offsets must be an int64 vector [recordings + 1] on {like.device}")
+    return t.contiguous()
+
+
 def _grad(name: str, g, like: torch.Tensor, shape=None) -> torch.Tensor:
     """An incoming gradient as the library takes it (None: zeros)."""
     if g is None:
@@ -294,10 +301,7 @@ class _Decay:
         else:
             if len(lead) != 1:
                 raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
-            if (not isinstance(offsets, torch.Tensor) or offsets.dtype is not torch.int64 or offsets.get_device() != q.get_device()
-                    or offsets.dim() != 1 or not offsets.numel()):
-                raise FlyguyError(f"offsets must be an int64 vector [recordings + 1] on {q.device}")
-            offsets = offsets.contiguous()
+            offsets = _offsets(offsets, q)
             batch, ticks = offsets.shape[0] - 1, lead[0]
         if log_decay.requires_grad:
             raise FlyguyError("log_decay is a constant of each head: it has no gradient")
@@ -444,9 +448,13 @@ class TickMemory(nn.Module):
 
     def forward(self, obs: torch.Tensor, state=None, positions=None, offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
         """obs [recordings, ticks, obs_dim], or [ticks, obs_dim] packed end to end with offsets: logits of every tick and
-        the states after the last. A recording carried on needs its states and positions (a rotation depends on them)."""
+        the states after the last. Positions are the ticks of each recording unless given. A recording carried on needs its
+        states and positions (a rotation depends on them)."""
         if state is not None and positions is None:
             raise FlyguyError("a recording carried on from a state needs its ticks' positions")
+        if offsets is not None and positions is None and obs.dim() == 2:   # (the states that come out are step's to go on from)
+            offsets, tick = _offsets(offsets, obs), torch.arange(len(obs), device=obs.device)
+            positions = tick - offsets[(torch.searchsorted(offsets, tick, right=True) - 1).clamp(min=0)]
         q, k, v = self._qkv(obs, positions)
         o, end = decay_attention(q, k, v, self.log_decay, state, offsets=offsets)
         return self._logits(o), end

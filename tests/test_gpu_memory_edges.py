@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from flyguy_b200 import memory
+from flyguy_b200.native import FlyguyError
 
 pytestmark = pytest.mark.gpu
 TOL = {torch.float32: 5e-6, torch.bfloat16: 4e-3, torch.float16: 5e-4}
@@ -162,3 +163,30 @@ def test_ticks_of_no_recording_are_zero(offsets, dims, typ, cuda):
     for got, want in ((o, o1), *zip(grads[:3], grads1[:3])):
         assert torch.equal(got[a:z], want) and not got[:a].any() and not got[z:].any()
     assert torch.equal(end, end1) and torch.equal(grads[3], grads1[3])
+
+
+@pytest.mark.parametrize("offsets", [[0, 70, 70, 100], [5, 30, 96]])
+def test_states_of_packed_recordings_go_on_tick_by_tick(offsets, cuda):
+    """What a packed forward hands on is what playing the same recordings one by one hands on, and a step from it answers alike: a
+    tick's position is its place in its own recording. fp32: the same products in another order (1e-5 of the norm)."""
+    torch.manual_seed(0)
+    m = memory.TickMemory(24, 6, heads=4, key_heads=2, dim=64, dtype=torch.float32).cuda()
+    torch.nn.init.normal_(m.out.weight, std=0.1)
+    obs, then = torch.randn(offsets[-1] + 3, 24, device="cuda"), torch.randn(len(offsets) - 1, 24, device="cuda")
+    with torch.no_grad():
+        _, end = m(obs, offsets=torch.tensor(offsets, device="cuda"))
+        states = m.states(len(offsets) - 1)
+        for i, (a, z) in enumerate(zip(offsets, offsets[1:])):
+            for t in range(z - a):
+                m.step(obs[a + t].unsqueeze(0), states[i:i + 1], torch.full((1,), t, device="cuda"))
+        assert _off(end, states.double()) <= 1e-5
+        ticks = torch.tensor([z - a for a, z in zip(offsets, offsets[1:])], device="cuda")
+        want = m.step(then, states, ticks)
+        assert _off(m.step(then, end, ticks), want.double()) <= 1e-5
+
+
+def test_offsets_of_a_memory_are_checked(cuda):
+    m, obs = memory.TickMemory(8, 4, heads=2, key_heads=1, dim=16).cuda(), torch.zeros(6, 8, device=cuda)
+    for offsets in ([0, 6], torch.tensor([0, 6]), torch.tensor([0.0, 6.0], device=cuda), torch.zeros(0, dtype=torch.int64, device=cuda)):
+        with pytest.raises(FlyguyError, match="offsets"):
+            m(obs, offsets=offsets)
