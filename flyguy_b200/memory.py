@@ -153,7 +153,7 @@ class _Rotation:
         batch, ticks = (shape[0], shape[1]) if len(shape) == 4 else (1, shape[0])
         if layout not in LAYOUTS:
             raise FlyguyError(f"layout must be one of {list(LAYOUTS)}, not {layout!r}")
-        turned = at = 0
+        turned = 0
         if turns is not None:
             if not isinstance(turns, torch.Tensor) or turns.dtype is not torch.int64 or turns.get_device() != q.get_device() or turns.dim() != 1:
                 raise FlyguyError(f"turns must be an int64 vector on {q.device} (rotary_turns)")
@@ -162,28 +162,38 @@ class _Rotation:
                 raise FlyguyError(f"turns are of {turned} values, a head has {dim}")
             if not turns.is_contiguous():
                 turns = turns.contiguous()
-            at = turns.data_ptr()
-        pos = (0, 0, 0, 8)
         if positions is not None:
             if not isinstance(positions, torch.Tensor) or positions.get_device() != q.get_device() or positions.dtype not in (torch.int64, torch.int32):
                 raise FlyguyError(f"positions must be int64 or int32 on {q.device}")
-            p = positions
-            if p.shape != (batch, ticks):
+            if positions.shape != (batch, ticks):
                 try:
-                    p = p.expand(batch, ticks)
+                    positions = positions.expand(batch, ticks)
                 except RuntimeError:
                     raise FlyguyError(f"positions {tuple(positions.shape)} do not fit {batch} x {ticks} ticks") from None
-            pos = (p.data_ptr(), p.stride(0), p.stride(1), p.element_size())
-        self.keep = (turns, positions)                        # (their memory, until the backward has run)
+        self.turns, self.positions = turns, positions
         self.dim, self.device = dim, q.get_device()
-        self.fields = (shape[-2], 0 if k is None else k.shape[-2], batch, ticks, dim, turned, at, *pos, TYPES[q.dtype],
-                       LAYOUTS[layout], int(eps is not None), float(eps or 1.0), float(amplitude))
+        self.sizes = (shape[-2], 0 if k is None else k.shape[-2], batch, ticks, dim, turned)
+        self.settings = (TYPES[q.dtype], LAYOUTS[layout], int(eps is not None), float(eps or 1.0), float(amplitude))
+
+    def let_go(self) -> tuple:
+        """The plan and the positions, for autograd to keep (and to guard against changes in place) until the backward."""
+        kept = self.turns, self.positions
+        self.turns = self.positions = None
+        return kept
+
+    def take_up(self, turns, positions):
+        """This call with the tensors that autograd has kept."""
+        again = object.__new__(_Rotation)
+        again.__dict__.update(self.__dict__, turns=turns, positions=positions)
+        return again
 
     def pack(self, x, z=_NONE, y=_NONE, yk=_NONE, gy=_NONE, gz=_NONE, gx=_NONE, gk=_NONE, wq=None, wk=None, gwq=None, gwk=None,
              work=(0, 0)) -> bytes:
+        p = self.positions
+        pos = (0, 0, 0, 8) if p is None else (p.data_ptr(), *p.stride(), p.element_size())
         return _ROTATE.pack(*x, *z, *y, *yk, *gy, *gz, *gx, *gk, _ptr(wq), _ptr(wk),
                             self.dim if wq is not None and wq.dim() == 2 else 0, self.dim if wk is not None and wk.dim() == 2 else 0,
-                            _ptr(gwq), _ptr(gwk), *self.fields, *work)
+                            _ptr(gwq), _ptr(gwk), *self.sizes, _ptr(self.turns), *pos, *self.settings, *work)
 
     def forward(self, q, k=None, wq=None, wk=None):
         y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -213,12 +223,14 @@ class _Rotation:
 class _RotateFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rotation):
+        y = rotation.forward(x)
         ctx.rotation = rotation
-        return rotation.forward(x)
+        ctx.save_for_backward(*rotation.let_go())
+        return y
 
     @staticmethod
     def backward(ctx, gy):
-        return ctx.rotation.backward(_grad("the gradient", gy, gy)), None
+        return ctx.rotation.take_up(*ctx.saved_tensors).backward(_grad("the gradient", gy, gy)), None
 
 
 class _NormRotateFn(torch.autograd.Function):
@@ -226,15 +238,16 @@ class _NormRotateFn(torch.autograd.Function):
     def forward(ctx, q, k, wq, wk, rotation):
         ctx.set_materialize_grads(False)
         q, k = _values("q", q, (3, 4)), _values("k", k, (3, 4))
-        ctx.save_for_backward(q, k, wq, wk)
+        out = rotation.forward(q, k, wq, wk)
         ctx.rotation = rotation
-        return rotation.forward(q, k, wq, wk)
+        ctx.save_for_backward(q, k, wq, wk, *rotation.let_go())
+        return out
 
     @staticmethod
     def backward(ctx, gy, gz):
-        q, k, wq, wk = ctx.saved_tensors
+        q, k, wq, wk, *plan = ctx.saved_tensors
         gy, gz = _grad("the gradient of the queries", gy, q), _grad("the gradient of the keys", gz, k)
-        return *ctx.rotation.backward(gy, gz, q, k, wq, wk, ctx.needs_input_grad[2:4]), None
+        return *ctx.rotation.take_up(*plan).backward(gy, gz, q, k, wq, wk, ctx.needs_input_grad[2:4]), None
 
 
 def rotate(x, turns, positions=None, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:
@@ -312,6 +325,17 @@ class _Decay:
         self.sizes = (batch, ticks, heads, key_heads, dim, value_dim, TYPES[q.dtype])
         self.scale = float(dim ** -0.5 if scale is None else scale)
 
+    def let_go(self) -> tuple:
+        """The decays and the offsets, for autograd to keep until the backward."""
+        kept = self.log_decay, self.offsets
+        self.log_decay = self.offsets = None
+        return kept
+
+    def take_up(self, log_decay, offsets):
+        again = object.__new__(_Decay)
+        again.__dict__.update(self.__dict__, log_decay=log_decay, offsets=offsets)
+        return again
+
     def run(self, fn, backward: bool, tensors, state=None, state_out=None, gstate_out=None, gstate=None) -> None:
         room, work = _room(_decay_room(self.sizes, self.offsets is not None, backward), tensors[0].device)
         packed = _DECAY.pack(*(f for t in tensors for f in (_NONE if t is None else _ticks(t))), self.log_decay.data_ptr(),
@@ -341,13 +365,15 @@ class _DecayFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         q, k, v = (_values("q", t, (3, 4)) for t in (q, k, v))
         state = None if state is None else state.contiguous()
-        ctx.save_for_backward(q, k, v, state)
+        out = job.forward(q, k, v, state)
         ctx.job = job
-        return job.forward(q, k, v, state)
+        ctx.save_for_backward(q, k, v, state, *job.let_go())
+        return out
 
     @staticmethod
     def backward(ctx, go, gend):
-        return *ctx.job.backward(*ctx.saved_tensors, go, gend, ctx.needs_input_grad[3]), None
+        q, k, v, state, *kept = ctx.saved_tensors
+        return *ctx.job.take_up(*kept).backward(q, k, v, state, go, gend, ctx.needs_input_grad[3]), None
 
 
 def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,

@@ -190,3 +190,36 @@ def test_offsets_of_a_memory_are_checked(cuda):
     for offsets in ([0, 6], torch.tensor([0, 6]), torch.tensor([0.0, 6.0], device=cuda), torch.zeros(0, dtype=torch.int64, device=cuda)):
         with pytest.raises(FlyguyError, match="offsets"):
             m(obs, offsets=offsets)
+
+
+def _operators(cuda, typ=torch.bfloat16):
+    """name: (the tensors that a call reads beside its leaves, leaves, the call)"""
+    g = _gen(5)
+    x, k, wk = (_rand(g, 60, h, 64, typ=typ).requires_grad_() for h in (4, 2, 2))
+    w = (1 + 0.2 * _rand(g, 64)).requires_grad_()
+    turns, positions = memory.rotary_turns(64, device=cuda), torch.arange(60, device=cuda) + 7
+    ld, offsets = torch.tensor([-0.3, -0.1, -0.02, -0.01], device=cuda), torch.tensor([0, 25, 60], device=cuda)
+    state = _rand(g, 2, 4, 64, 64).requires_grad_()
+    return {
+        "rotate": ([turns, positions], [x], lambda: (memory.rotate(x, turns, positions),)),
+        "norm_rotate": ([turns, positions], [x, k, w], lambda: memory.norm_rotate(x, k, turns, w, None, positions)),
+        "decay_attention": ([ld, offsets], [x, k, wk, state], lambda: memory.decay_attention(x, k, wk, ld, state, offsets=offsets)),
+    }
+
+
+@pytest.mark.parametrize("name", ["rotate", "norm_rotate", "decay_attention"])
+def test_what_a_backward_reads_is_guarded(name, cuda):
+    """Plans, positions, decays and offsets changed in place between forward and backward: an error, as for any saved tensor,
+    not gradients of another call; unchanged, or kept elsewhere meanwhile, the same gradients."""
+    reads, leaves, call = _operators(cuda)[name]
+    want = torch.autograd.grad([y.float().sum() for y in call()], leaves)
+    with torch.autograd.graph.save_on_cpu():
+        outs = call()
+    for a, b in zip(torch.autograd.grad([y.float().sum() for y in outs], leaves), want):
+        assert torch.equal(a, b)
+    for t in reads:
+        outs = call()
+        t += 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad([y.float().sum() for y in outs], leaves)
+        t -= 1
