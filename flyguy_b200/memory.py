@@ -24,6 +24,7 @@ from functools import lru_cache
 
 import torch
 from torch import nn
+from torch.autograd.graph import increment_version
 
 from .native import FlyguyError, lib
 
@@ -430,6 +431,7 @@ def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None
     packed = _STEP.pack(*f, log_decay.data_ptr(), state.data_ptr(), _ptr(slots), state.shape[0], batch, heads, key_heads, dim,
                         value_dim, TYPES[q.dtype], float(dim ** -0.5 if scale is None else scale))
     _call(lib().fg_decay_step, packed, q.get_device())
+    increment_version(state)                              # (autograd sees that it has changed, should it have kept it)
     return o
 
 

@@ -223,3 +223,17 @@ def test_what_a_backward_reads_is_guarded(name, cuda):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad([y.float().sum() for y in outs], leaves)
         t -= 1
+
+
+def test_a_state_that_a_backward_needs_is_not_stepped_over_unseen(cuda):
+    """decay_step changes its states in place: a backward that kept them says so."""
+    g = _gen(6)
+    q = _rand(g, 2, 9, 2, 64).requires_grad_()
+    state, ld = _rand(g, 2, 2, 64, 64), torch.tensor([-0.1, -0.01], device=cuda)
+    o, _ = memory.decay_attention(q, q, q, ld, state)
+    x = q.detach()[:, 0]
+    before = state._version
+    memory.decay_step(x, x, x, ld, state)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
