@@ -9,7 +9,8 @@ at once and played a tick at a time with a state of fixed size:
   decay_step        the same for one tick, the states updated in place
 
 They run in the library (fg_norm_rotate, fg_decay_attn, fg_decay_step of include/flyguy_b200.h) on CUDA tensors, on
-torch's current stream; rotate, norm_rotate and decay_attention have gradients. TickMemory puts them together.
+torch's current stream; rotate, norm_rotate and decay_attention have gradients (of the first order). TickMemory puts them
+together.
 
 Queries, keys and values are float32, bfloat16 or float16 of one type, [batch, ticks, heads, dim] or, for recordings packed
 end to end, [ticks, heads, dim]; any strides with a head's values adjacent (others are copied first). Norms, sums,
@@ -20,7 +21,7 @@ from __future__ import annotations
 import math
 import struct
 from decimal import Decimal, localcontext
-from functools import lru_cache
+from functools import lru_cache, wraps
 
 import torch
 from torch import nn
@@ -104,6 +105,32 @@ def _grad(name: str, g, like: torch.Tensor, shape=None) -> torch.Tensor:
         return torch.zeros(like.shape if shape is None else shape, dtype=like.dtype, device=like.device)
     g = _values(name, g if g.dtype is like.dtype else g.to(like.dtype), (like.dim(),))
     return g if 0 not in g.stride() else g.contiguous()   # (an expanded sum)
+
+
+class _AgainFn(torch.autograd.Function):
+    """The first `n` tensors as they are, and an error for whoever differentiates them."""
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise FlyguyError("gradients of the memory operators cannot be differentiated again")
+
+
+def _once(backward):
+    """A backward whose gradients, where a graph of them is asked for (create_graph), are not taken for constants."""
+    @wraps(backward)
+    def once(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            outs = backward(ctx, *grads)
+        of = (t for t in (*ctx.saved_tensors, *grads) if t is not None)
+        given = [t for t in outs if isinstance(t, torch.Tensor)]
+        kept = iter(_AgainFn.apply(len(given), *given, *of))
+        return tuple(next(kept) if isinstance(t, torch.Tensor) else None for t in outs)
+    return once
 
 
 # ---- rotation ------------------------------------------------------------------------------------------------------
@@ -230,6 +257,7 @@ class _RotateFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_once
     def backward(ctx, gy):
         return ctx.rotation.take_up(*ctx.saved_tensors).backward(_grad("the gradient", gy, gy)), None
 
@@ -245,6 +273,7 @@ class _NormRotateFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_once
     def backward(ctx, gy, gz):
         q, k, wq, wk, *plan = ctx.saved_tensors
         gy, gz = _grad("the gradient of the queries", gy, q), _grad("the gradient of the keys", gz, k)
@@ -372,6 +401,7 @@ class _DecayFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_once
     def backward(ctx, go, gend):
         q, k, v, state, *kept = ctx.saved_tensors
         return *ctx.job.take_up(*kept).backward(q, k, v, state, go, gend, ctx.needs_input_grad[3]), None

@@ -237,3 +237,25 @@ def test_a_state_that_a_backward_needs_is_not_stepped_over_unseen(cuda):
     assert state._version > before
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["rotate", "norm_rotate", "decay_attention"])
+def test_gradients_are_not_taken_for_constants(name, cuda):
+    """With create_graph the first gradients are the same; a penalty on them is refused, not lost."""
+    _, leaves, call = _operators(cuda, torch.float32)[name]
+    want = torch.autograd.grad([y.square().sum() for y in call()], leaves)
+    got = torch.autograd.grad([y.square().sum() for y in call()], leaves, create_graph=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b) and a.requires_grad
+        with pytest.raises(FlyguyError, match="again"):
+            torch.autograd.grad(a.square().sum(), leaves, allow_unused=True, retain_graph=True)
+    flat = torch.autograd.grad([y.sum() for y in call()], leaves, create_graph=True)
+    if name == "rotate":                                                    # linear: these are constants
+        assert not flat[0].requires_grad
+    else:
+        with pytest.raises(FlyguyError, match="again"):
+            flat[0].square().sum().backward()
+    torch.autograd.backward([y.square().sum() for y in call()], create_graph=True)
+    for t, b in zip(leaves, want):
+        assert torch.equal(t.grad, b)
+        t.grad = None
