@@ -25,6 +25,7 @@ from functools import lru_cache, wraps
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from .native import FlyguyError, lib
@@ -61,6 +62,12 @@ def _ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
     """fg_ticks of [batch, ticks, heads, dim] or [ticks, heads, dim]."""
     st = t.stride()
     return (t.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (t.data_ptr(), 0, st[0], st[1])
+
+
+def _no_tangents(*tensors) -> None:
+    """Tangents would be dropped: they are refused."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise FlyguyError("the memory operators have no forward-mode derivatives")
 
 
 _NONE = (0, 0, 0, 0)
@@ -287,6 +294,7 @@ def rotate(x, turns, positions=None, layout: str = "half", amplitude: float = 1.
     positions: int64 / int32 that expand to [batch, ticks] (None: 0, 1, ..). layout "half": pairs (i, i + turned / 2);
     "interleaved": (2i, 2i + 1). The gradient is the rotation back."""
     x = _values("x", x, (3, 4))
+    _no_tangents(x)
     r = _Rotation(x, None, turns, positions, layout, amplitude, None)
     if x.requires_grad and torch.is_grad_enabled():
         return _RotateFn.apply(x, r)
@@ -306,6 +314,7 @@ def norm_rotate(q, k, turns=None, q_weight=None, k_weight=None, positions=None, 
         q_weight = _float32("q_weight", q_weight, q, q.shape[-1:], q.shape[-2:])
     if k_weight is not None:
         k_weight = _float32("k_weight", k_weight, k, k.shape[-1:], k.shape[-2:])
+    _no_tangents(q, k, q_weight, k_weight)
     r = _Rotation(q, k, turns, positions, layout, amplitude, eps)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
@@ -420,6 +429,7 @@ def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,
     q = _values("q", q, (3, 4))
     k, v = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
     job = _Decay(q, k, v, log_decay, state, scale, offsets)
+    _no_tangents(q, k, v, state, job.log_decay)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
         return _DecayFn.apply(q, k, v, state, job)
@@ -445,6 +455,7 @@ def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None
         raise FlyguyError(f"state must be contiguous float32 {('slots', heads, dim, value_dim)} on {q.device}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise FlyguyError("decay_step has no gradient (decay_attention has): call it under torch.no_grad()")
+    _no_tangents(q, k, v, state, log_decay)
     if slots is not None:
         if (not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.get_device() != q.get_device()
                 or slots.shape != (batch,)):

@@ -259,3 +259,23 @@ def test_gradients_are_not_taken_for_constants(name, cuda):
     for t, b in zip(leaves, want):
         assert torch.equal(t.grad, b)
         t.grad = None
+
+
+def test_tangents_are_not_dropped(cuda):
+    """Forward-mode derivatives of any operand are refused, with gradients on or off; tensors without one go as ever."""
+    from torch.autograd import forward_ad
+    g = _gen(7)
+    x, w, state = _rand(g, 2, 5, 2, 64), 1 + _rand(g, 64), _rand(g, 2, 2, 64, 64)
+    turns, ld = memory.rotary_turns(64, device=cuda), torch.tensor([-0.1, -0.01], device=cuda)
+    y, s = x[:, 0].contiguous(), state.clone()
+    calls = [(lambda x: memory.rotate(x, turns), (x,)), (lambda q, k, w: memory.norm_rotate(q, k, turns, w, w), (x, x, w)),
+             (lambda q, k, v, s: memory.decay_attention(q, k, v, ld, s), (x, x, x, state)),
+             (lambda q, k, v, s: memory.decay_step(q, k, v, ld, s), (y, y, y, s))]
+    for fn, args in calls:
+        for i in range(len(args)):
+            for on in (True, False):
+                with forward_ad.dual_level(), torch.set_grad_enabled(on):
+                    fn(*args)
+                    dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+                    with pytest.raises(FlyguyError, match="forward-mode"):
+                        fn(*dual)
