@@ -334,7 +334,10 @@ _STEP = struct.Struct("=16q10qd")
 @lru_cache(maxsize=256)
 def _decay_room(sizes: tuple, packed: bool, backward: bool) -> int:
     """Bytes of workspace that a call of these sizes needs (fg_decay_work)."""
-    return lib().fg_decay_work(_DECAY.pack(*(0,) * 37, int(packed), *sizes, 1.0, 0, 0), int(backward))
+    size = lib().fg_decay_work(_DECAY.pack(*(0,) * 37, int(packed), *sizes, 1.0, 0, 0), int(backward))
+    if size < 0:                                          # (raised here: an error is not kept)
+        raise FlyguyError(lib().fg_mem_last_error().decode())
+    return size
 
 
 class _Decay:
