@@ -358,9 +358,9 @@ class _Decay:
                 raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
             offsets = _offsets(offsets, q)
             batch, ticks = offsets.shape[0] - 1, lead[0]
+        self.log_decay = _float32("log_decay", log_decay, q, (heads,))
         if log_decay.requires_grad:
             raise FlyguyError("log_decay is a constant of each head: it has no gradient")
-        self.log_decay = _float32("log_decay", log_decay, q, (heads,))
         self.states, self.device, self.offsets = (batch, heads, dim, value_dim), q.get_device(), offsets
         if state is not None:
             _float32("state", state, q, self.states)

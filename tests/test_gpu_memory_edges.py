@@ -279,3 +279,12 @@ def test_tangents_are_not_dropped(cuda):
                     dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
                     with pytest.raises(FlyguyError, match="forward-mode"):
                         fn(*dual)
+
+
+def test_decays_that_are_no_tensor_are_refused(cuda):
+    x, state = torch.zeros(1, 2, 2, 64, device=cuda), torch.zeros(2, 2, 64, 64, device=cuda)
+    for ld in ([-0.1, -0.1], -0.1, None):
+        with pytest.raises(FlyguyError, match="log_decay"):
+            memory.decay_attention(x, x, x, ld)
+        with pytest.raises(FlyguyError, match="log_decay"):
+            memory.decay_step(x[:, 0], x[:, 0], x[:, 0], ld, state)
