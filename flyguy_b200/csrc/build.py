@@ -21,9 +21,8 @@ LIB = PKG / "libflyguy_b200.so"
 TRAIN = PKG / "fg_train"                             # the trainer executable (a main() over fg_train_main)
 SOURCES = [HERE / "fg_core.cu", HERE / "fg_noalloc.cu", HERE / "fg_hopop.cu", HERE / "fg_train.cu", HERE / "fg_fly.cu",
            HERE / "fg_rotate.cu", HERE / "fg_decay.cu"]
-DEPS = SOURCES + [HERE / "fg_kernels.cuh", HERE / "fg_tcgen05.cuh", HERE / "fg_outtc.cuh", HERE / "fg_memory.cuh", HERE / "fg_decay_tc.cuh",
-                  HERE / "fg_decay_mma.cuh",
-                  REPO / "include" / "flyguy_b200.h"]
+DEPS = SOURCES + [HERE / "fg_kernels.cuh", HERE / "fg_tcgen05.cuh", HERE / "fg_outtc.cuh", HERE / "fg_memory.cuh", HERE / "fg_once.h",
+                  HERE / "fg_decay_tc.cuh", HERE / "fg_decay_mma.cuh", REPO / "include" / "flyguy_b200.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

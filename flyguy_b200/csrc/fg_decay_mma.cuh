@@ -303,12 +303,11 @@ __global__ void __launch_bounds__(kMmThreads, DP + EP < 256 ? 2 : 1) k_decay_mma
 template <class T, int DP, int EP, bool BACK>
 void mma_launch_as(const Scan& s, cudaStream_t st) {
     constexpr int bytes = MmLayout<DP, EP>::floats * 4;
-    static const bool once = [] {
-        MCK(cudaFuncSetAttribute(k_decay_mma<T, DP, EP, BACK, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        MCK(cudaFuncSetAttribute(k_decay_mma<T, DP, EP, BACK, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        return true;
-    }();
-    (void)once;
+    static OnEachDevice here;
+    here.first(current_device(), [] {
+        allow_shared(k_decay_mma<T, DP, EP, BACK, false>, bytes);
+        allow_shared(k_decay_mma<T, DP, EP, BACK, true>, bytes);
+    });
     const auto by4 = [&](const Operand& o) {
         return reinterpret_cast<uintptr_t>(o.p) % (4 * sizeof(T)) == 0 && o.batch % 4 == 0 && o.tick % 4 == 0 && o.head % 4 == 0;
     };

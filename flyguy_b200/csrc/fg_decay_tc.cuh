@@ -663,12 +663,11 @@ inline CUtensorMap tile_map(const Scan& s, const Operand& o, int dim, bool f32 =
 template <int DP, int EP, bool BACK, bool F32>
 void tc_launch_as(const Scan& s, cudaStream_t st) {
     constexpr int bytes = TcLayout<DP, EP>::bytes;
-    static const bool once = [] {
-        MCK(cudaFuncSetAttribute(k_decay_tc<DP, EP, BACK, F32, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        MCK(cudaFuncSetAttribute(k_decay_tc<DP, EP, BACK, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        return true;
-    }();
-    (void)once;
+    static OnEachDevice here;
+    here.first(current_device(), [] {
+        allow_shared(k_decay_tc<DP, EP, BACK, F32, false>, bytes);
+        allow_shared(k_decay_tc<DP, EP, BACK, false, true>, bytes);
+    });
     const TcMaps maps{tile_map(s, s.a, s.D), tile_map(s, s.b, s.D), tile_map(s, s.c, s.E), tile_map(s, s.out, s.E, F32)};
     const unsigned rows = (unsigned)(s.batch * s.heads);
     if (s.parts > 1) k_decay_tc<DP, EP, BACK, false, true><<<dim3(rows, s.parts - 1), kTcThreads, bytes, st>>>(s, maps);

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <string>
 
+#include "fg_once.h"
 #include "flyguy_b200.h"
 
 namespace fgm {
@@ -92,15 +93,15 @@ void by_type(long long type, F&& f) {
     else throw MemErr{"unknown type"};
 }
 
-inline int sm_count() {
-    static thread_local int dev = -1, n = 0;
+// kernel may be launched with so many bytes of shared memory on the current device
+template <class K>
+void allow_shared(K* kernel, int bytes) {
+    MCK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+inline int current_device() {
     int d = 0;
     MCK(cudaGetDevice(&d));
-    if (d != dev) {
-        MCK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d));
-        dev = d;
-    }
-    return n;
+    return d;
 }
 
 }  // namespace fgm

@@ -1,4 +1,7 @@
 """The memory-over-ticks operators' errors on the host. Without a GPU."""
+import ctypes
+import subprocess
+
 import pytest
 
 from flyguy_b200 import memory, native
@@ -13,3 +16,36 @@ def test_a_refused_size_is_refused_in_the_same_words_again():
             memory._room(memory._decay_room(bad, False, False), None)
         assert native.lib().fg_decay_work(memory._DECAY.pack(*(0,) * 38, *good, 1.0, 0, 0), 0) == 0
         assert native.lib().fg_mem_last_error() == b""
+
+
+def test_kernels_are_set_up_on_every_device(tmp_path):
+    """fg_once.h: once a device, on each device, again after a failure; numbers past 63 each time."""
+    src = tmp_path / "once.cpp"
+    src.write_text("""
+#include "fg_once.h"
+extern "C" int setups(const int* devices, const int* fails, int n, int* ran) {
+    fgm::OnEachDevice here;
+    int thrown = 0;
+    for (int i = 0; i < n; ++i) {
+        ran[i] = 0;
+        try {
+            here.first(devices[i], [&] { ran[i] = 1; if (fails[i]) throw 1; });
+        } catch (int) { ++thrown; }
+    }
+    return thrown;
+}
+""")
+    lib = tmp_path / "once.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", str(native.PKG / "csrc"), "-o", str(lib), str(src)], check=True)
+    devices, fails = [0, 0, 1, 1, 0, 63, 63, 64, 64, 2, 2, 2], [0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 0, 0]
+    n = len(devices)
+    ran = (ctypes.c_int * n)()
+    assert ctypes.CDLL(str(lib)).setups((ctypes.c_int * n)(*devices), (ctypes.c_int * n)(*fails), n, ran) == 1
+    assert list(ran) == [1, 0, 1, 0, 0, 1, 0, 1, 1, 1, 1, 0]
+
+
+def test_no_kernel_is_set_up_once_for_all_devices():
+    """Attributes are set at every launch or by OnEachDevice, never behind a flag of the process."""
+    for f in ("fg_decay.cu", "fg_decay_mma.cuh", "fg_decay_tc.cuh", "fg_rotate.cu"):
+        text = (native.PKG / "csrc" / f).read_text()
+        assert "static const bool" not in text and "static bool" not in text, f
