@@ -673,7 +673,11 @@ void launch_units(const Rotate& a, float* part, UnitPlan& plan, cudaStream_t st)
     if (MODE == kBackwardW) bytes = std::max(bytes, (size_t)groups * a.dim * 4);
     bytes += kAhead * kUnits<NORM, MODE> * 256 * 16;
     auto* k = k_rotate_units<T, INTER, NORM, MODE>;
-    if (bytes > 48 * 1024) MCK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    // (the most any sizes ask for, once: set to each call's own, another thread's call could lower it before this one's launch)
+    constexpr int most_bytes = 64 * 1024 + 2048 * 16 + kAhead * kUnits<NORM, MODE> * 256 * 16;
+    need(bytes <= (size_t)most_bytes, "fg_norm_rotate: the tiles do not fit shared memory");
+    static OnEachDevice here;
+    here.first(current_device(), [] { allow_shared(k_rotate_units<T, INTER, NORM, MODE>, most_bytes); });
     k<<<plan.blocks[0] + plan.blocks[1], 256, bytes, st>>>(a, plan, part);
     MCK(cudaGetLastError());
 }

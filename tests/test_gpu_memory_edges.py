@@ -288,3 +288,27 @@ def test_decays_that_are_no_tensor_are_refused(cuda):
             memory.decay_attention(x, x, x, ld)
         with pytest.raises(FlyguyError, match="log_decay"):
             memory.decay_step(x[:, 0], x[:, 0], x[:, 0], ld, state)
+
+
+def test_two_threads_with_tiles_of_different_sizes(cuda):
+    """Backward calls from several threads at once (autograd itself makes them from one), one with much more shared memory than
+    the other: neither's launch is refused, and the results are each thread's own."""
+    import threading
+    turns, wrong = memory.rotary_turns(128, device=cuda), []
+
+    def work(heads, seed):
+        g = _gen(seed)
+        x, w = _rand(g, 4, 8, heads, 128, typ=torch.bfloat16), torch.ones(heads, 128, device=cuda)
+        try:
+            call = memory._Rotation(x, x[:, :, :0], turns, None, "half", 1.0, 1e-6)
+            runs = [call.backward(x, x[:, :, :0], x, x[:, :, :0], w, None, (True, False)) for _ in range(1500)]
+            assert all(torch.equal(runs[0][i], runs[-1][i]) for i in (0, 2))
+        except Exception as e:                                              # noqa: BLE001  (told by the test's own thread)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in ((1, 8), (120, 9), (1, 10), (64, 11))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
