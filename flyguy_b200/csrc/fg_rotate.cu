@@ -724,6 +724,8 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
         need(reinterpret_cast<uintptr_t>(g->work) % 16 == 0, "fg_norm_rotate_bwd: the workspace is not 16-byte aligned");
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         float* norms = need_bytes ? static_cast<float*>(g->work) : nullptr;
+        for (int i = 0; i < 2; ++i)                           // (weights that no head has used)
+            if (a.s[i].gw && !a.s[i].heads && !g->w_head[i]) MCK(cudaMemsetAsync(a.s[i].gw, 0, a.dim * sizeof(float), st));
         by_type(g->type, [&](auto t) {
             using T = decltype(t);
             float* part = norms ? norms + (rows + 3) / 4 * 4 : nullptr;

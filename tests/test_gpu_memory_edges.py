@@ -312,3 +312,23 @@ def test_two_threads_with_tiles_of_different_sizes(cuda):
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("shape", [(2, 5, 3, 0), (2, 5, 0, 3), (0, 5, 2, 2), (2, 0, 2, 2), (1, 1, 0, 0)])
+def test_weights_that_nothing_used_have_zero_gradients(shape, cuda):
+    """No heads on a side, no recordings or no ticks: a weight's gradient is zeros, not what its memory held."""
+    B, T, H, K = shape
+    g = _gen(10)
+    q, k = _rand(g, B, T, H, 64), _rand(g, B, T, K, 64)
+    wq, wk = (1 + 0.2 * _rand(g, 64) for _ in range(2))
+    for t in (q, k, wq, wk):
+        t.requires_grad_()
+    y = memory.norm_rotate(q, k, memory.rotary_turns(64, device=cuda), wq, wk)
+    for n in range(8):
+        torch.full((64 << n,), float("nan"), device=cuda)                   # (freed at once: what the gradients may be made from)
+    got = torch.autograd.grad(y, (q, k, wq, wk), [torch.ones_like(t) for t in y])
+    for heads, t in ((H, got[2]), (K, got[3])):
+        if not (B and T and heads):
+            assert not t.any()
+        else:
+            assert t.isfinite().all() and t.any()
