@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
         float* to = PARTS ? s.partial + (((long long)b * s.heads + h) * s.parts + part) * D * E : hand_on ? s.last + state0 : nullptr;
         if (to && mine) {
             const bool across = !PARTS && s.last_t;
-            // (a wait that ran out says so in what is handed on, too)
+            // (a wait that ran out shows in what is handed on and, below, in all of out)
             const float f = *gave_up ? __int_as_float(0x7fc00000) : !PARTS && BACK && sp.n ? pw[1] : 1.f;
 #pragma unroll
             for (int j = 0; j < EP / 32; ++j) {
@@ -621,6 +621,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
+    if (!PARTS && *gave_up) {                                 // (all stores are over: warp 19 has waited for its own)
+        const long long at = batch * s.out.batch + (long long)(BACK ? begin - total : begin) * s.out.tick + h * s.out.head;
+        for (long long i = tid; i < (long long)total * E; i += kTcThreads) {
+            const long long to = at + i / E * s.out.tick + i % E;
+            if (F32) reinterpret_cast<uint32_t*>(s.out.p)[to] = 0x7fc00000u;
+            else reinterpret_cast<uint16_t*>(s.out.p)[to] = 0x7fc0;
+        }
+    }
     if (last_block) wait_for_previous();
     if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }

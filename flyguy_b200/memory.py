@@ -7,6 +7,7 @@ at once and played a tick at a time with a state of fixed size:
   norm_rotate       the norms of queries and keys for each head and the rotation in one pass
   decay_attention   linear attention with a decay for each head over whole recordings (also packed end to end)
   decay_step        the same for one tick, the states updated in place
+  sync              waits for their work and tells whether a kernel gave up
 
 They run in the library (fg_norm_rotate, fg_decay_attn, fg_decay_step of include/flyguy_b200.h) on CUDA tensors, on
 torch's current stream; rotate, norm_rotate and decay_attention have gradients (of the first order). TickMemory puts them
@@ -477,6 +478,14 @@ def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None
     _call(lib().fg_decay_step, packed, q.get_device())
     increment_version(state)                              # (autograd sees that it has changed, should it have kept it)
     return o
+
+
+def sync(device=None) -> None:
+    """Waits for the current stream of `device` (None: the current one). An error if a wait inside a kernel of these operators has
+    run out on it, now or earlier in this process; what that call left holds NaN."""
+    with torch.cuda.device(device):
+        if lib().fg_mem_sync(_raw_stream(_device())):
+            raise FlyguyError(lib().fg_mem_last_error().decode())
 
 
 # ---- the operators together ---------------------------------------------------------------------------------------

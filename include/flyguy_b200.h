@@ -290,8 +290,8 @@ typedef struct fg_step_args {
 
 /* One tick of fg_decay_attn for each row, its state updated in place. */
 int fg_decay_step(const fg_step_args* args, void* stream);
-/* Waits for the stream; -1 if a call of these on the current device gave up a wait on the tensor cores (about 2 s; its
- * states then hold NaN). */
+/* Waits for the stream; -1 if a call of these on the current device gave up a wait on the tensor cores (about 2 s; the outputs,
+ * gradients and states of its recording and head then hold NaN), now or earlier in this process. */
 int fg_mem_sync(void* stream);
 /* Why the calling thread's last call of these failed ("" after a success). */
 const char* fg_mem_last_error(void);

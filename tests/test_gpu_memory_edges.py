@@ -332,3 +332,11 @@ def test_weights_that_nothing_used_have_zero_gradients(shape, cuda):
             assert not t.any()
         else:
             assert t.isfinite().all() and t.any()
+
+
+def test_sync_after_calls_that_went_well(cuda):
+    x = _rand(_gen(11), 2, 300, 2, 64, typ=torch.bfloat16)
+    o, _ = memory.decay_attention(x, x, x, torch.tensor([-0.1, -0.01], device=cuda))
+    memory.sync()
+    memory.sync(cuda)
+    assert torch.cuda.current_stream().query() and o.isfinite().all()

@@ -1,4 +1,5 @@
 """The memory-over-ticks operators' errors on the host. Without a GPU."""
+import contextlib
 import ctypes
 import subprocess
 
@@ -49,3 +50,27 @@ def test_no_kernel_is_set_up_once_for_all_devices():
     for f in ("fg_decay.cu", "fg_decay_mma.cuh", "fg_decay_tc.cuh", "fg_rotate.cu"):
         text = (native.PKG / "csrc" / f).read_text()
         assert "static const bool" not in text and "static bool" not in text, f
+
+
+def test_a_wait_that_ran_out_is_told(monkeypatch):
+    """memory.sync on a library whose fg_mem_sync reports a wait that ran out, and on one that reports none."""
+    class Library:
+        status, asked = 0, []
+
+        def fg_mem_sync(self, stream):
+            self.asked.append(stream)
+            return self.status
+
+        def fg_mem_last_error(self):
+            return b"fg_decay_attn: a wait on the tensor cores ran out"
+
+    fake = Library()
+    monkeypatch.setattr(memory, "lib", lambda: fake)
+    monkeypatch.setattr(memory, "_raw_stream", lambda device: 7)
+    monkeypatch.setattr(memory, "_device", lambda: 0)
+    monkeypatch.setattr(memory.torch.cuda, "device", lambda device: contextlib.nullcontext())
+    memory.sync()
+    fake.status = -1
+    with pytest.raises(native.FlyguyError, match="ran out"):
+        memory.sync()
+    assert fake.asked == [7, 7]
