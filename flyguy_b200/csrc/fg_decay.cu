@@ -228,8 +228,8 @@ template <class T>
 void share_sum(const float* in, const Operand& out, long long batch, long long ticks, int heads, int key_heads, int dim, cudaStream_t st) {
     const bool four = dim % 4 == 0;                          // (`in` is the workspace's: aligned)
     const long long units = batch * ticks * key_heads * dim / (four ? 4 : 1);
-    const unsigned blocks = (unsigned)std::min<long long>((units + 255) / 256, 148 * 32);
-    const bool small = units < (1ll << 31) - 148 * 32 * 256;  // 32-bit divisions: a third of the time
+    const unsigned blocks = (unsigned)std::min<long long>((units + 255) / 256, kSms * 32);
+    const bool small = units < (1ll << 31) - kSms * 32 * 256;  // 32-bit divisions: a third of the time
     if (small && four) k_share_sum<T, 4, uint32_t><<<blocks, 256, 0, st>>>(in, out, (uint32_t)ticks, heads, key_heads, dim, (uint32_t)units);
     else if (small) k_share_sum<T, 1, uint32_t><<<blocks, 256, 0, st>>>(in, out, (uint32_t)ticks, heads, key_heads, dim, (uint32_t)units);
     else k_share_sum<T, 1, long long><<<blocks, 256, 0, st>>>(in, out, ticks, heads, key_heads, dim, batch * ticks * key_heads * dim);
@@ -280,7 +280,7 @@ void clear_outside(const fg_decay_args* g, const fg_ticks* const (&to)[3], const
     a.batch = g->batch;
     a.ticks = g->ticks;
     auto* kernel = piece == 16 ? k_clear_outside<uint4> : piece == 4 ? k_clear_outside<uint32_t> : k_clear_outside<uint16_t>;
-    kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, 148 * 4), n), 256, 0, st>>>(a);
+    kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, kSms * 4), n), 256, 0, st>>>(a);
     MCK(cudaGetLastError());
 }
 
@@ -423,7 +423,7 @@ int parts_of(const fg_decay_args* g) {
     const bool mma = g->dim <= 128 && g->value_dim <= 128;
     const bool tc = mma && g->type == FG_BF16 && g->dim % 16 == 0 && g->value_dim % 16 == 0;
     const long long blocks = mma ? rows : rows * ((std::min(g->dim, g->value_dim) + kRecCols - 1) / kRecCols);
-    const long long want = (tc ? 148 : mma ? 2 * 148 : 4 * 148) / blocks, most = mean / (tc ? 512 : 256);
+    const long long want = (tc ? kSms : mma ? 2 * kSms : 4 * kSms) / blocks, most = mean / (tc ? 512 : 256);
     return (int)std::min<long long>(64, std::max<long long>(1, std::min(want, most)));
 }
 long long partial_floats(const fg_decay_args* g) {

@@ -14,6 +14,8 @@
 
 namespace fgm {
 
+constexpr int kSms = 148;                                    // of a B200, the only device these are built for
+
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }

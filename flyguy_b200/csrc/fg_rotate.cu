@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(256, MODE != kForward && NORM ? 2 : 3) k_rotat
     }
 }
 
-constexpr int kSplits = 148 * 4;                             // blocks with sums of their own, at most
+constexpr int kSplits = kSms * 4;                            // blocks with sums of their own, at most
 
 void strides(long long (&to)[3], const fg_ticks& t) {
     to[0] = t.batch;
@@ -656,7 +656,7 @@ void launch_units(const Rotate& a, float* part, UnitPlan& plan, cudaStream_t st)
     const int rows = a.s[0].heads + a.s[1].heads;
     plan = UnitPlan{{1, 1}, {0, 0}, 1, (uint32_t)(((1ull << 32) + a.ticks - 1) / a.ticks)};
     while (plan.lanes < items) plan.lanes *= 2;
-    const int groups = 256 / plan.lanes, most = MODE >= kBackwardW ? kSplits : 148 * 12;
+    const int groups = 256 / plan.lanes, most = MODE >= kBackwardW ? kSplits : kSms * 12;
     size_t bytes = 0;
     for (int i = 0; i < 2; ++i) {
         const int heads = a.s[i].heads;
@@ -665,7 +665,7 @@ void launch_units(const Rotate& a, float* part, UnitPlan& plan, cudaStream_t st)
         // tick costs by itself (its place, its angles) is spread over its heads. With the sizes above 2 blocks an SM take
         // 41 and 74 us, 8 take 57 and 87; 2,048 angles twice are 32 KB of an SM's shared memory a block.
         int per = MODE == kBackwardEach ? 1 : groups;
-        while (per > 1 && ((total + per - 1) / per < 148 * 2 || (size_t)per * half > 2048)) per /= 2;
+        while (per > 1 && ((total + per - 1) / per < kSms * 2 || (size_t)per * half > 2048)) per /= 2;
         plan.per[i] = per;
         bytes = std::max(bytes, (size_t)per * half * 16 + (MODE == kBackwardEach ? (size_t)heads * a.dim * 4 : 0));
         plan.blocks[i] = std::max(1, std::min((total + per - 1) / per, (int)((long long)most * heads / rows)));
