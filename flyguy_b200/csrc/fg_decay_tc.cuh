@@ -525,20 +525,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
 #pragma unroll
             for (int i = 0; i < 16; ++i) S[j][i] = 0.f;
         const long long state0 = ((long long)b * s.heads + h) * D * E;
-        // S += f * the state at p, which may lie [E][D] or, a caller's, begin at any float: then value by value
+        // S += f * the state at p, which may lie [E][D]
         auto add = [&](const float* p, float f, bool across) {
-            const bool single = across || reinterpret_cast<uintptr_t>(p) % 16;
-            const int step = across ? D : 1;
 #pragma unroll
             for (int j = 0; j < EP / 32; ++j) {
                 const int e0 = (2 * j + half) * 16;
                 if (!mine || e0 >= E) continue;
-                const float* at = p + (across ? e0 * D + row : row * E + e0);
-                if (single) {
+                if (across) {
+                    const float* q = p + (long long)e0 * D + row;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i, at += step) S[j][i] = fmaf(f, *at, S[j][i]);
+                    for (int i = 0; i < 16; ++i, q += D) S[j][i] = fmaf(f, *q, S[j][i]);
                 } else {
-                    const float4* q = reinterpret_cast<const float4*>(at);
+                    const float4* q = reinterpret_cast<const float4*>(p + row * E + e0);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float4 v = q[i];
@@ -642,7 +640,8 @@ inline bool whole_units(const Scan& s, const Operand& o) {
 inline bool tc_fits(const Scan& s) {
     return s.D % 16 == 0 && s.E % 16 == 0 && s.D <= 128 && s.E <= 128 && s.ticks < (1ll << 31) && s.ticks > 0 &&
            s.batch < (1ll << 31) && whole_units(s, s.a) && whole_units(s, s.b) && whole_units(s, s.c) &&
-           whole_units(s, s.out) && reinterpret_cast<uintptr_t>(s.last) % 16 == 0;
+           whole_units(s, s.out) && reinterpret_cast<uintptr_t>(s.last) % 16 == 0 &&
+           (s.first_t || reinterpret_cast<uintptr_t>(s.first) % 16 == 0);   // (read value by value where it lies [E][D])
 }
 // [batch][ticks][heads][dim] as tiles of 128 bytes x 128 ticks, zeros outside
 inline CUtensorMap tile_map(const Scan& s, const Operand& o, int dim, bool f32 = false) {

@@ -59,6 +59,14 @@ def _float32(name: str, t, like: torch.Tensor, *shapes) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _state(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A state, or its gradient, as the kernels read it fastest: contiguous, from a 16-byte boundary on."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
     """fg_ticks of [batch, ticks, heads, dim] or [ticks, heads, dim]."""
     st = t.stride()
@@ -395,7 +403,7 @@ class _Decay:
     def backward(self, q, k, v, state, go, gend, want_state: bool):
         go = _grad("the gradient of o", go, q, (*q.shape[:-1], v.shape[-1]))
         if gend is not None:
-            gend = gend.float().contiguous()
+            gend = _state(gend.float())
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         gstate = torch.empty(self.states, dtype=torch.float32, device=q.device) if want_state else None
         self.run(lib().fg_decay_attn_bwd, True, (q, k, v, None, go, gq, gk, gv), state, None, gend, gstate)
@@ -407,7 +415,7 @@ class _DecayFn(torch.autograd.Function):
     def forward(ctx, q, k, v, state, job):
         ctx.set_materialize_grads(False)
         q, k, v = (_values("q", t, (3, 4)) for t in (q, k, v))
-        state = None if state is None else state.contiguous()
+        state = _state(state)
         out = job.forward(q, k, v, state)
         ctx.job = job
         ctx.save_for_backward(q, k, v, state, *job.let_go())
@@ -437,7 +445,7 @@ def decay_attention(q, k, v, log_decay, state=None, scale: float | None = None,
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
         return _DecayFn.apply(q, k, v, state, job)
-    return job.forward(q, k, v, None if state is None else state.contiguous())
+    return job.forward(q, k, v, _state(state))
 
 
 def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None) -> torch.Tensor:

@@ -340,3 +340,22 @@ def test_sync_after_calls_that_went_well(cuda):
     memory.sync()
     memory.sync(cuda)
     assert torch.cuda.current_stream().query() and o.isfinite().all()
+
+
+@pytest.mark.parametrize("dims", [(2, 1, 64, 64), (2, 2, 128, 128)])
+def test_the_library_takes_states_at_any_float(dims, cuda):
+    """The same below memory's own copy: the kernel that reads such states value by value."""
+    H, K, D, E = dims
+    g = _gen(12)
+    q, k, v = (_rand(g, 1, 300, h, n, typ=torch.bfloat16) for h, n in ((H, D), (K, D), (K, E)))
+    state, go, gend = _rand(g, 1, H, D, E), _rand(g, 1, 300, H, E, typ=torch.bfloat16), _rand(g, 1, H, D, E, scale=0.3)
+    job = memory._Decay(q, k, v, torch.tensor([-0.1, -0.01], device=cuda), state, None, None)
+    runs = []
+    for move in (lambda t: t, lambda t: _at_float(t, 1)):
+        o, end = job.forward(q, k, v, move(state))
+        job_end = move(gend)
+        gq, gk, gv, gs = (torch.empty_like(t) for t in (q, k, v, state))
+        job.run(memory.lib().fg_decay_attn_bwd, True, (q, k, v, None, go, gq, gk, gv), move(state), None, job_end, gs)
+        runs.append((o, end, gq, gk, gv, gs))
+    for a, b in zip(*runs):
+        assert _off(b, a.double()) <= 2 * TOL[a.dtype]
