@@ -619,13 +619,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_decay_tc(const __grid_constan
     fg::tc_fence_before();
     __syncthreads();
     fg::tc_fence_after();
-    if (!PARTS && *gave_up) {                                 // (all stores are over: warp 19 has waited for its own)
-        const long long at = batch * s.out.batch + (long long)(BACK ? begin - total : begin) * s.out.tick + h * s.out.head;
-        for (long long i = tid; i < (long long)total * E; i += kTcThreads) {
-            const long long to = at + i / E * s.out.tick + i % E;
-            if (F32) reinterpret_cast<uint32_t*>(s.out.p)[to] = 0x7fc00000u;
-            else reinterpret_cast<uint16_t*>(s.out.p)[to] = 0x7fc0;
-        }
+    if (!PARTS && warp >= 8 && warp < 16 && *gave_up) {       // (all stores are over: warp 19 has waited for its own)
+        // the block's place anew: kept, it would cost every role registers
+        int x, y;
+        asm volatile("mov.u32 %0, %%ctaid.x;\n\tmov.u32 %1, %%ctaid.y;" : "=r"(x), "=r"(y));
+        const Span all = span_of(s, x / s.heads);
+        const long long size = part_ticks(all.n, s.parts), from = min(all.n, y * size), to = min(all.n, from + size);
+        const long long at = (s.offsets ? 0 : x / s.heads) * s.out.batch + (x % s.heads) * s.out.head;
+#pragma unroll 1
+        for (long long t = from + warp - 8; t < to; t += 8)
+#pragma unroll 1
+            for (int e = lane; e < E; e += 32) {
+                const long long i = at + (all.start + (BACK ? all.n - 1 - t : t)) * s.out.tick + e;
+                if (F32) reinterpret_cast<uint32_t*>(s.out.p)[i] = 0x7fc00000u;
+                else reinterpret_cast<uint16_t*>(s.out.p)[i] = 0x7fc0;
+            }
     }
     if (last_block) wait_for_previous();
     if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
