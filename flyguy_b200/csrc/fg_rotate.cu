@@ -744,7 +744,7 @@ int fg_norm_rotate_bwd(const fg_rotate_args* g, void* stream) {
                     const int n0 = a.s[0].gw && a.s[0].heads ? sums[0].n : 0, n1 = a.s[1].gw && a.s[1].heads ? sums[1].n : 0;
                     sums[0].n = n0;
                     sums[1].n = n1;
-                    k_rotate_gw_sum<<<dim3((std::max(n0, n1) + 31) / 32, 2), 1024, 0, st>>>(sums[0], sums[1]);
+                    if (n0 || n1) k_rotate_gw_sum<<<dim3((std::max(n0, n1) + 31) / 32, 2), 1024, 0, st>>>(sums[0], sums[1]);
                     MCK(cudaGetLastError());
                 }
                 return;

@@ -359,3 +359,13 @@ def test_the_library_takes_states_at_any_float(dims, cuda):
         runs.append((o, end, gq, gk, gv, gs))
     for a, b in zip(*runs):
         assert _off(b, a.double()) <= 2 * TOL[a.dtype]
+
+
+@pytest.mark.parametrize("D", [64, 7])
+def test_only_weights_of_no_heads_learn(D, cuda):
+    """No key heads, and nothing but their weights asks for a gradient beside the queries."""
+    q, k = _rand(_gen(13), 2, 5, 3, D).requires_grad_(), torch.zeros(2, 5, 0, D, device=cuda)
+    wk = torch.ones(D, device=cuda).requires_grad_()
+    y, z = memory.norm_rotate(q, k, None, None, wk)
+    torch.autograd.backward((y, z), (torch.ones_like(y), torch.ones_like(z)))
+    assert not wk.grad.any() and q.grad.isfinite().all()
