@@ -55,9 +55,9 @@ __device__ __forceinline__ float power(float log_decay, float n) { return n > 0.
 
 // Scans that need nothing of one another overlap: a launch that may run beside the one before it begins once all of that
 // one's blocks have begun, and takes the SMs that its last blocks leave free. 512 blocks on 148 SMs are 3.5 rounds: 64
-// recordings of 1,024 ticks, 8 heads of 128 in bf16, forward and the three scans back take 631 us, in turn 698. What follows
-// must follow both, so one block of the later launch ends after the earlier one has. (With parts the launch before is the
-// parts', whose states are read.)
+// recordings of 1,024 ticks, 8 heads of 128 in bf16, forward and the three scans back take 650 us, in turn 719 (pass after
+// pass; with the L2 flushed in between 707 and 755). What follows must follow both, so one block of the later launch ends after
+// the earlier one has. (With parts the launch before is the parts', whose states are read.)
 __device__ __forceinline__ void next_may_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class... Rest>
@@ -92,8 +92,8 @@ namespace {
 // state; lane = column, warp w holds rows w R .. w R + R - 1 in registers. 16 ticks of a and b are staged in shared
 // memory as fp32 and read as broadcasts; the warps' shares of out meet in shared memory once per 16 ticks. It is what runs
 // for a dim or value_dim over 128, where neither of the other kernels has room for the state. Bound by the multiply-adds,
-// two a value of S and tick on the fp32 units, and the barriers between 16 ticks: 32 recordings of 509 ticks, 8 heads of 64 in
-// fp32 with gradients take 2,825 us here and 379 as products of chunks (bf16, 64 of 1,024, 8 heads of 128: 49,100 and 706).
+// two a value of S and tick on the fp32 units, and the barriers between 16 ticks: 32 recordings of 509 ticks, 4 heads of 64 in
+// fp32 with gradients take 2,825 us here and 379 as products of chunks (bf16, 64 of 1,024, 8 heads of 128: 49,100 and 720).
 constexpr int kRecTicks = 16, kRecWarps = 8, kRecCols = 32;
 constexpr int kRecRows = kMaxDim / kRecWarps;
 
@@ -238,7 +238,8 @@ void share_sum(const float* in, const Operand& out, long long batch, long long t
 
 // Zeros for the ticks that no recording covers, before the first and after the last (a packed buffer with room to spare): the
 // scans write recordings only, and what reads these outputs, the gradient of a projection's weights say, sums over all ticks.
-// Rows of `units` pieces of U of each head; up to three outputs, one a grid row.
+// Rows of `units` pieces of U of each head; up to three outputs, one a grid row. With nothing to clear it is the cost of a launch,
+// 3 us beside the scans' 190.
 struct Outside {
     struct {
         char* p;
@@ -280,7 +281,7 @@ void clear_outside(const fg_decay_args* g, const fg_ticks* const (&to)[3], const
     a.batch = g->batch;
     a.ticks = g->ticks;
     auto* kernel = piece == 16 ? k_clear_outside<uint4> : piece == 4 ? k_clear_outside<uint32_t> : k_clear_outside<uint16_t>;
-    kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, kSms * 4), n), 256, 0, st>>>(a);
+    kernel<<<dim3((unsigned)std::min<long long>((most + 255) / 256, kSms), n), 256, 0, st>>>(a);
     MCK(cudaGetLastError());
 }
 
@@ -415,7 +416,7 @@ void check_sizes(const Sizes& z, const char* who) {
 
 // Parts a recording. A part costs its b and c read twice, so: as many as keep the blocks within one round of the SMs (the
 // tcgen05 kernel takes a SM to itself, two blocks of the mma.sync kernel share one), of at least four chunks. The
-// recurrence's blocks are slow and share a SM: more of them. (1 recording of 65,536 ticks, 8 heads of 128 in bf16: 287 us in 18
+// recurrence's blocks are slow and share a SM: more of them. (1 recording of 65,536 ticks, 8 heads of 128 in bf16: 289 us in 18
 // parts a head; unsplit, 512 chunks of 4.7 us follow one another.)
 int parts_of(const fg_decay_args* g) {
     const long long rows = std::max<long long>(1, g->batch * g->heads);
@@ -472,7 +473,7 @@ Scan scan_of(const fg_decay_args* g) {
 }
 
 // By what fits: bf16 tiles that TMA takes go to the tcgen05 kernel, other types and strides up to 128 to mma.sync (fp32
-// needs its terms; 64 recordings of 1,024 ticks, 8 heads of 128 with gradients: 706 us and, in fp16, 5.4 ms), the rest to the recurrence.
+// needs its terms; 64 recordings of 1,024 ticks, 8 heads of 128 with gradients: 720 us and, in fp16, 5.4 ms), the rest to the recurrence.
 template <class T>
 void launch(const Scan& s, cudaStream_t st) {
     if (std::is_same<T, __nv_bfloat16>::value && tc_fits(s)) return tc_launch(s, st);

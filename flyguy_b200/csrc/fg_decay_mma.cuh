@@ -11,7 +11,9 @@
 // chunk's operand. Tensor instructions that reach further (tcgen05 kind::tf32) want operands of 4 bytes a value split
 // beforehand, two planes each: at dim 128 one chunk's would not fit beside S in 227 KB.
 //
-// 32 recordings of 509 ticks, 8 heads of 64 in fp32: 131 us a scan (52 MB; 13 GFLOP as 3 products of terms), 379 us forward and
+// A NaN or an infinity reaches all ticks of its chunk, and an infinity becomes a NaN in its terms (hi infinite, lo not a number).
+//
+// 32 recordings of 509 ticks, 4 heads of 64 in fp32: 131 us a scan (52 MB in; 6.4 GFLOP as 3 products of terms), 379 us forward and
 // back, the three scans back overlapping. Bound by waits: 8 warps of a block share the four products of a chunk, with a
 // barrier between each, and a block or two share an SM; the tensor pipe is 14% busy, issue slots 21%, DRAM 5%.
 #pragma once

@@ -9,8 +9,10 @@
 //   O2 [128 x E]   = W c                  W = A . gamma^{t-s} rounded to bf16, over A in TMEM
 //   dS [D x E]     = b'^T c               b' = gamma^{n-1-s} b as three bf16 terms (2^-25)
 // S itself stays in fp32 registers for the whole recording, thread = row, so states are as good as fp32 sums. The roundings
-// of S in O1 and of W in O2 are of the size of the rounding of out itself, and apart from one another: the three together
-// leave out sqrt(2) as far from exact as its own rounding alone.
+// of S in O1 and of W in O2 are of the size of the rounding of out itself, and apart from one another: out is 2.3e-3 of its norm
+// off where its own rounding alone is 1.7e-3. Second terms would take them away, but at 128 S's needs 32 KB more shared memory
+// than there is (and W's alone leaves S's); callers are told. A tile is worked on at once, so a NaN or an infinity in c reaches
+// all rows of its chunk (its weight for those before it is 0, and 0 times NaN is NaN), and an infinity in b' becomes a NaN.
 //
 // Tiles lie in shared memory as TMA writes them, 64 values (128 bytes, swizzled) of a tick in a row: read along the values
 // or along the ticks that is the K-major or the MN-major form of the same bytes, so nothing is transposed. 227 KB hold two
@@ -22,12 +24,12 @@
 // out. The roles meet at mbarriers only, so a
 // chunk's elementwise work runs beside its MMAs and the next chunk's copies.
 //
-// 64 recordings of 1,024 ticks, 8 heads of 128, forward: 185 us (403 MB in, 137 MB out; at the rate of a plain copy 82 us), 8
+// 64 recordings of 1,024 ticks, 8 heads of 128, forward: 189 us (403 MB in, 137 MB out; at the rate of a plain copy 82 us), 8
 // chunks of 4.7 us a block and some 8 us around them, four rounds of blocks. What bounds it is the chain from one state to the
 // next: S copied, O1, b' made (b is read and three terms written, 128 KB of shared memory at 128), 24 MMAs of dS (64 clocks
-// each, for both operands come from shared memory), S read back. The tensor pipe is 26% busy, DRAM 36%, issue slots 31%. At dim
-// 64 b' is made while O1 runs: 97,500 ticks, 8 heads, 180 us (250 MB). Blocks that took over one recording after another
-// instead of ending (with the next one's first tiles on their way) lost more a chunk than they saved: forward and back 713 us, 698 without.
+// each, for both operands come from shared memory), S read back. The tensor pipe is 26% busy, DRAM 35%, issue slots 31%. At dim
+// 64 b' is made while O1 runs: 97,500 ticks, 8 heads, 190 us (250 MB). Blocks that took over one recording after another
+// instead of ending (with the next one's first tiles on their way) lost more a chunk than they saved: forward and back took 2% longer.
 #pragma once
 #include <cuda.h>
 

@@ -225,10 +225,10 @@ __global__ void __launch_bounds__(1024) k_rotate_gw_sum(const SumSide queries, c
 // The bound is the memory: 2 passes over the values forward (read, write), 3 back. What it takes to get near it: kAhead
 // heads of each lane are on their way into shared memory at any time (a lane reads only what it asked for itself, so no
 // barrier is needed), and the arithmetic is done on pairs of floats, for the kernel is half bound by its instructions. In
-// bf16, half layout, 128 recordings of 128 ticks, 16 + 4 heads of 128, forward and back with the sums of gw: 41 and 74 us,
+// bf16, half layout, 128 recordings of 128 ticks, 16 + 4 heads of 128, forward and back with the sums of gw: 42 and 75 us,
 // where one head ahead in registers takes 49 and 99, and a row for each group, with its angles and weights fetched anew,
 // 73 and 95; the bytes alone are 26 and 39 us. In fp16, 32 recordings of 2,048 ticks, 8 + 8 heads of 128, the first 96
-// values turned as neighbours: 115 us (bytes: 82); where the lane's two units are neighbours too, 182.
+// values turned as neighbours: 118 us (bytes: 82); where the lane's two units are neighbours too, 182.
 
 // 16 bytes of T as pairs of floats, n values in all
 template <class T>
@@ -663,7 +663,7 @@ void launch_units(const Rotate& a, float* part, UnitPlan& plan, cudaStream_t st)
         if (!heads) continue;
         // a group takes a tick's heads one after another, unless the ticks are too few to give each SM two blocks: what a
         // tick costs by itself (its place, its angles) is spread over its heads. With the sizes above 2 blocks an SM take
-        // 41 and 74 us, 8 take 57 and 87; 2,048 angles twice are 32 KB of an SM's shared memory a block.
+        // 42 and 75 us, 8 take 57 and 87; 2,048 angles twice are 32 KB of an SM's shared memory a block.
         int per = MODE == kBackwardEach ? 1 : groups;
         while (per > 1 && ((total + per - 1) / per < kSms * 2 || (size_t)per * half > 2048)) per /= 2;
         plan.per[i] = per;

@@ -269,8 +269,10 @@ typedef struct fg_decay_args {
 
 /* For every recording and head h (keys and values of head h / (heads / key_heads)):
  *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t.
- * States are fp32. Ticks before the first recording and after the last get zeros. Offsets may not fall; outside 0..ticks, or falling,
- * they are clamped, never followed out of the buffers (falling ones leave the ticks that two recordings then name undefined). */
+ * States are fp32. Outputs may overlap neither one another nor inputs. Ticks before the first recording and after the last
+ * get zeros. Offsets may not fall; outside 0..ticks, or falling, they are clamped, never followed out of the buffers (falling
+ * ones leave the ticks that two recordings then name undefined). Ticks are worked on in tiles: a NaN or an infinity reaches all
+ * ticks of its tile of 64 or 128, of its recording and head. */
 int fg_decay_attn(const fg_decay_args* args, void* stream);
 /* With R_t = exp(log_decay) R_{t+1} + scale q_t go_t^T (the last also + gstate_out):
  *   gq_t = scale S_t go_t, gk_t = R_t v_t, gv_t = R_t^T k_t (summed over the query heads that share them), gstate =
