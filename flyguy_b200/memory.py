@@ -86,6 +86,11 @@ _NONE = (0, 0, 0, 0)
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice   # (torch.cuda's own, without its objects)
 
 
+def _kept(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t for autograd to keep (it keeps none that was made in inference mode)."""
+    return t.clone() if t is not None and t.is_inference() else t
+
+
 def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -224,7 +229,7 @@ class _Rotation:
 
     def let_go(self) -> tuple:
         """The plan and the positions, for autograd to keep (and to guard against changes in place) until the backward."""
-        kept = self.turns, self.positions
+        kept = _kept(self.turns), _kept(self.positions)
         self.turns = self.positions = None
         return kept
 
@@ -381,7 +386,7 @@ class _Decay:
 
     def let_go(self) -> tuple:
         """The decays and the offsets, for autograd to keep until the backward."""
-        kept = self.log_decay, self.offsets
+        kept = _kept(self.log_decay), _kept(self.offsets)
         self.log_decay = self.offsets = None
         return kept
 

@@ -369,3 +369,17 @@ def test_only_weights_of_no_heads_learn(D, cuda):
     y, z = memory.norm_rotate(q, k, None, None, wk)
     torch.autograd.backward((y, z), (torch.ones_like(y), torch.ones_like(z)))
     assert not wk.grad.any() and q.grad.isfinite().all()
+
+
+@pytest.mark.parametrize("name", ["rotate", "norm_rotate", "decay_attention"])
+def test_plans_made_in_inference_mode(name, cuda):
+    """Positions, plans, decays and offsets from inference mode learn as others do."""
+    reads, leaves, call = _operators(cuda)[name]
+    want = torch.autograd.grad([y.float().sum() for y in call()], leaves)
+    with torch.inference_mode():
+        made = [t.clone() for t in reads]
+    fns = {"rotate": lambda a, b: (memory.rotate(leaves[0], a, b),),
+           "norm_rotate": lambda a, b: memory.norm_rotate(*leaves[:2], a, leaves[2], None, b),
+           "decay_attention": lambda a, b: memory.decay_attention(*leaves[:3], a, leaves[3], offsets=b)}
+    for a, b in zip(torch.autograd.grad([y.float().sum() for y in fns[name](*made)], leaves), want):
+        assert torch.equal(a, b)
