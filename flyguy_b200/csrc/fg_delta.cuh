@@ -1,0 +1,177 @@
+// Pieces of the gated delta rule's kernels: operands as terms of bf16, tiles in shared memory, fragments of mma.sync.
+//
+// A value is taken as one to three bf16 terms (8 bits each: x = hi + mid + lo), a product of two values as the products of their
+// terms i and j with i + j < N, N the terms that the result deserves: 2^-9, 2^-17 or 2^-24 of each product is dropped. bf16 values
+// are one term as they are, fp16 values two. (mma.sync of tf32 takes twice the time of bf16 for the same product: two bf16 terms
+// cost as much as one of tf32 and keep 16 bits instead of 11.)
+//
+// mma.sync m16n8k16: a thread (g = lane / 4, t4 = lane % 4) of the warp has of a 16 x 8 result the values (g, 2 t4), (g, 2 t4 + 1),
+// (g + 8, 2 t4), (g + 8, 2 t4 + 1); two such results side by side are, packed in pairs, the 16 x 16 left operand of the next product.
+#pragma once
+#include "fg_heads.cuh"
+
+namespace {
+using namespace fgm;
+using bf16 = __nv_bfloat16;
+
+constexpr int kTicks = 64;               // of a chunk
+constexpr int kSquare = kTicks + 8;      // a row of a 64 x 64 tile in shared memory: 8 rows of 16 bytes lie in 32 banks
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void stsm_t(uint32_t at, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3])
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// a pair of values as N packed terms
+template <int N>
+__device__ __forceinline__ void terms(float x, float y, uint32_t (&t)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        t[i] = pack(x, y);
+        if (i + 1 < N) {
+            x -= low(t[i]);
+            y -= high(t[i]);
+        }
+    }
+}
+// two 16 x 8 results side by side as a left operand of N terms
+template <int N>
+__device__ __forceinline__ void left(const float (&x)[4], const float (&y)[4], uint32_t (&a)[N][4]) {
+    const float* v[4] = {&x[0], &x[2], &y[0], &y[2]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t t[N];
+        terms<N>(v[i][0], v[i][1], t);
+#pragma unroll
+        for (int n = 0; n < N; ++n) a[n][i] = t[n];
+    }
+}
+
+// Where a lane's 16 bytes of four 8 x 8 blocks lie in a tile with rows of `stride` values (a byte offset):
+// right operand from rows n of values k: blocks (n 0-7, k 0-7), (n 0-7, k 8-15), (n 8-15, k 0-7), (n 8-15, k 8-15)
+__device__ __forceinline__ uint32_t at_rows_n(int lane, int stride) { return 2 * (((lane & 7) + ((lane >> 4) << 3)) * stride + ((lane >> 3) & 1) * 8); }
+// left operand from rows m of values k, or (transposed) right operand from rows k of values n:
+// blocks (0-7, 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+__device__ __forceinline__ uint32_t at_rows_m(int lane, int stride) { return 2 * ((lane & 15) * stride + (lane >> 4) * 8); }
+// transposed: left operand from rows k of values m: the same blocks as at_rows_n
+__device__ __forceinline__ uint32_t at_rows_k(int lane, int stride) { return at_rows_n(lane, stride); }
+
+struct Operand {
+    char* p;
+    long long batch, tick, head;
+    int share;               // heads to one head of this operand
+    int fast;                // whole 16 bytes of 8 values (32 of fp32) at 16-byte boundaries
+};
+struct Gate {
+    float* p;
+    long long batch, tick, head;
+};
+struct Span {
+    long long start, n;      // ticks of the recording
+};
+
+__device__ __forceinline__ void async16(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows 0 .. 63 of an operand (`rows` of them there, the rest zeros), columns 0 .. COLS - 1 of `cols`, as N planes of terms
+// with rows of STRIDE values. bf16 at 16-byte boundaries goes by asynchronous copies.
+template <class T, int N, int COLS, int STRIDE, int THREADS>
+__device__ __forceinline__ void load_tile(bf16* to, const T* p, long long row, int rows, int cols, bool fast, int tid) {
+    constexpr int kUnits = COLS / 8, kPlane = kTicks * STRIDE;
+    for (int i = tid; i < kTicks * kUnits; i += THREADS) {
+        const int r = i / kUnits, c = (i - r * kUnits) * 8;
+        bf16* at = to + r * STRIDE + c;
+        const bool in = r < rows && c < cols;
+        const T* q = p + (in ? r * row + c : 0);
+        if constexpr (N == 1 && std::is_same<T, bf16>::value) {
+            if (fast) {
+                async16(smem_at(at), q, in);
+                continue;
+            }
+        }
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        if (in) {
+            if (fast) {
+                constexpr int kLoads = 8 * (int)sizeof(T) / 16;
+                uint4 u[kLoads];
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j) u[j] = reinterpret_cast<const uint4*>(q)[j];
+                const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = to_f(e[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (c + j < cols) x[j] = to_f(q[j]);
+            }
+        }
+        uint32_t t[4][N];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) terms<N>(x[2 * j], x[2 * j + 1], t[j]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(at + n * kPlane) = make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]);
+    }
+}
+// N planes of a 64 x 64 tile from the workspace (rows of 64) to rows of kSquare
+template <int N, int THREADS>
+__device__ __forceinline__ void load_square(bf16* to, const bf16* p, int tid) {
+    for (int i = tid; i < N * kTicks * 8; i += THREADS) async16(smem_at(to + (i >> 3) * kSquare + (i & 7) * 8), p + i * 8, true);
+}
+
+// 16 sums over the 8 lanes with the same t4, of v[2 j + i] = a value of column 8 j + 2 t4 + i: lane g keeps columns 8 g + 2 t4, + 1
+__device__ __forceinline__ float2 column_sums(float (&v)[16], int lane) {
+#pragma unroll
+    for (int half = 8; half >= 2; half >>= 1) {
+        const int bit = half * 2;                            // lanes 16, 8, 4 apart
+        const bool upper = lane & bit;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float give = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
+    }
+    return make_float2(v[0], v[1]);
+}
+
+// the types' terms: of inputs, of what is carried (states, corrections), of outputs
+template <class T> struct Terms;
+template <> struct Terms<bf16> { static constexpr int in = 1, kept = 2, out = 1; };
+template <> struct Terms<__half> { static constexpr int in = 2, kept = 2, out = 2; };
+template <> struct Terms<float> { static constexpr int in = 3, kept = 3, out = 3; };
+
+}  // namespace

@@ -1,0 +1,257 @@
+// The gradients of q, k and the gates, every chunk by itself, from what the chain forward (S before the chunk, U) and the chain back
+// (R behind it, dN, rows of dots) have left:
+//
+//   dP = dO U^T . M on and below the diagonal, D = -dN U^T . M below it
+//   dQ = scale (e^G dO S^T + dP K),  dK = scale dP^T Q + (D + D^T) K - e^G dN S^T + e^{G_63 - G} U R^T
+//   dbeta: the tiles' rows added;  dlog_decay_t = <R, S> + sum over t' >= t of (o dO - v dN)_t'
+//
+// A block of 8 warps makes 64 columns of one chunk of one head: warp = 16 ticks x 32 columns. The products with S and R run over blocks of 64 of
+// their columns; S and R arrive as the chain's left operands and go through shared memory, where reading across turns them.
+#pragma once
+#include "fg_delta_chain.cuh"
+
+namespace {
+
+template <class T>
+struct GradLayout {
+    static constexpr int in = Terms<T>::in, kept = in == 1 ? 1 : Terms<T>::kept, plane = kTicks * kSquare;
+    static constexpr int q = 0, k = q + in * plane, go = k + in * plane, dn = go + in * plane, u = dn + kept * plane, s = u + kept * plane,
+                         r = s + kept * plane, values = r + kept * plane;
+    static constexpr int dp = go, d = dp + kept * plane;     // later, over what is read by then
+    static constexpr int bytes = 2 * values + 4 * kGates * kTicks;
+    static_assert(2 * kept <= in + 4 * kept && bytes <= 227 * 1024, "room");
+};
+
+template <class T>
+__global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(const __grid_constant__ Delta s) {
+    using Lay = GradLayout<T>;
+    constexpr int NI = Lay::in, NK = Lay::kept, kPlane = Lay::plane;
+    constexpr int NB = Terms<T>::kept;                       // terms that a product keeps where both sides have several
+    constexpr int kKeep = NI == 1 ? 1 : NB;
+    extern __shared__ __align__(16) unsigned char smem[];
+    bf16* tiles = reinterpret_cast<bf16*>(smem);
+    float* gates = reinterpret_cast<float*>(smem + 2 * Lay::values);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const long long slot = blockIdx.x, place = slot * s.heads + blockIdx.y;
+    const int h = blockIdx.y, d_block = 64 * blockIdx.z, all_d = (s.D + 15) / 16, tiles_e = (s.E + 15) / 16;
+    const int padded_d = s.D > 64 ? 8 : 4;                   // the chain's 16-value pieces of a column
+    const Chunk c = chunk_of(s, slot);
+    if (c.n == 0) return;
+    const long long tick = (s.offsets ? span_of(s, c.b).start : 0) + c.first;
+    const int wt = warp >> 1, wd = warp & 1;                 // ticks 16 wt .., columns (of d, or ticks s) 32 wd ..
+
+    load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::q, row_of<const T>(s, s.q, c.b, h, tick) + d_block, s.q.tick, c.n, s.D - d_block, s.q.fast, tid);
+    load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::k, row_of<const T>(s, s.k, c.b, h, tick) + d_block, s.k.tick, c.n, s.D - d_block, s.k.fast, tid);
+    for (int i = tid; i < kGates * kTicks; i += 256) gates[i] = s.gates[place * kGates * kTicks + i];
+
+    // the gates' gradients
+    if (blockIdx.z == 0 && warp == 0) {
+        float dot[2] = {}, db[2] = {}, anchor = 0.f;
+        for (int e = 0; e < tiles_e; ++e) {
+            const long long at = (place * tiles_e + e) * kTicks + 2 * lane;
+            const float2 o = *reinterpret_cast<const float2*>(s.od + at), v = *reinterpret_cast<const float2*>(s.vdn + at),
+                         x = *reinterpret_cast<const float2*>(s.db + at);
+            dot[0] += o.x - v.x;
+            dot[1] += o.y - v.y;
+            db[0] += x.x;
+            db[1] += x.y;
+            anchor += s.anchor[place * tiles_e + e];
+        }
+        float after = dot[0] + dot[1];                       // of this lane's ticks and all later ones
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float x = __shfl_down_sync(0xffffffffu, after, o);
+            if (lane + o < 32) after += x;
+        }
+        const float next = __shfl_down_sync(0xffffffffu, after, 1);
+        const float rest = (lane < 31 ? next : 0.f) + anchor;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = 2 * lane + i;
+            if (t >= c.n) continue;
+            *gate_of(s, s.glog_decay, c.b, h, tick + t) = i ? rest + dot[1] : rest + dot[1] + dot[0];
+            *gate_of(s, s.gbeta, c.b, h, tick + t) = db[i];
+        }
+    }
+
+    float dq[4][4] = {}, dk[4][4] = {}, du[4][4] = {}, dp[4][4] = {}, dd[4][4] = {};
+    const uint32_t at_m = smem_at(tiles) + at_rows_m(lane, kSquare), at_n = smem_at(tiles) + at_rows_n(lane, kSquare);
+    const bool below = 32 * wd <= 16 * wt;                   // this warp's ticks s x t meet the diagonal's lower side
+#pragma unroll 1
+    for (int e0 = 0; e0 < s.E; e0 += 64) {
+        if (e0) __syncthreads();
+        load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::go, row_of<const T>(s, s.go, c.b, h, tick) + e0, s.go.tick, c.n, s.E - e0, s.go.fast, tid);
+        if (s.dn_f32)
+            load_tile<float, NK, 64, kSquare, 256>(tiles + Lay::dn, row_of<const float>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0,
+                                                   s.dn.fast, tid);
+        else if constexpr (sizeof(T) == 2)
+            load_tile<T, NK, 64, kSquare, 256>(tiles + Lay::dn, row_of<const T>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast,
+                                               tid);
+        using U = std::conditional_t<NI == 1, bf16, float>;
+        load_tile<U, NK, 64, kSquare, 256>(tiles + Lay::u, reinterpret_cast<const U*>(s.u) + place * kTicks * 16 * tiles_e + e0, 16 * tiles_e,
+                                           kTicks, 16 * tiles_e - e0, true, tid);
+        async_commit();
+        // S and R: left operands of 16 columns x 16 values -> rows of columns
+        for (int i = warp; i < 2 * NK * 16; i += 8) {
+            const int which = i & 1, n = (i >> 1) % NK, piece = (i >> 1) / NK, te = piece >> 2, td = piece & 3, e = e0 / 16 + te;
+            uint32_t r[4] = {0, 0, 0, 0};
+            if (e < tiles_e && d_block / 16 + td < all_d) {
+                const int kept = which ? NK : NB;
+                const uint4 u = (which ? s.gstates : s.states)[(((place * tiles_e + e) * kept + n) * padded_d + d_block / 16 + td) * 32 + lane];
+                r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
+            }
+            const uint32_t to = smem_at(tiles) + 2 * ((which ? Lay::r : Lay::s) + n * kPlane + 16 * te * kSquare + 16 * td) + at_rows_m(lane, kSquare);
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                         : "memory");
+        }
+        async_wait<0>();
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t go[NI][4], dn[NK][4], u[NK][4];
+#pragma unroll
+            for (int n = 0; n < NI; ++n) ldsm(go[n], at_m + 2 * (Lay::go + n * kPlane + 16 * wt * kSquare + 16 * e));
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                ldsm(dn[n], at_m + 2 * (Lay::dn + n * kPlane + 16 * wt * kSquare + 16 * e));
+                ldsm(u[n], at_m + 2 * (Lay::u + n * kPlane + 16 * wt * kSquare + 16 * e));
+            }
+#pragma unroll
+            for (int jp = 0; jp < 2; ++jp)
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    uint32_t b[4];
+                    ldsm_t(b, at_m + 2 * (Lay::s + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * jp));
+#pragma unroll
+                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
+                        if (t < NI) {
+                            mma(dq[2 * jp], go[t < NI ? t : 0], b[0], b[1]);
+                            mma(dq[2 * jp + 1], go[t < NI ? t : 0], b[2], b[3]);
+                        }
+                        mma(dk[2 * jp], dn[t], b[0], b[1]);
+                        mma(dk[2 * jp + 1], dn[t], b[2], b[3]);
+                    }
+                    ldsm_t(b, at_m + 2 * (Lay::r + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * jp));
+#pragma unroll
+                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
+                        mma(du[2 * jp], u[t], b[0], b[1]);
+                        mma(du[2 * jp + 1], u[t], b[2], b[3]);
+                    }
+                    if (below) {
+                        ldsm(b, at_n + 2 * (Lay::u + j * kPlane + (32 * wd + 16 * jp) * kSquare + 16 * e));
+#pragma unroll
+                        for (int t = 0; t < NK && t + j < kKeep; ++t) {
+                            if (t < NI) {
+                                mma(dp[2 * jp], go[t < NI ? t : 0], b[0], b[1]);
+                                mma(dp[2 * jp + 1], go[t < NI ? t : 0], b[2], b[3]);
+                            }
+                            mma(dd[2 * jp], dn[t], b[0], b[1]);
+                            mma(dd[2 * jp + 1], dn[t], b[2], b[3]);
+                        }
+                    }
+                }
+        }
+    }
+    __syncthreads();                                          // dO, dN and U have been read
+    const float *from0 = gates, *to_end = gates + kTicks, *gh = gates + 3 * kTicks, *gl = gates + 4 * kTicks;
+    if (below) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = 16 * wt + g + 8 * i, c0 = 32 * wd + 8 * j + 2 * t4;
+                float x[2], y[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float f = t >= c0 + e ? expf((gh[t] - gh[c0 + e]) + (gl[t] - gl[c0 + e])) : 0.f;
+                    x[e] = t >= c0 + e ? dp[j][2 * i + e] * (f * s.scale) : 0.f;
+                    y[e] = t > c0 + e ? -dd[j][2 * i + e] * f : 0.f;
+                }
+                uint32_t a[NK], b[NK];
+                terms<NK>(x[0], x[1], a);
+                terms<NK>(y[0], y[1], b);
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    *reinterpret_cast<uint32_t*>(tiles + Lay::dp + n * kPlane + t * kSquare + c0) = a[n];
+                    *reinterpret_cast<uint32_t*>(tiles + Lay::d + n * kPlane + t * kSquare + c0) = b[n];
+                }
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = 16 * wt + g + 8 * i;
+        const float f = from0[t], k = to_end[t];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 2 * i; e < 2 * i + 2; ++e) {
+                dq[j][e] *= f * s.scale;
+                dk[j][e] = fmaf(-f, dk[j][e], k * du[j][e]);
+            }
+    }
+    __syncthreads();
+    // rows of dP and D by K; columns of dP by Q, of D by K
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint32_t a[NK][4], b[NK][4], kk[NI][2][4], qq[NI][2][4];
+        const bool row = k <= wt, column = k >= wt;
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int jp = 0; jp < 2; ++jp) {
+                ldsm_t(kk[n][jp], at_m + 2 * (Lay::k + n * kPlane + 16 * k * kSquare + 32 * wd + 16 * jp));
+                if (column) ldsm_t(qq[n][jp], at_m + 2 * (Lay::q + n * kPlane + 16 * k * kSquare + 32 * wd + 16 * jp));
+            }
+        if (row) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                ldsm(a[n], at_m + 2 * (Lay::dp + n * kPlane + 16 * wt * kSquare + 16 * k));
+                ldsm(b[n], at_m + 2 * (Lay::d + n * kPlane + 16 * wt * kSquare + 16 * k));
+            }
+#pragma unroll
+            for (int jp = 0; jp < 2; ++jp)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
+                        mma(dq[2 * jp], a[t], kk[j][jp][0], kk[j][jp][1]);
+                        mma(dq[2 * jp + 1], a[t], kk[j][jp][2], kk[j][jp][3]);
+                        mma(dk[2 * jp], b[t], kk[j][jp][0], kk[j][jp][1]);
+                        mma(dk[2 * jp + 1], b[t], kk[j][jp][2], kk[j][jp][3]);
+                    }
+        }
+        if (column) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                ldsm_t(a[n], at_n + 2 * (Lay::dp + n * kPlane + 16 * k * kSquare + 16 * wt));
+                ldsm_t(b[n], at_n + 2 * (Lay::d + n * kPlane + 16 * k * kSquare + 16 * wt));
+            }
+#pragma unroll
+            for (int jp = 0; jp < 2; ++jp)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
+                        mma(dk[2 * jp], a[t], qq[j][jp][0], qq[j][jp][1]);
+                        mma(dk[2 * jp + 1], a[t], qq[j][jp][2], qq[j][jp][3]);
+                        mma(dk[2 * jp], b[t], kk[j][jp][0], kk[j][jp][1]);
+                        mma(dk[2 * jp + 1], b[t], kk[j][jp][2], kk[j][jp][3]);
+                    }
+        }
+    }
+    const auto put = [&](const Operand& o, int f32, const float (&x)[4][4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = 16 * wt + g + 8 * (e >> 1), d = d_block + 32 * wd + 8 * j + 2 * t4 + (e & 1);
+                if (t >= c.n || d >= s.D) continue;
+                if (f32) row_of<float>(s, o, c.b, h, tick + t)[d] = x[j][e];
+                else row_of<T>(s, o, c.b, h, tick + t)[d] = from_f<T>(x[j][e]);
+            }
+    };
+    put(s.gq, s.gq_f32, dq);
+    put(s.gk, s.gk_f32, dk);
+}
+
+}  // namespace

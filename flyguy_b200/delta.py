@@ -1,0 +1,207 @@
+"""A memory over ticks that overwrites (beside flyguy_b200.memory, whose states only fade): the gated delta rule.
+
+  delta_attention   the rule over whole recordings (also packed end to end), with gradients of all its inputs
+  delta_step        the same for one tick, the states updated in place
+
+S_t = g_t S_{t-1} + k_t u_t^T with u_t = beta_t (v_t - g_t k_t S_{t-1}): what the state holds at a tick's key is moved towards the tick's
+value by beta, everything else fades by g = exp(log_decay). Both gates are each tick's own. o_t = scale q_t S_t. Bounded where
+beta |k|^2 is at most 2: keys of about unit length (memory.norm_rotate with k_weight dim^-0.5).
+
+They run in the library (fg_delta_attn, fg_delta_step of include/flyguy_b200.h) on CUDA tensors, on torch's current stream.
+Queries, keys and values are float32, bfloat16 or float16 of one type, any strides with a head's values adjacent (others are copied
+first); gates and states are float32. Gradients are of the first order. DeltaMemory puts the operators together.
+
+Products run on the tensor cores in bfloat16 terms: what is carried from chunk to chunk (states, corrections and their gradients)
+has two terms, 2^-17 of each value, three and 2^-24 where the inputs are float32, and sums are float32. Outputs and the gradients of q, k
+and v of bfloat16 are made of once rounded operands, each of the size of the result's own rounding."""
+from __future__ import annotations
+
+import math
+import struct
+from functools import lru_cache
+
+import torch
+from torch import nn
+from torch.autograd.graph import increment_version
+
+from . import layers, memory
+from .memory import TYPES, _call, _float32, _grad, _kept, _no_tangents, _NONE, _offsets, _once, _ptr, _room, _state, _ticks, _values
+from .native import FlyguyError, lib
+
+# fg_delta_args: q, k, v, o, go, gq, gk, gv, log_decay, beta, glog_decay, gbeta (fg_ticks), state, state_out, gstate_out, gstate, offsets,
+# batch, ticks, heads, query_heads, key_heads, value_heads, dim, value_dim, type, scale, work, work_bytes
+_DELTA = struct.Struct("=48q5q9qd2q")
+# fg_delta_step_args: q, k, v, o, log_decay, beta (fg_ticks), state, slots, n_slots, batch, heads, query_heads, key_heads, value_heads, dim,
+# value_dim, type, scale
+_STEP = struct.Struct("=24q11qd")
+
+
+def _gate(name: str, t, lead: tuple, like: torch.Tensor) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != like.get_device():
+        raise FlyguyError(f"{name} must be a float32 tensor on {like.device}")
+    if t.dim() != len(lead) + 1 or t.shape[:-1] != lead:
+        raise FlyguyError(f"{name} must be {(*lead, 'heads')}, not {tuple(t.shape)}")
+    return t
+
+
+def _head_counts(q, k, v, log_decay, beta) -> tuple[int, int, int, int]:
+    """heads, query heads, key heads, value heads."""
+    heads = log_decay.shape[-1]
+    if beta.shape != log_decay.shape:
+        raise FlyguyError(f"beta must be {tuple(log_decay.shape)} as log_decay is, not {tuple(beta.shape)}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.shape[-2] or not heads or heads % t.shape[-2]:
+            raise FlyguyError(f"{heads} heads (of the gates) cannot share {t.shape[-2]} heads of {name}")
+    return heads, q.shape[-2], k.shape[-2], v.shape[-2]
+
+
+def _gate_ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
+    """fg_ticks of [batch, ticks, heads] or [ticks, heads]."""
+    st = t.stride()
+    return (t.data_ptr(), *st) if len(st) == 3 else (t.data_ptr(), 0, *st)
+
+
+@lru_cache(maxsize=256)
+def _delta_room(sizes: tuple, packed: bool, backward: bool) -> int:
+    """Bytes of workspace that a call of these sizes needs (fg_delta_work)."""
+    size = lib().fg_delta_work(_DELTA.pack(*(0,) * 52, int(packed), *sizes, 1.0, 0, 0), int(backward))
+    if size < 0:                                          # (raised here: an error is not kept)
+        raise FlyguyError(lib().fg_mem_last_error().decode())
+    return size
+
+
+class _Delta:
+    """What forward and backward of one call share."""
+
+    def __init__(self, q, k, v, log_decay, beta, state, scale, offsets):
+        lead, dim, value_dim = q.shape[:-2], q.shape[-1], v.shape[-1]
+        if k.shape[:-2] != lead or k.shape[-1] != dim or v.shape[:-2] != lead:
+            raise FlyguyError(f"k and v must be {(*lead, 'key heads', dim)} and {(*lead, 'value heads', 'value dim')}, not "
+                              f"{tuple(k.shape)} and {tuple(v.shape)}")
+        if offsets is None:
+            batch, ticks = lead if len(lead) == 2 else (1, lead[0])
+        else:
+            if len(lead) != 1:
+                raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
+            offsets = _offsets(offsets, q)
+            batch, ticks = offsets.shape[0] - 1, lead[0]
+        heads = _head_counts(q, k, v, log_decay, beta)
+        self.states, self.device, self.offsets = (batch, heads[0], dim, value_dim), q.get_device(), offsets
+        if state is not None:
+            _float32("state", state, q, self.states)
+        self.sizes = (batch, ticks, *heads, dim, value_dim, TYPES[q.dtype])
+        self.scale = float(dim ** -0.5 if scale is None else scale)
+
+    def let_go(self) -> torch.Tensor | None:
+        """The offsets, for autograd to keep until the backward."""
+        kept, self.offsets = _kept(self.offsets), None
+        return kept
+
+    def take_up(self, offsets):
+        again = object.__new__(_Delta)
+        again.__dict__.update(self.__dict__, offsets=offsets)
+        return again
+
+    def run(self, fn, backward: bool, tensors, gates, state=None, state_out=None, gstate_out=None, gstate=None) -> None:
+        room, work = _room(_delta_room(self.sizes, self.offsets is not None, backward), tensors[0].device)
+        packed = _DELTA.pack(*(f for t in tensors for f in (_NONE if t is None else _ticks(t))),
+                             *(f for t in gates for f in (_NONE if t is None else _gate_ticks(t))), _ptr(state), _ptr(state_out),
+                             _ptr(gstate_out), _ptr(gstate), _ptr(self.offsets), *self.sizes, self.scale, *work)
+        _call(fn, packed, self.device)
+
+    def forward(self, q, k, v, log_decay, beta, state):
+        o = torch.empty((*q.shape[:-2], self.states[1], v.shape[-1]), dtype=q.dtype, device=q.device)
+        end = torch.empty(self.states, dtype=torch.float32, device=q.device)
+        self.run(lib().fg_delta_attn, False, (q, k, v, o, None, None, None, None), (log_decay, beta, None, None), state, end)
+        return o, end
+
+    def backward(self, q, k, v, log_decay, beta, state, go, gend, want_state: bool):
+        go = _grad("the gradient of o", go, q, (*q.shape[:-2], self.states[1], v.shape[-1]))
+        if gend is not None:
+            gend = _state(gend.float())
+        gq, gk, gv, gl, gb = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, log_decay, beta))
+        gstate = torch.empty(self.states, dtype=torch.float32, device=q.device) if want_state else None
+        self.run(lib().fg_delta_attn_bwd, True, (q, k, v, None, go, gq, gk, gv), (log_decay, beta, gl, gb), state, None, gend, gstate)
+        return gq, gk, gv, gl, gb, gstate
+
+
+class _DeltaFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, beta, state, job):
+        ctx.set_materialize_grads(False)
+        q, k, v = (_values("q", t, (3, 4)) for t in (q, k, v))
+        state = _state(state)
+        out = job.forward(q, k, v, log_decay, beta, state)
+        ctx.job = job
+        ctx.save_for_backward(q, k, v, log_decay, beta, state, job.let_go())
+        return out
+
+    @staticmethod
+    @_once
+    def backward(ctx, go, gend):
+        *ins, offsets = ctx.saved_tensors
+        return *ctx.job.take_up(offsets).backward(*ins, go, gend, ctx.needs_input_grad[5]), None
+
+
+def delta_attention(q, k, v, log_decay, beta, state=None, scale: float | None = None,
+                    offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gated delta rule for every recording and head: S_t = exp(log_decay_t) S_{t-1} + k_t u_t^T, u_t = beta_t (v_t -
+    exp(log_decay_t) k_t S_{t-1}), o_t = scale q_t S_t.
+
+    log_decay and beta float32 [batch, ticks, heads]; q [batch, ticks, query heads, dim], k [.., key heads, dim] and v [.., value
+    heads, value dim], each number of heads a divisor of `heads` (head h has query head h / (heads / query heads), and so on). Or
+    [ticks, ..] with recordings packed end to end and offsets int64 [recordings + 1], not falling (recordings may be empty; ticks
+    before the first and after the last get zeros, in o and in the gradients). state float32 [recordings, heads, dim, value
+    dim] before the first ticks (None: zeros). scale: dim^-0.5 when None. dim at most 128, value dim at most 256.
+    log_decay is at most 0, minus infinity forgets the state (anything below -256 does, in float32).
+    Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v, log_decay, beta and state.
+
+    A recording's ticks are worked on in tiles of 64: a NaN or an infinity stays in its recording and head and out of the tiles
+    before it, but reaches all ticks of its own and those after it, and infinities become NaN (delta_step goes tick by tick)."""
+    q = _values("q", q, (3, 4))
+    k, v = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
+    log_decay, beta = _gate("log_decay", log_decay, q.shape[:-2], q), _gate("beta", beta, q.shape[:-2], q)
+    job = _Delta(q, k, v, log_decay, beta, state, scale, offsets)
+    _no_tangents(q, k, v, log_decay, beta, state)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, beta, state)):
+        return _DeltaFn.apply(q, k, v, log_decay, beta, state, job)
+    return job.forward(q, k, v, log_decay, beta, _state(state))
+
+
+def delta_step(q, k, v, log_decay, beta, state, scale: float | None = None, slots=None) -> torch.Tensor:
+    """One tick of delta_attention for a batch: q [batch, query heads, dim], k [batch, key heads, dim], v [batch, value heads, value
+    dim], log_decay and beta float32 [batch, heads]. state float32 [slots, heads, dim, value dim], contiguous, is updated in place
+    at each row's slot (slots int64 [batch], no two alike; None: row b's is b); a row whose slot is outside answers 0 and changes
+    nothing. dim and value dim at most 256. Returns o [batch, heads, value dim]. No gradient: for learning, delta_attention."""
+    q, k, v = _values("q", q, (3,)), _values("k", k, (3,), q), _values("v", v, (3,), q)
+    batch, _, dim = q.shape
+    value_dim = v.shape[-1]
+    if k.shape[0] != batch or k.shape[-1] != dim or v.shape[0] != batch:
+        raise FlyguyError(f"k and v must be {(batch, 'key heads', dim)} and {(batch, 'value heads', 'value dim')}, not "
+                          f"{tuple(k.shape)} and {tuple(v.shape)}")
+    log_decay, beta = _gate("log_decay", log_decay, (batch,), q), _gate("beta", beta, (batch,), q)
+    heads = _head_counts(q, k, v, log_decay, beta)
+    if (not isinstance(state, torch.Tensor) or state.dtype is not torch.float32 or state.get_device() != q.get_device()
+            or state.dim() != 4 or state.shape[1:] != (heads[0], dim, value_dim) or not state.is_contiguous()):
+        raise FlyguyError(f"state must be contiguous float32 {('slots', heads[0], dim, value_dim)} on {q.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, beta, state)):
+        raise FlyguyError("delta_step has no gradient (delta_attention has): call it under torch.no_grad()")
+    _no_tangents(q, k, v, log_decay, beta, state)
+    if slots is not None:
+        if (not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.get_device() != q.get_device()
+                or slots.shape != (batch,)):
+            raise FlyguyError(f"slots must be int64 [{batch}] on {q.device}")
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
+    elif state.shape[0] < batch:
+        raise FlyguyError(f"{batch} rows need as many states, not {state.shape[0]}")
+    o = torch.empty((batch, heads[0], value_dim), dtype=q.dtype, device=q.device)
+    f = []
+    for t in (q, k, v, o, log_decay, beta):
+        st = t.stride()
+        f += (t.data_ptr(), st[0], 0, st[1])
+    packed = _STEP.pack(*f, state.data_ptr(), _ptr(slots), state.shape[0], batch, *heads, dim, value_dim, TYPES[q.dtype],
+                        float(dim ** -0.5 if scale is None else scale))
+    _call(lib().fg_delta_step, packed, q.get_device())
+    increment_version(state)                              # (autograd sees that it has changed, should it have kept it)
+    return o

@@ -65,6 +65,14 @@ SIGNATURES = {
     "fg_decay_attn_bwd": (_ci, [_vp, _vp]),
     "fg_decay_work": (_cll, [_vp, _ci]),
     "fg_decay_step": (_ci, [_vp, _vp]),
+    "fg_delta_attn": (_ci, [_vp, _vp]),
+    "fg_delta_attn_bwd": (_ci, [_vp, _vp]),
+    "fg_delta_work": (_cll, [_vp, _ci]),
+    "fg_delta_step": (_ci, [_vp, _vp]),
+    "fg_layer_norm": (_ci, [_vp, _vp]),
+    "fg_layer_norm_bwd": (_ci, [_vp, _vp]),
+    "fg_layer_norm_work": (_cll, [_vp]),
+    "fg_dropout": (_ci, [_vp, _vp]),
     "fg_mem_sync": (_ci, [_vp]),
     "fg_mem_last_error": (ctypes.c_char_p, []),
     "fg_train_main": (_ci, [_ci, ctypes.POINTER(ctypes.c_char_p)]),

@@ -292,11 +292,87 @@ typedef struct fg_step_args {
 
 /* One tick of fg_decay_attn for each row, its state updated in place. */
 int fg_decay_step(const fg_step_args* args, void* stream);
+typedef struct fg_delta_args {
+    fg_ticks q, k, v, o;              /* [.., query_heads, dim], [.., key_heads, dim], [.., value_heads, value_dim], [.., heads, value_dim] */
+    fg_ticks go, gq, gk, gv;          /* backward */
+    fg_ticks log_decay, beta;         /* fp32 [.., heads] */
+    fg_ticks glog_decay, gbeta;       /* backward, fp32 */
+    const float* state;               /* [batch, heads, dim, value_dim] before the first tick, or NULL: zeros */
+    float* state_out;                 /* after the last tick (may not overlap state) */
+    const float* gstate_out;          /* backward: gradient of state_out, or NULL: zeros */
+    float* gstate;                    /* backward: gradient of state, or NULL: not wanted; neither state nor gstate_out */
+    const long long* offsets;         /* [batch + 1] first ticks of recordings packed end to end, or NULL: all of `ticks` */
+    long long batch, ticks;           /* with offsets: ticks of all recordings together */
+    long long heads, query_heads, key_heads, value_heads, dim, value_dim, type;
+    double scale;
+    void* work;                       /* fg_delta_work bytes, 16-byte aligned */
+    long long work_bytes;
+} fg_delta_args;
+
+/* The gated delta rule. For every recording and head h (queries, keys and values of head h / (heads / query_heads) and so on), with
+ * g_t = exp(log_decay_t):
+ *   S_t = g_t S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - g_t k_t S_{t-1}),   o_t = scale q_t S_t.
+ * Bounded where beta |k|^2 is at most 2. log_decay is at most 0; below -256 it is taken as -256, a state forgotten. dim to 128,
+ * value_dim to 256. As with fg_decay_attn: states are fp32, outputs overlap nothing, ticks of no recording get zeros, offsets may not
+ * fall and are clamped, and a NaN or an infinity reaches all ticks of its tile of 64 and all later ones of its recording and head. */
+int fg_delta_attn(const fg_delta_args* args, void* stream);
+/* Gradients of q, k, v, log_decay, beta and state; o and state_out are unused. */
+int fg_delta_attn_bwd(const fg_delta_args* args, void* stream);
+long long fg_delta_work(const fg_delta_args* args, int backward);
+
+typedef struct fg_delta_step_args {
+    fg_ticks q, k, v, o;              /* one tick: the tick stride is unused */
+    fg_ticks log_decay, beta;         /* fp32 [batch, heads] */
+    float* state;                     /* [slots, heads, dim, value_dim], updated in place */
+    const long long* slots;           /* as in fg_step_args */
+    long long n_slots;
+    long long batch, heads, query_heads, key_heads, value_heads, dim, value_dim, type;
+    double scale;
+} fg_delta_step_args;
+
+/* One tick of fg_delta_attn for each row, its state updated in place; dim and value_dim to 256. */
+int fg_delta_step(const fg_delta_step_args* args, void* stream);
+
 /* Waits for the stream; -1 if a call of these on the current device gave up a wait on the tensor cores (about 2 s; the outputs,
  * gradients and states of its recording and head then hold NaN), now or earlier in this process. */
 int fg_mem_sync(void* stream);
 /* Why the calling thread's last call of these failed ("" after a success). */
 const char* fg_mem_last_error(void);
+
+/* ---- the layers around a memory -----------------------------------------------------------------------------------
+ * In the manner of the memory's operators above: the caller's buffers and stream, 8-byte fields, 0 or -1 with the reason in
+ * fg_mem_last_error(). */
+
+typedef struct fg_norm_args {
+    const void *x;                    /* rows of `dim` adjacent values, x_row apart */
+    void *y;                          /* [rows, dim] */
+    const void *gy;                   /* backward: rows gy_row apart */
+    void *gx;                         /* backward: [rows, dim] */
+    const float *w, *b;               /* [dim], or NULL: ones, zeros */
+    float *gw, *gb;                   /* backward: written; NULL: not wanted */
+    long long rows, dim, x_row, gy_row, type;
+    double eps;
+    void* work;                       /* backward with gw or gb: fg_layer_norm_work bytes, 16-byte aligned */
+    long long work_bytes;
+} fg_norm_args;
+
+/* y = (x - mean) / sqrt(mean((x - mean)^2) + eps) w + b of each row; statistics and products in fp32, rounded once. */
+int fg_layer_norm(const fg_norm_args* args, void* stream);
+/* gx, gw and gb from x and gy (y and b unused). The sums of gw and gb run in a fixed order. */
+int fg_layer_norm_bwd(const fg_norm_args* args, void* stream);
+long long fg_layer_norm_work(const fg_norm_args* args);
+
+typedef struct fg_dropout_args {
+    const void *x, *add;              /* n adjacent values each; add may be NULL (zeros) */
+    void* y;                          /* may be x or add */
+    const long long* seed;            /* on the device, read when the kernel runs; or NULL: seed_value */
+    long long seed_value, call, n, least, type;
+} fg_dropout_args;
+
+/* y = add + (bits(i) >= least ? x 65536 / (65536 - least) : 0), least 0..65535. bits(i): the 16 bits of number (i mod 8), low halves
+ * first, in the four words that Philox4x32-10 makes of the counter (i / 8, call), low words first, with the key seed. The gradient
+ * is the same of y's. */
+int fg_dropout(const fg_dropout_args* args, void* stream);
 
 /* ---- the standalone teaching trainer (replaces the reference's flyguy_train executable, flyguy/native/
  * flyguy_train.cu main() at 631-788): argv as the command line "fg_train NET.bin PARAMS.bin DATA_DIR OUT_PREFIX
