@@ -516,6 +516,7 @@ int fg_mem_sync(void* stream) {
         MCK(cudaMemcpyFromSymbolAsync(&bad, g_tc_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
         MCK(cudaStreamSynchronize(st));
         need(!bad, "fg_decay_attn: a wait on the tensor cores ran out; its results are not to be used");
+        need(!step_gave_up(st), "fg_delta_step: a wait for a state ran out; its results are not to be used");
         return 0;
     });
 }

@@ -25,9 +25,10 @@ struct Step {
 };
 // A block takes 32 columns of a row's state of one head, whole in registers: V columns a thread of every (256 V / 32)-th row. One
 // pass over them gives k S and q S, and o = q S + (q k) u needs no second one. State in and out is the cost.
-template <class T, int V>
-__global__ void __launch_bounds__(256) k_delta_step(const __grid_constant__ Step s) {
-    constexpr int kAcross = 32 / V, kRows = 256 / kAcross, kPer = kMaxStep / kRows;
+// V columns and PER rows a thread
+template <class T, int V, int PER>
+__global__ void __launch_bounds__(256, PER * V <= 16 ? 5 : 3) k_delta_step(const __grid_constant__ Step s) {
+    constexpr int kAcross = 32 / V, kRows = 256 / kAcross, kPer = PER;
     __shared__ float sq[kMaxStep], sk[kMaxStep], pred[8][32], out[8][32], qk_part[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     long long item = blockIdx.x;
@@ -125,6 +126,206 @@ __global__ void __launch_bounds__(256) k_delta_step(const __grid_constant__ Step
                 o[e0 + j] = from_f<T>(fmaf(qk, u[j], p) * s.scale);
             }
         }
+    }
+}
+
+// Many rows: a block goes from one (row, head) to the next with three places for a state in shared memory. A warp of its own brings whole
+// states as bulk copies, the next two while one is worked on, and sends them off again; 16 warps work, V = 4 columns a thread of every R-th
+// row. D E at most 16,384 (64 KB), at most 32 values a thread.
+constexpr int kWideThreads = 512, kWidePer = 8, kWidePlaces = 3, kWideSums = 2 * 16 * kWideThreads;
+__device__ int g_step_error;              // a wait ran out (fg_mem_sync)
+struct WideLayout {
+    int state, bytes;                // of a place, of the block
+    __host__ __device__ WideLayout(int D, int E) : state(D * E * 4), bytes(kWidePlaces * D * E * 4 + kWideSums + 4 * 5 * kMaxStep + 64) {}
+};
+// a phase of a barrier, given up after about 2 s
+__device__ __forceinline__ bool phase_of(uint32_t bar, uint32_t parity) {
+    uint32_t done = 0;
+    for (int tries = 0; !done && tries < 20000; ++tries)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    return done != 0;
+}
+// the workers' barrier; whether all of them say yes
+__device__ __forceinline__ bool workers(bool yes) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "barrier.cta.red.and.pred p, 1, 512, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)yes)
+        : "memory");
+    return all != 0;
+}
+template <class T>
+__global__ void __launch_bounds__(kWideThreads + 32, 1) k_delta_step_wide(const __grid_constant__ Step s, uint32_t items) {
+    static_assert(kWideThreads == 512, "the workers' barrier");
+    extern __shared__ __align__(128) unsigned char smem[];
+    const WideLayout lay(s.D, s.E);
+    float4* part = reinterpret_cast<float4*>(smem + kWidePlaces * lay.state);          // [R][E / 4] of k S, then of q S
+    float* row = reinterpret_cast<float*>(smem + kWidePlaces * lay.state + kWideSums);   // two places: k, q; then u
+    uint64_t* bars = reinterpret_cast<uint64_t*>(row + 5 * kMaxStep);
+    const int tid = threadIdx.x, C = s.E / 4, R = kWideThreads / C, r = tid / C, c = tid - r * C;
+    const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), full = (uint32_t)__cvta_generic_to_shared(bars), done = full + 8 * kWidePlaces;
+    if (tid < 2 * kWidePlaces)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full + 8 * tid), "r"(tid < kWidePlaces ? 1 : kWideThreads / 32) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    // this block's i-th item is blockIdx.x + i gridDim.x; its state goes to place i mod 3. An item without a slot uses no place.
+    const auto nth = [&](uint32_t i) { return blockIdx.x + i * gridDim.x; };
+    const auto slot_of = [&](uint32_t item) {
+        const uint32_t b = item / (uint32_t)s.heads;
+        const long long slot = s.slots ? s.slots[b] : b;
+        return slot >= 0 && slot < s.n_slots ? slot : -1;
+    };
+    if (tid >= kWideThreads) {
+        if (tid != kWideThreads) return;
+        uint32_t fetched = 0, phases = 0, open = 0;          // open: places whose copy has been asked for, and not answered by the workers
+        long long slots[kWidePlaces];
+        const auto fetch = [&]() {
+            const uint32_t item = nth(fetched), place = fetched % kWidePlaces;
+            ++fetched;
+            if (item >= items) return;
+            const long long slot = slots[place] = slot_of(item);
+            if (slot < 0) return;
+            open |= 1u << place;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * place), "r"(lay.state) : "memory");
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(sm + place * lay.state),
+                         "l"(s.state + (slot * s.heads + item % (uint32_t)s.heads) * s.D * s.E), "r"(lay.state), "r"(full + 8 * place)
+                         : "memory");
+        };
+        for (int i = 0; i < kWidePlaces; ++i) fetch();
+        for (uint32_t i = 0; nth(i) < items; ++i) {
+            const uint32_t place = i % kWidePlaces;
+            if (slots[place] >= 0) {
+                if (!phase_of(done + 8 * place, (phases >> place) & 1)) {
+                    atomicExch(&g_step_error, 1);
+                    break;
+                }
+                phases ^= 1u << place;
+                open &= ~(1u << place);
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                                 s.state + (slots[place] * s.heads + nth(i) % (uint32_t)s.heads) * s.D * s.E),
+                             "r"(sm + place * lay.state), "r"(lay.state)
+                             : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+            fetch();
+        }
+        // (after a wait that ran out) copies land before the block ends
+        for (uint32_t place = 0; place < kWidePlaces; ++place)
+            if (open >> place & 1) phase_of(full + 8 * place, (phases >> place) & 1);
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        return;
+    }
+    const bool busy = r < R;
+    // what else an item needs, one item ahead in registers, as it comes (whatever is done to it here would wait for it)
+    T nk = from_f<T>(0.f), nq = nk, nv = nk;
+    float ndecay = 0.f, nbeta = 0.f;
+    long long nslot = -1;
+    const auto ahead = [&](uint32_t i) {
+        const uint32_t item = nth(i);
+        if (item >= items) return;
+        const long long b = item / (uint32_t)s.heads;
+        const int h = (int)(item - (uint32_t)b * (uint32_t)s.heads);
+        nslot = s.slots ? s.slots[b] : b;
+        if (tid < s.D) {
+            nk = reinterpret_cast<const T*>(s.k.p)[b * s.k.batch + (h / s.k_share) * s.k.head + tid];
+            nq = reinterpret_cast<const T*>(s.q.p)[b * s.q.batch + (h / s.q_share) * s.q.head + tid];
+        }
+        if (tid < s.E) nv = reinterpret_cast<const T*>(s.v.p)[b * s.v.batch + (h / s.v_share) * s.v.head + tid];
+        ndecay = s.log_decay[b * s.log_batch + h * s.log_head];
+        nbeta = s.beta[b * s.beta_batch + h * s.beta_head];
+    };
+    ahead(0);
+    uint32_t phases = 0;
+    for (uint32_t i = 0; nth(i) < items; ++i) {
+        const uint32_t item = nth(i), place = i % kWidePlaces;
+        const long long b = item / (uint32_t)s.heads, slot = nslot;
+        const int h = (int)(item - (uint32_t)b * (uint32_t)s.heads);
+        float *sk = row + (i & 1) * 2 * kMaxStep, *sq = sk + kMaxStep;
+        if (tid < s.D) {
+            sk[tid] = to_f(nk);
+            sq[tid] = to_f(nq);
+        }
+        const float v = to_f(nv), decay = expf(ndecay), beta = nbeta;
+        ahead(i + 1);
+        T* o = reinterpret_cast<T*>(s.o.p) + b * s.o.batch + h * s.o.head;
+        workers(true);                                        // k and q are there
+        if (slot < 0 || slot >= s.n_slots) {                  // (the same for all threads)
+            for (int e = tid; e < s.E; e += kWideThreads) o[e] = from_f<T>(0.f);
+            continue;
+        }
+        const bool there = phase_of(full + 8 * place, (phases >> place) & 1);
+        phases ^= 1u << place;
+        float4* S = reinterpret_cast<float4*>(smem + place * lay.state) + c;
+        float4 x[kWidePer];
+        float ks[4] = {}, qs[4] = {};
+        if (busy) {
+#pragma unroll
+            for (int n = 0; n < kWidePer; ++n) {
+                const int d = r + n * R;
+                if (d >= s.D) break;
+                x[n] = S[d * C];
+                float* p = &x[n].x;
+                const float kd = sk[d], qd = sq[d];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] *= decay;
+                    ks[j] = fmaf(kd, p[j], ks[j]);
+                    qs[j] = fmaf(qd, p[j], qs[j]);
+                }
+            }
+            part[tid] = make_float4(ks[0], ks[1], ks[2], ks[3]);
+            part[kWideThreads + tid] = make_float4(qs[0], qs[1], qs[2], qs[3]);
+        }
+        float qk = 0.f;
+        for (int d = tid & 31; d < s.D; d += 32) qk = fmaf(sk[d], sq[d], qk);
+        qk = warp_sum(qk);
+        if (!workers(there)) {                                // (for all threads, if for one: the state stays as it was)
+            for (int e = tid; e < s.E; e += kWideThreads) o[e] = from_f<T>(__int_as_float(0x7fffffff));
+            if (tid == 0) atomicExch(&g_step_error, 1);
+            break;
+        }
+        // columns' sums, u and o by a thread each, and u for all
+        float* us = row + 4 * kMaxStep;
+        if (tid < s.E) {
+            const float *p = reinterpret_cast<const float*>(part) + tid, *q = p + 4 * kWideThreads;
+            float a = 0.f, y = 0.f;
+            for (int n = 0; n < R; ++n) {
+                a += p[n * s.E];
+                y += q[n * s.E];
+            }
+            const float u = beta * (v - a);
+            us[tid] = u;
+            o[tid] = from_f<T>(fmaf(qk, u, y) * s.scale);
+        }
+        workers(true);
+        if (busy) {
+            const float4 u = *reinterpret_cast<const float4*>(us + 4 * c);
+#pragma unroll
+            for (int n = 0; n < kWidePer; ++n) {
+                const int d = r + n * R;
+                if (d >= s.D) break;
+                const float kd = sk[d];
+                x[n].x = fmaf(kd, u.x, x[n].x);
+                x[n].y = fmaf(kd, u.y, x[n].y);
+                x[n].z = fmaf(kd, u.z, x[n].z);
+                x[n].w = fmaf(kd, u.w, x[n].w);
+                S[d * C] = x[n];
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((tid & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(done + 8 * place) : "memory");
     }
 }
 
@@ -403,7 +604,18 @@ int fg_delta_step(const fg_delta_step_args* g, void* stream) {
         s.scale = (float)g->scale;
         const bool by4 = g->value_dim % 4 == 0 && reinterpret_cast<uintptr_t>(g->state) % 16 == 0;
         by_type(g->type, [&](auto t) {
-            auto* kernel = by4 ? k_delta_step<decltype(t), 4> : k_delta_step<decltype(t), 1>;
+            using T = decltype(t);
+            const long long items = g->batch * g->heads;
+            // whole states through shared memory where each SM has several (2,048 rows, 8 heads of 128 x 128: 476 us by columns)
+            if (by4 && items >= 8 * kSms && s.D * s.E <= 16384 && s.E * 2 <= 4 * kWideThreads && s.D * (s.E / 4) <= kWidePer * (kWideThreads / (s.E / 4)) * (s.E / 4)) {
+                const int bytes = WideLayout(s.D, s.E).bytes;
+                static OnEachDevice here;
+                here.first(current_device(), [] { allow_shared(k_delta_step_wide<T>, WideLayout(128, 128).bytes); });
+                k_delta_step_wide<T><<<kSms, kWideThreads + 32, bytes, static_cast<cudaStream_t>(stream)>>>(s, (uint32_t)items);
+                return;
+            }
+            auto* kernel = by4 ? s.D <= 64 ? k_delta_step<T, 4, 2> : s.D <= 128 ? k_delta_step<T, 4, 4> : k_delta_step<T, 4, 8>
+                               : s.D <= 64 ? k_delta_step<T, 1, 8> : k_delta_step<T, 1, 32>;
             kernel<<<(unsigned)(g->batch * g->heads * s.tiles), 256, 0, static_cast<cudaStream_t>(stream)>>>(s);
         });
         MCK(cudaGetLastError());
@@ -412,3 +624,12 @@ int fg_delta_step(const fg_delta_step_args* g, void* stream) {
 }
 
 }  // extern "C"
+
+namespace fgm {
+int step_gave_up(cudaStream_t st) {
+    int bad = 0;
+    MCK(cudaMemcpyFromSymbolAsync(&bad, g_step_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+    MCK(cudaStreamSynchronize(st));
+    return bad;
+}
+}  // namespace fgm

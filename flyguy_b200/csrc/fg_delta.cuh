@@ -19,22 +19,20 @@ constexpr int kSquare = kTicks + 8;      // a row of a 64 x 64 tile in shared me
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// (volatile: they stay between the barriers around them; loads from global memory may pass them)
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(at)
-                 : "memory");
+                 : "r"(at));
 }
 __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(at)
-                 : "memory");
+                 : "r"(at));
 }
 __device__ __forceinline__ void stsm_t(uint32_t at, const uint32_t (&r)[4]) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
@@ -110,15 +108,18 @@ __device__ __forceinline__ void async_wait() {
 // with rows of STRIDE values. bf16 at 16-byte boundaries goes by asynchronous copies.
 template <class T, int N, int COLS, int STRIDE, int THREADS>
 __device__ __forceinline__ void load_tile(bf16* to, const T* p, long long row, int rows, int cols, bool fast, int tid) {
-    constexpr int kUnits = COLS / 8, kPlane = kTicks * STRIDE;
-    for (int i = tid; i < kTicks * kUnits; i += THREADS) {
-        const int r = i / kUnits, c = (i - r * kUnits) * 8;
-        bf16* at = to + r * STRIDE + c;
-        const bool in = r < rows && c < cols;
-        const T* q = p + (in ? r * row + c : 0);
+    constexpr int kUnits = COLS / 8, kPlane = kTicks * STRIDE, kStep = THREADS / kUnits;
+    static_assert(THREADS % kUnits == 0 && kTicks % kStep == 0, "a thread keeps its columns");
+    const int r0 = tid / kUnits, c = tid % kUnits * 8;
+    const bool has = c < cols;
+    const T* q = p + (has ? r0 * row + c : 0);
+    bf16* at = to + r0 * STRIDE + c;
+#pragma unroll 4
+    for (int r = r0; r < kTicks; r += kStep, q += kStep * row, at += kStep * STRIDE) {
+        const bool in = has && r < rows;
         if constexpr (N == 1 && std::is_same<T, bf16>::value) {
             if (fast) {
-                async16(smem_at(at), q, in);
+                async16(smem_at(at), in ? q : p, in);
                 continue;
             }
         }

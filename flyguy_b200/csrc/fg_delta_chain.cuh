@@ -216,7 +216,13 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
             const float* row = sl + (16 * warp + t) * 68 + 16 * warp;
             float v = row[lane];
 #pragma unroll
-            for (int k = 0; k < t; ++k) v = fmaf(-row[k], y[k], v);
+            for (int k = 0; k < t; k += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(row + k);
+                v = fmaf(-l.x, y[k], v);
+                if (k + 1 < t) v = fmaf(-l.y, y[k + 1], v);
+                if (k + 2 < t) v = fmaf(-l.z, y[k + 2], v);
+                if (k + 3 < t) v = fmaf(-l.w, y[k + 3], v);
+            }
             y[t] = v * beta[16 * warp + t];
             uint32_t u[NS];
             terms<NS>(v, 0.f, u);
@@ -643,6 +649,8 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_chain(const __grid_constan
     if (s.last) each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { s.last[state0 + at] = v; });
 }
 
+__device__ __forceinline__ void prefetch(const char* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // Back. s.last is the state after the recording's last tick.
 template <class T, int DP, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant__ Delta s) {
@@ -685,6 +693,17 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
         // R^T K^T, and <R, S> behind the chunk
         float anchor = 0.f;
         const uint4* behind = s.states + ((place + s.heads) * tiles_e + e0 / 16) * NS * (DP / 16) * 32 + lane;
+        const bool inner = i + 1 < chunks;
+        uint4 ahead[NS];
+        if (inner) {
+#pragma unroll
+            for (int k = 0; k < NS; ++k) ahead[k] = __ldg(behind + k * (DP / 16) * 32);
+        }
+        if (i > 0) {                                          // what the next chunk reads of this, on its way to L2
+            const char* states = reinterpret_cast<const char*>(s.states + warp_place * NS * (DP / 16) * 32);
+            for (int at = lane * 128; at < NS * (DP / 16) * 512; at += 32 * 128) prefetch(states + at);
+            prefetch(reinterpret_cast<const char*>(s.w + (warp_place - (long long)s.heads * tiles_e) * 8 * 32) + lane * 128);
+        }
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
             uint32_t a[NS][4];
@@ -692,10 +711,11 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
 #pragma unroll
             for (int k = 0; k < NG; ++k)
                 s.gstates[((warp_place * NG + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
-            if (i + 1 < chunks) {
+            if (inner) {
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
-                    const uint4 u = behind[(k * (DP / 16) + d) * 32];
+                    const uint4 u = ahead[k];
+                    if (d + 1 < DP / 16) ahead[k] = __ldg(behind + (k * (DP / 16) + d + 1) * 32);
                     const uint32_t* p = &u.x;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -749,6 +769,9 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
         // dR = dU - X^T B dU
         {
             float Y[8][4];
+            float4 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = __ldg(s.w + (warp_place * 8 + j) * 32 + lane);
 #pragma unroll
             for (int j = 0; j < 8; ++j) Y[j][0] = Y[j][1] = Y[j][2] = Y[j][3] = 0.f;
 #pragma unroll
@@ -778,11 +801,10 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
             float sums[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float4 w = s.w[(warp_place * 8 + j) * 32 + lane];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) N[j][e] -= Y[j][e];
-                sums[2 * j] = N[j][0] * w.x + N[j][2] * w.z;
-                sums[2 * j + 1] = N[j][1] * w.y + N[j][3] * w.w;
+                sums[2 * j] = N[j][0] * w[j].x + N[j][2] * w[j].z;
+                sums[2 * j + 1] = N[j][1] * w[j].y + N[j][3] * w[j].w;
             }
             const float2 db = column_sums(sums, lane);
             *reinterpret_cast<float2*>(s.db + warp_place * kTicks + 8 * (lane >> 2) + 2 * (lane & 3)) = db;

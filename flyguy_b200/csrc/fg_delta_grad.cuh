@@ -19,7 +19,7 @@ struct GradLayout {
                          r = s + kept * plane, values = r + kept * plane;
     static constexpr int dp = go, d = dp + kept * plane;     // later, over what is read by then
     static constexpr int bytes = 2 * values + 4 * kGates * kTicks;
-    static_assert(2 * kept <= in + 4 * kept && bytes <= 227 * 1024, "room");
+    static_assert(2 * kept <= in + 4 * kept && 2 * kept * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
 };
 
 template <class T>
@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     float* gates = reinterpret_cast<float*>(smem + 2 * Lay::values);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const long long slot = blockIdx.x, place = slot * s.heads + blockIdx.y;
-    const int h = blockIdx.y, d_block = 64 * blockIdx.z, all_d = (s.D + 15) / 16, tiles_e = (s.E + 15) / 16;
+    const int h = blockIdx.y, d_block = 64 * blockIdx.z, tiles_e = (s.E + 15) / 16;
     const int padded_d = s.D > 64 ? 8 : 4;                   // the chain's 16-value pieces of a column
     const Chunk c = chunk_of(s, slot);
     if (c.n == 0) return;
@@ -92,17 +92,26 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                                            kTicks, 16 * tiles_e - e0, true, tid);
         async_commit();
         // S and R: left operands of 16 columns x 16 values -> rows of columns
-        for (int i = warp; i < 2 * NK * 16; i += 8) {
-            const int which = i & 1, n = (i >> 1) % NK, piece = (i >> 1) / NK, te = piece >> 2, td = piece & 3, e = e0 / 16 + te;
-            uint32_t r[4] = {0, 0, 0, 0};
-            if (e < tiles_e && d_block / 16 + td < all_d) {
-                const int kept = which ? NK : NB;
-                const uint4 u = (which ? s.gstates : s.states)[(((place * tiles_e + e) * kept + n) * padded_d + d_block / 16 + td) * 32 + lane];
-                r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
-            }
-            const uint32_t to = smem_at(tiles) + 2 * ((which ? Lay::r : Lay::s) + n * kPlane + 16 * te * kSquare + 16 * td) + at_rows_m(lane, kSquare);
-            asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-                         : "memory");
+        {
+            // warp: columns 16 (warp / 2).., of S or R
+            const int which = warp & 1, te = warp >> 1, e = e0 / 16 + te, kept = which ? NK : NB;
+            const uint4* from = (which ? s.gstates : s.states) + (((place * tiles_e + e) * kept) * padded_d + d_block / 16) * 32 + lane;
+            const uint32_t to = smem_at(tiles) + 2 * ((which ? Lay::r : Lay::s) + 16 * te * kSquare) + at_rows_m(lane, kSquare);
+            uint4 u[NK][4];
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int td = 0; td < 4; ++td) {
+                    u[n][td] = make_uint4(0, 0, 0, 0);
+                    if (e < tiles_e) u[n][td] = __ldg(from + (n * padded_d + td) * 32);
+                }
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int td = 0; td < 4; ++td)
+                    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to + 2 * (n * kPlane + 16 * td)),
+                                 "r"(u[n][td].x), "r"(u[n][td].y), "r"(u[n][td].z), "r"(u[n][td].w)
+                                 : "memory");
         }
         async_wait<0>();
         __syncthreads();
@@ -239,18 +248,50 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                     }
         }
     }
+    // by way of shared memory (over S and R), so that a row leaves in whole sectors
+    float* stage = reinterpret_cast<float*>(tiles + Lay::s);
+    constexpr int kRow = 68;
     const auto put = [&](const Operand& o, int f32, const float (&x)[4][4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = 16 * wt + g + 8 * (e >> 1), d = d_block + 32 * wd + 8 * j + 2 * t4 + (e & 1);
-                if (t >= c.n || d >= s.D) continue;
-                if (f32) row_of<float>(s, o, c.b, h, tick + t)[d] = x[j][e];
-                else row_of<T>(s, o, c.b, h, tick + t)[d] = from_f<T>(x[j][e]);
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<float2*>(stage + (16 * wt + g + 8 * i) * kRow + 32 * wd + 8 * j + 2 * t4) = make_float2(x[j][2 * i], x[j][2 * i + 1]);
+        __syncthreads();
+        const int r0 = tid >> 3, col = (tid & 7) * 8, d = d_block + col;
+        if (d < s.D) {
+#pragma unroll
+            for (int r = r0; r < kTicks; r += 32) {
+                if (r >= c.n) break;
+                float v[8];
+                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stage + r * kRow + col);
+                *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(stage + r * kRow + col + 4);
+                if (f32) {
+                    float* to = row_of<float>(s, o, c.b, h, tick + r) + d;
+                    if (o.fast) {
+                        reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        for (int j = 0; j < 8 && d + j < s.D; ++j) to[j] = v[j];
+                    }
+                } else if constexpr (sizeof(T) == 2) {
+                    T* to = row_of<T>(s, o, c.b, h, tick + r) + d;
+                    T w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = from_f<T>(v[j]);
+                    if (o.fast) {
+                        *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(w);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (d + j < s.D) to[j] = w[j];
+                    }
+                }
             }
+        }
     };
     put(s.gq, s.gq_f32, dq);
+    __syncthreads();
     put(s.gk, s.gk_f32, dk);
 }
 

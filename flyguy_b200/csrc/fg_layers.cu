@@ -12,28 +12,33 @@
 namespace {
 using namespace fgm;
 
-// V values of T: 16 bytes, or one
+// V values of T as they lie in memory: 16 bytes, or one value
 template <class T, int V>
-__device__ __forceinline__ void load(const T* p, float (&x)[V]) {
-    if constexpr (V == 1) {
-        x[0] = to_f(*p);
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = to_f(e[i]);
-    }
+struct alignas(V > 1 ? 16 : sizeof(T)) Unit {
+    T v[V];
+};
+template <class T, int V>
+__device__ __forceinline__ Unit<T, V> load(const T* p) {
+    return *reinterpret_cast<const Unit<T, V>*>(p);
 }
 template <class T, int V>
 __device__ __forceinline__ void store(T* p, const float (&x)[V]) {
-    if constexpr (V == 1) {
-        *p = from_f<T>(x[0]);
-    } else {
-        uint4 u;
-        T* e = reinterpret_cast<T*>(&u);
+    Unit<T, V> u;
 #pragma unroll
-        for (int i = 0; i < V; ++i) e[i] = from_f<T>(x[i]);
-        *reinterpret_cast<uint4*>(p) = u;
+    for (int i = 0; i < V; ++i) u.v[i] = from_f<T>(x[i]);
+    *reinterpret_cast<Unit<T, V>*>(p) = u;
+}
+// V values of the weight or the bias (aligned where V is over 1; NULL: `other`)
+template <int V>
+__device__ __forceinline__ void load_w(const float* p, int c, float other, float (&w)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = other;
+    if (!p) return;
+    if constexpr (V == 1) {
+        w[0] = p[c];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(w + i) = *reinterpret_cast<const float4*>(p + c + i);
     }
 }
 
@@ -47,13 +52,15 @@ struct Norm {
     float eps;
 };
 
-// sums over the threads that share a row: a warp, or the block
-template <bool WARP, int N>
+// sums over the threads that share a row: GROUP lanes, or (0) the block
+template <int GROUP, int N>
 __device__ __forceinline__ void row_sums(float (&s)[N], float* room, int& turn) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = warp_sum(s[i]);
-    if constexpr (!WARP) {
-        float* at = room + (turn ^= 1) * 32 * N;              // (two places in turn: one barrier a sum)
+    for (int o = (GROUP ? GROUP : 32) / 2; o; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+    if constexpr (GROUP == 0) {
+        float* at = room + (turn ^= 1) * 16 * N;              // (two places in turn: one barrier a sum)
         const int warps = blockDim.x >> 5;
         if ((threadIdx.x & 31) == 0) {
 #pragma unroll
@@ -69,72 +76,92 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float* room, int& turn) 
     }
 }
 
-// A row's PER units of V values in this thread as d = x - mean (0 past the row's end); r
-template <class T, int V, int PER, bool WARP>
-__device__ __forceinline__ float centred(const Norm& a, const T* p, int me, int step, float (&d)[PER][V], float* room, int& turn) {
-    float s[1] = {0.f};
+// What a thread has of ROWS rows: PER units of V values of each, kept as they came so that 16-bit values take half the registers
+template <class T, int V, int PER, int GROUP, int ROWS>
+struct Rows {
+    Unit<T, V> u[ROWS][PER];
+    int me, step;
+    __device__ __forceinline__ int column(int j) const { return (me + j * step) * V; }
+    __device__ __forceinline__ void fetch(const char* p, long long row, long long rows, long long stride, int dim) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int c = (me + j * step) * V;
-        if (c < a.dim) load<T, V>(p + c, d[j]);
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (row + r < rows && column(j) < dim) u[r][j] = load<T, V>(reinterpret_cast<const T*>(p) + (row + r) * stride + column(j));
     }
+    // means and 1 / deviations; rows past the last are worked on as they are
+    __device__ __forceinline__ void stats(int dim, float eps, float (&mean)[ROWS], float (&inv)[ROWS], float* room, int& turn) const {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        if ((me + j * step) * V < a.dim) {
+        for (int r = 0; r < ROWS; ++r) {
+            mean[r] = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[0] += d[j][i];
+            for (int j = 0; j < PER; ++j)
+                if (column(j) < dim) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) mean[r] += to_f(u[r][j].v[i]);
+                }
         }
-    }
-    row_sums<WARP, 1>(s, room, turn);
-    const float mean = s[0] / (float)a.dim;
-    s[0] = 0.f;
+        row_sums<GROUP, ROWS>(mean, room, turn);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const bool in = (me + j * step) * V < a.dim;
+        for (int r = 0; r < ROWS; ++r) {
+            mean[r] /= (float)dim;
+            inv[r] = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            d[j][i] = in ? d[j][i] - mean : 0.f;
-            s[0] = fmaf(d[j][i], d[j][i], s[0]);
+            for (int j = 0; j < PER; ++j)
+                if (column(j) < dim) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float d = to_f(u[r][j].v[i]) - mean[r];
+                        inv[r] = fmaf(d, d, inv[r]);
+                    }
+                }
         }
+        row_sums<GROUP, ROWS>(inv, room, turn);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) inv[r] = 1.f / sqrtf(inv[r] / (float)dim + eps);
     }
-    row_sums<WARP, 1>(s, room, turn);
-    return 1.f / sqrtf(s[0] / (float)a.dim + a.eps);
-}
+};
 
-template <class T, int V, int PER, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm(const __grid_constant__ Norm a) {
-    __shared__ float room[64];
+template <class T, int V, int PER, int GROUP, int ROWS>
+__global__ void __launch_bounds__(GROUP ? 256 : 512) k_norm(const __grid_constant__ Norm a) {
+    __shared__ float room[32 * ROWS];
     int turn = 0;
-    const int me = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x;
-    const long long row = WARP ? blockIdx.x * (long long)(blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.rows) return;
-    float d[PER][V];
-    const float r = centred<T, V, PER, WARP>(a, reinterpret_cast<const T*>(a.x) + row * a.x_row, me, step, d, room, turn);
-    T* y = reinterpret_cast<T*>(a.y) + row * a.dim;
+    Rows<T, V, PER, GROUP, ROWS> x;
+    x.me = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
+    x.step = GROUP ? GROUP : blockDim.x;
+    const long long row = (GROUP ? blockIdx.x * (long long)(blockDim.x / (GROUP ? GROUP : 1)) + threadIdx.x / (GROUP ? GROUP : 1) : blockIdx.x) * ROWS;
+    x.fetch(a.x, row, a.rows, a.x_row, a.dim);
+    float mean[ROWS], inv[ROWS];
+    x.stats(a.dim, a.eps, mean, inv, room, turn);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int c = (me + j * step) * V;
+        const int c = x.column(j);
         if (c >= a.dim) continue;
-        float w[V], o[V];
+        float w[V], b[V];
+        load_w<V>(a.w, c, 1.f, w);
+        load_w<V>(a.b, c, 0.f, b);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            w[i] = a.w ? a.w[c + i] : 1.f;
-            o[i] = a.b ? a.b[c + i] : 0.f;
+        for (int r = 0; r < ROWS; ++r) {
+            if (row + r >= a.rows) break;
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = fmaf((to_f(x.u[r][j].v[i]) - mean[r]) * inv[r], w[i], b[i]);
+            store<T, V>(reinterpret_cast<T*>(a.y) + (row + r) * a.dim + c, o);
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = fmaf(d[j][i] * r, w[i], o[i]);
-        store<T, V>(y + c, o);
     }
 }
 
-// gx of rows, and this block's sums for gw and gb
-template <class T, int V, int PER, bool WARP, bool SUMS>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_bwd(const __grid_constant__ Norm a) {
-    __shared__ float room[128];
-    extern __shared__ float sums[];                           // WARP: [warps][32 V] of one unit column
+// gx of rows, and this block's sums for gw and gb. While a group of rows is worked on the next one is on its way.
+template <class T, int V, int PER, int GROUP, int ROWS, bool SUMS>
+__global__ void __launch_bounds__(GROUP ? 128 : 512, GROUP ? 3 : 1) k_norm_bwd(const __grid_constant__ Norm a) {
+    __shared__ float room[64 * ROWS];
+    extern __shared__ float sums[];                           // GROUP: [groups][GROUP V] of one unit column
+    constexpr int kGroup = GROUP ? GROUP : 1;
     int turn = 0;
-    const int me = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x;
-    const int group = WARP ? threadIdx.x >> 5 : 0, groups = WARP ? blockDim.x >> 5 : 1;
+    const int group = GROUP ? threadIdx.x / kGroup : 0, groups = GROUP ? blockDim.x / kGroup : 1;
+    Rows<T, V, PER, GROUP, ROWS> x, g, next_x, next_g;
+    x.me = g.me = next_x.me = next_g.me = GROUP ? threadIdx.x % kGroup : threadIdx.x;
+    x.step = g.step = next_x.step = next_g.step = GROUP ? GROUP : blockDim.x;
     float aw[SUMS ? PER : 1][V], ab[SUMS ? PER : 1][V];
     if constexpr (SUMS) {
 #pragma unroll
@@ -142,52 +169,65 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_bwd(const __grid_con
 #pragma unroll
             for (int i = 0; i < V; ++i) aw[j][i] = ab[j][i] = 0.f;
     }
-    for (long long row = blockIdx.x * (long long)groups + group; row < a.rows; row += gridDim.x * (long long)groups) {
-        float d[PER][V], g[PER][V];
-        const T* gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_row;
+    const long long step = gridDim.x * (long long)groups * ROWS, first = (blockIdx.x * (long long)groups) * ROWS;
+    next_x.fetch(a.x, first + group * ROWS, a.rows, a.x_row, a.dim);
+    next_g.fetch(a.gy, first + group * ROWS, a.rows, a.gy_row, a.dim);
+    for (long long base = first; base < a.rows; base += step) {   // (the block's groups stay together)
+        const long long row = base + group * ROWS;
+        x = next_x;
+        g = next_g;
+        next_x.fetch(a.x, row + step, a.rows, a.x_row, a.dim);
+        next_g.fetch(a.gy, row + step, a.rows, a.gy_row, a.dim);
+        float mean[ROWS], inv[ROWS], s[2 * ROWS];
+        x.stats(a.dim, a.eps, mean, inv, room, turn);
+#pragma unroll
+        for (int r = 0; r < 2 * ROWS; ++r) s[r] = 0.f;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int c = (me + j * step) * V;
-            if (c < a.dim) load<T, V>(gy + c, g[j]);
-        }
-        const float r = centred<T, V, PER, WARP>(a, reinterpret_cast<const T*>(a.x) + row * a.x_row, me, step, d, room, turn);
-        float s[2] = {0.f, 0.f};
+            const int c = x.column(j);
+            if (c >= a.dim) continue;
+            float w[V];
+            load_w<V>(a.w, c, 1.f, w);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int c = (me + j * step) * V;
-            const bool in = c < a.dim;
+            for (int r = 0; r < ROWS; ++r) {
+                if (row + r >= a.rows) break;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                d[j][i] *= r;
-                if (!in) g[j][i] = 0.f;
-                if constexpr (SUMS) {
-                    aw[j][i] = fmaf(g[j][i], d[j][i], aw[j][i]);
-                    ab[j][i] += g[j][i];
+                for (int i = 0; i < V; ++i) {
+                    const float d = (to_f(x.u[r][j].v[i]) - mean[r]) * inv[r], y = to_f(g.u[r][j].v[i]), z = y * w[i];
+                    if constexpr (SUMS) {
+                        aw[j][i] = fmaf(y, d, aw[j][i]);
+                        ab[j][i] += y;
+                    }
+                    s[2 * r] += z;
+                    s[2 * r + 1] = fmaf(z, d, s[2 * r + 1]);
                 }
-                if (a.w) g[j][i] *= in ? a.w[c + i] : 0.f;
-                s[0] += g[j][i];
-                s[1] = fmaf(g[j][i], d[j][i], s[1]);
             }
         }
-        row_sums<WARP, 2>(s, room, turn);
-        const float m = s[0] / (float)a.dim, k = s[1] / (float)a.dim;
-        T* gx = reinterpret_cast<T*>(a.gx) + row * a.dim;
+        row_sums<GROUP, 2 * ROWS>(s, room, turn);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int c = (me + j * step) * V;
+            const int c = x.column(j);
             if (c >= a.dim) continue;
-            float o[V];
+            float w[V];
+            load_w<V>(a.w, c, 1.f, w);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = r * (g[j][i] - m - d[j][i] * k);
-            store<T, V>(gx + c, o);
+            for (int r = 0; r < ROWS; ++r) {
+                if (row + r >= a.rows) break;
+                const float m = s[2 * r] / (float)a.dim, k = s[2 * r + 1] / (float)a.dim;
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    o[i] = inv[r] * (to_f(g.u[r][j].v[i]) * w[i] - m - (to_f(x.u[r][j].v[i]) - mean[r]) * inv[r] * k);
+                store<T, V>(reinterpret_cast<T*>(a.gx) + (row + r) * a.dim + c, o);
+            }
         }
     }
     if constexpr (SUMS) {
         float* part = a.part + (long long)blockIdx.x * 2 * a.dim;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int c = (me + j * step) * V;
-            if constexpr (!WARP) {
+            const int c = x.column(j);
+            if constexpr (GROUP == 0) {
                 if (c < a.dim) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
@@ -197,20 +237,309 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) k_norm_bwd(const __grid_con
                 }
             } else {
 #pragma unroll
-                for (int which = 0; which < 2; ++which) {     // the warps' sums in order
+                for (int which = 0; which < 2; ++which) {     // the groups' sums in order
                     __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < V; ++i) sums[group * 32 * V + me * V + i] = which ? ab[j][i] : aw[j][i];
+                    for (int i = 0; i < V; ++i) sums[(group * GROUP + x.me) * V + i] = which ? ab[j][i] : aw[j][i];
                     __syncthreads();
-                    for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) {
+                    for (int e = threadIdx.x; e < GROUP * V; e += blockDim.x) {
                         float t = 0.f;
-                        for (int k = 0; k < groups; ++k) t += sums[k * 32 * V + e];
-                        const int at = j * 32 * V + e;
+                        for (int k = 0; k < groups; ++k) t += sums[k * GROUP * V + e];
+                        const int at = j * GROUP * V + e;
                         if (at < a.dim) part[which * a.dim + at] = t;
                     }
                 }
             }
         }
+    }
+}
+
+// Many rows, a warp each, that copy themselves ahead: a lane's units of the next DEPTH - 1 rows are on their way to places in shared
+// memory that it alone reads, so that nothing but its own copies is waited for. With the rows in shared memory (read again for each
+// step) the registers are the sums', 16 warps share an SM and 16 x DEPTH rows are in flight.
+// SHIFT: rows that begin anywhere, at the same place in 16 bytes in x, gy and what comes out. A warp takes every so many-th row, a multiple of
+// 8, so its rows all begin alike; its first and last units reach into the neighbours, whose values count for nothing.
+template <class T, int V, bool BACK>
+struct Ring {
+    static constexpr int depth = BACK ? 3 : 4, warps = 4, tensors = BACK ? 2 : 1;
+    static int units(int dim, bool shift) { return (dim + (shift ? V - 1 : 0) + V - 1) / V; }
+    // rows' places, in rounds of 32 units, and the weight, with a shift as each warp reads it
+    static int bytes(int rounds, bool shift) { return (depth * tensors * 512 * warps + (BACK ? 128 * V * (shift ? warps : 1) : 0)) * rounds; }
+};
+__device__ __forceinline__ void copy_ahead(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// Values as fp32, in pairs (one instruction for two) where a unit has several
+template <int V>
+using Lane = std::conditional_t<(V > 1), uint64_t, float>;
+template <class P>
+__device__ __forceinline__ P same(float x) {
+    if constexpr (std::is_same<P, float>::value) return x;
+    else return two(x, x);
+}
+__device__ __forceinline__ float plus(float x, float y) { return x + y; }
+__device__ __forceinline__ uint64_t plus(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ float times(float x, float y) { return x * y; }
+__device__ __forceinline__ uint64_t times(uint64_t x, uint64_t y) { return mul2(x, y); }
+__device__ __forceinline__ float times_plus(float x, float y, float z) { return fmaf(x, y, z); }
+__device__ __forceinline__ uint64_t times_plus(uint64_t x, uint64_t y, uint64_t z) { return fma2(x, y, z); }
+__device__ __forceinline__ float both(float x) { return x; }
+__device__ __forceinline__ float both(uint64_t x) { return sum2(x); }
+template <class T, int V>
+__device__ __forceinline__ Lane<V> lane_of(const Unit<T, V>& u, int i) {
+    if constexpr (V == 1) return to_f(u.v[0]);
+    else return two(to_f(u.v[2 * i]), to_f(u.v[2 * i + 1]));
+}
+template <int V>
+__device__ __forceinline__ Lane<V> lane_of(const float (&w)[V], int i) {
+    if constexpr (V == 1) return w[0];
+    else return two(w[2 * i], w[2 * i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void values_of(Lane<V> p, int i, float (&v)[V]) {
+    if constexpr (V == 1) v[0] = p;
+    else halves(p, v[2 * i], v[2 * i + 1]);
+}
+
+template <class T, int V, int PER, bool SHIFT, bool BACK, bool SUMS>
+__global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ Norm a, int rounds) {
+    using R = Ring<T, V, BACK>;
+    using P = Lane<V>;
+    constexpr int N = V / 2;
+    extern __shared__ __align__(16) unsigned char ring[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, place_bytes = rounds * 512, stage = R::tensors * place_bytes;
+    unsigned char* mine = ring + warp * R::depth * stage + lane * 16;
+    const long long step = gridDim.x * (long long)R::warps;
+    long long row = blockIdx.x * (long long)R::warps + warp;
+    const int shift = SHIFT ? (int)((reinterpret_cast<uintptr_t>(a.x) / sizeof(T) + (unsigned long long)(row * a.x_row)) % V) : 0;
+    const auto column = [&](int j) { return (lane + 32 * j) * V - shift; };   // may be up to V - 1 before the row
+    const auto edge = [&](int c) { return SHIFT && (c < 0 || c + V > a.dim); };
+    const auto inside = [&](int c) { return c >= 0 && c < a.dim; };
+    const auto fetch = [&](long long row, int place) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int c = column(j);
+                if (c >= a.dim) break;
+                unsigned char* to = mine + place * stage + j * 512;
+#pragma unroll
+                for (int k = 0; k < R::tensors; ++k) {
+                    const T* p = reinterpret_cast<const T*>(k ? a.gy : a.x) + row * (k ? a.gy_row : a.x_row) + c;
+                    if (SHIFT && c + V > a.dim && row + 1 == a.rows) {   // (nothing is read behind the last row)
+                        Unit<T, V> u{};
+                        for (int i = 0; i < V; ++i)
+                            if (inside(c + i)) u.v[i] = p[i];
+                        *reinterpret_cast<Unit<T, V>*>(to + k * place_bytes) = u;
+                    } else {
+                        copy_ahead((uint32_t)__cvta_generic_to_shared(to + k * place_bytes), p);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // forward the weight and the bias stay in registers; back the sums do, and the weight lies in shared memory as the lanes read it
+    P w[BACK ? 1 : PER][N], b[BACK ? 1 : PER][N], aw[SUMS ? PER : 1][N], ab[SUMS ? PER : 1][N];
+    float* sw = reinterpret_cast<float*>(ring + R::warps * R::depth * stage) + (SHIFT ? warp * 32 * V * rounds : 0) + lane * 4;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int c = column(j);
+        float v[V], o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[i] = a.w && inside(c + i) ? a.w[c + i] : 1.f;
+            o[i] = !BACK && a.b && inside(c + i) ? a.b[c + i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (!BACK) {
+                w[j][i] = lane_of<V>(v, i);
+                b[j][i] = lane_of<V>(o, i);
+            }
+            if constexpr (SUMS) aw[j][i] = ab[j][i] = same<P>(0.f);
+        }
+        if (BACK && c < a.dim && (SHIFT || warp == 0)) {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(sw + (j * V + i) * 32) = *reinterpret_cast<const float4*>(v + i);
+        }
+    }
+    if (BACK && !SHIFT) __syncthreads();
+    const auto weight = [&](int j, P(&to)[N]) {
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(sw + (j * V + i) * 32);
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = lane_of<V>(v, i);
+    };
+    // pairs outside the row as zeros
+    const auto keep = [&](int c, P(&v)[N]) {
+        if (edge(c)) {
+            float x[V];
+#pragma unroll
+            for (int i = 0; i < N; ++i) values_of<V>(v[i], i, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (!inside(c + i)) x[i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = lane_of<V>(x, i);
+        }
+    };
+    const auto put = [&](T* p, int c, const float (&o)[V]) {
+        if (edge(c)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (inside(c + i)) p[c + i] = from_f<T>(o[i]);
+        } else {
+            store<T, V>(p + c, o);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < R::depth - 1; ++k) fetch(row + k * step, k);
+    int place = 0;
+    for (; row < a.rows; row += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(R::depth - 2) : "memory");
+        fetch(row + (R::depth - 1) * step, place ? place - 1 : R::depth - 1);
+        const unsigned char* at = mine + place * stage;
+        place = place + 1 == R::depth ? 0 : place + 1;
+        const auto unit = [&](int j) { return *reinterpret_cast<const Unit<T, V>*>(at + j * 512); };
+        const auto gunit = [&](int j) { return *reinterpret_cast<const Unit<T, V>*>(at + place_bytes + j * 512); };
+        P sum = same<P>(0.f);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int c = column(j);
+            if (c >= a.dim) break;
+            const Unit<T, V> x = unit(j);
+            P d[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = lane_of<T, V>(x, i);
+            keep(c, d);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = plus(sum, d[i]);
+        }
+        const P off = same<P>(-warp_sum(both(sum)) / (float)a.dim);   // - mean
+        sum = same<P>(0.f);
+        const auto centred = [&](int j, int c, P(&d)[N]) {
+            const Unit<T, V> x = unit(j);
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = plus(lane_of<T, V>(x, i), off);
+            keep(c, d);
+        };
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int c = column(j);
+            if (c >= a.dim) break;
+            P d[N];
+            centred(j, c, d);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = times_plus(d[i], d[i], sum);
+        }
+        const P inv = same<P>(1.f / sqrtf(warp_sum(both(sum)) / (float)a.dim + a.eps));
+        if constexpr (!BACK) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int c = column(j);
+                if (c >= a.dim) break;
+                P d[N];
+                centred(j, c, d);
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < N; ++i) values_of<V>(times_plus(times(d[i], inv), w[j][i], b[j][i]), i, o);
+                put(reinterpret_cast<T*>(a.y) + row * a.dim, c, o);
+            }
+        } else {
+            P s0 = same<P>(0.f), s1 = s0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int c = column(j);
+                if (c >= a.dim) break;
+                const Unit<T, V> g = gunit(j);
+                P d[N], y[N], v[N];
+                centred(j, c, d);
+                weight(j, v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = lane_of<T, V>(g, i);
+                keep(c, y);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const P h = times(d[i], inv), z = times(y[i], v[i]);
+                    if constexpr (SUMS) {
+                        aw[j][i] = times_plus(y[i], h, aw[j][i]);
+                        ab[j][i] = plus(ab[j][i], y[i]);
+                    }
+                    s0 = plus(s0, z);
+                    s1 = times_plus(z, h, s1);
+                }
+            }
+            const P m = same<P>(-warp_sum(both(s0)) / (float)a.dim), k = same<P>(-warp_sum(both(s1)) / (float)a.dim);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int c = column(j);
+                if (c >= a.dim) break;
+                const Unit<T, V> x = unit(j), g = gunit(j);
+                P v[N];
+                weight(j, v);
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const P d = times(plus(lane_of<T, V>(x, i), off), inv);
+                    values_of<V>(times(times_plus(d, k, times_plus(lane_of<T, V>(g, i), v[i], m)), inv), i, o);
+                }
+                put(reinterpret_cast<T*>(a.gx) + row * a.dim, c, o);
+            }
+        }
+    }
+    if constexpr (SUMS) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        float* part = a.part + (long long)blockIdx.x * 2 * a.dim;
+        float* sums = reinterpret_cast<float*>(ring);         // without a shift [warps][32 V] of one round's columns, with one [dim]
+        if constexpr (!SHIFT) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    float v[V];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) values_of<V>(which ? ab[j][i] : aw[j][i], i, v);
+                    __syncthreads();
+#pragma unroll
+                    for (int i = 0; i < V; i += 4)
+                        *reinterpret_cast<float4*>(sums + threadIdx.x * V + i) = *reinterpret_cast<const float4*>(v + i);
+                    __syncthreads();
+                    for (int e = threadIdx.x; e < 32 * V; e += 128) {
+                        float t = 0.f;
+#pragma unroll
+                        for (int k = 0; k < R::warps; ++k) t += sums[k * 32 * V + e];
+                        const int c = j * 32 * V + e;
+                        if (c < a.dim) part[which * a.dim + c] = t;
+                    }
+                }
+            return;
+        }
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+            for (int k = 0; k < R::warps; ++k) {              // one warp after another: the order is fixed
+                __syncthreads();
+                if (k != warp) continue;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    if (column(j) >= a.dim) break;
+                    float v[V];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) values_of<V>(which ? ab[j][i] : aw[j][i], i, v);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const int c = column(j) + i;
+                        if (!inside(c)) continue;
+                        const float t = k ? sums[c] + v[i] : v[i];
+                        if (k + 1 < R::warps) sums[c] = t;
+                        else part[which * a.dim + c] = t;
+                    }
+                }
+            }
     }
 }
 
@@ -223,14 +552,14 @@ __global__ void __launch_bounds__(512) k_norm_any(const __grid_constant__ Norm a
         const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
         float s[1] = {0.f};
         for (int c = threadIdx.x; c < a.dim; c += 512) s[0] += to_f(x[c]);
-        row_sums<false, 1>(s, room, turn);
+        row_sums<0, 1>(s, room, turn);
         const float mean = s[0] / (float)a.dim;
         s[0] = 0.f;
         for (int c = threadIdx.x; c < a.dim; c += 512) {
             const float d = to_f(x[c]) - mean;
             s[0] = fmaf(d, d, s[0]);
         }
-        row_sums<false, 1>(s, room, turn);
+        row_sums<0, 1>(s, room, turn);
         const float r = 1.f / sqrtf(s[0] / (float)a.dim + a.eps);
         if (!a.gy) {
             T* y = reinterpret_cast<T*>(a.y) + row * a.dim;
@@ -245,7 +574,7 @@ __global__ void __launch_bounds__(512) k_norm_any(const __grid_constant__ Norm a
             t[0] += g;
             t[1] = fmaf(g, (to_f(x[c]) - mean) * r, t[1]);
         }
-        row_sums<false, 2>(t, room, turn);
+        row_sums<0, 2>(t, room, turn);
         const float m = t[0] / (float)a.dim, k = t[1] / (float)a.dim;
         T* gx = reinterpret_cast<T*>(a.gx) + row * a.dim;
         for (int c = threadIdx.x; c < a.dim; c += 512)
@@ -281,6 +610,7 @@ __global__ void __launch_bounds__(512) k_norm_sums(const float* __restrict__ par
     if (!to) return;
     float t = 0.f;
     if (c < dim)
+#pragma unroll 8
         for (int k = w; k < blocks; k += 16) t += part[(2ll * k + blockIdx.y) * dim + c];
     s[w][lane] = t;
     __syncthreads();
@@ -292,13 +622,13 @@ __global__ void __launch_bounds__(512) k_norm_sums(const float* __restrict__ par
     }
 }
 
-constexpr int kNormBlocks = 4 * kSms;                         // partial sums of a backward pass at most
-constexpr int kLongest = 16384;                               // values of a row that the registers of a block hold
+constexpr int kNormBlocks = 12 * kSms;                         // partial sums of a backward pass at most
+constexpr int kLongest = 8192;                                // values of a row that the registers of a block hold
 
 int vector_of(const fg_norm_args* g, bool backward) {
     const int v = g->type == FG_F32 ? 4 : 8;
     const auto fits = [&](const void* p, long long row) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % v == 0; };
-    return g->dim % v == 0 && fits(g->x, g->x_row) && (backward ? fits(g->gy, g->gy_row) && fits(g->gx, 0) : fits(g->y, 0)) ? v : 1;
+    return g->dim % v == 0 && fits(g->x, g->x_row) && fits(g->w, 0) && fits(g->b, 0) && (backward ? fits(g->gy, g->gy_row) && fits(g->gx, 0) : fits(g->y, 0)) ? v : 1;
 }
 Norm norm_of(const fg_norm_args* g) {
     Norm a{};
@@ -330,28 +660,76 @@ long long norm_work(const fg_norm_args* g) {
     return (kNormBlocks * 2 * g->dim + (any_length(g) ? 2 * g->rows : 0)) * 4;
 }
 
-// f(vector width, units a thread, whether a warp takes a row) as types, and the threads that share a row
+constexpr int kSumThreads = 128;                              // of a backward block whose lanes share rows
+
+// f(V, PER, GROUP, rows at once forward and back) as types, and the threads that share a row. Lanes of a warp share a row where they hold it in
+// 32 values of 16 bits or 20 of fp32 each: no barriers (65,536 rows of 1,024 in bf16 and back: 55 + 160 us, as blocks of 4 warps 87 + 218).
 template <class T, class F>
 void by_shape(int v, int dim, F&& f) {
-    using std::integral_constant;
-    using W = std::true_type;
-    using B = std::false_type;
     const int units = (dim + v - 1) / v;
     constexpr int wide = 16 / (int)sizeof(T);
+    const auto is = [](auto x) { return x; };
+    using std::integral_constant;
+#define SHAPE(V, PER, GROUP, ROWS, BACK, THREADS)                                                                                  \
+    f(is(integral_constant<int, V>()), is(integral_constant<int, PER>()), is(integral_constant<int, GROUP>()),                     \
+      is(integral_constant<int, ROWS>()), is(integral_constant<int, BACK>()), THREADS)
+    const auto block = [&](int per) { return (units + 32 * per - 1) / (32 * per) * 32; };
     if (v > 1) {
-        using V = integral_constant<int, wide>;
-        if (units <= 32) f(V(), integral_constant<int, 1>(), W(), 32);
-        else if (units <= 64) f(V(), integral_constant<int, 2>(), W(), 32);
-        else if (units <= 128) f(V(), integral_constant<int, 4>(), W(), 32);
-        else if (units <= 1024) f(V(), integral_constant<int, 1>(), B(), (units + 31) / 32 * 32);
-        else f(V(), integral_constant<int, 4>(), B(), (units + 127) / 128 * 32);
+        if (units <= 8) SHAPE(wide, 1, 8, 2, 2, 8);
+        else if (units <= 16) SHAPE(wide, 2, 8, 1, 1, 8);
+        else if (units <= 32) SHAPE(wide, 1, 32, 2, 2, 32);
+        else if (units <= 64) SHAPE(wide, 2, 32, 2, 1, 32);
+        else if (units <= 512) SHAPE(wide, 1, 0, 4, 2, block(1));
+        else SHAPE(wide, 16 / wide, 0, 1, 1, block(16 / wide));
     } else {
-        using V = integral_constant<int, 1>;
-        if (units <= 128) f(V(), integral_constant<int, 4>(), W(), 32);
-        else if (units <= 544) f(V(), integral_constant<int, 17>(), W(), 32);
-        else if (units <= 4096) f(V(), integral_constant<int, 4>(), B(), (units + 127) / 128 * 32);
-        else f(V(), integral_constant<int, 16>(), B(), (units + 511) / 512 * 32);
+        if (units <= 32) SHAPE(1, 4, 8, 1, 1, 8);
+        else if (units <= 128) SHAPE(1, 4, 32, 2, 2, 32);
+        else if (units <= 2048) SHAPE(1, 4, 0, 4, 2, block(4));
+        else SHAPE(1, 16, 0, 1, 1, block(16));
     }
+#undef SHAPE
+}
+
+// f(PER, SHIFT) as types where rows are many and go through the ring: up to 128 units of 16 bytes, beginning at one place in 16 bytes in
+// all that is read and written
+template <class T, class F>
+bool by_ring(const fg_norm_args* g, bool back, F&& f) {
+    constexpr int V = 16 / (int)sizeof(T);
+    using std::integral_constant;
+    const auto fits = [&](const void* p, long long row) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (row - g->dim) % V == 0; };
+    if (g->rows < 16 * kSms || !fits(g->x, g->x_row)) return false;
+    if (back ? !fits(g->gy, g->gy_row) || !fits(g->gx, g->dim) : !fits(g->y, g->dim)) return false;
+    const bool shift = g->dim % V != 0;
+    if (shift && (g->x_row < g->dim || (back && g->gy_row < g->dim))) return false;   // (behind a row lies another)
+    const int units = Ring<T, V, false>::units((int)g->dim, shift);
+    constexpr int most = 32 / V;                             // 32 values a lane
+    if (units <= 16 || units > 32 * most) return false;      // (short rows: several to a warp)
+    const auto by_per = [&](auto per) {
+        if (shift) f(per, std::true_type());
+        else f(per, std::false_type());
+    };
+    if (units <= 32) by_per(integral_constant<int, 1>());
+    else if (units <= 64) by_per(integral_constant<int, 2>());
+    else if (units <= 128 || most == 4) by_per(integral_constant<int, 4>());
+    else by_per(integral_constant<int, most>());
+    return true;
+}
+// As many as run at once (a second round of them would find the SMs half empty: 137 instead of 89 us), and an even number: 4 rows a
+// block, so a warp's rows are a multiple of 8 apart.
+template <class T, bool SHIFT, bool BACK>
+int ring_blocks(int dim) {
+    using R = Ring<T, 16 / (int)sizeof(T), BACK>;
+    return kSms * std::min(4, 220 * 1024 / (R::bytes((R::units(dim, SHIFT) + 31) / 32, SHIFT) + 1024));
+}
+template <class T, int PER, bool SHIFT, bool BACK, bool SUMS>
+void ring_launch(const Norm& a, cudaStream_t st) {
+    constexpr int V = 16 / (int)sizeof(T);
+    using R = Ring<T, V, BACK>;
+    auto* kernel = k_norm_ring<T, V, PER, SHIFT, BACK, SUMS>;
+    static OnEachDevice here;
+    here.first(current_device(), [&] { allow_shared(kernel, R::bytes(PER, SHIFT)); });
+    const int rounds = (R::units(a.dim, SHIFT) + 31) / 32;
+    kernel<<<ring_blocks<T, SHIFT, BACK>(a.dim), 128, R::bytes(rounds, SHIFT), st>>>(a, rounds);
 }
 
 template <class T>
@@ -361,13 +739,14 @@ void norm_forward(const fg_norm_args* g, cudaStream_t st) {
         k_norm_any<T><<<(unsigned)std::min<long long>(a.rows, kSms * 4), 512, 0, st>>>(a, nullptr);
         return;
     }
-    by_shape<T>(vector_of(g, false), a.dim, [&](auto v, auto per, auto warp, int threads) {
-        constexpr bool W = decltype(warp)::value;
-        // a warp a row: few rows spread over the SMs
-        const int warps = W ? (int)std::min<long long>(8, (a.rows + kSms - 1) / kSms) : 1;
-        const long long blocks = (a.rows + warps - 1) / warps;
+    if (by_ring<T>(g, false, [&](auto per, auto shift) { ring_launch<T, decltype(per)::value, decltype(shift)::value, false, false>(a, st); })) return;
+    by_shape<T>(vector_of(g, false), a.dim, [&](auto v, auto per, auto group, auto rows, auto, int threads) {
+        constexpr int G = decltype(group)::value, R = decltype(rows)::value;
+        // few rows: a warp a block, spread over the SMs
+        const int block = G ? a.rows >= 16 * kSms * R ? 256 : 32 : threads;
+        const long long at_once = (G ? block / threads : 1) * R, blocks = (a.rows + at_once - 1) / at_once;
         need(blocks < (1ll << 31), "fg_layer_norm: too many rows");
-        k_norm<T, decltype(v)::value, decltype(per)::value, W><<<(unsigned)blocks, W ? 32 * warps : threads, 0, st>>>(a);
+        k_norm<T, decltype(v)::value, decltype(per)::value, G, R><<<(unsigned)blocks, block, 0, st>>>(a);
     });
 }
 
@@ -384,14 +763,19 @@ void norm_backward(const fg_norm_args* g, cudaStream_t st) {
             blocks = (int)std::min<long long>(a.rows, 64);
             k_norm_columns<T><<<dim3((unsigned)((a.dim + 255) / 256), blocks), 256, 0, st>>>(a, stats);
         }
+    } else if (by_ring<T>(g, true, [&](auto per, auto shift) {
+                   blocks = ring_blocks<T, decltype(shift)::value, true>(a.dim);
+                   if (sums) ring_launch<T, decltype(per)::value, decltype(shift)::value, true, true>(a, st);
+                   else ring_launch<T, decltype(per)::value, decltype(shift)::value, true, false>(a, st);
+               })) {
     } else {
-        by_shape<T>(vector_of(g, true), a.dim, [&](auto v, auto per, auto warp, int threads) {
-            constexpr int V = decltype(v)::value, PER = decltype(per)::value;
-            constexpr bool W = decltype(warp)::value;
-            const int warps = W ? (int)std::min<long long>(8, (a.rows + kSms - 1) / kSms) : 1;
-            blocks = (int)std::min<long long>(kNormBlocks, (a.rows + warps - 1) / warps);
-            if (sums) k_norm_bwd<T, V, PER, W, true><<<blocks, W ? 32 * warps : threads, W ? warps * 32 * V * 4 : 0, st>>>(a);
-            else k_norm_bwd<T, V, PER, W, false><<<blocks, W ? 32 * warps : threads, 0, st>>>(a);
+        by_shape<T>(vector_of(g, true), a.dim, [&](auto v, auto per, auto group, auto, auto rows, int threads) {
+            constexpr int V = decltype(v)::value, PER = decltype(per)::value, G = decltype(group)::value, R = decltype(rows)::value;
+            const int block = G ? kSumThreads : threads;
+            const long long at_once = (G ? block / threads : 1) * R;
+            blocks = (int)std::min<long long>(G ? 3 * kSms : std::min(kNormBlocks, kSms * std::max(1, 768 / block)), (a.rows + at_once - 1) / at_once);
+            if (sums) k_norm_bwd<T, V, PER, G, R, true><<<blocks, block, G ? block * V * 4 : 0, st>>>(a);
+            else k_norm_bwd<T, V, PER, G, R, false><<<blocks, block, 0, st>>>(a);
         });
     }
     MCK(cudaGetLastError());
@@ -438,13 +822,15 @@ __global__ void __launch_bounds__(256) k_dropout(const __grid_constant__ Drop a)
         if (WIDE && block * 8 + 8 <= a.n) {
 #pragma unroll
             for (int u = 0; u < 8; u += V) {
-                float v[V], o[V];
-                load<T, V>(x + u, v);
+                const Unit<T, V> v = load<T, V>(x + u);
+                Unit<T, V> r{};
+                float o[V];
+                if (add) r = load<T, V>(add + u);
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = 0.f;
-                if (add) load<T, V>(add + u, o);
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = bits[u + i] >= a.least ? fmaf(v[i], a.by, o[i]) : o[i];
+                for (int i = 0; i < V; ++i) {
+                    const float b = add ? to_f(r.v[i]) : 0.f;
+                    o[i] = bits[u + i] >= a.least ? fmaf(to_f(v.v[i]), a.by, b) : b;
+                }
                 store<T, V>(y + u, o);
             }
         } else {

@@ -60,6 +60,7 @@ struct MemErr {
     std::string msg;
 };
 std::string& last_error();
+int step_gave_up(cudaStream_t st);       // whether a wait of fg_delta_step has run out (the stream is waited for)
 
 #define MCK(call)                                                                                         \
     do {                                                                                                  \
