@@ -371,17 +371,35 @@ struct Room {
 struct Wide {
     float *q = nullptr, *k = nullptr, *v = nullptr, *last = nullptr;
 };
+// Parts of a recording (k_delta_join): as many as keep the blocks within one round of the SMs, of 512 ticks at least; four at least, or
+// the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: PARTS us in 27 parts, 5,230 in one.
+int parts_of(const fg_delta_args* g) {
+    const long long rows = std::max<long long>(1, g->batch * g->heads), mean = g->offsets ? g->ticks / std::max<long long>(1, g->batch) : g->ticks;
+    const long long parts = std::min<long long>(64, std::min(12 * kSms / (rows * ((g->value_dim + 15) / 16)), mean / 512));
+    return parts >= 4 ? (int)parts : 1;
+}
 // places s's parts; returns their size
 long long lay_out(const fg_delta_args* g, bool backward, Delta& s, Wide& wide) {
     Room room{static_cast<char*>(g->work)};
-    const int in = g->type == FG_F32 ? 3 : g->type == FG_F16 ? 2 : 1, kept = std::max(in, 2);
+    const auto of = [&](auto f) {
+        return g->type == FG_F32 ? f(Terms<float>()) : g->type == FG_F16 ? f(Terms<__half>()) : f(Terms<bf16>());
+    };
+    const int in = of([](auto t) { return t.in; }), out = of([](auto t) { return t.out; }), square = of([](auto t) { return t.square; }),
+              saved = of([](auto t) { return t.saved; }), grad = of([](auto t) { return t.grad; });
     const long long places = slots_of(g) * g->heads, tiles = (g->value_dim + 15) / 16, pieces = g->dim > 64 ? 8 : 4;
-    room.take(s.x, places * kept * kTicks * kTicks * 2);
-    room.take(s.p, places * (backward ? kept : in) * kTicks * kTicks * 2);
+    room.take(s.x, places * square * 2 * kChunk * kChunk * 2);
+    room.take(s.p, places * (backward ? square : out) * 2 * kChunk * kChunk * 2);
     room.take(s.gates, places * kGates * kTicks * 4);
+    s.parts = parts_of(g);
+    if (s.parts > 1) {
+        const long long all = g->batch * g->heads * s.parts * 4, dim = 16 * pieces;
+        room.take(s.own, all * 16 * tiles * dim);
+        room.take(s.turn, all * dim * dim);
+        room.take(s.start, all * 16 * tiles * dim);
+    }
     if (!backward) return room.used;
-    room.take(s.states, places * tiles * kept * pieces * 512);
-    room.take(s.gstates, places * tiles * (in == 1 ? 1 : kept) * pieces * 512);
+    room.take(s.states, places * tiles * saved * pieces * 512);
+    room.take(s.gstates, places * tiles * grad * pieces * 512);
     room.take(s.w, places * tiles * 8 * 512);
     room.take(s.u, places * kTicks * 16 * tiles * (in == 1 ? 2 : 4));
     room.take(s.od, places * tiles * kTicks * 4);
@@ -451,18 +469,25 @@ void prepare(const Delta& s, cudaStream_t st) {
     if (s.slots) launch(k_delta_prep<T, DP, NP>, dim3((unsigned)s.slots, s.heads), 128, PrepLayout<T, DP>::bytes, here, st, s);
 }
 // WARPS: 16 columns of values each
-template <class T, int DP, int WARPS, bool KEEP>
+template <class T, int DP, int WARPS, int MODE>
 void chain(const Delta& s, cudaStream_t st) {
     static OnEachDevice here;
-    using Lay = ChainLayout<T, DP, WARPS, KEEP ? Terms<T>::kept : Terms<T>::out, KEEP>;
-    const long long blocks = s.batch * s.heads * ((s.E + 16 * WARPS - 1) / (16 * WARPS));
-    launch(k_delta_chain<T, DP, WARPS, KEEP>, dim3((unsigned)blocks), 32 * WARPS, Lay::bytes, here, st, s);
+    using Lay = ChainLayout<T, DP, WARPS, MODE == kKeep ? Terms<T>::square : Terms<T>::out, MODE == kKeep>;
+    const int tiles = (s.E + 15) / 16 + (MODE >= kParts ? (s.D + 15) / 16 : 0);
+    const long long blocks = s.batch * s.heads * ((tiles + WARPS - 1) / WARPS);
+    launch(k_delta_chain<T, DP, WARPS, MODE>, dim3((unsigned)blocks, s.parts), 32 * WARPS, Lay::bytes, here, st, s);
 }
-template <class T, int DP, int WARPS>
+template <class T, int DP, int WARPS, bool PARTS>
 void chain_back(const Delta& s, cudaStream_t st) {
     static OnEachDevice here;
     const long long blocks = s.batch * s.heads * ((s.E + 16 * WARPS - 1) / (16 * WARPS));
-    launch(k_delta_back<T, DP, WARPS>, dim3((unsigned)blocks), 32 * WARPS, ChainLayout<T, DP, WARPS, Terms<T>::kept, true>::bytes, here, st, s);
+    launch(k_delta_back<T, DP, WARPS, PARTS>, dim3((unsigned)blocks, s.parts), 32 * WARPS, ChainLayout<T, DP, WARPS, Terms<T>::square, true>::bytes,
+           here, st, s);
+}
+template <int DP, bool BACK>
+void join(const Delta& s, cudaStream_t st) {
+    k_delta_join<DP, BACK><<<(unsigned)(s.batch * s.heads * ((s.E + 15) / 16)), 2 * DP, 0, st>>>(s);
+    MCK(cudaGetLastError());
 }
 template <class T>
 void gradients(const Delta& s, cudaStream_t st) {
@@ -470,28 +495,34 @@ void gradients(const Delta& s, cudaStream_t st) {
     if (s.slots) launch(k_delta_grads<T>, dim3((unsigned)s.slots, s.heads, (s.D + 63) / 64), 256, GradLayout<T>::bytes, here, st, s);
 }
 
+// the state that each part of a recording begins with
+template <class T, int DP, int MODE>
+void parts_forward(const Delta& s, cudaStream_t st) {
+    if (s.parts == 1) return;
+    chain<T, DP, 4, MODE>(s, st);
+    join<DP, false>(s, st);
+}
 template <class T, int DP>
 void forward(const Delta& s, cudaStream_t st) {
     prepare<T, DP, Terms<T>::out>(s, st);
-    if constexpr (Terms<T>::in == 1) {
-        if (s.E > 64) return chain<T, DP, 8, false>(s, st);
-    }
-    chain<T, DP, 4, false>(s, st);
+    parts_forward<T, DP, kParts>(s, st);
+    chain<T, DP, 4, kForward>(s, st);
 }
 template <class T, int DP>
 void backward(Delta s, float* last, cudaStream_t st) {
-    prepare<T, DP, Terms<T>::kept>(s, st);
+    prepare<T, DP, Terms<T>::square>(s, st);
     s.last = last;
-    constexpr bool wide = Terms<T>::in == 1;
-    if (wide && s.E > 64) {
-        if constexpr (wide) {
-            chain<T, DP, 8, true>(s, st);
-            chain_back<T, DP, 8>(s, st);
-        }
-    } else {
-        chain<T, DP, 4, true>(s, st);
-        chain_back<T, DP, 4>(s, st);
+    parts_forward<T, DP, Terms<T>::learn == Terms<T>::forward ? kParts : kPartsKeep>(s, st);
+    // 64 or 128 columns of values a block; 16 warps an SM where 128 registers a thread do (the chain back, W = 4 and 8: 863 and 758 us)
+    constexpr int wide = Terms<T>::in == 1 && DP == 128 ? 8 : 4;
+    if (s.E > 64) chain<T, DP, wide, kKeep>(s, st);
+    else chain<T, DP, 4, kKeep>(s, st);
+    if (s.parts > 1) {
+        chain_back<T, DP, 4, true>(s, st);
+        join<DP, true>(s, st);
     }
+    if (s.E > 64) chain_back<T, DP, wide, false>(s, st);
+    else chain_back<T, DP, 4, false>(s, st);
     gradients<T>(s, st);
 }
 

@@ -14,8 +14,10 @@ namespace {
 using namespace fgm;
 using bf16 = __nv_bfloat16;
 
-constexpr int kTicks = 64;               // of a chunk
+constexpr int kTicks = 64;               // of a slot: where states are kept for the gradients
+constexpr int kChunk = 32;               // of a chunk of the chain, two to a slot
 constexpr int kSquare = kTicks + 8;      // a row of a 64 x 64 tile in shared memory: 8 rows of 16 bytes lie in 32 banks
+constexpr int kSmall = kChunk + 8;       // and of a 32 x 32 one
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -47,6 +49,12 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// the product without a sum before it
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // a pair of values as N packed terms
 template <int N>
 __device__ __forceinline__ void terms(float x, float y, uint32_t (&t)[N]) {
@@ -104,18 +112,18 @@ __device__ __forceinline__ void async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Rows 0 .. 63 of an operand (`rows` of them there, the rest zeros), columns 0 .. COLS - 1 of `cols`, as N planes of terms
+// Rows 0 .. ROWS - 1 of an operand (`rows` of them there, the rest zeros), columns 0 .. COLS - 1 of `cols`, as N planes of terms
 // with rows of STRIDE values. bf16 at 16-byte boundaries goes by asynchronous copies.
-template <class T, int N, int COLS, int STRIDE, int THREADS>
+template <class T, int N, int COLS, int STRIDE, int THREADS, int ROWS = kTicks>
 __device__ __forceinline__ void load_tile(bf16* to, const T* p, long long row, int rows, int cols, bool fast, int tid) {
-    constexpr int kUnits = COLS / 8, kPlane = kTicks * STRIDE, kStep = THREADS / kUnits;
-    static_assert(THREADS % kUnits == 0 && kTicks % kStep == 0, "a thread keeps its columns");
+    constexpr int kUnits = COLS / 8, kPlane = ROWS * STRIDE, kStep = THREADS / kUnits;
+    static_assert(THREADS % kUnits == 0 && ROWS % kStep == 0, "a thread keeps its columns");
     const int r0 = tid / kUnits, c = tid % kUnits * 8;
     const bool has = c < cols;
     const T* q = p + (has ? r0 * row + c : 0);
     bf16* at = to + r0 * STRIDE + c;
 #pragma unroll 4
-    for (int r = r0; r < kTicks; r += kStep, q += kStep * row, at += kStep * STRIDE) {
+    for (int r = r0; r < ROWS; r += kStep, q += kStep * row, at += kStep * STRIDE) {
         const bool in = has && r < rows;
         if constexpr (N == 1 && std::is_same<T, bf16>::value) {
             if (fast) {
@@ -148,17 +156,17 @@ __device__ __forceinline__ void load_tile(bf16* to, const T* p, long long row, i
         for (int n = 0; n < N; ++n) *reinterpret_cast<uint4*>(at + n * kPlane) = make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]);
     }
 }
-// N planes of a 64 x 64 tile from the workspace (rows of 64) to rows of kSquare
+// N planes of a 32 x 32 tile from the workspace (rows of 32) to rows of kSmall
 template <int N, int THREADS>
-__device__ __forceinline__ void load_square(bf16* to, const bf16* p, int tid) {
-    for (int i = tid; i < N * kTicks * 8; i += THREADS) async16(smem_at(to + (i >> 3) * kSquare + (i & 7) * 8), p + i * 8, true);
+__device__ __forceinline__ void load_small(bf16* to, const bf16* p, int tid) {
+    for (int i = tid; i < N * kChunk * 4; i += THREADS) async16(smem_at(to + (i >> 2) * kSmall + (i & 3) * 8), p + i * 8, true);
 }
 
-// 16 sums over the 8 lanes with the same t4, of v[2 j + i] = a value of column 8 j + 2 t4 + i: lane g keeps columns 8 g + 2 t4, + 1
-__device__ __forceinline__ float2 column_sums(float (&v)[16], int lane) {
+// 8 sums over the 8 lanes g with the same t4, of v[2 j + i] = a value of column 8 j + 2 t4 + i: lane g keeps column 8 (g / 2) + 2 t4 + g % 2
+__device__ __forceinline__ float column_sums(float (&v)[8], int lane) {
 #pragma unroll
-    for (int half = 8; half >= 2; half >>= 1) {
-        const int bit = half * 2;                            // lanes 16, 8, 4 apart
+    for (int half = 4; half >= 1; half >>= 1) {
+        const int bit = half * 4;                            // lanes 16, 8, 4 apart
         const bool upper = lane & bit;
 #pragma unroll
         for (int i = 0; i < half; ++i) {
@@ -166,13 +174,16 @@ __device__ __forceinline__ float2 column_sums(float (&v)[16], int lane) {
             v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
         }
     }
-    return make_float2(v[0], v[1]);
+    return v[0];
 }
 
-// the types' terms: of inputs, of what is carried (states, corrections), of outputs
+// Terms by type: of inputs; of what a chunk corrects by (X, P and what they meet); of states, of their gradients and of what is added to
+// them, on the way forward and where gradients are wanted; of states as they are kept for those; of operands of q's and k's gradients.
+// With bf16 inputs states are 4e-6 of their norm off at two terms, 1.5e-6 at three. Two are enough for o and the last states; the gates'
+// gradients are differences of what they give (1e-5 at two, 4e-6 at three; 64 recordings of 1,024 ticks, 8 heads of 128: TIMES).
 template <class T> struct Terms;
-template <> struct Terms<bf16> { static constexpr int in = 1, kept = 2, out = 1; };
-template <> struct Terms<__half> { static constexpr int in = 2, kept = 2, out = 2; };
-template <> struct Terms<float> { static constexpr int in = 3, kept = 3, out = 3; };
+template <> struct Terms<bf16> { static constexpr int in = 1, square = 2, forward = 2, learn = 3, saved = 2, grad = 1, out = 1; };
+template <> struct Terms<__half> { static constexpr int in = 2, square = 3, forward = 3, learn = 3, saved = 3, grad = 2, out = 2; };
+template <> struct Terms<float> { static constexpr int in = 3, square = 3, forward = 3, learn = 3, saved = 3, grad = 3, out = 3; };
 
 }  // namespace

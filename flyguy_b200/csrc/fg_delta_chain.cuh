@@ -1,21 +1,22 @@
-// The gated delta rule over chunks of 64 ticks. With G the log decays added up from the chunk's first tick on, M_ts = exp(G_t - G_s),
+// The gated delta rule over chunks of 32 ticks. With G the log decays added up from the chunk's first tick on, M_ts = exp(G_t - G_s),
 // L = K K^T . M below the diagonal, P = scale Q K^T . M on and below it, B = diag(beta):
 //
 //   X = (I + L B)^-1 L
 //   N = V - e^G K S,  W = N - X B N,  U = B W            W_t = v_t - g_t k_t S_{t-1}, what a tick's key did not foretell
-//   O = scale e^G Q S + P U,  S <- e^{G_63} S + (e^{G_63 - G} K)^T U
+//   O = scale e^G Q S + P U,  S <- e^{G_31} S + (e^{G_31 - G} K)^T U
 //
 // and back, R the gradient of the state behind the chunk:
-//   dU = e^{G_63 - G} K R + P^T dO,  dR = dU - X^T B dU,  dN = B dR = dV,  dbeta = rows of dR . W
-//   R <- e^{G_63} R + (scale e^G dO)^T Q - (e^G dN)^T K   (transposed)
-//   dlog_decay_t: o_t dO_t - v_t dN_t, added up from the chunk's last tick on, behind which it is <R, S>
+//   dU = e^{G_31 - G} K R + P^T dO,  dR = dU - X^T B dU,  dN = B dR = dV,  dbeta = rows of dR . W
+//   R <- e^{G_31} R + (scale e^G dO)^T Q - (e^G dN)^T K   (transposed)
+//   dlog_decay_t: o_t dO_t - v_t dN_t, added up from a slot's last tick on, behind which it is <R, S>
 //
 // k_delta_prep makes X, P and the gates of every chunk, all at once. What is left runs from chunk to chunk, and there each column of the
 // state goes its own way: a warp owns 16 of them, S transposed (16 columns x dim) in registers as an accumulator, and every product has
 // them for rows: N^T = V^T - S^T K^T, W^T = N^T - (N^T B) X^T, O^T = S^T Q^T + U^T P^T, S^T += U^T K. An accumulator is the next
 // product's left operand as it lies, so states, corrections and outputs never leave the registers, and warps meet only to have tiles of
 // K, Q, V, X, P loaded (mma.sync: 25% of the tensor cores' rate, but the chain from state to state has no trip through shared
-// memory or TMEM in it).
+// memory or TMEM in it). Chunks of 32 ticks leave room for 16 warps an SM at dim 128; with 64 ticks, 8 warps, the products were the same
+// and waited twice as long on one another.
 #pragma once
 #include "fg_delta.cuh"
 
@@ -33,13 +34,16 @@ struct Delta {
     long long batch, ticks, slots;
     int heads, D, E, gq_f32, gk_f32, dn_f32;
     float scale;
-    bf16 *x, *p;                     // [slot][head][term][64][64]
-    float* gates;                    // [slot][head][5][64]: e^G, e^{G_63 - G}, beta, G as two floats
-    uint4 *states, *gstates;         // [slot][head][tile of 16 columns][term][DP / 16][32]: S and R as left operands
-    float4* w;                       // [slot][head][tile][8][32]: W^T as accumulators
+    bf16 *x, *p;                     // [slot][head][chunk][term][32][32]
+    float* gates;                    // [slot][head][5][64]: e^G and e^{G_31 - G} of the chunks, beta, G of the slot as two floats
+    uint4 *states, *gstates;         // [slot][head][tile of 16 columns][term][DP / 16][32]: S before and R behind as left operands
+    float4* w;                       // [slot][head][chunk][tile][4][32]: W^T as accumulators
     char* u;                         // [slot][head][64][16 tiles]: U in bf16 (inputs of one term) or fp32
     float *od, *vdn, *db;            // [slot][head][tile][64]: rows of o dO, v dN, dbeta
-    float* anchor;                   // [slot][head][tile]
+    float* anchor;                   // [slot][head][tile]: <R, S> behind
+    // few long recordings are split into parts, see k_delta_join
+    int parts;
+    float *own, *turn, *start;       // [batch][heads][part] of [16 tiles][DP], [DP][DP], [16 tiles][DP], all transposed
 };
 
 __device__ __forceinline__ Span span_of(const Delta& s, long long b) {
@@ -47,16 +51,16 @@ __device__ __forceinline__ Span span_of(const Delta& s, long long b) {
     const long long lo = min(max(s.offsets[b], 0ll), s.ticks), hi = min(max(s.offsets[b + 1], lo), s.ticks);
     return {lo, hi - lo};
 }
-// the chunks of recording b have the slots from here on; recordings end to end, of n ticks each, take ceil(n / 64) and leave at most one
+// recording b has the slots from here on; recordings end to end, of n ticks each, take ceil(n / 64) and leave at most one
 // slot between them, ticks / 64 + batch in all
 __device__ __forceinline__ long long slot_of(const Delta& s, long long b, long long start) {
     return s.offsets ? start / kTicks + b : b * ((s.ticks + kTicks - 1) / kTicks);
 }
-struct Chunk {
+struct Slot {
     long long b, first;              // recording, first tick (of the recording's)
     int n;                           // ticks, 0: this slot is empty
 };
-__device__ __forceinline__ Chunk chunk_of(const Delta& s, long long slot) {
+__device__ __forceinline__ Slot ticks_of(const Delta& s, long long slot) {
     if (!s.offsets) {
         const long long per = (s.ticks + kTicks - 1) / kTicks, b = slot / per, first = (slot - b * per) * kTicks;
         return {b, first, (int)min((long long)kTicks, s.ticks - first)};
@@ -71,6 +75,15 @@ __device__ __forceinline__ Chunk chunk_of(const Delta& s, long long slot) {
     const long long first = (slot - slot_of(s, lo, sp.start)) * kTicks;
     return {lo, first, first < 0 ? 0 : (int)max(0ll, min((long long)kTicks, sp.n - first))};
 }
+// the chunks of a part: whole slots, as many in each but the last ones
+struct Part {
+    int first, end;
+};
+__device__ __forceinline__ Part part_of(const Delta& s, long long n, int part) {
+    const long long slots = (n + kTicks - 1) / kTicks, per = 2 * ((slots + s.parts - 1) / s.parts);
+    const int chunks = (int)((n + kChunk - 1) / kChunk);
+    return {(int)min((long long)chunks, part * per), (int)min((long long)chunks, (part + 1) * per)};
+}
 template <class T>
 __device__ __forceinline__ T* row_of(const Delta& s, const Operand& o, long long b, int h, long long tick) {
     return reinterpret_cast<T*>(o.p) + (s.offsets ? 0 : b * o.batch) + tick * o.tick + (h / o.share) * o.head;
@@ -83,29 +96,29 @@ __device__ __forceinline__ float* gate_of(const Delta& s, const Gate& o, long lo
 
 template <class T, int DP>
 struct PrepLayout {
-    static constexpr int in = Terms<T>::in, kept = Terms<T>::kept, stride = DP + 8, tile = in * kTicks * stride,
-                         square = kept * kTicks * kSquare;
-    static constexpr int tiles = 2 * tile > 2 * square ? 2 * tile : 2 * square;   // K and Q, later L B and X
-    static constexpr int l = kTicks * 68, bytes = 2 * tiles + 4 * (l + 4 * kTicks);
+    static constexpr int in = Terms<T>::in, square = Terms<T>::square, stride = DP + 8, tile = in * kTicks * stride,
+                         small = 2 * square * kChunk * kSmall;                       // of both chunks
+    static constexpr int tiles = 2 * tile > 2 * small ? 2 * tile : 2 * small;        // K and Q, later L B and X
+    static constexpr int lrow = kChunk + 4, l = kTicks * lrow, bytes = 2 * tiles + 4 * (l + 3 * kTicks);
 };
 
-// NP: terms of P. A block of 4 warps makes one chunk of one head: warp w the rows 16 w .. of K K^T and Q K^T, then the block (w, w) of X
-// by substitution, then X's column block w downwards, X^T as an accumulator like the states of the chain.
+// NP: terms of P. A block of 4 warps makes one slot of one head: warp w rows 16 w .. of its chunk's K K^T and Q K^T, then its block of X
+// on the diagonal by substitution; the block below that by products, X^T as an accumulator like the states of the chain.
 template <class T, int DP, int NP>
 __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delta s) {
     using Lay = PrepLayout<T, DP>;
-    constexpr int NI = Lay::in, NS = Lay::kept, kStride = Lay::stride, kPlane = kTicks * kStride, kSq = kTicks * kSquare;
+    constexpr int NI = Lay::in, NX = Lay::square, kStride = Lay::stride, kPlane = kTicks * kStride, kSm = kChunk * kSmall, kL = Lay::lrow;
     extern __shared__ __align__(16) unsigned char smem[];
-    bf16 *sk = reinterpret_cast<bf16*>(smem), *sq = sk + Lay::tile, *sa = sk, *sx = sk + Lay::square;
+    bf16 *sk = reinterpret_cast<bf16*>(smem), *sa = sk, *sx = sk + Lay::small;
     float *sl = reinterpret_cast<float*>(smem + 2 * Lay::tiles), *gh = sl + Lay::l, *gl = gh + kTicks, *beta = gl + kTicks;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, chunk = warp >> 1, lower = warp & 1;
     const long long slot = blockIdx.x;
     const int h = blockIdx.y;
-    const Chunk c = chunk_of(s, slot);
+    const Slot c = ticks_of(s, slot);
     if (c.n == 0) return;
     const long long tick = (s.offsets ? span_of(s, c.b).start : 0) + c.first;
     load_tile<T, NI, DP, kStride, 128>(sk, row_of<const T>(s, s.k, c.b, h, tick), s.k.tick, c.n, s.D, s.k.fast, tid);
-    load_tile<T, NI, DP, kStride, 128>(sq, row_of<const T>(s, s.q, c.b, h, tick), s.q.tick, c.n, s.D, s.q.fast, tid);
+    load_tile<T, NI, DP, kStride, 128>(sk + Lay::tile, row_of<const T>(s, s.q, c.b, h, tick), s.q.tick, c.n, s.D, s.q.fast, tid);
     async_commit();
     const long long place = slot * s.heads + h;
     if (warp == 0) {
@@ -113,11 +126,12 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
         // fp32, so nothing lower is needed, and minus infinity (a state forgotten) stays out of the differences.
         double sum[2];
         float lv[2], bv[2];
+        const float *lp = gate_of(s, s.log_decay, c.b, h, tick), *bp = gate_of(s, s.beta, c.b, h, tick);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = 2 * lane + i;
-            lv[i] = r < c.n ? *gate_of(s, s.log_decay, c.b, h, tick + r) : 0.f;
-            bv[i] = r < c.n ? *gate_of(s, s.beta, c.b, h, tick + r) : 0.f;
+            lv[i] = r < c.n ? lp[r * s.log_decay.tick] : 0.f;
+            bv[i] = r < c.n ? bp[r * s.beta.tick] : 0.f;
             lv[i] = lv[i] < -256.f ? -256.f : lv[i];
         }
         sum[0] = lv[0];
@@ -128,7 +142,7 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
             const double x = __shfl_up_sync(0xffffffffu, before, o);
             if (lane >= o) before += x;
         }
-        const double all = __shfl_sync(0xffffffffu, before, 31);
+        const double end = __shfl_sync(0xffffffffu, before, lane | 15), middle = __shfl_sync(0xffffffffu, before, 15);
         before -= sum[1];
         float* out = s.gates + place * kGates * kTicks;
 #pragma unroll
@@ -138,8 +152,8 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
             gh[r] = (float)v;
             gl[r] = (float)(v - (double)gh[r]);
             beta[r] = bv[i];
-            out[r] = expf((float)v);
-            out[kTicks + r] = expf((float)(all - v));
+            out[r] = expf((float)(lane < 16 ? v : v - middle));
+            out[kTicks + r] = expf((float)(end - v));
             out[2 * kTicks + r] = bv[i];
             out[3 * kTicks + r] = gh[r];
             out[4 * kTicks + r] = gl[r];
@@ -148,72 +162,78 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
     async_wait<0>();
     __syncthreads();
 
-    const uint32_t rows_m = at_rows_m(lane, kStride) + smem_at(sk) + 2 * (16 * warp * kStride), rows_n = at_rows_n(lane, kStride) + smem_at(sk);
-    const uint32_t to_q = 2 * Lay::tile;
-    bf16* p_out = s.p + place * NP * kTicks * kTicks;
-    const int r0 = 16 * warp + g;
-#pragma unroll 1
-    for (int jp = 0; jp <= warp; ++jp) {
-        float kk[2][4] = {}, qk[2][4] = {};
+    const uint32_t rows_m = at_rows_m(lane, kStride) + smem_at(sk) + 2 * (16 * warp * kStride),
+                   rows_n = at_rows_n(lane, kStride) + smem_at(sk) + 2 * (kChunk * chunk * kStride);
+    constexpr uint32_t to_q = 2 * Lay::tile;
+    bf16* p_out = s.p + (2 * place + chunk) * NP * kChunk * kChunk;
+    // the block left of the diagonal (of the lower rows), then the one on it
+    float kk[2][2][4] = {}, qk[2][2][4] = {};
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-            uint32_t a[NI][4], q[NI][4], b[4];
+    for (int d = 0; d < DP / 16; ++d) {
+        uint32_t a[NI][4], q[NI][4], b[4];
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                ldsm(a[i], rows_m + 2 * (i * kPlane + 16 * d));
-                ldsm(q[i], rows_m + to_q + 2 * (i * kPlane + 16 * d));
-            }
+        for (int i = 0; i < NI; ++i) {
+            ldsm(a[i], rows_m + 2 * (i * kPlane + 16 * d));
+            ldsm(q[i], rows_m + to_q + 2 * (i * kPlane + 16 * d));
+        }
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+            if (jp > lower) break;
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 ldsm(b, rows_n + 2 * (j * kPlane + 16 * jp * kStride + 16 * d));
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    if (i + j >= NS) continue;
-                    mma(kk[0], a[i], b[0], b[1]);
-                    mma(kk[1], a[i], b[2], b[3]);
-                    mma(qk[0], q[i], b[0], b[1]);
-                    mma(qk[1], q[i], b[2], b[3]);
+                    if (i + j >= NX) continue;
+                    mma(kk[jp][0], a[i], b[0], b[1]);
+                    mma(kk[jp][1], a[i], b[2], b[3]);
+                    mma(qk[jp][0], q[i], b[0], b[1]);
+                    mma(qk[jp][1], q[i], b[2], b[3]);
                 }
             }
         }
+    }
+    __syncthreads();                                          // K and Q have been read: L B goes over them
+    float* l_rows = sl + (kChunk * chunk) * kL;
+    bf16 *a_rows = sa + chunk * NX * kSm, *x_rows = sx + chunk * NX * kSm;
+    const float *ch = gh + kChunk * chunk, *cl = gl + kChunk * chunk, *cb = beta + kChunk * chunk;
+#pragma unroll
+    for (int jp = 0; jp < 2; ++jp) {
+        if (jp > lower) break;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int t = r0 + 8 * i, c0 = 16 * jp + 8 * j + 2 * t4;
+                const int t = 16 * lower + g + 8 * i, c0 = 16 * jp + 8 * j + 2 * t4;
                 float l[2], p[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float f = expf((gh[t] - gh[c0 + e]) + (gl[t] - gl[c0 + e]));
-                    l[e] = t > c0 + e ? kk[j][2 * i + e] * f : 0.f;
-                    p[e] = t >= c0 + e ? qk[j][2 * i + e] * (f * s.scale) : 0.f;
+                    const float f = expf((ch[t] - ch[c0 + e]) + (cl[t] - cl[c0 + e]));
+                    l[e] = t > c0 + e ? kk[jp][j][2 * i + e] * f : 0.f;
+                    p[e] = t >= c0 + e ? qk[jp][j][2 * i + e] * (f * s.scale) : 0.f;
                 }
-                *reinterpret_cast<float2*>(sl + t * 68 + c0) = make_float2(l[0], l[1]);
+                *reinterpret_cast<float2*>(l_rows + t * kL + c0) = make_float2(l[0], l[1]);
                 uint32_t u[NP];
                 terms<NP>(p[0], p[1], u);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) *reinterpret_cast<uint32_t*>(p_out + (n * kTicks + t) * kTicks + c0) = u[n];
+                for (int n = 0; n < NP; ++n) *reinterpret_cast<uint32_t*>(p_out + (n * kChunk + t) * kChunk + c0) = u[n];
+                if (jp < lower) {                             // L B left of the diagonal
+                    uint32_t v[NX];
+                    terms<NX>(l[0] * cb[c0], l[1] * cb[c0 + 1], v);
+#pragma unroll
+                    for (int n = 0; n < NX; ++n) *reinterpret_cast<uint32_t*>(a_rows + n * kSm + t * kSmall + c0) = v[n];
+                }
             }
     }
-    __syncthreads();                                          // K and Q have been read, L is there
-
-    // L B as terms, blocks on and below the diagonal
-    for (int i = tid; i < kTicks * 8; i += 128) {
-        const int r = i >> 3, c0 = (i & 7) * 8;
-        if (c0 / 16 > r / 16) continue;
-        uint32_t u[4][NS];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            terms<NS>(sl[r * 68 + c0 + 2 * j] * beta[c0 + 2 * j], sl[r * 68 + c0 + 2 * j + 1] * beta[c0 + 2 * j + 1], u[j]);
-#pragma unroll
-        for (int n = 0; n < NS; ++n) *reinterpret_cast<uint4*>(sa + n * kSq + r * kSquare + c0) = make_uint4(u[0][n], u[1][n], u[2][n], u[3][n]);
-    }
-    // X's block (w, w): lane = column, rows one after another
+    __syncwarp();
+    // X's block on the diagonal: lane = column, rows one after another
     if (lane < 16) {
+        const float* block = l_rows + 16 * lower * (kL + 1);
+        const float* b = cb + 16 * lower;
         float y[16];
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
-            const float* row = sl + (16 * warp + t) * 68 + 16 * warp;
+            const float* row = block + t * kL;
             float v = row[lane];
 #pragma unroll
             for (int k = 0; k < t; k += 4) {
@@ -223,82 +243,59 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
                 if (k + 2 < t) v = fmaf(-l.z, y[k + 2], v);
                 if (k + 3 < t) v = fmaf(-l.w, y[k + 3], v);
             }
-            y[t] = v * beta[16 * warp + t];
-            uint32_t u[NS];
-            terms<NS>(v, 0.f, u);
+            y[t] = v * b[t];
+            uint32_t u[NX];
+            terms<NX>(v, 0.f, u);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-                reinterpret_cast<unsigned short*>(sx)[n * kSq + (16 * warp + t) * kSquare + 16 * warp + lane] = (unsigned short)u[n];
+            for (int n = 0; n < NX; ++n)
+                reinterpret_cast<unsigned short*>(x_rows)[n * kSm + (16 * lower + t) * kSmall + 16 * lower + lane] = (unsigned short)u[n];
         }
     }
     __syncthreads();
-    // X's blocks below it: X_ij = (I - X_ii B) (L_ij - sum_k (L B)_ik X_kj)
-    {
-        const uint32_t n_at = at_rows_n(lane, kSquare), a_at = smem_at(sa) + n_at, x_at = smem_at(sx) + n_at;
-        const int j0 = 16 * warp;
-        uint32_t xf[3][NS][4];
+    // the block below: X_10 = (I - X_11 B) (L_10 - (L B)_10 X_00)
+    if (!lower) {
+        const uint32_t n_at = at_rows_n(lane, kSmall), a_at = smem_at(a_rows) + n_at, x_at = smem_at(x_rows) + n_at;
+        uint32_t x[NX][4];
+        float acc[2][4] = {}, y[2][4], by[2][4];
 #pragma unroll
-        for (int n = 0; n < NS; ++n) ldsm_t(xf[0][n], x_at + 2 * (n * kSq + j0 * kSquare + j0));
+        for (int n = 0; n < NX; ++n) ldsm_t(x[n], x_at + 2 * (n * kSm));
+        const auto products = [&](uint32_t at) {
 #pragma unroll
-        for (int di = 1; di < 4; ++di) {
-            const int i0 = j0 + 16 * di;
-            if (i0 >= kTicks) break;
-            float acc[2][4] = {};
-#pragma unroll
-            for (int k = 0; k < di; ++k)
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    uint32_t b[4];
-                    ldsm(b, a_at + 2 * (j * kSq + i0 * kSquare + j0 + 16 * k));
-#pragma unroll
-                    for (int i = 0; i + j < NS; ++i) {
-                        mma(acc[0], xf[k][i], b[0], b[1]);
-                        mma(acc[1], xf[k][i], b[2], b[3]);
-                    }
-                }
-            float y[2][4], by[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int t = i0 + 8 * j + 2 * t4 + (e & 1);
-                    y[j][e] = sl[t * 68 + j0 + g + 8 * (e >> 1)] - acc[j][e];
-                    by[j][e] = y[j][e] * -beta[t];
-                }
-            uint32_t a[NS][4];
-            left<NS>(by[0], by[1], a);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < NS; ++j) {
+            for (int j = 0; j < NX; ++j) {
                 uint32_t b[4];
-                ldsm(b, x_at + 2 * (j * kSq + i0 * kSquare + i0));
+                ldsm(b, at + 2 * (j * kSm));
 #pragma unroll
-                for (int i = 0; i + j < NS; ++i) {
-                    mma(acc[0], a[i], b[0], b[1]);
-                    mma(acc[1], a[i], b[2], b[3]);
+                for (int i = 0; i + j < NX; ++i) {
+                    mma(acc[0], x[i], b[0], b[1]);
+                    mma(acc[1], x[i], b[2], b[3]);
                 }
             }
+        };
+        products(a_at + 2 * (16 * kSmall));
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[j][e] += acc[j][e];
-            left<NS>(y[0], y[1], a);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                stsm_t(x_at + 2 * (n * kSq + i0 * kSquare + j0), a[n]);
-                if (di < 3) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) xf[di][n][i] = a[n][i];
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int t = 16 + 8 * j + 2 * t4 + (e & 1);
+                y[j][e] = l_rows[t * kL + g + 8 * (e >> 1)] - acc[j][e];
+                by[j][e] = y[j][e] * -cb[t];
+                acc[j][e] = 0.f;
             }
-        }
+        left<NX>(by[0], by[1], x);
+        products(x_at + 2 * (16 * kSmall + 16));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[j][e] += acc[j][e];
+        left<NX>(y[0], y[1], x);
+#pragma unroll
+        for (int n = 0; n < NX; ++n) stsm_t(x_at + 2 * (n * kSm + 16 * kSmall), x[n]);
     }
     __syncthreads();
-    bf16* x_out = s.x + place * NS * kTicks * kTicks;
-    for (int i = tid; i < NS * kTicks * 8; i += 128)
-        if ((i & 7) / 2 <= (i >> 3 & 63) / 16)
-            *reinterpret_cast<uint4*>(x_out + i * 8) = *reinterpret_cast<const uint4*>(sx + (i >> 3) * kSquare + (i & 7) * 8);
+    bf16* x_out = s.x + 2 * place * NX * kChunk * kChunk;
+    for (int i = tid; i < 2 * NX * kChunk * 4; i += 128)
+        if ((i & 3) / 2 <= (i >> 2 & 31) / 16)
+            *reinterpret_cast<uint4*>(x_out + i * 8) = *reinterpret_cast<const uint4*>(sx + (i >> 2) * kSmall + (i & 3) * 8);
 }
 
 // ---- from chunk to chunk ------------------------------------------------------------------------------------------------
@@ -306,37 +303,45 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
 // Tiles of one chunk, in values of bf16
 template <class T, int DP, int WARPS, int NP, bool GO>
 struct ChainLayout {
-    static constexpr int in = Terms<T>::in, kept = Terms<T>::kept, stride = DP + 8, vstride = 16 * WARPS + 8;
-    static constexpr int k = 0, q = k + in * kTicks * stride, v = q + in * kTicks * stride, go = v + in * kTicks * vstride,
-                         x = go + (GO ? in * kTicks * vstride : 0), p = x + kept * kTicks * kSquare, gates = p + NP * kTicks * kSquare,
-                         stage = gates + 3 * kTicks * 2;
+    static constexpr int in = Terms<T>::in, square = Terms<T>::square, stride = DP + 8, vstride = 16 * WARPS + 8;
+    static constexpr int k = 0, q = k + in * kChunk * stride, v = q + in * kChunk * stride, go = v + in * kChunk * vstride,
+                         x = go + (GO ? in * kChunk * vstride : 0), p = x + square * kChunk * kSmall, gates = p + NP * kChunk * kSmall,
+                         stage = gates + 3 * kChunk * 2;
     static constexpr int stages = in == 1 ? 2 : 1, bytes = 2 * stage * stages;
     static_assert(bytes <= 227 * 1024, "the tiles fit");
 };
-template <class T, int DP, int WARPS, int NP, bool GO>
-__device__ __forceinline__ void load_chunk(const Delta& s, bf16* to, long long b, int h, long long tick, int n, long long slot, int e0) {
+// What a block reads and writes of its recording and head
+template <class T>
+struct Source {
+    const T *k, *q, *v, *go;
+    long long place;                 // of its first slot, in slots times heads
+};
+template <class T, int DP, int WARPS, int NP, bool GO, bool Q = true>
+__device__ __forceinline__ void load_chunk(const Delta& s, const Source<T>& from, bf16* to, int i, int n, int cols) {
     using Lay = ChainLayout<T, DP, WARPS, NP, GO>;
-    constexpr int kThreads = 32 * WARPS;
+    constexpr int kThreads = 32 * WARPS, kTile = kChunk * kChunk;
     const int tid = threadIdx.x;
-    const long long place = slot * s.heads + h;
-    load_tile<T, Lay::in, DP, Lay::stride, kThreads>(to + Lay::k, row_of<const T>(s, s.k, b, h, tick), s.k.tick, n, s.D, s.k.fast, tid);
-    load_tile<T, Lay::in, DP, Lay::stride, kThreads>(to + Lay::q, row_of<const T>(s, s.q, b, h, tick), s.q.tick, n, s.D, s.q.fast, tid);
-    load_tile<T, Lay::in, 16 * WARPS, Lay::vstride, kThreads>(to + Lay::v, row_of<const T>(s, s.v, b, h, tick) + e0, s.v.tick, n, s.E - e0,
-                                                             s.v.fast, tid);
+    const long long t = (long long)i * kChunk, place = from.place + (long long)(i >> 1) * s.heads, half = 2 * place + (i & 1);
+    load_tile<T, Lay::in, DP, Lay::stride, kThreads, kChunk>(to + Lay::k, from.k + t * s.k.tick, s.k.tick, n, s.D, s.k.fast, tid);
+    load_tile<T, Lay::in, 16 * WARPS, Lay::vstride, kThreads, kChunk>(to + Lay::v, from.v + t * s.v.tick, s.v.tick, n, cols, s.v.fast, tid);
+    load_small<Lay::square, kThreads>(to + Lay::x, s.x + half * Lay::square * kTile, tid);
+    if (tid < 24) {
+        const int row = tid >> 3, c = (tid & 7) * 4;
+        async16(smem_at(to + Lay::gates) + tid * 16, s.gates + (place * kGates + row) * kTicks + (i & 1) * kChunk + c, true);
+    }
+    if constexpr (Q) load_tile<T, Lay::in, DP, Lay::stride, kThreads, kChunk>(to + Lay::q, from.q + t * s.q.tick, s.q.tick, n, s.D, s.q.fast, tid);
     if constexpr (GO)
-        load_tile<T, Lay::in, 16 * WARPS, Lay::vstride, kThreads>(to + Lay::go, row_of<const T>(s, s.go, b, h, tick) + e0, s.go.tick, n,
-                                                                 s.E - e0, s.go.fast, tid);
-    load_square<Lay::kept, kThreads>(to + Lay::x, s.x + place * Lay::kept * kTicks * kTicks, tid);
-    load_square<NP, kThreads>(to + Lay::p, s.p + place * NP * kTicks * kTicks, tid);
-    if (tid < 48) async16(smem_at(to + Lay::gates) + tid * 16, s.gates + place * kGates * kTicks + tid * 4, true);
+        load_tile<T, Lay::in, 16 * WARPS, Lay::vstride, kThreads, kChunk>(to + Lay::go, from.go + t * s.go.tick, s.go.tick, n, cols, s.go.fast, tid);
+    if constexpr (Q) load_small<NP, kThreads>(to + Lay::p, s.p + half * NP * kTile, tid);
     async_commit();
 }
 
-// The chunks of a recording in turn (from the last one on): f(stage, chunk)
+// The chunks of a part in turn (from the last one on): f(stage, chunk)
 template <class Lay, class Load, class F>
-__device__ __forceinline__ void each_chunk(bf16* tiles, int chunks, bool back, Load&& load, F&& f) {
+__device__ __forceinline__ void each_chunk(bf16* tiles, Part part, bool back, Load&& load, F&& f) {
+    const int chunks = part.end - part.first;
     if (!chunks) return;
-    const auto nth = [&](int i) { return back ? chunks - 1 - i : i; };
+    const auto nth = [&](int i) { return back ? part.end - 1 - i : part.first + i; };
     if (Lay::stages == 2) load(tiles, nth(0));
 #pragma unroll 1
     for (int i = 0; i < chunks; ++i) {
@@ -352,6 +357,7 @@ __device__ __forceinline__ void each_chunk(bf16* tiles, int chunks, bool back, L
     }
 }
 
+__device__ __forceinline__ void clear(float (&x)[4]) { x[0] = x[1] = x[2] = x[3] = 0.f; }
 // S (or R) transposed between memory [D][E] and a warp's registers: rows e0 + g, e0 + g + 8
 template <int DP, class F>
 __device__ __forceinline__ void each_value(float (&S)[DP / 8][4], int D, int E, int e0, int lane, F&& f) {
@@ -364,15 +370,24 @@ __device__ __forceinline__ void each_value(float (&S)[DP / 8][4], int D, int E, 
         }
 }
 
-// A warp's 16 columns of 64 rows, x[j] the transposed accumulators, to `to` (rows `row` values apart) by way of the warp's own columns of
+// the same of a part's rows [16 tiles][DP]
+template <int DP, class F>
+__device__ __forceinline__ void each_pair(float (&S)[DP / 8][4], int e0, int lane, F&& f) {
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) f((e0 + (lane >> 2) + 8 * i) * DP + 8 * j + 2 * (lane & 3), S[j][2 * i], S[j][2 * i + 1]);
+}
+
+// A warp's 16 columns of 32 rows, x[j] the transposed accumulators, to `to` (rows `row` values apart) by way of the warp's own columns of
 // the planes of a tile that it has read already: n rows, `cols` columns there.
 template <class T, int VS>
-__device__ __forceinline__ void store_rows(const float (&x)[8][4], bf16* tile, T* to, long long row, int n, int cols, bool fast, int lane) {
-    constexpr int kPlane = kTicks * VS, kHalves = sizeof(T) / 2;
+__device__ __forceinline__ void store_rows(const float (&x)[4][4], bf16* tile, T* to, long long row, int n, int cols, bool fast, int lane) {
+    constexpr int kPlane = kChunk * VS, kHalves = sizeof(T) / 2;
     const uint32_t at = smem_at(tile) + at_rows_n(lane, VS);
     __syncwarp();
 #pragma unroll
-    for (int jp = 0; jp < 4; ++jp) {
+    for (int jp = 0; jp < 2; ++jp) {
         uint32_t r[kHalves][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -389,12 +404,12 @@ __device__ __forceinline__ void store_rows(const float (&x)[8][4], bf16* tile, T
         for (int k = 0; k < kHalves; ++k) stsm_t(at + 2 * (k * kPlane + 16 * jp * VS), r[k]);
     }
     __syncwarp();
-    const int half = lane & 1, c = 8 * half;
+    const int c = 8 * (lane & 1);
+    T* q = to + (lane >> 1) * row + c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i, q += 16 * row) {
         const int t = 16 * i + (lane >> 1);
         if (t >= n || c >= cols) continue;
-        T* q = to + t * row + c;
         uint4 u[kHalves];
 #pragma unroll
         for (int k = 0; k < kHalves; ++k) u[k] = *reinterpret_cast<const uint4*>(tile + k * kPlane + t * VS + c);
@@ -421,13 +436,13 @@ __device__ __forceinline__ void store_rows(const float (&x)[8][4], bf16* tile, T
     __syncwarp();
 }
 
-// x[j] of the warp's columns from NI planes of a tile, transposed as accumulators; j = 2 jp, 2 jp + 1
+// the warp's columns of 16 ticks from NI planes of a tile, transposed as two accumulators
 template <int NI, int VS>
 __device__ __forceinline__ void two_columns(uint32_t at, int jp, float (&x)[2][4]) {
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
         uint32_t r[4];
-        ldsm_t(r, at + 2 * (n * kTicks * VS + 16 * jp * VS));
+        ldsm_t(r, at + 2 * (n * kChunk * VS + 16 * jp * VS));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float(&v)[4] = x[i >> 1];
@@ -437,226 +452,264 @@ __device__ __forceinline__ void two_columns(uint32_t at, int jp, float (&x)[2][4
         }
     }
 }
-// two neighbouring values of a 64-value gate for columns 8 j + 2 t4, + 1
+// two neighbouring values of a gate for columns 8 j + 2 t4, + 1
 __device__ __forceinline__ float2 gate2(const float* gates, int j, int lane) {
     return *reinterpret_cast<const float2*>(gates + 8 * j + 2 * (lane & 3));
 }
+__device__ __forceinline__ void scale2(float (&x)[4], float2 f) {
+    x[0] *= f.x, x[1] *= f.y, x[2] *= f.x, x[3] *= f.y;
+}
+// x = x f + y
+__device__ __forceinline__ void scale_add(float (&x)[4], float2 f, const float (&y)[4]) {
+    x[0] = fmaf(x[0], f.x, y[0]), x[1] = fmaf(x[1], f.y, y[1]), x[2] = fmaf(x[2], f.x, y[2]), x[3] = fmaf(x[3], f.y, y[3]);
+}
+__device__ __forceinline__ void subtract(float (&x)[4], const float (&y)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] -= y[e];
+}
 
-// Forward. KEEP: nothing but what the way back needs is written (S before each chunk, W, U, rows of o dO), and o is made to as many
-// terms as the states.
-template <class T, int DP, int WARPS, bool KEEP>
-__global__ void __launch_bounds__(32 * WARPS) k_delta_chain(const __grid_constant__ Delta s) {
-    constexpr int NI = Terms<T>::in, NS = Terms<T>::kept, NO = KEEP ? NS : Terms<T>::out;
+// sum[2 J] += a b for J pairs of 8 x 16 right operands from planes of NB terms at(j, pair), products with term numbers below KEEP; term
+// by term over all pairs, so that no product waits for the one just before. `first`: sum = a b.
+template <int NA, int NB, int KEEP, int J, bool TRANS, class At>
+__device__ __forceinline__ void products(float (*sum)[4], const uint32_t (&a)[NA][4], At&& at, bool first = false) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        uint32_t r[J][4];
+#pragma unroll
+        for (int p = 0; p < J; ++p) {
+            if (TRANS) ldsm_t(r[p], at(j, p));
+            else ldsm(r[p], at(j, p));
+        }
+#pragma unroll
+        for (int k = 0; k < NA && k + j < KEEP; ++k)
+#pragma unroll
+            for (int p = 0; p < J; ++p) {
+                if (first && j + k == 0) {
+                    mma_first(sum[2 * p], a[k], r[p][0], r[p][1]);
+                    mma_first(sum[2 * p + 1], a[k], r[p][2], r[p][3]);
+                } else {
+                    mma(sum[2 * p], a[k], r[p][0], r[p][1]);
+                    mma(sum[2 * p + 1], a[k], r[p][2], r[p][3]);
+                }
+            }
+    }
+}
+
+// blocks of an SM at once: 16 warps with 128 registers a thread, 12 with 168
+template <int DP>
+constexpr int chain_blocks(int warps) { return warps == 8 ? 2 : (DP > 64 ? 12 : 16) / warps; }
+
+// Forward. kKeep: nothing but what the way back needs is written (S before each slot, W, U, rows of o dO), and o is made to as many
+// terms as the corrections. kParts: what a part makes of a state of zeros, and (tiles past those of the columns) of the columns of 1;
+// kPartsKeep: for what is kept.
+enum { kForward, kKeep, kParts, kPartsKeep };
+template <class T, int DP, int WARPS, int MODE>
+__global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<DP>(WARPS) : DP > 64 ? 2 : 3)
+    k_delta_chain(const __grid_constant__ Delta s) {
+    constexpr bool KEEP = MODE == kKeep, PARTS = MODE >= kParts;
+    constexpr int NI = Terms<T>::in, NX = Terms<T>::square, NS = KEEP || MODE == kPartsKeep ? Terms<T>::learn : Terms<T>::forward, NO = KEEP ? NX : Terms<T>::out,
+                  kSaved = Terms<T>::saved;
+    // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: forward with 168 registers 415 and 380 us (64 recordings
+    // of 1,024 ticks, 8 heads of 128), with what is kept and 128 registers 675 and 747
+    constexpr bool kTogether = WARPS == 8;
     using Lay = ChainLayout<T, DP, WARPS, NO, KEEP>;
-    constexpr int kPlane = kTicks * Lay::stride, kSq = kTicks * kSquare;
+    constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int blocks_e = (s.E + 16 * WARPS - 1) / (16 * WARPS), tiles_e = (s.E + 15) / 16;
+    const int tiles_e = (s.E + 15) / 16, all_tiles = tiles_e + (PARTS ? (s.D + 15) / 16 : 0), blocks_e = (all_tiles + WARPS - 1) / WARPS;
     long long item = blockIdx.x;
     const int e_block = (int)(item % blocks_e) * 16 * WARPS, e0 = e_block + 16 * warp;
     item /= blocks_e;
     const int h = (int)(item % s.heads);
     const long long b = item / s.heads;
     const Span sp = span_of(s, b);
-    const int chunks = (int)((sp.n + kTicks - 1) / kTicks);
-    const long long slot0 = slot_of(s, b, sp.start), state0 = (b * s.heads + h) * s.D * s.E;
-    const bool mine = e0 < s.E;
+    const int chunks = (int)((sp.n + kChunk - 1) / kChunk);
+    const Part part = part_of(s, sp.n, blockIdx.y);
+    const long long part_place = (b * s.heads + h) * s.parts + blockIdx.y;
+    const long long state0 = (b * s.heads + h) * s.D * s.E;
+    const bool mine = e0 < 16 * all_tiles;
+    const Source<T> from{row_of<const T>(s, s.k, b, h, sp.start), row_of<const T>(s, s.q, b, h, sp.start),
+                         row_of<const T>(s, s.v, b, h, sp.start) + e_block, KEEP ? row_of<const T>(s, s.go, b, h, sp.start) + e_block : nullptr,
+                         slot_of(s, b, sp.start) * s.heads + h};
+    T* out = MODE == kForward ? row_of<T>(s, s.o, b, h, sp.start) + e0 : nullptr;
+    const auto ticks = [&](int i) { return (int)min((long long)kChunk, sp.n - (long long)i * kChunk); };
 
     float S[DP / 8][4];
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j) S[j][0] = S[j][1] = S[j][2] = S[j][3] = 0.f;
-    if (s.first) each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.first[state0 + at]; });
+    for (int j = 0; j < DP / 8; ++j) clear(S[j]);
+    if constexpr (PARTS) {
+        const int one = e0 - 16 * tiles_e + (lane >> 2) - 2 * (lane & 3);   // the value d = row, counted from the thread's first
+        if (e0 >= 16 * tiles_e) {
+#pragma unroll
+            for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[j][i] = 8 * j + (i & 1) == one + 8 * (i >> 1) ? 1.f : 0.f;
+        }
+    } else if (blockIdx.y) {
+        if (mine) {
+            const float* from = s.start + part_place * 16 * tiles_e * DP;
+            each_pair<DP>(S, e0, lane, [&](int at, float& x, float& y) {
+                const float2 v = *reinterpret_cast<const float2*>(from + at);
+                x = v.x, y = v.y;
+            });
+        }
+    } else if (s.first) {
+        each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.first[state0 + at]; });
+    }
 
-    const auto load = [&](bf16* to, int i) {
-        load_chunk<T, DP, WARPS, NO, KEEP>(s, to, b, h, sp.start + (long long)i * kTicks, (int)min((long long)kTicks, sp.n - (long long)i * kTicks),
-                                           slot0 + i, e_block);
-    };
-    each_chunk<Lay>(tiles, chunks, false, load, [&](bf16* now, int i) {
+    const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NO, KEEP, !PARTS>(s, from, to, i, ticks(i), s.E - e_block); };
+    each_chunk<Lay>(tiles, part, false, load, [&](bf16* now, int i) {
         if (!mine) return;
-        const int n = (int)min((long long)kTicks, sp.n - (long long)i * kTicks);
-        const long long place = (slot0 + i) * s.heads + h, warp_place = place * tiles_e + e0 / 16;
-        const uint32_t rows_n = smem_at(now) + at_rows_n(lane, Lay::stride), rows_m = smem_at(now) + at_rows_m(lane, Lay::stride);
-        const uint32_t square_n = smem_at(now) + at_rows_n(lane, kSquare), columns = smem_at(now) + at_rows_k(lane, Lay::vstride) + 32 * warp;
-        const float *from0 = reinterpret_cast<const float*>(now + Lay::gates), *to_end = from0 + kTicks, *beta = to_end + kTicks;
-        float N[8][4], O[8][4];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) N[j][e] = O[j][e] = 0.f;
-        // S^T K^T and S^T Q^T
+        const uint32_t tile = smem_at(now), rows_n = tile + at_rows_n(lane, Lay::stride), rows_m = tile + at_rows_m(lane, Lay::stride),
+                       square_n = tile + at_rows_n(lane, kSmall), columns = tile + at_rows_k(lane, Lay::vstride) + 32 * warp;
+        const float *from0 = reinterpret_cast<const float*>(now + Lay::gates), *to_end = from0 + kChunk, *beta = to_end + kChunk;
+        const long long place = from.place + (long long)(i >> 1) * s.heads, warp_place = place * tiles_e + e0 / 16;
+        float N[4][4], O[4][4];
+        const auto query = [&](const auto& a, int d) {
+            products<sizeof(a) / 16, NI, NO, 2, false>(O, a, [&](int j, int p) { return rows_n + 2 * (Lay::q + j * kPlane + 16 * p * Lay::stride + 16 * d); },
+                                                       d == 0);
+        };
+        // N = V - e^G K S
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
             uint32_t a[NS][4];
             left<NS>(S[2 * d], S[2 * d + 1], a);
-            if constexpr (KEEP) {
+            if (KEEP && !(i & 1)) {
 #pragma unroll
-                for (int k = 0; k < NS; ++k)
-                    s.states[((warp_place * NS + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
+                for (int k = 0; k < kSaved; ++k)
+                    s.states[((warp_place * kSaved + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
             }
-#pragma unroll
-            for (int jp = 0; jp < 4; ++jp)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    uint32_t r[4];
-                    ldsm(r, rows_n + 2 * (Lay::k + j * kPlane + 16 * jp * Lay::stride + 16 * d));
-#pragma unroll
-                    for (int k = 0; k + j < NS; ++k) {
-                        mma(N[2 * jp], a[k], r[0], r[1]);
-                        mma(N[2 * jp + 1], a[k], r[2], r[3]);
-                    }
-                    ldsm(r, rows_n + 2 * (Lay::q + j * kPlane + 16 * jp * Lay::stride + 16 * d));
-#pragma unroll
-                    for (int k = 0; k + j < NO; ++k) {
-                        mma(O[2 * jp], a[k], r[0], r[1]);
-                        mma(O[2 * jp + 1], a[k], r[2], r[3]);
-                    }
-                }
+            products<NS, NI, NS, 2, false>(N, a, [&](int j, int p) { return rows_n + 2 * (Lay::k + j * kPlane + 16 * p * Lay::stride + 16 * d); }, d == 0);
+            if (kTogether && !PARTS) query(a, d);
         }
-        // N = V - e^G K S; scale e^G Q S
 #pragma unroll
-        for (int jp = 0; jp < 4; ++jp) {
+        for (int jp = 0; jp < 2; ++jp) {
             float v[2][4];
             two_columns<NI, Lay::vstride>(columns + 2 * Lay::v, jp, v);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float2 f = gate2(from0, 2 * jp + j, lane);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float ge = e & 1 ? f.y : f.x;
-                    N[2 * jp + j][e] = fmaf(-ge, N[2 * jp + j][e], v[j][e]);
-                    O[2 * jp + j][e] *= ge * s.scale;
-                }
+                scale_add(N[2 * jp + j], make_float2(-f.x, -f.y), v[j]);
             }
         }
-        // W = N - X B N
+        // W = N - X B N; U = B W
         {
-            float Y[8][4];
+            float Y[4][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) Y[j][0] = Y[j][1] = Y[j][2] = Y[j][3] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 float x[2][4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float2 f = gate2(beta, 2 * k + j, lane);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[j][e] = N[2 * k + j][e] * (e & 1 ? f.y : f.x);
+                    for (int e = 0; e < 4; ++e) x[j][e] = N[2 * k + j][e];
+                    scale2(x[j], gate2(beta, 2 * k + j, lane));
                 }
-                uint32_t a[NS][4];
-                left<NS>(x[0], x[1], a);
-#pragma unroll
-                for (int jp = k; jp < 4; ++jp)
-#pragma unroll
-                    for (int j = 0; j < NS; ++j) {
-                        uint32_t r[4];
-                        ldsm(r, square_n + 2 * (Lay::x + j * kSq + 16 * jp * kSquare + 16 * k));
-#pragma unroll
-                        for (int t = 0; t + j < NS; ++t) {
-                            mma(Y[2 * jp], a[t], r[0], r[1]);
-                            mma(Y[2 * jp + 1], a[t], r[2], r[3]);
-                        }
-                    }
+                uint32_t a[NX][4];
+                left<NX>(x[0], x[1], a);
+                const auto at = [&](int j, int p) { return square_n + 2 * (Lay::x + j * kSm + 16 * (p + k) * kSmall + 16 * k); };
+                if (k == 0) products<NX, NX, NX, 2, false>(Y, a, at, true);
+                else products<NX, NX, NX, 1, false>(Y + 2, a, at);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) N[j][e] -= Y[j][e];
+            for (int j = 0; j < 4; ++j) subtract(N[j], Y[j]);
         }
         if constexpr (KEEP) {
+            const long long w_place = (2 * place + (i & 1)) * tiles_e + e0 / 16;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s.w[(warp_place * 8 + j) * 32 + lane] = make_float4(N[j][0], N[j][1], N[j][2], N[j][3]);
-        }
-        // U = B W; O += P U
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = gate2(beta, j, lane);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) N[j][e] *= e & 1 ? f.y : f.x;
+            for (int j = 0; j < 4; ++j) s.w[(w_place * 4 + j) * 32 + lane] = make_float4(N[j][0], N[j][1], N[j][2], N[j][3]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            uint32_t a[NO][4];
-            left<NO>(N[2 * k], N[2 * k + 1], a);
+        for (int j = 0; j < 4; ++j) scale2(N[j], gate2(beta, j, lane));
+        // O = scale e^G Q S + P U
+        if constexpr (!PARTS) {
+            if (!kTogether) {
 #pragma unroll
-            for (int jp = k; jp < 4; ++jp)
-#pragma unroll
-                for (int j = 0; j < NO; ++j) {
-                    uint32_t r[4];
-                    ldsm(r, square_n + 2 * (Lay::p + j * kSq + 16 * jp * kSquare + 16 * k));
-#pragma unroll
-                    for (int t = 0; t + j < NO; ++t) {
-                        mma(O[2 * jp], a[t], r[0], r[1]);
-                        mma(O[2 * jp + 1], a[t], r[2], r[3]);
-                    }
+                for (int d = 0; d < DP / 16; ++d) {
+                    uint32_t a[NO][4];
+                    left<NO>(S[2 * d], S[2 * d + 1], a);
+                    query(a, d);
                 }
-        }
-        if constexpr (!KEEP) {
-            store_rows<T, Lay::vstride>(O, now + Lay::v + 16 * warp, row_of<T>(s, s.o, b, h, sp.start + (long long)i * kTicks) + e0, s.o.tick, n,
-                                        s.E - e0, s.o.fast, lane);
-        } else {
-            float sums[16];
-#pragma unroll
-            for (int jp = 0; jp < 4; ++jp) {
-                float v[2][4];
-                two_columns<NI, Lay::vstride>(columns + 2 * Lay::go, jp, v);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) sums[4 * jp + 2 * j + e] = O[2 * jp + j][e] * v[j][e] + O[2 * jp + j][e + 2] * v[j][e + 2];
             }
-            const float2 od = column_sums(sums, lane);
-            *reinterpret_cast<float2*>(s.od + warp_place * kTicks + 8 * (lane >> 2) + 2 * (lane & 3)) = od;
-            using U = std::conditional_t<NI == 1, bf16, float>;
-            store_rows<U, Lay::vstride>(N, now + Lay::v + 16 * warp, reinterpret_cast<U*>(s.u) + place * kTicks * 16 * tiles_e + e0,
-                                        16 * tiles_e, kTicks, 16, true, lane);
-        }
-        // S = e^{G_63} S + (e^{G_63 - G} K)^T U
-        uint32_t a[4][NS][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float x[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float2 f = gate2(to_end, 2 * k + j, lane);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[j][e] = N[2 * k + j][e] * (e & 1 ? f.y : f.x);
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = gate2(from0, j, lane);
+                scale2(O[j], make_float2(f.x * s.scale, f.y * s.scale));
             }
-            left<NS>(x[0], x[1], a[k]);
-        }
-        const float fade = from0[kTicks - 1];
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-            float acc[2][4] = {};
+            for (int k = 0; k < 2; ++k) {
+                uint32_t a[NO][4];
+                left<NO>(N[2 * k], N[2 * k + 1], a);
+                const auto at = [&](int j, int p) { return square_n + 2 * (Lay::p + j * kSm + 16 * (p + k) * kSmall + 16 * k); };
+                if (k == 0) products<NO, NO, NO, 2, false>(O, a, at);
+                else products<NO, NO, NO, 1, false>(O + 2, a, at);
+            }
+            if constexpr (!KEEP) {
+                store_rows<T, Lay::vstride>(O, now + Lay::v + 16 * warp, out + (long long)i * kChunk * s.o.tick, s.o.tick, ticks(i), s.E - e0, s.o.fast, lane);
+            } else {
+                float sums[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+                for (int jp = 0; jp < 2; ++jp) {
+                    float v[2][4];
+                    two_columns<NI, Lay::vstride>(columns + 2 * Lay::go, jp, v);
 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    uint32_t r[4];
-                    ldsm_t(r, rows_m + 2 * (Lay::k + j * kPlane + 16 * k * Lay::stride + 16 * d));
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int t = 0; t + j < NS; ++t) {
-                        mma(acc[0], a[k][t], r[0], r[1]);
-                        mma(acc[1], a[k][t], r[2], r[3]);
-                    }
+                        for (int e = 0; e < 2; ++e) sums[4 * jp + 2 * j + e] = O[2 * jp + j][e] * v[j][e] + O[2 * jp + j][e + 2] * v[j][e + 2];
                 }
+                s.od[warp_place * kTicks + (i & 1) * kChunk + 8 * (lane >> 3) + 2 * (lane & 3) + (lane >> 2 & 1)] = column_sums(sums, lane);
+                using U = std::conditional_t<NI == 1, bf16, float>;
+                store_rows<U, Lay::vstride>(N, now + Lay::v + 16 * warp,
+                                            reinterpret_cast<U*>(s.u) + (place * kTicks + (i & 1) * kChunk) * 16 * tiles_e + e0, 16 * tiles_e, kChunk, 16,
+                                            true, lane);
+            }
+        }
+        // S = e^{G_31} S + (e^{G_31 - G} K)^T U
+        uint32_t a[2][NS][4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[2 * d + j][e] = fmaf(S[2 * d + j][e], fade, acc[j][e]);
+            for (int j = 0; j < 2; ++j) scale2(N[2 * k + j], gate2(to_end, 2 * k + j, lane));
+            left<NS>(N[2 * k], N[2 * k + 1], a[k]);
+        }
+        const float fade = from0[kChunk - 1];
+#pragma unroll
+        for (int d = 0; d < DP / 16; d += 2) {
+            float acc[4][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                products<NS, NI, NS, 2, true>(acc, a[k], [&](int j, int p) { return rows_m + 2 * (Lay::k + j * kPlane + 16 * k * Lay::stride + 16 * (d + p)); }, k == 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) scale_add(S[2 * d + j], make_float2(fade, fade), acc[j]);
         }
     });
-    if (s.last) each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { s.last[state0 + at] = v; });
+    // a slot whose second chunk has no ticks: nothing is foretold there, and nothing added
+    if (KEEP && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {
+        const long long place = from.place + (long long)(chunks >> 1) * s.heads;
+        s.od[(place * tiles_e + e0 / 16) * kTicks + kChunk + lane] = 0.f;
+        using U = std::conditional_t<NI == 1, bf16, float>;
+        U* u = reinterpret_cast<U*>(s.u) + (place * kTicks + kChunk) * 16 * tiles_e + e0;
+        for (int c = 0; c < 16; ++c) u[(long long)lane * 16 * tiles_e + c] = from_f<U>(0.f);
+    }
+    if constexpr (PARTS) {
+        if (!mine) return;
+        const bool turn = e0 >= 16 * tiles_e;
+        float* to = turn ? s.turn + part_place * DP * DP : s.own + part_place * 16 * tiles_e * DP;
+        each_pair<DP>(S, turn ? e0 - 16 * tiles_e : e0, lane, [&](int at, float& x, float& y) { *reinterpret_cast<float2*>(to + at) = make_float2(x, y); });
+    } else if (s.last && (chunks ? part.first < chunks && part.end == chunks : blockIdx.y == 0)) {
+        each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { s.last[state0 + at] = v; });
+    }
 }
 
 __device__ __forceinline__ void prefetch(const char* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// Back. s.last is the state after the recording's last tick.
-template <class T, int DP, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant__ Delta s) {
-    constexpr int NI = Terms<T>::in, NS = Terms<T>::kept, NG = NI == 1 ? 1 : NS;   // NG: terms of R that the gradients of q and k need
-    using Lay = ChainLayout<T, DP, WARPS, NS, true>;
-    constexpr int kPlane = kTicks * Lay::stride, kSq = kTicks * kSquare;
+// Back. s.last is the state after the recording's last tick. PARTS: what a part leaves of a gradient of zeros, and nothing else.
+template <class T, int DP, int WARPS, bool PARTS>
+__global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<DP>(WARPS) : DP > 64 ? 2 : 3)
+    k_delta_back(const __grid_constant__ Delta s) {
+    constexpr int NI = Terms<T>::in, NX = Terms<T>::square, NS = Terms<T>::learn, NG = Terms<T>::grad, kSaved = Terms<T>::saved;
+    using Lay = ChainLayout<T, DP, WARPS, NX, true>;
+    constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -667,56 +720,76 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
     const int h = (int)(item % s.heads);
     const long long b = item / s.heads;
     const Span sp = span_of(s, b);
-    const int chunks = (int)((sp.n + kTicks - 1) / kTicks);
-    const long long slot0 = slot_of(s, b, sp.start), state0 = (b * s.heads + h) * s.D * s.E;
+    const int chunks = (int)((sp.n + kChunk - 1) / kChunk);
+    const Part part = part_of(s, sp.n, blockIdx.y);
+    const long long part_place = (b * s.heads + h) * s.parts + blockIdx.y;
+    const long long state0 = (b * s.heads + h) * s.D * s.E;
     const bool mine = e0 < s.E;
+    const Source<T> from{row_of<const T>(s, s.k, b, h, sp.start), row_of<const T>(s, s.q, b, h, sp.start),
+                         row_of<const T>(s, s.v, b, h, sp.start) + e_block, row_of<const T>(s, s.go, b, h, sp.start) + e_block,
+                         slot_of(s, b, sp.start) * s.heads + h};
+    const auto ticks = [&](int i) { return (int)min((long long)kChunk, sp.n - (long long)i * kChunk); };
 
     float R[DP / 8][4];
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j) R[j][0] = R[j][1] = R[j][2] = R[j][3] = 0.f;
-    if (s.glast) each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.glast[state0 + at]; });
+    for (int j = 0; j < DP / 8; ++j) clear(R[j]);
+    if (PARTS) {
+    } else if ((int)blockIdx.y + 1 < s.parts) {
+        if (mine) {
+            const float* at_end = s.start + part_place * 16 * tiles_e * DP;
+            each_pair<DP>(R, e0, lane, [&](int at, float& x, float& y) {
+                const float2 v = *reinterpret_cast<const float2*>(at_end + at);
+                x = v.x, y = v.y;
+            });
+        }
+    } else if (s.glast) {
+        each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.glast[state0 + at]; });
+    }
+    if (!PARTS && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {                               // a slot's second chunk without ticks
+        const long long at = ((from.place + (long long)(chunks >> 1) * s.heads) * tiles_e + e0 / 16) * kTicks + kChunk + lane;
+        s.vdn[at] = s.db[at] = 0.f;
+    }
 
-    const auto load = [&](bf16* to, int i) {
-        load_chunk<T, DP, WARPS, NS, true>(s, to, b, h, sp.start + (long long)i * kTicks, (int)min((long long)kTicks, sp.n - (long long)i * kTicks),
-                                           slot0 + i, e_block);
-    };
-    each_chunk<Lay>(tiles, chunks, true, load, [&](bf16* now, int i) {
+    const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NX, true>(s, from, to, i, ticks(i), s.E - e_block); };
+    each_chunk<Lay>(tiles, part, true, load, [&](bf16* now, int i) {
         if (!mine) return;
-        const int n = (int)min((long long)kTicks, sp.n - (long long)i * kTicks);
-        const long long place = (slot0 + i) * s.heads + h, warp_place = place * tiles_e + e0 / 16;
-        const uint32_t rows_n = smem_at(now) + at_rows_n(lane, Lay::stride), rows_m = smem_at(now) + at_rows_m(lane, Lay::stride);
-        const uint32_t square_m = smem_at(now) + at_rows_m(lane, kSquare), columns = smem_at(now) + at_rows_k(lane, Lay::vstride) + 32 * warp;
-        const float *from0 = reinterpret_cast<const float*>(now + Lay::gates), *to_end = from0 + kTicks, *beta = to_end + kTicks;
-        float N[8][4];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) N[j][0] = N[j][1] = N[j][2] = N[j][3] = 0.f;
-        // R^T K^T, and <R, S> behind the chunk
+        const uint32_t tile = smem_at(now), rows_n = tile + at_rows_n(lane, Lay::stride), rows_m = tile + at_rows_m(lane, Lay::stride),
+                       square_m = tile + at_rows_m(lane, kSmall), columns = tile + at_rows_k(lane, Lay::vstride) + 32 * warp;
+        const float *from0 = reinterpret_cast<const float*>(now + Lay::gates), *to_end = from0 + kChunk, *beta = to_end + kChunk;
+        const long long place = from.place + (long long)(i >> 1) * s.heads, warp_place = place * tiles_e + e0 / 16;
+        const long long w_place = (2 * place + (i & 1)) * tiles_e + e0 / 16;
+        const bool last = i + 1 == chunks, slot_end = !PARTS && ((i & 1) || last);   // R is the one behind the slot
+        const uint4* behind = s.states + (warp_place + (long long)s.heads * tiles_e) * kSaved * (DP / 16) * 32 + lane;
+        if (!PARTS && i > part.first) {                       // what the next chunk reads of this, on its way to L2
+            if (!(i & 1)) {
+                const char* states = reinterpret_cast<const char*>(s.states + warp_place * kSaved * (DP / 16) * 32);
+                for (int at = lane * 128; at < kSaved * (DP / 16) * 512; at += 32 * 128) prefetch(states + at);
+            }
+            const long long before = (2 * (place - (i & 1 ? 0 : s.heads)) + !(i & 1)) * tiles_e + e0 / 16;
+            if (lane < 16) prefetch(reinterpret_cast<const char*>(s.w + before * 4 * 32) + lane * 128);
+        }
+        float N[4][4];
+        // R^T K^T, and <R, S> behind the slot
         float anchor = 0.f;
-        const uint4* behind = s.states + ((place + s.heads) * tiles_e + e0 / 16) * NS * (DP / 16) * 32 + lane;
-        const bool inner = i + 1 < chunks;
-        uint4 ahead[NS];
-        if (inner) {
-#pragma unroll
-            for (int k = 0; k < NS; ++k) ahead[k] = __ldg(behind + k * (DP / 16) * 32);
-        }
-        if (i > 0) {                                          // what the next chunk reads of this, on its way to L2
-            const char* states = reinterpret_cast<const char*>(s.states + warp_place * NS * (DP / 16) * 32);
-            for (int at = lane * 128; at < NS * (DP / 16) * 512; at += 32 * 128) prefetch(states + at);
-            prefetch(reinterpret_cast<const char*>(s.w + (warp_place - (long long)s.heads * tiles_e) * 8 * 32) + lane * 128);
-        }
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
+            uint4 kept[kSaved];
+            if (slot_end && !last) {
+#pragma unroll
+                for (int k = 0; k < kSaved; ++k) kept[k] = __ldg(behind + (k * (DP / 16) + d) * 32);
+            }
             uint32_t a[NS][4];
             left<NS>(R[2 * d], R[2 * d + 1], a);
+            if (slot_end) {
 #pragma unroll
-            for (int k = 0; k < NG; ++k)
-                s.gstates[((warp_place * NG + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
-            if (inner) {
+                for (int k = 0; k < NG; ++k)
+                    s.gstates[((warp_place * NG + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
+            }
+            products<NS, NI, NS, 2, false>(N, a, [&](int j, int p) { return rows_n + 2 * (Lay::k + j * kPlane + 16 * p * Lay::stride + 16 * d); }, d == 0);
+            if (slot_end && !last) {
 #pragma unroll
-                for (int k = 0; k < NS; ++k) {
-                    const uint4 u = ahead[k];
-                    if (d + 1 < DP / 16) ahead[k] = __ldg(behind + (k * (DP / 16) + d + 1) * 32);
-                    const uint32_t* p = &u.x;
+                for (int k = 0; k < kSaved; ++k) {
+                    const uint32_t* p = &kept[k].x;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float(&v)[4] = R[2 * d + (j >> 1)];
@@ -725,109 +798,79 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
                     }
                 }
             }
-#pragma unroll
-            for (int jp = 0; jp < 4; ++jp)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    uint32_t r[4];
-                    ldsm(r, rows_n + 2 * (Lay::k + j * kPlane + 16 * jp * Lay::stride + 16 * d));
-#pragma unroll
-                    for (int k = 0; k + j < NS; ++k) {
-                        mma(N[2 * jp], a[k], r[0], r[1]);
-                        mma(N[2 * jp + 1], a[k], r[2], r[3]);
-                    }
-                }
         }
-        if (i + 1 == chunks) each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { anchor = fmaf(v, s.last[state0 + at], anchor); });
-        anchor = warp_sum(anchor);
-        if (lane == 0) s.anchor[warp_place] = anchor;
-        // dU = e^{G_63 - G} K R + P^T dO
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = gate2(to_end, j, lane);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) N[j][e] *= e & 1 ? f.y : f.x;
+        if (last && !PARTS) each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { anchor = fmaf(v, s.last[state0 + at], anchor); });
+        if (slot_end) {
+            anchor = warp_sum(anchor);
+            if (lane == 0) s.anchor[warp_place] = anchor;
         }
+        // dU = e^{G_31 - G} K R + P^T dO
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int j = 0; j < 4; ++j) scale2(N[j], gate2(to_end, j, lane));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
             uint32_t a[NI][4];
 #pragma unroll
-            for (int t = 0; t < NI; ++t) ldsm_t(a[t], columns + 2 * (Lay::go + t * kTicks * Lay::vstride + 16 * k * Lay::vstride));
-#pragma unroll
-            for (int jp = 0; jp <= k; ++jp)
-#pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    uint32_t r[4];
-                    ldsm_t(r, square_m + 2 * (Lay::p + j * kSq + 16 * k * kSquare + 16 * jp));
-#pragma unroll
-                    for (int t = 0; t < NI && t + j < NS; ++t) {
-                        mma(N[2 * jp], a[t], r[0], r[1]);
-                        mma(N[2 * jp + 1], a[t], r[2], r[3]);
-                    }
-                }
+            for (int t = 0; t < NI; ++t) ldsm_t(a[t], columns + 2 * (Lay::go + t * kChunk * Lay::vstride + 16 * k * Lay::vstride));
+            const auto at = [&](int j, int p) { return square_m + 2 * (Lay::p + j * kSm + 16 * k * kSmall + 16 * p); };
+            if (k == 0) products<NI, NX, NX, 1, true>(N, a, at);
+            else products<NI, NX, NX, 2, true>(N, a, at);
         }
         // dR = dU - X^T B dU
+        const int column = (i & 1) * kChunk + 8 * (lane >> 3) + 2 * (lane & 3) + (lane >> 2 & 1);
         {
-            float Y[8][4];
-            float4 w[8];
+            float Y[4][4];
+            float4 w[4];
+            if constexpr (!PARTS) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = __ldg(s.w + (warp_place * 8 + j) * 32 + lane);
+                for (int j = 0; j < 4; ++j) w[j] = __ldg(s.w + (w_place * 4 + j) * 32 + lane);
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) Y[j][0] = Y[j][1] = Y[j][2] = Y[j][3] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 1; k >= 0; --k) {
                 float x[2][4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float2 f = gate2(beta, 2 * k + j, lane);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[j][e] = N[2 * k + j][e] * (e & 1 ? f.y : f.x);
+                    for (int e = 0; e < 4; ++e) x[j][e] = N[2 * k + j][e];
+                    scale2(x[j], gate2(beta, 2 * k + j, lane));
                 }
-                uint32_t a[NS][4];
-                left<NS>(x[0], x[1], a);
-#pragma unroll
-                for (int jp = 0; jp <= k; ++jp)
-#pragma unroll
-                    for (int j = 0; j < NS; ++j) {
-                        uint32_t r[4];
-                        ldsm_t(r, square_m + 2 * (Lay::x + j * kSq + 16 * k * kSquare + 16 * jp));
-#pragma unroll
-                        for (int t = 0; t + j < NS; ++t) {
-                            mma(Y[2 * jp], a[t], r[0], r[1]);
-                            mma(Y[2 * jp + 1], a[t], r[2], r[3]);
-                        }
-                    }
+                uint32_t a[NX][4];
+                left<NX>(x[0], x[1], a);
+                const auto at = [&](int j, int p) { return square_m + 2 * (Lay::x + j * kSm + 16 * k * kSmall + 16 * p); };
+                if (k == 0) products<NX, NX, NX, 1, true>(Y, a, at);
+                else products<NX, NX, NX, 2, true>(Y, a, at, true);
             }
-            float sums[16];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) subtract(N[j], Y[j]);
+            // dN = B dR; rows of dR W and of v dN
+            float sums[8];
+            if constexpr (!PARTS) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) N[j][e] -= Y[j][e];
-                sums[2 * j] = N[j][0] * w[j].x + N[j][2] * w[j].z;
-                sums[2 * j + 1] = N[j][1] * w[j].y + N[j][3] * w[j].w;
-            }
-            const float2 db = column_sums(sums, lane);
-            *reinterpret_cast<float2*>(s.db + warp_place * kTicks + 8 * (lane >> 2) + 2 * (lane & 3)) = db;
-            // dN = B dR, rows of v dN
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float v[2][4];
-                two_columns<NI, Lay::vstride>(columns + 2 * Lay::v, k, v);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float2 f = gate2(beta, 2 * k + j, lane);
-                    float(&x)[4] = N[2 * k + j];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] *= e & 1 ? f.y : f.x;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) sums[4 * k + 2 * j + e] = x[e] * v[j][e] + x[e + 2] * v[j][e + 2];
+                for (int j = 0; j < 4; ++j) {
+                    sums[2 * j] = N[j][0] * w[j].x + N[j][2] * w[j].z;
+                    sums[2 * j + 1] = N[j][1] * w[j].y + N[j][3] * w[j].w;
                 }
+                s.db[warp_place * kTicks + column] = column_sums(sums, lane);
             }
-            const float2 vdn = column_sums(sums, lane);
-            *reinterpret_cast<float2*>(s.vdn + warp_place * kTicks + 8 * (lane >> 2) + 2 * (lane & 3)) = vdn;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) scale2(N[j], gate2(beta, j, lane));
+            if constexpr (!PARTS) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float v[2][4];
+                    two_columns<NI, Lay::vstride>(columns + 2 * Lay::v, k, v);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            sums[4 * k + 2 * j + e] = N[2 * k + j][e] * v[j][e] + N[2 * k + j][e + 2] * v[j][e + 2];
+                }
+                s.vdn[warp_place * kTicks + column] = column_sums(sums, lane);
+            }
         }
-        {
-            const long long tick = sp.start + (long long)i * kTicks;
+        if constexpr (!PARTS) {
+            const long long tick = sp.start + (long long)i * kChunk;
+            const int n = ticks(i);
             bf16* room = now + Lay::v + 16 * warp;
             if (sizeof(T) == 2 && !s.dn_f32)
                 store_rows<T, Lay::vstride>(N, room, row_of<T>(s, s.dn, b, h, tick) + e0, s.dn.tick, n, s.E - e0, s.dn.fast, lane);
@@ -836,7 +879,7 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
             else {                                            // (one plane: fp32 straight from the registers)
                 float* to = row_of<float>(s, s.dn, b, h, tick) + e0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int t = 8 * j + 2 * (lane & 3) + (e & 1), c = (lane >> 2) + 8 * (e >> 1);
@@ -844,54 +887,128 @@ __global__ void __launch_bounds__(32 * WARPS) k_delta_back(const __grid_constant
                     }
             }
         }
-        // R = e^{G_63} R + (scale e^G dO)^T Q - (e^G dN)^T K
-        const float fade = from0[kTicks - 1];
-        uint32_t a[4][NS][4], q[4][NS][4];
+        // R = e^{G_31} R + (scale e^G dO)^T Q - (e^G dN)^T K
+        const float fade = from0[kChunk - 1];
+        uint32_t a[2][NS][4], q[2][NX][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float v[2][4], x[2][4];
+        for (int k = 0; k < 2; ++k) {
+            float v[2][4];
             two_columns<NI, Lay::vstride>(columns + 2 * Lay::go, k, v);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float2 f = gate2(from0, 2 * k + j, lane);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float ge = e & 1 ? f.y : f.x;
-                    x[j][e] = N[2 * k + j][e] * -ge;
-                    v[j][e] *= ge * s.scale;
-                }
+                scale2(N[2 * k + j], make_float2(-f.x, -f.y));
+                scale2(v[j], make_float2(f.x * s.scale, f.y * s.scale));
             }
-            left<NS>(x[0], x[1], a[k]);
-            left<NS>(v[0], v[1], q[k]);
+            left<NS>(N[2 * k], N[2 * k + 1], a[k]);
+            left<NX>(v[0], v[1], q[k]);
         }
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-            float acc[2][4] = {};
+        for (int d = 0; d < DP / 16; d += 2) {
+            float acc[4][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 2; ++k) {
+                products<NS, NI, NS, 2, true>(acc, a[k], [&](int j, int p) { return rows_m + 2 * (Lay::k + j * kPlane + 16 * k * Lay::stride + 16 * (d + p)); }, k == 0);
+                products<NX, NI, NX, 2, true>(acc, q[k], [&](int j, int p) { return rows_m + 2 * (Lay::q + j * kPlane + 16 * k * Lay::stride + 16 * (d + p)); });
+            }
 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    uint32_t r[4];
-                    ldsm_t(r, rows_m + 2 * (Lay::k + j * kPlane + 16 * k * Lay::stride + 16 * d));
+            for (int j = 0; j < 4; ++j) scale_add(R[2 * d + j], make_float2(fade, fade), acc[j]);
+        }
+    });
+    if constexpr (PARTS) {
+        float* to = s.own + part_place * 16 * tiles_e * DP;
+        if (mine) each_pair<DP>(R, e0, lane, [&](int at, float& x, float& y) { *reinterpret_cast<float2*>(to + at) = make_float2(x, y); });
+    } else if (s.gfirst && blockIdx.y == 0) {
+        each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { s.gfirst[state0 + at] = v; });
+    }
+}
+
+// ---- parts ----------------------------------------------------------------------------------------------------------------
+
+// A long recording in parts, all at once: a part turns the state S before it into Z + F S, Z what it makes of zeros and F what it
+// makes of the columns of 1 (dim more columns). Those are put together here, part after part, and then every part runs from the
+// state that it begins with; back it is Y + F^T R. That is 2.6 times the work on as many times the SMs as there are parts.
+//
+// A block goes through the parts with 16 columns: the state as terms in shared memory, a warp makes 16 of its values a part; F is read one
+// part ahead. s.start: BACK: R behind each part but the last, else S before each part but the first.
+template <int DP, bool BACK>
+__global__ void __launch_bounds__(2 * DP) k_delta_join(const __grid_constant__ Delta s) {
+    constexpr int kStride = DP + 8, kPlane = 16 * kStride, NS = 3;
+    __shared__ __align__(16) bf16 sm[2][NS * kPlane];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3, d0 = 16 * warp;
+    const int tiles_e = (s.E + 15) / 16, tile = blockIdx.x % tiles_e, rows = 16 * tiles_e * DP;
+    const long long bh = blockIdx.x / tiles_e;
+    const float* before = BACK ? s.glast : s.first;
+    float x[2][4];
 #pragma unroll
-                    for (int t = 0; t + j < NS; ++t) {
-                        mma(acc[0], a[k][t], r[0], r[1]);
-                        mma(acc[1], a[k][t], r[2], r[3]);
-                    }
-                    ldsm_t(r, rows_m + 2 * (Lay::q + j * kPlane + 16 * k * Lay::stride + 16 * d));
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int t = 0; t + j < NS; ++t) {
-                        mma(acc[0], q[k][t], r[0], r[1]);
-                        mma(acc[1], q[k][t], r[2], r[3]);
-                    }
-                }
+        for (int i = 0; i < 4; ++i) {
+            const int e = 16 * tile + g + 8 * (i >> 1), d = d0 + 8 * j + 2 * t4 + (i & 1);
+            x[j][i] = before && d < s.D && e < s.E ? before[(bh * s.D + d) * s.E + e] : 0.f;
+        }
+    float f[DP / 16][2][4];                                  // right operands (k, n) of F or its transpose, n this warp's values
+    const int written = (s.D + 15) / 16 * 16;                // rows of F that a part has
+    const auto fetch = [&](int p) {
+        const float* turn = s.turn + (bh * s.parts + p) * DP * DP;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) R[2 * d + j][e] = fmaf(R[2 * d + j][e], fade, acc[j][e]);
+                for (int i = 0; i < 4; ++i) {
+                    const int kk = 16 * k + 2 * t4 + (i & 1) + 8 * (i >> 1), n = d0 + 8 * j + g;
+                    f[k][j][i] = (BACK ? n : kk) < written ? turn[BACK ? n * DP + kk : kk * DP + n] : 0.f;
+                }
+    };
+    fetch(BACK ? s.parts - 1 : 0);
+    for (int i = 0; i + 1 < s.parts; ++i) {
+        const int p = BACK ? s.parts - 1 - i : i;            // the part that is gone through
+        bf16* now = sm[i & 1];
+        uint32_t a[NS][4];
+        left<NS>(x[0], x[1], a);
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint32_t*>(now + n * kPlane + (g + 8 * (e & 1)) * kStride + d0 + 2 * t4 + 8 * (e >> 1)) = a[n][e];
+        uint32_t b[DP / 16][2][2][NS];
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) terms<NS>(f[k][j][2 * e], f[k][j][2 * e + 1], b[k][j][e]);
+        if (i + 2 < s.parts) fetch(BACK ? p - 1 : p + 1);
+        const float* own = s.own + (bh * s.parts + p) * rows + 16 * tile * DP;
+        float z[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[j][e] = own[(g + 8 * (e >> 1)) * DP + d0 + 8 * j + 2 * t4 + (e & 1)];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) clear(x[j]);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) ldsm(a[n], smem_at(now + n * kPlane + 16 * k) + at_rows_m(lane, kStride));
+#pragma unroll
+            for (int m = 0; m < NS; ++m)
+#pragma unroll
+                for (int n = 0; n + m < NS; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) mma(x[j], a[n], b[k][j][0][m], b[k][j][1][m]);
         }
-    });
-    if (s.gfirst) each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { s.gfirst[state0 + at] = v; });
+        float* to = s.start + (bh * s.parts + (BACK ? p - 1 : p + 1)) * rows + 16 * tile * DP;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[j][e] += z[j][e];
+                to[(g + 8 * (e >> 1)) * DP + d0 + 8 * j + 2 * t4 + (e & 1)] = x[j][e];
+            }
+    }
 }
 
 }  // namespace

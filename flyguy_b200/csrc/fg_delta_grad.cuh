@@ -1,11 +1,11 @@
-// The gradients of q, k and the gates, every chunk by itself, from what the chain forward (S before the chunk, U) and the chain back
+// The gradients of q, k and the gates, every slot of 64 ticks by itself (a chunk as in fg_delta_chain.cuh, of 64: the same formulas), from what the chain forward (S before the chunk, U) and the chain back
 // (R behind it, dN, rows of dots) have left:
 //
 //   dP = dO U^T . M on and below the diagonal, D = -dN U^T . M below it
 //   dQ = scale (e^G dO S^T + dP K),  dK = scale dP^T Q + (D + D^T) K - e^G dN S^T + e^{G_63 - G} U R^T
 //   dbeta: the tiles' rows added;  dlog_decay_t = <R, S> + sum over t' >= t of (o dO - v dN)_t'
 //
-// A block of 8 warps makes 64 columns of one chunk of one head: warp = 16 ticks x 32 columns. The products with S and R run over blocks of 64 of
+// A block of 8 warps makes 64 columns of one slot of one head: warp = 16 ticks x 32 columns. The products with S and R run over blocks of 64 of
 // their columns; S and R arrive as the chain's left operands and go through shared memory, where reading across turns them.
 #pragma once
 #include "fg_delta_chain.cuh"
@@ -14,7 +14,7 @@ namespace {
 
 template <class T>
 struct GradLayout {
-    static constexpr int in = Terms<T>::in, kept = in == 1 ? 1 : Terms<T>::kept, plane = kTicks * kSquare;
+    static constexpr int in = Terms<T>::in, kept = Terms<T>::grad, plane = kTicks * kSquare;
     static constexpr int q = 0, k = q + in * plane, go = k + in * plane, dn = go + in * plane, u = dn + kept * plane, s = u + kept * plane,
                          r = s + kept * plane, values = r + kept * plane;
     static constexpr int dp = go, d = dp + kept * plane;     // later, over what is read by then
@@ -26,8 +26,7 @@ template <class T>
 __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(const __grid_constant__ Delta s) {
     using Lay = GradLayout<T>;
     constexpr int NI = Lay::in, NK = Lay::kept, kPlane = Lay::plane;
-    constexpr int NB = Terms<T>::kept;                       // terms that a product keeps where both sides have several
-    constexpr int kKeep = NI == 1 ? 1 : NB;
+    constexpr int NB = Terms<T>::saved, kKeep = NK;          // (terms i and j are kept with i + j < kKeep)
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
     float* gates = reinterpret_cast<float*>(smem + 2 * Lay::values);
@@ -35,7 +34,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     const long long slot = blockIdx.x, place = slot * s.heads + blockIdx.y;
     const int h = blockIdx.y, d_block = 64 * blockIdx.z, tiles_e = (s.E + 15) / 16;
     const int padded_d = s.D > 64 ? 8 : 4;                   // the chain's 16-value pieces of a column
-    const Chunk c = chunk_of(s, slot);
+    const Slot c = ticks_of(s, slot);
     if (c.n == 0) return;
     const long long tick = (s.offsets ? span_of(s, c.b).start : 0) + c.first;
     const int wt = warp >> 1, wd = warp & 1;                 // ticks 16 wt .., columns (of d, or ticks s) 32 wd ..
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
         }
     }
     __syncthreads();                                          // dO, dN and U have been read
-    const float *from0 = gates, *to_end = gates + kTicks, *gh = gates + 3 * kTicks, *gl = gates + 4 * kTicks;
+    const float *gh = gates + 3 * kTicks, *gl = gates + 4 * kTicks;
     if (below) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -189,7 +188,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int t = 16 * wt + g + 8 * i;
-        const float f = from0[t], k = to_end[t];
+        const float f = expf(gh[t] + gl[t]), k = expf((gh[kTicks - 1] - gh[t]) + (gl[kTicks - 1] - gl[t]));
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
