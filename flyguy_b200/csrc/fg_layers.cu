@@ -5,8 +5,9 @@
 //
 //   y = add + (kept ? x / (1 - p) : 0)                                                                    (gx: the same of gy)
 //
-// A row stays in registers between its statistics (the mean, then the squares of what is left: two sums, so that a mean far
-// from zero costs no digits) and its result, so x is read once. The mask is made anew wherever it is needed.
+// A row stays on the chip between its statistics and its result, so x is read once. The statistics are the mean m, as good as fp32 sums
+// make it, and then of d = x - m the sum, for what m lacks, and the squares: d r = (x - m) r - mean(d) r, var = mean(d^2) - mean(d)^2, so
+// that a mean far from zero costs no digits. The mask is made anew wherever it is needed.
 #include "fg_memory.cuh"
 
 namespace {
@@ -76,6 +77,12 @@ __device__ __forceinline__ void row_sums(float (&s)[N], float* room, int& turn) 
     }
 }
 
+// from the means of d and of d^2
+__device__ __forceinline__ void deviation(float mean, float square, float eps, float& inv, float& lack) {
+    inv = 1.f / sqrtf(fmaxf(fmaf(-mean, mean, square), 0.f) + eps);
+    lack = -mean * inv;
+}
+
 // What a thread has of ROWS rows: PER units of V values of each, kept as they came so that 16-bit values take half the registers
 template <class T, int V, int PER, int GROUP, int ROWS>
 struct Rows {
@@ -89,8 +96,8 @@ struct Rows {
             for (int j = 0; j < PER; ++j)
                 if (row + r < rows && column(j) < dim) u[r][j] = load<T, V>(reinterpret_cast<const T*>(p) + (row + r) * stride + column(j));
     }
-    // means and 1 / deviations; rows past the last are worked on as they are
-    __device__ __forceinline__ void stats(int dim, float eps, float (&mean)[ROWS], float (&inv)[ROWS], float* room, int& turn) const {
+    // the values d r are (x - mean) inv + lack; rows past the last are worked on as they are
+    __device__ __forceinline__ void stats(int dim, float eps, float (&mean)[ROWS], float (&inv)[ROWS], float (&lack)[ROWS], float* room, int& turn) const {
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             mean[r] = 0.f;
@@ -102,37 +109,39 @@ struct Rows {
                 }
         }
         row_sums<GROUP, ROWS>(mean, room, turn);
+        float s[2 * ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             mean[r] /= (float)dim;
-            inv[r] = 0.f;
+            s[2 * r] = s[2 * r + 1] = 0.f;
 #pragma unroll
             for (int j = 0; j < PER; ++j)
                 if (column(j) < dim) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         const float d = to_f(u[r][j].v[i]) - mean[r];
-                        inv[r] = fmaf(d, d, inv[r]);
+                        s[2 * r] += d;
+                        s[2 * r + 1] = fmaf(d, d, s[2 * r + 1]);
                     }
                 }
         }
-        row_sums<GROUP, ROWS>(inv, room, turn);
+        row_sums<GROUP, 2 * ROWS>(s, room, turn);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) inv[r] = 1.f / sqrtf(inv[r] / (float)dim + eps);
+        for (int r = 0; r < ROWS; ++r) deviation(s[2 * r] / (float)dim, s[2 * r + 1] / (float)dim, eps, inv[r], lack[r]);
     }
 };
 
 template <class T, int V, int PER, int GROUP, int ROWS>
 __global__ void __launch_bounds__(GROUP ? 256 : 512) k_norm(const __grid_constant__ Norm a) {
-    __shared__ float room[32 * ROWS];
+    __shared__ float room[64 * ROWS];
     int turn = 0;
     Rows<T, V, PER, GROUP, ROWS> x;
     x.me = GROUP ? threadIdx.x % (GROUP ? GROUP : 1) : threadIdx.x;
     x.step = GROUP ? GROUP : blockDim.x;
     const long long row = (GROUP ? blockIdx.x * (long long)(blockDim.x / (GROUP ? GROUP : 1)) + threadIdx.x / (GROUP ? GROUP : 1) : blockIdx.x) * ROWS;
     x.fetch(a.x, row, a.rows, a.x_row, a.dim);
-    float mean[ROWS], inv[ROWS];
-    x.stats(a.dim, a.eps, mean, inv, room, turn);
+    float mean[ROWS], inv[ROWS], lack[ROWS];
+    x.stats(a.dim, a.eps, mean, inv, lack, room, turn);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int c = x.column(j);
@@ -145,7 +154,7 @@ __global__ void __launch_bounds__(GROUP ? 256 : 512) k_norm(const __grid_constan
             if (row + r >= a.rows) break;
             float o[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = fmaf((to_f(x.u[r][j].v[i]) - mean[r]) * inv[r], w[i], b[i]);
+            for (int i = 0; i < V; ++i) o[i] = fmaf(fmaf(to_f(x.u[r][j].v[i]) - mean[r], inv[r], lack[r]), w[i], b[i]);
             store<T, V>(reinterpret_cast<T*>(a.y) + (row + r) * a.dim + c, o);
         }
     }
@@ -178,8 +187,8 @@ __global__ void __launch_bounds__(GROUP ? 128 : 512, GROUP ? 3 : 1) k_norm_bwd(c
         g = next_g;
         next_x.fetch(a.x, row + step, a.rows, a.x_row, a.dim);
         next_g.fetch(a.gy, row + step, a.rows, a.gy_row, a.dim);
-        float mean[ROWS], inv[ROWS], s[2 * ROWS];
-        x.stats(a.dim, a.eps, mean, inv, room, turn);
+        float mean[ROWS], inv[ROWS], lack[ROWS], s[2 * ROWS];
+        x.stats(a.dim, a.eps, mean, inv, lack, room, turn);
 #pragma unroll
         for (int r = 0; r < 2 * ROWS; ++r) s[r] = 0.f;
 #pragma unroll
@@ -193,7 +202,7 @@ __global__ void __launch_bounds__(GROUP ? 128 : 512, GROUP ? 3 : 1) k_norm_bwd(c
                 if (row + r >= a.rows) break;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float d = (to_f(x.u[r][j].v[i]) - mean[r]) * inv[r], y = to_f(g.u[r][j].v[i]), z = y * w[i];
+                    const float d = fmaf(to_f(x.u[r][j].v[i]) - mean[r], inv[r], lack[r]), y = to_f(g.u[r][j].v[i]), z = y * w[i];
                     if constexpr (SUMS) {
                         aw[j][i] = fmaf(y, d, aw[j][i]);
                         ab[j][i] += y;
@@ -217,7 +226,7 @@ __global__ void __launch_bounds__(GROUP ? 128 : 512, GROUP ? 3 : 1) k_norm_bwd(c
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    o[i] = inv[r] * (to_f(g.u[r][j].v[i]) * w[i] - m - (to_f(x.u[r][j].v[i]) - mean[r]) * inv[r] * k);
+                    o[i] = inv[r] * (to_f(g.u[r][j].v[i]) * w[i] - m - fmaf(to_f(x.u[r][j].v[i]) - mean[r], inv[r], lack[r]) * k);
                 store<T, V>(reinterpret_cast<T*>(a.gx) + (row + r) * a.dim + c, o);
             }
         }
@@ -421,7 +430,8 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
             for (int i = 0; i < N; ++i) sum = plus(sum, d[i]);
         }
         const P off = same<P>(-warp_sum(both(sum)) / (float)a.dim);   // - mean
-        sum = same<P>(0.f);
+        P squares = same<P>(0.f);
+        sum = squares;
         const auto centred = [&](int j, int c, P(&d)[N]) {
             const Unit<T, V> x = unit(j);
 #pragma unroll
@@ -435,9 +445,14 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
             P d[N];
             centred(j, c, d);
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum = times_plus(d[i], d[i], sum);
+            for (int i = 0; i < N; ++i) {
+                sum = plus(sum, d[i]);
+                squares = times_plus(d[i], d[i], squares);
+            }
         }
-        const P inv = same<P>(1.f / sqrtf(warp_sum(both(sum)) / (float)a.dim + a.eps));
+        float one, other;
+        deviation(warp_sum(both(sum)) / (float)a.dim, warp_sum(both(squares)) / (float)a.dim, a.eps, one, other);
+        const P inv = same<P>(one), lack = same<P>(other);
         if constexpr (!BACK) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
@@ -447,7 +462,7 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
                 centred(j, c, d);
                 float o[V];
 #pragma unroll
-                for (int i = 0; i < N; ++i) values_of<V>(times_plus(times(d[i], inv), w[j][i], b[j][i]), i, o);
+                for (int i = 0; i < N; ++i) values_of<V>(times_plus(times_plus(d[i], inv, lack), w[j][i], b[j][i]), i, o);
                 put(reinterpret_cast<T*>(a.y) + row * a.dim, c, o);
             }
         } else {
@@ -465,7 +480,7 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
                 keep(c, y);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const P h = times(d[i], inv), z = times(y[i], v[i]);
+                    const P h = times_plus(d[i], inv, lack), z = times(y[i], v[i]);
                     if constexpr (SUMS) {
                         aw[j][i] = times_plus(y[i], h, aw[j][i]);
                         ab[j][i] = plus(ab[j][i], y[i]);
@@ -485,7 +500,7 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const P d = times(plus(lane_of<T, V>(x, i), off), inv);
+                    const P d = times_plus(plus(lane_of<T, V>(x, i), off), inv, lack);
                     values_of<V>(times(times_plus(d, k, times_plus(lane_of<T, V>(g, i), v[i], m)), inv), i, o);
                 }
                 put(reinterpret_cast<T*>(a.gx) + row * a.dim, c, o);
@@ -554,17 +569,18 @@ __global__ void __launch_bounds__(512) k_norm_any(const __grid_constant__ Norm a
         for (int c = threadIdx.x; c < a.dim; c += 512) s[0] += to_f(x[c]);
         row_sums<0, 1>(s, room, turn);
         const float mean = s[0] / (float)a.dim;
-        s[0] = 0.f;
+        float q[2] = {0.f, 0.f}, r, lack;
         for (int c = threadIdx.x; c < a.dim; c += 512) {
             const float d = to_f(x[c]) - mean;
-            s[0] = fmaf(d, d, s[0]);
+            q[0] += d;
+            q[1] = fmaf(d, d, q[1]);
         }
-        row_sums<0, 1>(s, room, turn);
-        const float r = 1.f / sqrtf(s[0] / (float)a.dim + a.eps);
+        row_sums<0, 2>(q, room, turn);
+        deviation(q[0] / (float)a.dim, q[1] / (float)a.dim, a.eps, r, lack);
         if (!a.gy) {
             T* y = reinterpret_cast<T*>(a.y) + row * a.dim;
             for (int c = threadIdx.x; c < a.dim; c += 512)
-                y[c] = from_f<T>(fmaf((to_f(x[c]) - mean) * r, a.w ? a.w[c] : 1.f, a.b ? a.b[c] : 0.f));
+                y[c] = from_f<T>(fmaf(fmaf(to_f(x[c]) - mean, r, lack), a.w ? a.w[c] : 1.f, a.b ? a.b[c] : 0.f));
             continue;
         }
         const T* gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_row;
@@ -572,16 +588,17 @@ __global__ void __launch_bounds__(512) k_norm_any(const __grid_constant__ Norm a
         for (int c = threadIdx.x; c < a.dim; c += 512) {
             const float g = to_f(gy[c]) * (a.w ? a.w[c] : 1.f);
             t[0] += g;
-            t[1] = fmaf(g, (to_f(x[c]) - mean) * r, t[1]);
+            t[1] = fmaf(g, fmaf(to_f(x[c]) - mean, r, lack), t[1]);
         }
         row_sums<0, 2>(t, room, turn);
         const float m = t[0] / (float)a.dim, k = t[1] / (float)a.dim;
         T* gx = reinterpret_cast<T*>(a.gx) + row * a.dim;
         for (int c = threadIdx.x; c < a.dim; c += 512)
-            gx[c] = from_f<T>(r * (to_f(gy[c]) * (a.w ? a.w[c] : 1.f) - m - (to_f(x[c]) - mean) * r * k));
+            gx[c] = from_f<T>(r * (to_f(gy[c]) * (a.w ? a.w[c] : 1.f) - m - fmaf(to_f(x[c]) - mean, r, lack) * k));
         if (stats && threadIdx.x == 0) {
-            stats[2 * row] = mean;
-            stats[2 * row + 1] = r;
+            stats[3 * row] = mean;
+            stats[3 * row + 1] = r;
+            stats[3 * row + 2] = lack;
         }
     }
 }
@@ -593,8 +610,8 @@ __global__ void __launch_bounds__(256) k_norm_columns(const __grid_constant__ No
     float sw = 0.f, sb = 0.f;
     for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float g = to_f(reinterpret_cast<const T*>(a.gy)[row * a.gy_row + c]);
-        const float d = to_f(reinterpret_cast<const T*>(a.x)[row * a.x_row + c]) - stats[2 * row];
-        sw = fmaf(g, d * stats[2 * row + 1], sw);
+        const float d = to_f(reinterpret_cast<const T*>(a.x)[row * a.x_row + c]) - stats[3 * row];
+        sw = fmaf(g, fmaf(d, stats[3 * row + 1], stats[3 * row + 2]), sw);
         sb += g;
     }
     float* part = a.part + (long long)blockIdx.y * 2 * a.dim;
@@ -657,7 +674,7 @@ void check(const fg_norm_args* g, const char* who) {
 bool any_length(const fg_norm_args* g) { return g->dim > kLongest; }
 long long norm_work(const fg_norm_args* g) {
     if (!g->gw && !g->gb) return 0;
-    return (kNormBlocks * 2 * g->dim + (any_length(g) ? 2 * g->rows : 0)) * 4;
+    return (kNormBlocks * 2 * g->dim + (any_length(g) ? 3 * g->rows : 0)) * 4;
 }
 
 constexpr int kSumThreads = 128;                              // of a backward block whose lanes share rows

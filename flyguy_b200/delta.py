@@ -16,7 +16,6 @@ has two terms, 2^-17 of each value, three and 2^-24 where the inputs are float32
 and v of bfloat16 are made of once rounded operands, each of the size of the result's own rounding."""
 from __future__ import annotations
 
-import math
 import struct
 from functools import lru_cache
 
@@ -205,3 +204,56 @@ def delta_step(q, k, v, log_decay, beta, state, scale: float | None = None, slot
     _call(lib().fg_delta_step, packed, q.get_device())
     increment_version(state)                              # (autograd sees that it has changed, should it have kept it)
     return o
+
+
+# ---- the operators together ---------------------------------------------------------------------------------------
+
+class DeltaMemory(memory.TickMemory):
+    """TickMemory with the gated delta rule: a memory that can replace what it holds, with gates that the observations set.
+
+    The observations are normed (layer_norm) and projected in `dtype` to key_heads queries and keys of unit length (norm_rotate), heads
+    values, and each head's gates: beta = sigmoid(b) and log_decay = -softplus(a) / span, the heads' spans spread from ticks[0] to
+    ticks[1]. delta_attention carries the states, each head's output is normed, some of it dropped while learning (in training mode:
+    dropout with `seed`, one call of the generator a forward), and a last projection, zero at first, gives the logits."""
+
+    def __init__(self, obs_dim: int, n_actions: int, heads: int = 8, key_heads: int = 2, dim: int = 64,
+                 ticks: tuple[float, float] = (16.0, 4096.0), base: float = 10000.0, dropout: float = 0.0, seed: int = 0,
+                 dtype: torch.dtype = torch.bfloat16):
+        super().__init__(obs_dim, n_actions, heads, key_heads, dim, ticks, base, dtype)
+        self.dropout, self.seed, self.calls = dropout, seed, 0
+        self.qkv = nn.Linear(obs_dim, (2 * key_heads + heads) * dim, bias=False)
+        self.gates = nn.Linear(obs_dim, 2 * heads)
+        nn.init.zeros_(self.gates.weight)
+        nn.init.zeros_(self.gates.bias)
+        with torch.no_grad():
+            self.k_weight.fill_(dim ** -0.5)               # keys of unit length
+        self.obs_weight, self.obs_bias = nn.Parameter(torch.ones(obs_dim)), nn.Parameter(torch.zeros(obs_dim))
+        self.o_weight, self.o_bias = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.zeros(dim))
+
+    def _inputs(self, obs: torch.Tensor, positions):
+        obs = layers.layer_norm(obs.float(), self.obs_weight, self.obs_bias)
+        x = nn.functional.linear(obs.to(self.dtype), self.qkv.weight.to(self.dtype))
+        x = x.unflatten(-1, (2 * self.key_heads + self.heads, self.dim))
+        q, k, v = x.split((self.key_heads, self.key_heads, self.heads), -2)
+        a, b = nn.functional.linear(obs, self.gates.weight, self.gates.bias).chunk(2, -1)
+        q, k = memory.norm_rotate(q, k, self.turns, self.q_weight, self.k_weight, positions)
+        return q, k, v, nn.functional.softplus(a) * self.log_decay, torch.sigmoid(b)
+
+    def _normed(self, o: torch.Tensor) -> torch.Tensor:
+        return layers.layer_norm(o, self.o_weight, self.o_bias)
+
+    def forward(self, obs: torch.Tensor, state=None, positions=None, offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """As TickMemory.forward."""
+        offsets, positions = self._places(obs, state, positions, offsets)
+        o, end = delta_attention(*self._inputs(obs, positions), state, offsets=offsets)
+        o = self._normed(o)
+        if self.training and self.dropout:
+            o = layers.dropout(o, self.dropout, self.seed, call=self.calls)
+            self.calls += 1
+        return self._logits(o), end
+
+    @torch.no_grad()
+    def step(self, obs: torch.Tensor, state: torch.Tensor, positions: torch.Tensor, slots=None) -> torch.Tensor:
+        """As TickMemory.step; nothing is dropped."""
+        x = self._inputs(obs.unsqueeze(1), positions.unsqueeze(1))
+        return self._logits(self._normed(delta_step(*(t.squeeze(1) for t in x), state, slots=slots)))

@@ -537,6 +537,15 @@ class TickMemory(nn.Module):
         """The states of so many cars that remember nothing: float32 [cars, heads, dim, dim]."""
         return torch.zeros(cars, self.heads, self.dim, self.dim, device=self.log_decay.device)
 
+    def _places(self, obs: torch.Tensor, state, positions, offsets):
+        """Offsets and positions as forward's operators take them."""
+        if state is not None and positions is None:
+            raise FlyguyError("a recording carried on from a state needs its ticks' positions")
+        if offsets is not None and positions is None and obs.dim() == 2:   # (the states that come out are step's to go on from)
+            offsets, tick = _offsets(offsets, obs), torch.arange(len(obs), device=obs.device)
+            positions = tick - offsets[(torch.searchsorted(offsets, tick, right=True) - 1).clamp(min=0)]
+        return offsets, positions
+
     def _qkv(self, obs: torch.Tensor, positions):
         x = nn.functional.linear(obs.to(self.dtype), self.qkv.weight.to(self.dtype))
         x = x.unflatten(-1, (self.heads + 2 * self.key_heads, self.dim))
@@ -550,11 +559,7 @@ class TickMemory(nn.Module):
         """obs [recordings, ticks, obs_dim], or [ticks, obs_dim] packed end to end with offsets: logits of every tick and
         the states after the last. Positions are the ticks of each recording unless given. A recording carried on needs its
         states and positions (a rotation depends on them)."""
-        if state is not None and positions is None:
-            raise FlyguyError("a recording carried on from a state needs its ticks' positions")
-        if offsets is not None and positions is None and obs.dim() == 2:   # (the states that come out are step's to go on from)
-            offsets, tick = _offsets(offsets, obs), torch.arange(len(obs), device=obs.device)
-            positions = tick - offsets[(torch.searchsorted(offsets, tick, right=True) - 1).clamp(min=0)]
+        offsets, positions = self._places(obs, state, positions, offsets)
         q, k, v = self._qkv(obs, positions)
         o, end = decay_attention(q, k, v, self.log_decay, state, offsets=offsets)
         return self._logits(o), end

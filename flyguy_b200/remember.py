@@ -1,12 +1,13 @@
 """A memory over ticks beside a fly network, learned on whole recordings and played a tick at a time.
 
   python -m flyguy_b200.remember [--steps 200] [--recordings 64] [--ticks 128] [--ago 12] [--lr 3e-3] [--cars 8]
+                                 [--rule decay|delta] [--dropout 0]
 
 A made-up game that no actor without a memory can play: each tick's observation shows an action, and the right answer is
 the one shown `ago` ticks earlier. The fly network (a small synthetic one, its weights left alone) answers from the tick's
-observation; flyguy_b200.memory.TickMemory adds what it remembers. Learning is distillation as elsewhere in this package:
-the library's KL loss of the sum against the teacher's logits gives the gradient, here of a batch of whole recordings.
-Then `cars` cars play a recording tick by tick with the same weights."""
+observation; flyguy_b200.memory.TickMemory (or flyguy_b200.delta.DeltaMemory: --rule delta) adds what it remembers. Learning
+is distillation as elsewhere in this package: the library's KL loss of the sum against the teacher's logits gives the
+gradient, here of a batch of whole recordings. Then `cars` cars play a recording tick by tick with the same weights."""
 from __future__ import annotations
 
 import argparse
@@ -14,6 +15,7 @@ import argparse
 import torch
 
 from . import native, synth
+from .delta import DeltaMemory
 from .memory import TickMemory
 
 
@@ -30,14 +32,19 @@ def recordings(n: int, ticks: int, ago: int, obs_dim: int, n_act: int, generator
 class Game:
     """The fly network and the memory beside it."""
 
-    def __init__(self, seed: int = 0, max_batch: int = 8192, n_act: int = 16, device: str = "cuda"):
+    def __init__(self, seed: int = 0, max_batch: int = 8192, n_act: int = 16, device: str = "cuda", rule: str = "decay",
+                 dropout: float = 0.0):
         s, params = synth.make_synthetic(sizes=(300, 700, 500, 60), total_edges=30_000, seed=seed)
         self.device = torch.device(device)
         torch.manual_seed(seed)
         self.fly = native.Handle(s, max_batch, native.FG_INFER_ONLY)
         self.fly.set_params(params)
         self.obs_dim, self.all_actions, self.n_act = s["obs_dim"], s["n_act"], n_act
-        self.memory = TickMemory(self.obs_dim, self.all_actions, ticks=(8.0, 256.0)).to(self.device)
+        if rule == "delta":
+            self.memory = DeltaMemory(self.obs_dim, self.all_actions, ticks=(8.0, 256.0), dropout=dropout, seed=seed)
+        else:
+            self.memory = TickMemory(self.obs_dim, self.all_actions, ticks=(8.0, 256.0))
+        self.memory.to(self.device)
 
     def fly_logits(self, obs: torch.Tensor) -> torch.Tensor:
         """The fly network's logits [.., n_act] of observations [.., obs_dim] (in batches of a multiple of 32)."""
@@ -83,10 +90,13 @@ def main() -> None:
     ap.add_argument("--ago", type=int, default=12)
     ap.add_argument("--lr", type=float, default=3e-3)
     ap.add_argument("--cars", type=int, default=8)
+    ap.add_argument("--rule", choices=("decay", "delta"), default="decay")
+    ap.add_argument("--dropout", type=float, default=0.0, help="of the delta rule's outputs, while learning")
     a = ap.parse_args()
-    game = Game(max_batch=-(-max(a.recordings * a.ticks, a.cars) // 32) * 32)
+    game = Game(max_batch=-(-max(a.recordings * a.ticks, a.cars) // 32) * 32, rule=a.rule, dropout=a.dropout)
     game.learn(a.steps, a.recordings, a.ticks, a.ago, a.lr, log=print)
     obs, right = recordings(a.cars, a.ticks, a.ago, game.obs_dim, game.n_act, torch.Generator().manual_seed(99), game.device)
+    game.memory.eval()
     played = game.play(obs)
     with torch.no_grad():
         whole = game.fly_logits(obs) + game.memory(obs)[0]
