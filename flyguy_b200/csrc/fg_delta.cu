@@ -384,24 +384,22 @@ long long lay_out(const fg_delta_args* g, bool backward, Delta& s, Wide& wide) {
     const auto of = [&](auto f) {
         return g->type == FG_F32 ? f(Terms<float>()) : g->type == FG_F16 ? f(Terms<__half>()) : f(Terms<bf16>());
     };
-    const int in = of([](auto t) { return t.in; }), out = of([](auto t) { return t.out; }), square = of([](auto t) { return t.square; }),
-              saved = of([](auto t) { return t.saved; }), grad = of([](auto t) { return t.grad; });
-    const long long places = slots_of(g) * g->heads, tiles = (g->value_dim + 15) / 16, pieces = g->dim > 64 ? 8 : 4;
-    room.take(s.x, places * square * 2 * kChunk * kChunk * 2);
-    room.take(s.p, places * (backward ? square : out) * 2 * kChunk * kChunk * 2);
+    const int kept = of([](auto t) { return t.kept; }), out = of([](auto t) { return t.out_p; });
+    const long long places = slots_of(g) * g->heads, tiles = (g->value_dim + 15) / 16, padded = g->dim > 64 ? 128 : 64;
+    room.take(s.x, places * kept * 2 * kChunk * kChunk * 2);
+    room.take(s.p, places * (backward ? kept : out) * 2 * kChunk * kChunk * 2);
     room.take(s.gates, places * kGates * kTicks * 4);
     s.parts = parts_of(g);
     if (s.parts > 1) {
-        const long long all = g->batch * g->heads * s.parts * 4, dim = 16 * pieces;
+        const long long all = g->batch * g->heads * s.parts * 4, dim = padded;
         room.take(s.own, all * 16 * tiles * dim);
         room.take(s.turn, all * dim * dim);
         room.take(s.start, all * 16 * tiles * dim);
     }
     if (!backward) return room.used;
-    room.take(s.states, places * tiles * saved * pieces * 512);
-    room.take(s.gstates, places * tiles * grad * pieces * 512);
+    room.take(s.states, places * tiles * padded * 64);
+    room.take(s.gstates, places * tiles * padded * 64);
     room.take(s.w, places * tiles * 8 * 512);
-    room.take(s.u, places * kTicks * 16 * tiles * (in == 1 ? 2 : 4));
     room.take(s.od, places * tiles * kTicks * 4);
     room.take(s.vdn, places * tiles * kTicks * 4);
     room.take(s.db, places * tiles * kTicks * 4);
@@ -472,8 +470,8 @@ void prepare(const Delta& s, cudaStream_t st) {
 template <class T, int DP, int WARPS, int MODE>
 void chain(const Delta& s, cudaStream_t st) {
     static OnEachDevice here;
-    using Lay = ChainLayout<T, DP, WARPS, MODE == kKeep ? Terms<T>::square : Terms<T>::out, MODE == kKeep>;
-    const int tiles = (s.E + 15) / 16 + (MODE >= kParts ? (s.D + 15) / 16 : 0);
+    using Lay = ChainLayout<T, DP, WARPS, MODE == kKeep ? Terms<T>::kept : Terms<T>::out_p, MODE == kKeep>;
+    const int tiles = (s.E + 15) / 16 + (MODE == kParts ? (s.D + 15) / 16 : 0);
     const long long blocks = s.batch * s.heads * ((tiles + WARPS - 1) / WARPS);
     launch(k_delta_chain<T, DP, WARPS, MODE>, dim3((unsigned)blocks, s.parts), 32 * WARPS, Lay::bytes, here, st, s);
 }
@@ -481,7 +479,7 @@ template <class T, int DP, int WARPS, bool PARTS>
 void chain_back(const Delta& s, cudaStream_t st) {
     static OnEachDevice here;
     const long long blocks = s.batch * s.heads * ((s.E + 16 * WARPS - 1) / (16 * WARPS));
-    launch(k_delta_back<T, DP, WARPS, PARTS>, dim3((unsigned)blocks, s.parts), 32 * WARPS, ChainLayout<T, DP, WARPS, Terms<T>::square, true>::bytes,
+    launch(k_delta_back<T, DP, WARPS, PARTS>, dim3((unsigned)blocks, s.parts), 32 * WARPS, ChainLayout<T, DP, WARPS, Terms<T>::kept, true>::bytes,
            here, st, s);
 }
 template <int DP, bool BACK>
@@ -496,23 +494,23 @@ void gradients(const Delta& s, cudaStream_t st) {
 }
 
 // the state that each part of a recording begins with
-template <class T, int DP, int MODE>
+template <class T, int DP>
 void parts_forward(const Delta& s, cudaStream_t st) {
     if (s.parts == 1) return;
-    chain<T, DP, 4, MODE>(s, st);
+    chain<T, DP, 4, kParts>(s, st);
     join<DP, false>(s, st);
 }
 template <class T, int DP>
 void forward(const Delta& s, cudaStream_t st) {
-    prepare<T, DP, Terms<T>::out>(s, st);
-    parts_forward<T, DP, kParts>(s, st);
+    prepare<T, DP, Terms<T>::out_p>(s, st);
+    parts_forward<T, DP>(s, st);
     chain<T, DP, 4, kForward>(s, st);
 }
 template <class T, int DP>
 void backward(Delta s, float* last, cudaStream_t st) {
-    prepare<T, DP, Terms<T>::square>(s, st);
+    prepare<T, DP, Terms<T>::kept>(s, st);
     s.last = last;
-    parts_forward<T, DP, Terms<T>::learn == Terms<T>::forward ? kParts : kPartsKeep>(s, st);
+    parts_forward<T, DP>(s, st);
     // 64 or 128 columns of values a block; 16 warps an SM where 128 registers a thread do (the chain back, W = 4 and 8: 863 and 758 us)
     constexpr int wide = Terms<T>::in == 1 && DP == 128 ? 8 : 4;
     if (s.E > 64) chain<T, DP, wide, kKeep>(s, st);

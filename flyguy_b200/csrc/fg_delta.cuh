@@ -177,13 +177,80 @@ __device__ __forceinline__ float column_sums(float (&v)[8], int lane) {
     return v[0];
 }
 
-// Terms by type: of inputs; of what a chunk corrects by (X, P and what they meet); of states, of their gradients and of what is added to
-// them, on the way forward and where gradients are wanted; of states as they are kept for those; of operands of q's and k's gradients.
-// With bf16 inputs states are 4e-6 of their norm off at two terms, 1.5e-6 at three. Two are enough for o and the last states; the gates'
-// gradients are differences of what they give (1e-5 at two, 4e-6 at three; 64 recordings of 1,024 ticks, 8 heads of 128: TIMES).
+// Terms by type: of inputs; of all that is carried from chunk to chunk and what corrects it (states, X, their gradients); of S and of P
+// and U where they make o; for the gradients of q and k of U, dP and D, of S
+// and R, and of dN (gv in the type of v, where no heads share it).
+// Three terms keep states, their gradients and the gates' as good as fp32 products and sums would (64 recordings of 1,024 ticks, 8 heads of
+// 128 in bf16: 3e-7 to 8e-7 off; with two terms 4e-6 to 1e-5, in CHAINTWO instead of CHAIN us for the chain forward). o and the gradients of
+// q and k are rounded to 16 bits in the end, 1.65e-3 of their norm; with once rounded operands throughout they were 2.6e-3 to 3.0e-3 off,
+// with these terms GRADERR.
 template <class T> struct Terms;
-template <> struct Terms<bf16> { static constexpr int in = 1, square = 2, forward = 2, learn = 3, saved = 2, grad = 1, out = 1; };
-template <> struct Terms<__half> { static constexpr int in = 2, square = 3, forward = 3, learn = 3, saved = 3, grad = 2, out = 2; };
-template <> struct Terms<float> { static constexpr int in = 3, square = 3, forward = 3, learn = 3, saved = 3, grad = 3, out = 3; };
+template <> struct Terms<bf16> { static constexpr int in = 1, kept = 3, out_s = 2, out_p = 1, grad = 2, grad_s = 1, grad_n = 1; };
+template <> struct Terms<__half> { static constexpr int in = 2, kept = 3, out_s = 2, out_p = 2, grad = 2, grad_s = 2, grad_n = 2; };
+template <> struct Terms<float> { static constexpr int in = 3, kept = 3, out_s = 3, out_p = 3, grad = 3, grad_s = 3, grad_n = 3; };
+
+// sum[2 J] += a b for J pairs of 8 x 16 right operands from planes of NB terms at(j, pair), products with term numbers below KEEP; term
+// by term over all pairs, so that no product waits for the one just before. `first`: sum = a b. The tensor cores cut sums off, they do not
+// round them: where both operands have terms (so many products) the small ones are added up first, by themselves, and their sum with the
+// large one to `sum` in fp32 (1.0e-6 to 2.1e-6 off without that, 4e-7 to 7e-7 with it, 32 recordings of 509 ticks, 4 heads of 64 in fp32).
+template <int NA, int NB, int KEEP, int J, bool TRANS, class At>
+__device__ __forceinline__ void products(float (*sum)[4], const uint32_t (&a)[NA][4], At&& at, bool first = false) {
+    if constexpr (KEEP >= 3 && NB >= 2) {
+        uint32_t r[NB][J][4];
+        float x[2 * J][4];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int p = 0; p < J; ++p) {
+                if (TRANS) ldsm_t(r[j][p], at(j, p));
+                else ldsm(r[j][p], at(j, p));
+            }
+        constexpr int most = NA + NB - 2 < KEEP - 1 ? NA + NB - 2 : KEEP - 1;
+#pragma unroll
+        for (int s = most; s >= 0; --s)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int k = s - j;
+                if (k < 0 || k >= NA) continue;
+                const bool opens = s == most && (j == 0 || k == NA - 1);   // the first of all
+#pragma unroll
+                for (int p = 0; p < J; ++p) {
+                    if (opens) {
+                        mma_first(x[2 * p], a[k], r[j][p][0], r[j][p][1]);
+                        mma_first(x[2 * p + 1], a[k], r[j][p][2], r[j][p][3]);
+                    } else {
+                        mma(x[2 * p], a[k], r[j][p][0], r[j][p][1]);
+                        mma(x[2 * p + 1], a[k], r[j][p][2], r[j][p][3]);
+                    }
+                }
+            }
+#pragma unroll
+        for (int p = 0; p < 2 * J; ++p)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[p][e] = first ? x[p][e] : sum[p][e] + x[p][e];
+    } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            uint32_t r[J][4];
+#pragma unroll
+            for (int p = 0; p < J; ++p) {
+                if (TRANS) ldsm_t(r[p], at(j, p));
+                else ldsm(r[p], at(j, p));
+            }
+#pragma unroll
+            for (int k = 0; k < NA && k + j < KEEP; ++k)
+#pragma unroll
+                for (int p = 0; p < J; ++p) {
+                    if (first && j + k == 0) {
+                        mma_first(sum[2 * p], a[k], r[p][0], r[p][1]);
+                        mma_first(sum[2 * p + 1], a[k], r[p][2], r[p][3]);
+                    } else {
+                        mma(sum[2 * p], a[k], r[p][0], r[p][1]);
+                        mma(sum[2 * p + 1], a[k], r[p][2], r[p][3]);
+                    }
+                }
+        }
+    }
+}
 
 }  // namespace

@@ -36,9 +36,8 @@ struct Delta {
     float scale;
     bf16 *x, *p;                     // [slot][head][chunk][term][32][32]
     float* gates;                    // [slot][head][5][64]: e^G and e^{G_31 - G} of the chunks, beta, G of the slot as two floats
-    uint4 *states, *gstates;         // [slot][head][tile of 16 columns][term][DP / 16][32]: S before and R behind as left operands
+    float4 *states, *gstates;        // [slot][head][tile of 16 columns][DP / 8][32]: S before and R behind, transposed, as accumulators
     float4* w;                       // [slot][head][chunk][tile][4][32]: W^T as accumulators
-    char* u;                         // [slot][head][64][16 tiles]: U in bf16 (inputs of one term) or fp32
     float *od, *vdn, *db;            // [slot][head][tile][64]: rows of o dO, v dN, dbeta
     float* anchor;                   // [slot][head][tile]: <R, S> behind
     // few long recordings are split into parts, see k_delta_join
@@ -96,7 +95,7 @@ __device__ __forceinline__ float* gate_of(const Delta& s, const Gate& o, long lo
 
 template <class T, int DP>
 struct PrepLayout {
-    static constexpr int in = Terms<T>::in, square = Terms<T>::square, stride = DP + 8, tile = in * kTicks * stride,
+    static constexpr int in = Terms<T>::in, square = Terms<T>::kept, stride = DP + 8, tile = in * kTicks * stride,
                          small = 2 * square * kChunk * kSmall;                       // of both chunks
     static constexpr int tiles = 2 * tile > 2 * small ? 2 * tile : 2 * small;        // K and Q, later L B and X
     static constexpr int lrow = kChunk + 4, l = kTicks * lrow, bytes = 2 * tiles + 4 * (l + 3 * kTicks);
@@ -303,7 +302,7 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
 // Tiles of one chunk, in values of bf16
 template <class T, int DP, int WARPS, int NP, bool GO>
 struct ChainLayout {
-    static constexpr int in = Terms<T>::in, square = Terms<T>::square, stride = DP + 8, vstride = 16 * WARPS + 8;
+    static constexpr int in = Terms<T>::in, square = Terms<T>::kept, stride = DP + 8, vstride = 16 * WARPS + 8;
     static constexpr int k = 0, q = k + in * kChunk * stride, v = q + in * kChunk * stride, go = v + in * kChunk * vstride,
                          x = go + (GO ? in * kChunk * vstride : 0), p = x + square * kChunk * kSmall, gates = p + NP * kChunk * kSmall,
                          stage = gates + 3 * kChunk * 2;
@@ -468,51 +467,22 @@ __device__ __forceinline__ void subtract(float (&x)[4], const float (&y)[4]) {
     for (int e = 0; e < 4; ++e) x[e] -= y[e];
 }
 
-// sum[2 J] += a b for J pairs of 8 x 16 right operands from planes of NB terms at(j, pair), products with term numbers below KEEP; term
-// by term over all pairs, so that no product waits for the one just before. `first`: sum = a b.
-template <int NA, int NB, int KEEP, int J, bool TRANS, class At>
-__device__ __forceinline__ void products(float (*sum)[4], const uint32_t (&a)[NA][4], At&& at, bool first = false) {
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        uint32_t r[J][4];
-#pragma unroll
-        for (int p = 0; p < J; ++p) {
-            if (TRANS) ldsm_t(r[p], at(j, p));
-            else ldsm(r[p], at(j, p));
-        }
-#pragma unroll
-        for (int k = 0; k < NA && k + j < KEEP; ++k)
-#pragma unroll
-            for (int p = 0; p < J; ++p) {
-                if (first && j + k == 0) {
-                    mma_first(sum[2 * p], a[k], r[p][0], r[p][1]);
-                    mma_first(sum[2 * p + 1], a[k], r[p][2], r[p][3]);
-                } else {
-                    mma(sum[2 * p], a[k], r[p][0], r[p][1]);
-                    mma(sum[2 * p + 1], a[k], r[p][2], r[p][3]);
-                }
-            }
-    }
-}
-
 // blocks of an SM at once: 16 warps with 128 registers a thread, 12 with 168
 template <int DP>
 constexpr int chain_blocks(int warps) { return warps == 8 ? 2 : (DP > 64 ? 12 : 16) / warps; }
 
-// Forward. kKeep: nothing but what the way back needs is written (S before each slot, W, U, rows of o dO), and o is made to as many
-// terms as the corrections. kParts: what a part makes of a state of zeros, and (tiles past those of the columns) of the columns of 1;
-// kPartsKeep: for what is kept.
-enum { kForward, kKeep, kParts, kPartsKeep };
+// Forward. kKeep: nothing but what the way back needs is written (S before each slot, W, rows of o dO), and o is made to as many
+// terms as the corrections. kParts: what a part makes of a state of zeros, and (tiles past those of the columns) of the columns of 1.
+enum { kForward, kKeep, kParts };
 template <class T, int DP, int WARPS, int MODE>
 __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<DP>(WARPS) : DP > 64 ? 2 : 3)
     k_delta_chain(const __grid_constant__ Delta s) {
-    constexpr bool KEEP = MODE == kKeep, PARTS = MODE >= kParts;
-    constexpr int NI = Terms<T>::in, NX = Terms<T>::square, NS = KEEP || MODE == kPartsKeep ? Terms<T>::learn : Terms<T>::forward, NO = KEEP ? NX : Terms<T>::out,
-                  kSaved = Terms<T>::saved;
+    constexpr bool KEEP = MODE == kKeep, PARTS = MODE == kParts;
+    constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX, NO = KEEP ? NX : Terms<T>::out_s, NP = KEEP ? NX : Terms<T>::out_p;
     // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: forward with 168 registers 415 and 380 us (64 recordings
     // of 1,024 ticks, 8 heads of 128), with what is kept and 128 registers 675 and 747
     constexpr bool kTogether = WARPS == 8;
-    using Lay = ChainLayout<T, DP, WARPS, NO, KEEP>;
+    using Lay = ChainLayout<T, DP, WARPS, NP, KEEP>;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
@@ -558,7 +528,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
         each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.first[state0 + at]; });
     }
 
-    const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NO, KEEP, !PARTS>(s, from, to, i, ticks(i), s.E - e_block); };
+    const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NP, KEEP, !PARTS>(s, from, to, i, ticks(i), s.E - e_block); };
     each_chunk<Lay>(tiles, part, false, load, [&](bf16* now, int i) {
         if (!mine) return;
         const uint32_t tile = smem_at(now), rows_n = tile + at_rows_n(lane, Lay::stride), rows_m = tile + at_rows_m(lane, Lay::stride),
@@ -577,8 +547,8 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
             left<NS>(S[2 * d], S[2 * d + 1], a);
             if (KEEP && !(i & 1)) {
 #pragma unroll
-                for (int k = 0; k < kSaved; ++k)
-                    s.states[((warp_place * kSaved + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
+                for (int j = 2 * d; j < 2 * d + 2; ++j)
+                    s.states[(warp_place * (DP / 8) + j) * 32 + lane] = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
             }
             products<NS, NI, NS, 2, false>(N, a, [&](int j, int p) { return rows_n + 2 * (Lay::k + j * kPlane + 16 * p * Lay::stride + 16 * d); }, d == 0);
             if (kTogether && !PARTS) query(a, d);
@@ -638,11 +608,11 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                uint32_t a[NO][4];
-                left<NO>(N[2 * k], N[2 * k + 1], a);
+                uint32_t a[NP][4];
+                left<NP>(N[2 * k], N[2 * k + 1], a);
                 const auto at = [&](int j, int p) { return square_n + 2 * (Lay::p + j * kSm + 16 * (p + k) * kSmall + 16 * k); };
-                if (k == 0) products<NO, NO, NO, 2, false>(O, a, at);
-                else products<NO, NO, NO, 1, false>(O + 2, a, at);
+                if (k == 0) products<NP, NP, NP, 2, false>(O, a, at);
+                else products<NP, NP, NP, 1, false>(O + 2, a, at);
             }
             if constexpr (!KEEP) {
                 store_rows<T, Lay::vstride>(O, now + Lay::v + 16 * warp, out + (long long)i * kChunk * s.o.tick, s.o.tick, ticks(i), s.E - e0, s.o.fast, lane);
@@ -658,10 +628,6 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
                         for (int e = 0; e < 2; ++e) sums[4 * jp + 2 * j + e] = O[2 * jp + j][e] * v[j][e] + O[2 * jp + j][e + 2] * v[j][e + 2];
                 }
                 s.od[warp_place * kTicks + (i & 1) * kChunk + 8 * (lane >> 3) + 2 * (lane & 3) + (lane >> 2 & 1)] = column_sums(sums, lane);
-                using U = std::conditional_t<NI == 1, bf16, float>;
-                store_rows<U, Lay::vstride>(N, now + Lay::v + 16 * warp,
-                                            reinterpret_cast<U*>(s.u) + (place * kTicks + (i & 1) * kChunk) * 16 * tiles_e + e0, 16 * tiles_e, kChunk, 16,
-                                            true, lane);
             }
         }
         // S = e^{G_31} S + (e^{G_31 - G} K)^T U
@@ -683,13 +649,10 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
             for (int j = 0; j < 4; ++j) scale_add(S[2 * d + j], make_float2(fade, fade), acc[j]);
         }
     });
-    // a slot whose second chunk has no ticks: nothing is foretold there, and nothing added
+    // a slot's second chunk without ticks
     if (KEEP && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {
         const long long place = from.place + (long long)(chunks >> 1) * s.heads;
         s.od[(place * tiles_e + e0 / 16) * kTicks + kChunk + lane] = 0.f;
-        using U = std::conditional_t<NI == 1, bf16, float>;
-        U* u = reinterpret_cast<U*>(s.u) + (place * kTicks + kChunk) * 16 * tiles_e + e0;
-        for (int c = 0; c < 16; ++c) u[(long long)lane * 16 * tiles_e + c] = from_f<U>(0.f);
     }
     if constexpr (PARTS) {
         if (!mine) return;
@@ -707,7 +670,7 @@ __device__ __forceinline__ void prefetch(const char* p) { asm volatile("prefetch
 template <class T, int DP, int WARPS, bool PARTS>
 __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<DP>(WARPS) : DP > 64 ? 2 : 3)
     k_delta_back(const __grid_constant__ Delta s) {
-    constexpr int NI = Terms<T>::in, NX = Terms<T>::square, NS = Terms<T>::learn, NG = Terms<T>::grad, kSaved = Terms<T>::saved;
+    constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX;
     using Lay = ChainLayout<T, DP, WARPS, NX, true>;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -759,11 +722,11 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
         const long long place = from.place + (long long)(i >> 1) * s.heads, warp_place = place * tiles_e + e0 / 16;
         const long long w_place = (2 * place + (i & 1)) * tiles_e + e0 / 16;
         const bool last = i + 1 == chunks, slot_end = !PARTS && ((i & 1) || last);   // R is the one behind the slot
-        const uint4* behind = s.states + (warp_place + (long long)s.heads * tiles_e) * kSaved * (DP / 16) * 32 + lane;
+        const float4* behind = s.states + (warp_place + (long long)s.heads * tiles_e) * (DP / 8) * 32 + lane;
         if (!PARTS && i > part.first) {                       // what the next chunk reads of this, on its way to L2
             if (!(i & 1)) {
-                const char* states = reinterpret_cast<const char*>(s.states + warp_place * kSaved * (DP / 16) * 32);
-                for (int at = lane * 128; at < kSaved * (DP / 16) * 512; at += 32 * 128) prefetch(states + at);
+                const char* states = reinterpret_cast<const char*>(s.states + warp_place * (DP / 8) * 32);
+                for (int at = lane * 128; at < DP / 8 * 512; at += 32 * 128) prefetch(states + at);
             }
             const long long before = (2 * (place - (i & 1 ? 0 : s.heads)) + !(i & 1)) * tiles_e + e0 / 16;
             if (lane < 16) prefetch(reinterpret_cast<const char*>(s.w + before * 4 * 32) + lane * 128);
@@ -773,29 +736,24 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<D
         float anchor = 0.f;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
-            uint4 kept[kSaved];
+            float4 kept[2];
             if (slot_end && !last) {
 #pragma unroll
-                for (int k = 0; k < kSaved; ++k) kept[k] = __ldg(behind + (k * (DP / 16) + d) * 32);
+                for (int j = 0; j < 2; ++j) kept[j] = __ldg(behind + (2 * d + j) * 32);
+            }
+            if (slot_end) {
+#pragma unroll
+                for (int j = 2 * d; j < 2 * d + 2; ++j)
+                    s.gstates[(warp_place * (DP / 8) + j) * 32 + lane] = make_float4(R[j][0], R[j][1], R[j][2], R[j][3]);
             }
             uint32_t a[NS][4];
             left<NS>(R[2 * d], R[2 * d + 1], a);
-            if (slot_end) {
-#pragma unroll
-                for (int k = 0; k < NG; ++k)
-                    s.gstates[((warp_place * NG + k) * (DP / 16) + d) * 32 + lane] = make_uint4(a[k][0], a[k][1], a[k][2], a[k][3]);
-            }
             products<NS, NI, NS, 2, false>(N, a, [&](int j, int p) { return rows_n + 2 * (Lay::k + j * kPlane + 16 * p * Lay::stride + 16 * d); }, d == 0);
             if (slot_end && !last) {
 #pragma unroll
-                for (int k = 0; k < kSaved; ++k) {
-                    const uint32_t* p = &kept[k].x;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float(&v)[4] = R[2 * d + (j >> 1)];
-                        anchor = fmaf(v[2 * (j & 1)], low(p[j]), anchor);
-                        anchor = fmaf(v[2 * (j & 1) + 1], high(p[j]), anchor);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    const float(&v)[4] = R[2 * d + j];
+                    anchor = fmaf(v[0], kept[j].x, fmaf(v[1], kept[j].y, fmaf(v[2], kept[j].z, fmaf(v[3], kept[j].w, anchor))));
                 }
             }
         }

@@ -1,4 +1,4 @@
-// The gradients of q, k and the gates, every slot of 64 ticks by itself (a chunk as in fg_delta_chain.cuh, of 64: the same formulas), from what the chain forward (S before the chunk, U) and the chain back
+// The gradients of q, k and the gates, every slot of 64 ticks by itself (a chunk as in fg_delta_chain.cuh, of 64: the same formulas), from what the chain forward (S before the slot, W) and the chain back
 // (R behind it, dN, rows of dots) have left:
 //
 //   dP = dO U^T . M on and below the diagonal, D = -dN U^T . M below it
@@ -14,26 +14,26 @@ namespace {
 
 template <class T>
 struct GradLayout {
-    static constexpr int in = Terms<T>::in, kept = Terms<T>::grad, plane = kTicks * kSquare;
-    static constexpr int q = 0, k = q + in * plane, go = k + in * plane, dn = go + in * plane, u = dn + kept * plane, s = u + kept * plane,
-                         r = s + kept * plane, values = r + kept * plane;
-    static constexpr int dp = go, d = dp + kept * plane;     // later, over what is read by then
+    static constexpr int in = Terms<T>::in, terms_n = Terms<T>::grad_n, terms_s = Terms<T>::grad_s, terms = Terms<T>::grad, plane = kTicks * kSquare;
+    static constexpr int q = 0, k = q + in * plane, go = k + in * plane, dn = go + in * plane, u = dn + terms_n * plane, s = u + terms * plane,
+                         r = s + terms_s * plane, values = r + terms_s * plane;
+    static constexpr int dp = go, d = dp + terms * plane;     // later, over dO, dN and U
+    static constexpr int out = s;                             // and at last, fp32 rows over S and R
     static constexpr int bytes = 2 * values + 4 * kGates * kTicks;
-    static_assert(2 * kept <= in + 4 * kept && 2 * kept * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
+    static_assert(in + terms_n >= terms && 2 * terms_s * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
 };
 
 template <class T>
 __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(const __grid_constant__ Delta s) {
     using Lay = GradLayout<T>;
-    constexpr int NI = Lay::in, NK = Lay::kept, kPlane = Lay::plane;
-    constexpr int NB = Terms<T>::saved, kKeep = NK;          // (terms i and j are kept with i + j < kKeep)
+    constexpr int NI = Lay::in, NN = Lay::terms_n, NS = Lay::terms_s, NG = Lay::terms, kPlane = Lay::plane;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
     float* gates = reinterpret_cast<float*>(smem + 2 * Lay::values);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const long long slot = blockIdx.x, place = slot * s.heads + blockIdx.y;
     const int h = blockIdx.y, d_block = 64 * blockIdx.z, tiles_e = (s.E + 15) / 16;
-    const int padded_d = s.D > 64 ? 8 : 4;                   // the chain's 16-value pieces of a column
+    const int padded_d = s.D > 64 ? 16 : 8;                  // the chain's 8-value pieces of a column
     const Slot c = ticks_of(s, slot);
     if (c.n == 0) return;
     const long long tick = (s.offsets ? span_of(s, c.b).start : 0) + c.first;
@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
         }
     }
 
+    __syncthreads();                                          // the gates are there
     float dq[4][4] = {}, dk[4][4] = {}, du[4][4] = {}, dp[4][4] = {}, dd[4][4] = {};
     const uint32_t at_m = smem_at(tiles) + at_rows_m(lane, kSquare), at_n = smem_at(tiles) + at_rows_n(lane, kSquare);
     const bool below = 32 * wd <= 16 * wt;                   // this warp's ticks s x t meet the diagonal's lower side
@@ -81,86 +82,89 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
         if (e0) __syncthreads();
         load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::go, row_of<const T>(s, s.go, c.b, h, tick) + e0, s.go.tick, c.n, s.E - e0, s.go.fast, tid);
         if (s.dn_f32)
-            load_tile<float, NK, 64, kSquare, 256>(tiles + Lay::dn, row_of<const float>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0,
+            load_tile<float, NN, 64, kSquare, 256>(tiles + Lay::dn, row_of<const float>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0,
                                                    s.dn.fast, tid);
         else if constexpr (sizeof(T) == 2)
-            load_tile<T, NK, 64, kSquare, 256>(tiles + Lay::dn, row_of<const T>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast,
+            load_tile<T, NN, 64, kSquare, 256>(tiles + Lay::dn, row_of<const T>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast,
                                                tid);
-        using U = std::conditional_t<NI == 1, bf16, float>;
-        load_tile<U, NK, 64, kSquare, 256>(tiles + Lay::u, reinterpret_cast<const U*>(s.u) + place * kTicks * 16 * tiles_e + e0, 16 * tiles_e,
-                                           kTicks, 16 * tiles_e - e0, true, tid);
         async_commit();
-        // S and R: left operands of 16 columns x 16 values -> rows of columns
+        if (e0 + 64 < s.E) {                                  // the next columns on their way to L2
+            const int e = e0 / 16 + 4 + (warp >> 1);
+            if (e < tiles_e) {
+                prefetch(reinterpret_cast<const char*>((warp & 1 ? s.gstates : s.states) + ((place * tiles_e + e) * padded_d + d_block / 8) * 32) + lane * 128);
+                if (lane < 16) prefetch(reinterpret_cast<const char*>(s.w + ((2 * place + (warp & 1)) * tiles_e + e) * 4 * 32) + lane * 128);
+            }
+            const int row = tid & 63;
+            if (tid < 64 && row < c.n) prefetch(reinterpret_cast<const char*>(row_of<const T>(s, s.go, c.b, h, tick + row) + e0 + 64));
+            else if (tid < 128 && tid >= 64 && row < c.n)
+                prefetch(s.dn_f32 ? reinterpret_cast<const char*>(row_of<const float>(s, s.dn, c.b, h, tick + row) + e0 + 64)
+                                  : reinterpret_cast<const char*>(row_of<const T>(s, s.dn, c.b, h, tick + row) + e0 + 64));
+        }
+        // S and R, accumulators of 16 columns x 8 values -> terms in rows of columns; a warp: 16 columns of one of them
         {
-            // warp: columns 16 (warp / 2).., of S or R
-            const int which = warp & 1, te = warp >> 1, e = e0 / 16 + te, kept = which ? NK : NB;
-            const uint4* from = (which ? s.gstates : s.states) + (((place * tiles_e + e) * kept) * padded_d + d_block / 16) * 32 + lane;
+            const int which = warp & 1, te = warp >> 1, e = e0 / 16 + te;
+            const float4* from = (which ? s.gstates : s.states) + ((place * tiles_e + e) * padded_d + d_block / 8) * 32 + lane;
             const uint32_t to = smem_at(tiles) + 2 * ((which ? Lay::r : Lay::s) + 16 * te * kSquare) + at_rows_m(lane, kSquare);
-            uint4 u[NK][4];
+            float4 v[8];
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
+            for (int j = 0; j < 8; ++j) v[j] = e < tiles_e ? __ldg(from + j * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int td = 0; td < 4; ++td) {
-                    u[n][td] = make_uint4(0, 0, 0, 0);
-                    if (e < tiles_e) u[n][td] = __ldg(from + (n * padded_d + td) * 32);
-                }
+            for (int j = 0; j < 4; ++j) {
+                uint32_t a[NS][4];
+                const float x[2][4] = {{v[2 * j].x, v[2 * j].y, v[2 * j].z, v[2 * j].w}, {v[2 * j + 1].x, v[2 * j + 1].y, v[2 * j + 1].z, v[2 * j + 1].w}};
+                left<NS>(x[0], x[1], a);
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int td = 0; td < 4; ++td)
-                    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to + 2 * (n * kPlane + 16 * td)),
-                                 "r"(u[n][td].x), "r"(u[n][td].y), "r"(u[n][td].z), "r"(u[n][td].w)
+                for (int n = 0; n < NS; ++n)
+                    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to + 2 * (n * kPlane + 16 * j)), "r"(a[n][0]),
+                                 "r"(a[n][1]), "r"(a[n][2]), "r"(a[n][3])
                                  : "memory");
+            }
+        }
+        // U = B W; a warp: 16 columns of one chunk (without ticks: zeros)
+        {
+            const int te = warp >> 1, half = warp & 1, e = e0 / 16 + te;
+            const bool there = e < tiles_e && (half == 0 || c.n > kChunk);
+            const float4* from = s.w + ((2 * place + half) * tiles_e + e) * 4 * 32 + lane;
+            const uint32_t to = smem_at(tiles) + 2 * (Lay::u + 32 * half * kSquare + 16 * te) + at_rows_n(lane, kSquare);
+            float4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = there ? __ldg(from + j * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x[2][4] = {{v[2 * j].x, v[2 * j].y, v[2 * j].z, v[2 * j].w}, {v[2 * j + 1].x, v[2 * j + 1].y, v[2 * j + 1].z, v[2 * j + 1].w}};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) scale2(x[i], gate2(gates + 2 * kTicks + 32 * half, 2 * j + i, lane));
+                uint32_t a[NG][4];
+                left<NG>(x[0], x[1], a);
+#pragma unroll
+                for (int n = 0; n < NG; ++n) stsm_t(to + 2 * (n * kPlane + 16 * j * kSquare), a[n]);
+            }
         }
         async_wait<0>();
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            uint32_t go[NI][4], dn[NK][4], u[NK][4];
+            uint32_t go[NI][4], dn[NN][4], u[NG][4];
 #pragma unroll
             for (int n = 0; n < NI; ++n) ldsm(go[n], at_m + 2 * (Lay::go + n * kPlane + 16 * wt * kSquare + 16 * e));
 #pragma unroll
-            for (int n = 0; n < NK; ++n) {
-                ldsm(dn[n], at_m + 2 * (Lay::dn + n * kPlane + 16 * wt * kSquare + 16 * e));
+            for (int n = 0; n < NN; ++n) ldsm(dn[n], at_m + 2 * (Lay::dn + n * kPlane + 16 * wt * kSquare + 16 * e));
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
                 ldsm(u[n], at_m + 2 * (Lay::u + n * kPlane + 16 * wt * kSquare + 16 * e));
             }
-#pragma unroll
-            for (int jp = 0; jp < 2; ++jp)
-#pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    uint32_t b[4];
-                    ldsm_t(b, at_m + 2 * (Lay::s + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * jp));
-#pragma unroll
-                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
-                        if (t < NI) {
-                            mma(dq[2 * jp], go[t < NI ? t : 0], b[0], b[1]);
-                            mma(dq[2 * jp + 1], go[t < NI ? t : 0], b[2], b[3]);
-                        }
-                        mma(dk[2 * jp], dn[t], b[0], b[1]);
-                        mma(dk[2 * jp + 1], dn[t], b[2], b[3]);
-                    }
-                    ldsm_t(b, at_m + 2 * (Lay::r + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * jp));
-#pragma unroll
-                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
-                        mma(du[2 * jp], u[t], b[0], b[1]);
-                        mma(du[2 * jp + 1], u[t], b[2], b[3]);
-                    }
-                    if (below) {
-                        ldsm(b, at_n + 2 * (Lay::u + j * kPlane + (32 * wd + 16 * jp) * kSquare + 16 * e));
-#pragma unroll
-                        for (int t = 0; t < NK && t + j < kKeep; ++t) {
-                            if (t < NI) {
-                                mma(dp[2 * jp], go[t < NI ? t : 0], b[0], b[1]);
-                                mma(dp[2 * jp + 1], go[t < NI ? t : 0], b[2], b[3]);
-                            }
-                            mma(dd[2 * jp], dn[t], b[0], b[1]);
-                            mma(dd[2 * jp + 1], dn[t], b[2], b[3]);
-                        }
-                    }
-                }
+            const auto state = [&](int j, int p) { return at_m + 2 * (Lay::s + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * p); };
+            products<NI, NS, NG, 2, true>(dq, go, state);
+            products<NN, NS, NG, 2, true>(dk, dn, state);
+            products<NG, NS, NG, 2, true>(du, u, [&](int j, int p) { return at_m + 2 * (Lay::r + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * p); });
+            if (below) {
+                const auto at = [&](int j, int p) { return at_n + 2 * (Lay::u + j * kPlane + (32 * wd + 16 * p) * kSquare + 16 * e); };
+                products<NI, NG, NG, 2, false>(dp, go, at);
+                products<NN, NG, NG, 2, false>(dd, dn, at);
+            }
         }
     }
-    __syncthreads();                                          // dO, dN and U have been read
+    __syncthreads();                                          // dO, dN, U, S and R have been read
     const float *gh = gates + 3 * kTicks, *gl = gates + 4 * kTicks;
     if (below) {
 #pragma unroll
@@ -175,11 +179,11 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                     x[e] = t >= c0 + e ? dp[j][2 * i + e] * (f * s.scale) : 0.f;
                     y[e] = t > c0 + e ? -dd[j][2 * i + e] * f : 0.f;
                 }
-                uint32_t a[NK], b[NK];
-                terms<NK>(x[0], x[1], a);
-                terms<NK>(y[0], y[1], b);
+                uint32_t a[NG], b[NG];
+                terms<NG>(x[0], x[1], a);
+                terms<NG>(y[0], y[1], b);
 #pragma unroll
-                for (int n = 0; n < NK; ++n) {
+                for (int n = 0; n < NG; ++n) {
                     *reinterpret_cast<uint32_t*>(tiles + Lay::dp + n * kPlane + t * kSquare + c0) = a[n];
                     *reinterpret_cast<uint32_t*>(tiles + Lay::d + n * kPlane + t * kSquare + c0) = b[n];
                 }
@@ -201,54 +205,29 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     // rows of dP and D by K; columns of dP by Q, of D by K
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        uint32_t a[NK][4], b[NK][4], kk[NI][2][4], qq[NI][2][4];
-        const bool row = k <= wt, column = k >= wt;
+        uint32_t a[NG][4], b[NG][4];
+        const auto keys = [&](int j, int p) { return at_m + 2 * (Lay::k + j * kPlane + 16 * k * kSquare + 32 * wd + 16 * p); };
+        if (k <= wt) {
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
-#pragma unroll
-            for (int jp = 0; jp < 2; ++jp) {
-                ldsm_t(kk[n][jp], at_m + 2 * (Lay::k + n * kPlane + 16 * k * kSquare + 32 * wd + 16 * jp));
-                if (column) ldsm_t(qq[n][jp], at_m + 2 * (Lay::q + n * kPlane + 16 * k * kSquare + 32 * wd + 16 * jp));
-            }
-        if (row) {
-#pragma unroll
-            for (int n = 0; n < NK; ++n) {
+            for (int n = 0; n < NG; ++n) {
                 ldsm(a[n], at_m + 2 * (Lay::dp + n * kPlane + 16 * wt * kSquare + 16 * k));
                 ldsm(b[n], at_m + 2 * (Lay::d + n * kPlane + 16 * wt * kSquare + 16 * k));
             }
-#pragma unroll
-            for (int jp = 0; jp < 2; ++jp)
-#pragma unroll
-                for (int j = 0; j < NI; ++j)
-#pragma unroll
-                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
-                        mma(dq[2 * jp], a[t], kk[j][jp][0], kk[j][jp][1]);
-                        mma(dq[2 * jp + 1], a[t], kk[j][jp][2], kk[j][jp][3]);
-                        mma(dk[2 * jp], b[t], kk[j][jp][0], kk[j][jp][1]);
-                        mma(dk[2 * jp + 1], b[t], kk[j][jp][2], kk[j][jp][3]);
-                    }
+            products<NG, NI, NG, 2, true>(dq, a, keys);
+            products<NG, NI, NG, 2, true>(dk, b, keys);
         }
-        if (column) {
+        if (k >= wt) {
 #pragma unroll
-            for (int n = 0; n < NK; ++n) {
+            for (int n = 0; n < NG; ++n) {
                 ldsm_t(a[n], at_n + 2 * (Lay::dp + n * kPlane + 16 * k * kSquare + 16 * wt));
                 ldsm_t(b[n], at_n + 2 * (Lay::d + n * kPlane + 16 * k * kSquare + 16 * wt));
             }
-#pragma unroll
-            for (int jp = 0; jp < 2; ++jp)
-#pragma unroll
-                for (int j = 0; j < NI; ++j)
-#pragma unroll
-                    for (int t = 0; t < NK && t + j < kKeep; ++t) {
-                        mma(dk[2 * jp], a[t], qq[j][jp][0], qq[j][jp][1]);
-                        mma(dk[2 * jp + 1], a[t], qq[j][jp][2], qq[j][jp][3]);
-                        mma(dk[2 * jp], b[t], kk[j][jp][0], kk[j][jp][1]);
-                        mma(dk[2 * jp + 1], b[t], kk[j][jp][2], kk[j][jp][3]);
-                    }
+            products<NG, NI, NG, 2, true>(dk, a, [&](int j, int p) { return at_m + 2 * (Lay::q + j * kPlane + 16 * k * kSquare + 32 * wd + 16 * p); });
+            products<NG, NI, NG, 2, true>(dk, b, keys);
         }
     }
     // by way of shared memory (over S and R), so that a row leaves in whole sectors
-    float* stage = reinterpret_cast<float*>(tiles + Lay::s);
+    float* stage = reinterpret_cast<float*>(tiles + Lay::out);
     constexpr int kRow = 68;
     const auto put = [&](const Operand& o, int f32, const float (&x)[4][4]) {
 #pragma unroll
