@@ -24,7 +24,7 @@ from torch import nn
 from torch.autograd.graph import increment_version
 
 from . import layers, memory
-from .memory import TYPES, _call, _float32, _grad, _kept, _no_tangents, _NONE, _offsets, _once, _ptr, _room, _state, _ticks, _values
+from .memory import TYPES, _call, _float32, _grad, _kept, _no_tangents, _offsets, _once, _ptr, _room, _state, _ticks, _values
 from .native import FlyguyError, lib
 
 # fg_delta_args: q, k, v, o, go, gq, gk, gv, log_decay, beta, glog_decay, gbeta (fg_ticks), state, state_out, gstate_out, gstate, offsets,
@@ -33,6 +33,7 @@ _DELTA = struct.Struct("=48q5q9qd2q")
 # fg_delta_step_args: q, k, v, o, log_decay, beta (fg_ticks), state, slots, n_slots, batch, heads, query_heads, key_heads, value_heads, dim,
 # value_dim, type, scale
 _STEP = struct.Struct("=24q11qd")
+_STEP_HEAD, _DOUBLE = struct.Struct("=26q"), struct.Struct("=d")
 
 
 def _gate(name: str, t, lead: tuple, like: torch.Tensor) -> torch.Tensor:
@@ -48,10 +49,11 @@ def _head_counts(q, k, v, log_decay, beta) -> tuple[int, int, int, int]:
     heads = log_decay.shape[-1]
     if beta.shape != log_decay.shape:
         raise FlyguyError(f"beta must be {tuple(log_decay.shape)} as log_decay is, not {tuple(beta.shape)}")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not t.shape[-2] or not heads or heads % t.shape[-2]:
-            raise FlyguyError(f"{heads} heads (of the gates) cannot share {t.shape[-2]} heads of {name}")
-    return heads, q.shape[-2], k.shape[-2], v.shape[-2]
+    counts = q.shape[-2], k.shape[-2], v.shape[-2]
+    for name, n in zip("qkv", counts):
+        if not n or not heads or heads % n:
+            raise FlyguyError(f"{heads} heads (of the gates) cannot share {n} heads of {name}")
+    return heads, *counts
 
 
 def _gate_ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
@@ -61,34 +63,46 @@ def _gate_ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
 
 
 @lru_cache(maxsize=256)
-def _delta_room(sizes: tuple, packed: bool, backward: bool) -> int:
-    """Bytes of workspace that a call of these sizes needs (fg_delta_work)."""
-    size = lib().fg_delta_work(_DELTA.pack(*(0,) * 52, int(packed), *sizes, 1.0, 0, 0), int(backward))
-    if size < 0:                                          # (raised here: an error is not kept)
-        raise FlyguyError(lib().fg_mem_last_error().decode())
-    return size
+def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tuple, bytes, int, int]:
+    """Of a call of these shapes and this type: the states' and o's shape, its fields from batch to type, and the bytes of workspace
+    that it and its gradients need (fg_delta_work). recordings: None, or how many the offsets name."""
+    lead, dim, value_dim = q[:-2], q[-1], v[-1]
+    if recordings is None:
+        batch, ticks = lead if len(lead) == 2 else (1, lead[0])
+    else:
+        batch, ticks = recordings, lead[0]
+    heads = log_decay[-1]
+    sizes = (batch, ticks, heads, q[-2], k[-2], v[-2], dim, value_dim, TYPES[typ])
+    rooms = []
+    for backward in (0, 1):
+        rooms.append(lib().fg_delta_work(_DELTA.pack(*(0,) * 52, int(recordings is not None), *sizes, 1.0, 0, 0), backward))
+        if rooms[-1] < 0:                                 # (raised here: an error is not kept)
+            raise FlyguyError(lib().fg_mem_last_error().decode())
+    return (batch, heads, dim, value_dim), (*lead, heads, value_dim), struct.pack("=9q", *sizes), *rooms
+
+
+_NOTHING = bytes(32)                                      # an fg_ticks of NULL
+_TICKS, _POINTERS, _END = struct.Struct("=4q"), struct.Struct("=5q"), struct.Struct("=d2q")
 
 
 class _Delta:
     """What forward and backward of one call share."""
 
     def __init__(self, q, k, v, log_decay, beta, state, scale, offsets):
-        lead, dim, value_dim = q.shape[:-2], q.shape[-1], v.shape[-1]
+        lead, dim = q.shape[:-2], q.shape[-1]
         if k.shape[:-2] != lead or k.shape[-1] != dim or v.shape[:-2] != lead:
             raise FlyguyError(f"k and v must be {(*lead, 'key heads', dim)} and {(*lead, 'value heads', 'value dim')}, not "
                               f"{tuple(k.shape)} and {tuple(v.shape)}")
-        if offsets is None:
-            batch, ticks = lead if len(lead) == 2 else (1, lead[0])
-        else:
+        if offsets is not None:
             if len(lead) != 1:
                 raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
             offsets = _offsets(offsets, q)
-            batch, ticks = offsets.shape[0] - 1, lead[0]
-        heads = _head_counts(q, k, v, log_decay, beta)
-        self.states, self.device, self.offsets = (batch, heads[0], dim, value_dim), q.get_device(), offsets
+        _head_counts(q, k, v, log_decay, beta)
+        self.device, self.offsets = q.get_device(), offsets
+        self.states, self.o_shape, self.sizes, self.room, self.room_back = _delta_sizes(
+            q.shape, k.shape, v.shape, log_decay.shape, beta.shape, q.dtype, None if offsets is None else offsets.shape[0] - 1)
         if state is not None:
             _float32("state", state, q, self.states)
-        self.sizes = (batch, ticks, *heads, dim, value_dim, TYPES[q.dtype])
         self.scale = float(dim ** -0.5 if scale is None else scale)
 
     def let_go(self) -> torch.Tensor | None:
@@ -101,26 +115,29 @@ class _Delta:
         again.__dict__.update(self.__dict__, offsets=offsets)
         return again
 
-    def run(self, fn, backward: bool, tensors, gates, state=None, state_out=None, gstate_out=None, gstate=None) -> None:
-        room, work = _room(_delta_room(self.sizes, self.offsets is not None, backward), tensors[0].device)
-        packed = _DELTA.pack(*(f for t in tensors for f in (_NONE if t is None else _ticks(t))),
-                             *(f for t in gates for f in (_NONE if t is None else _gate_ticks(t))), _ptr(state), _ptr(state_out),
-                             _ptr(gstate_out), _ptr(gstate), _ptr(self.offsets), *self.sizes, self.scale, *work)
-        _call(fn, packed, self.device)
+    def run(self, fn, size: int, ticks: bytes, device, state=0, state_out=0, gstate_out=0, gstate=0) -> None:
+        room, work = _room(size, device)
+        _call(fn, ticks + _POINTERS.pack(state, state_out, gstate_out, gstate, _ptr(self.offsets)) + self.sizes + _END.pack(self.scale, *work),
+              self.device)
 
     def forward(self, q, k, v, log_decay, beta, state):
-        o = torch.empty((*q.shape[:-2], self.states[1], v.shape[-1]), dtype=q.dtype, device=q.device)
-        end = torch.empty(self.states, dtype=torch.float32, device=q.device)
-        self.run(lib().fg_delta_attn, False, (q, k, v, o, None, None, None, None), (log_decay, beta, None, None), state, end)
+        o = q.new_empty(self.o_shape)
+        end = log_decay.new_empty(self.states)
+        pack = _TICKS.pack
+        ticks = (pack(*_ticks(q)) + pack(*_ticks(k)) + pack(*_ticks(v)) + pack(*_ticks(o)) + 4 * _NOTHING + pack(*_gate_ticks(log_decay))
+                 + pack(*_gate_ticks(beta)) + 2 * _NOTHING)
+        self.run(lib().fg_delta_attn, self.room, ticks, q.device, _ptr(state), end.data_ptr())
         return o, end
 
     def backward(self, q, k, v, log_decay, beta, state, go, gend, want_state: bool):
-        go = _grad("the gradient of o", go, q, (*q.shape[:-2], self.states[1], v.shape[-1]))
+        go = _grad("the gradient of o", go, q, self.o_shape)
         if gend is not None:
             gend = _state(gend.float())
         gq, gk, gv, gl, gb = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, log_decay, beta))
         gstate = torch.empty(self.states, dtype=torch.float32, device=q.device) if want_state else None
-        self.run(lib().fg_delta_attn_bwd, True, (q, k, v, None, go, gq, gk, gv), (log_decay, beta, gl, gb), state, None, gend, gstate)
+        ticks = b"".join([_TICKS.pack(*_ticks(t)) for t in (q, k, v)] + [_NOTHING] + [_TICKS.pack(*_ticks(t)) for t in (go, gq, gk, gv)]
+                         + [_TICKS.pack(*_gate_ticks(t)) for t in (log_decay, beta, gl, gb)])
+        self.run(lib().fg_delta_attn_bwd, self.room_back, ticks, q.device, _ptr(state), 0, _ptr(gend), _ptr(gstate))
         return gq, gk, gv, gl, gb, gstate
 
 
@@ -162,16 +179,28 @@ def delta_attention(q, k, v, log_decay, beta, state=None, scale: float | None = 
     log_decay, beta = _gate("log_decay", log_decay, q.shape[:-2], q), _gate("beta", beta, q.shape[:-2], q)
     job = _Delta(q, k, v, log_decay, beta, state, scale, offsets)
     _no_tangents(q, k, v, log_decay, beta, state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or beta.requires_grad
+                                    or (state is not None and state.requires_grad)):
         return _DeltaFn.apply(q, k, v, log_decay, beta, state, job)
     return job.forward(q, k, v, log_decay, beta, _state(state))
 
 
-def delta_step(q, k, v, log_decay, beta, state, scale: float | None = None, slots=None) -> torch.Tensor:
-    """One tick of delta_attention for a batch: q [batch, query heads, dim], k [batch, key heads, dim], v [batch, value heads, value
-    dim], log_decay and beta float32 [batch, heads]. state float32 [slots, heads, dim, value dim], contiguous, is updated in place
-    at each row's slot (slots int64 [batch], no two alike; None: row b's is b); a row whose slot is outside answers 0 and changes
-    nothing. dim and value dim at most 256. Returns o [batch, heads, value dim]. No gradient: for learning, delta_attention."""
+@lru_cache(maxsize=256)
+def _step_sizes(q, k, v, log_decay, beta, state, *types) -> tuple[tuple, bytes]:
+    """(batch, heads, value dim) of a step of these shapes and types, and its fields from n_slots to type; an error without words."""
+    *types, own_slots = types
+    if not (len(q) == len(k) == len(v) == 3 and len(log_decay) == 2 and log_decay == beta and len(state) == 4 and types[0] in TYPES
+            and types[0] is types[1] is types[2] and types[3:] == [torch.float32] * 3):
+        raise FlyguyError
+    (batch, heads), (slots, *of_state), dim, value_dim = log_decay, state, q[2], v[2]
+    if not (q[0] == k[0] == v[0] == batch and k[2] == dim and of_state == [heads, dim, value_dim] and heads and q[1] and k[1] and v[1]
+            and not heads % q[1] and not heads % k[1] and not heads % v[1] and (slots >= batch or not own_slots)):
+        raise FlyguyError
+    return (batch, heads, value_dim), struct.pack("=9q", slots, batch, heads, q[1], k[1], v[1], dim, value_dim, TYPES[types[0]])
+
+
+def _step_inputs(q, k, v, log_decay, beta, state, slots) -> tuple:
+    """The inputs as the library takes them, or what is wrong with them."""
     q, k, v = _values("q", q, (3,)), _values("k", k, (3,), q), _values("v", v, (3,), q)
     batch, _, dim = q.shape
     value_dim = v.shape[-1]
@@ -183,25 +212,43 @@ def delta_step(q, k, v, log_decay, beta, state, scale: float | None = None, slot
     if (not isinstance(state, torch.Tensor) or state.dtype is not torch.float32 or state.get_device() != q.get_device()
             or state.dim() != 4 or state.shape[1:] != (heads[0], dim, value_dim) or not state.is_contiguous()):
         raise FlyguyError(f"state must be contiguous float32 {('slots', heads[0], dim, value_dim)} on {q.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, beta, state)):
+    if slots is None and state.shape[0] < batch:
+        raise FlyguyError(f"{batch} rows need as many states, not {state.shape[0]}")
+    return q, k, v, log_decay, beta
+
+
+def delta_step(q, k, v, log_decay, beta, state, scale: float | None = None, slots=None) -> torch.Tensor:
+    """One tick of delta_attention for a batch: q [batch, query heads, dim], k [batch, key heads, dim], v [batch, value heads, value
+    dim], log_decay and beta float32 [batch, heads]. state float32 [slots, heads, dim, value dim], contiguous, is updated in place
+    at each row's slot (slots int64 [batch], no two alike; None: row b's is b); a row whose slot is outside answers 0 and changes
+    nothing. dim and value dim at most 256. Returns o [batch, heads, value dim]. No gradient: for learning, delta_attention."""
+    try:                                                  # (what most calls are, by the sizes alone)
+        sizes, tail = _step_sizes(q.shape, k.shape, v.shape, log_decay.shape, beta.shape, state.shape, q.dtype, k.dtype, v.dtype,
+                                  log_decay.dtype, beta.dtype, state.dtype, slots is None)
+        at, device = [x.stride() for x in (q, k, v)], q.get_device()
+        if not (at[0][2] == at[1][2] == at[2][2] == 1 and state.is_contiguous() and device >= 0
+                and k.get_device() == v.get_device() == log_decay.get_device() == beta.get_device() == state.get_device() == device):
+            raise FlyguyError
+    except (AttributeError, FlyguyError):
+        q, k, v, log_decay, beta = _step_inputs(q, k, v, log_decay, beta, state, slots)
+        sizes, tail = _step_sizes(q.shape, k.shape, v.shape, log_decay.shape, beta.shape, state.shape, q.dtype, k.dtype, v.dtype,
+                                  log_decay.dtype, beta.dtype, state.dtype, slots is None)
+        at, device = [x.stride() for x in (q, k, v)], q.get_device()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or beta.requires_grad
+                                    or state.requires_grad):
         raise FlyguyError("delta_step has no gradient (delta_attention has): call it under torch.no_grad()")
     _no_tangents(q, k, v, log_decay, beta, state)
     if slots is not None:
-        if (not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.get_device() != q.get_device()
-                or slots.shape != (batch,)):
-            raise FlyguyError(f"slots must be int64 [{batch}] on {q.device}")
+        if not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.get_device() != device or slots.shape != sizes[:1]:
+            raise FlyguyError(f"slots must be int64 [{sizes[0]}] on {q.device}")
         if not slots.is_contiguous():
             slots = slots.contiguous()
-    elif state.shape[0] < batch:
-        raise FlyguyError(f"{batch} rows need as many states, not {state.shape[0]}")
-    o = torch.empty((batch, heads[0], value_dim), dtype=q.dtype, device=q.device)
-    f = []
-    for t in (q, k, v, o, log_decay, beta):
-        st = t.stride()
-        f += (t.data_ptr(), st[0], 0, st[1])
-    packed = _STEP.pack(*f, state.data_ptr(), _ptr(slots), state.shape[0], batch, *heads, dim, value_dim, TYPES[q.dtype],
-                        float(dim ** -0.5 if scale is None else scale))
-    _call(lib().fg_delta_step, packed, q.get_device())
+    o = q.new_empty(sizes)
+    (qb, qh, _), (kb, kh, _), (vb, vh, _), (lb, lh), (bb, bh) = *at, log_decay.stride(), beta.stride()
+    packed = _STEP_HEAD.pack(q.data_ptr(), qb, 0, qh, k.data_ptr(), kb, 0, kh, v.data_ptr(), vb, 0, vh, o.data_ptr(), sizes[1] * sizes[2], 0,
+                             sizes[2], log_decay.data_ptr(), lb, 0, lh, beta.data_ptr(), bb, 0, bh, state.data_ptr(),
+                             0 if slots is None else slots.data_ptr())
+    _call(lib().fg_delta_step, packed + tail + _DOUBLE.pack(q.shape[2] ** -0.5 if scale is None else scale), device)
     increment_version(state)                              # (autograd sees that it has changed, should it have kept it)
     return o
 

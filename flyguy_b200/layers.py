@@ -35,9 +35,10 @@ def _tensor(name: str, t, like=None) -> torch.Tensor:
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """t as rows that lie at equal distances, and that distance in values; copied if they do not."""
-    dim, shape, stride = t.shape[-1], t.shape, t.stride()
+    dim = t.shape[-1]
     if t.is_contiguous():
         return t, dim
+    shape, stride = t.shape, t.stride()
     if (stride[-1] == 1 or dim == 1) and t.dim() > 1:
         step = stride[-2] if shape[-2] > 1 else None
         at, even = (step or 0) * shape[-2], True
@@ -57,7 +58,7 @@ class _Norm:
     """What forward and backward of one call share."""
 
     def __init__(self, x, eps):
-        self.dim, self.eps, self.type, self.device = x.shape[-1], float(eps), TYPES[x.dtype], x.get_device()
+        self.dim, self.eps, self.type, self.device = x.shape[-1], eps, TYPES[x.dtype], x.get_device()
         self.rows = x.numel() // self.dim if self.dim else 0
 
     def pack(self, x, y=0, gy=0, gx=0, w=None, b=None, gw=None, gb=None, x_row=0, gy_row=0, work=(0, 0)) -> bytes:
@@ -66,8 +67,9 @@ class _Norm:
 
     def forward(self, x, w, b):
         x, step = _rows(x)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _call(lib().fg_layer_norm, self.pack(x.data_ptr(), y.data_ptr(), w=w, b=b, x_row=step), self.device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        _call(lib().fg_layer_norm, _NORM.pack(x.data_ptr(), y.data_ptr(), 0, 0, _ptr(w), _ptr(b), 0, 0, self.rows, self.dim, step, 0, self.type,
+                                              self.eps, 0, 0), self.device)
         return y
 
     def backward(self, x, w, b, gy, want_w, want_b):
@@ -113,7 +115,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
         bias = _float32("bias", bias, x, x.shape[-1:])
     _no_tangents(x, weight, bias)
     job = _Norm(x, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _NormFn.apply(x, weight, bias, job)
     return job.forward(x, weight, bias)
 
@@ -130,7 +133,7 @@ class _Drop:
     def run(self, x, add=None):
         x = x.contiguous()
         add = None if add is None else add.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x)
         _call(lib().fg_dropout, _DROPOUT.pack(x.data_ptr(), _ptr(add), y.data_ptr(), _ptr(self.seed), self.value, self.call, x.numel(),
                                               self.least, TYPES[x.dtype]), self.device)
         return y
