@@ -511,7 +511,8 @@ void backward(Delta s, float* last, cudaStream_t st) {
     prepare<T, DP, Terms<T>::kept>(s, st);
     s.last = last;
     parts_forward<T, DP>(s, st);
-    // 64 or 128 columns of values a block; 16 warps an SM where 128 registers a thread do (the chain back, W = 4 and 8: 863 and 758 us)
+    // 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 777 and 917 us, as
+    // blocks of 4 warps with 168 registers 1,185 and 1,030)
     constexpr int wide = Terms<T>::in == 1 && DP == 128 ? 8 : 4;
     if (s.E > 64) chain<T, DP, wide, kKeep>(s, st);
     else chain<T, DP, 4, kKeep>(s, st);

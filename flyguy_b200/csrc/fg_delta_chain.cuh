@@ -61,7 +61,8 @@ struct Slot {
 };
 __device__ __forceinline__ Slot ticks_of(const Delta& s, long long slot) {
     if (!s.offsets) {
-        const long long per = (s.ticks + kTicks - 1) / kTicks, b = slot / per, first = (slot - b * per) * kTicks;
+        const uint32_t per = (uint32_t)((s.ticks + kTicks - 1) / kTicks), b = (uint32_t)slot / per;   // (slots are fewer than 2^31)
+        const long long first = (long long)((uint32_t)slot - b * per) * kTicks;
         return {b, first, (int)min((long long)kTicks, s.ticks - first)};
     }
     long long lo = 0, hi = s.batch - 1;                      // the last recording whose slots begin at or before this one
@@ -85,7 +86,7 @@ __device__ __forceinline__ Part part_of(const Delta& s, long long n, int part) {
 }
 template <class T>
 __device__ __forceinline__ T* row_of(const Delta& s, const Operand& o, long long b, int h, long long tick) {
-    return reinterpret_cast<T*>(o.p) + (s.offsets ? 0 : b * o.batch) + tick * o.tick + (h / o.share) * o.head;
+    return reinterpret_cast<T*>(o.p) + (s.offsets ? 0 : b * o.batch) + tick * o.tick + (uint32_t)h / (uint32_t)o.share * o.head;
 }
 __device__ __forceinline__ float* gate_of(const Delta& s, const Gate& o, long long b, int h, long long tick) {
     return o.p + (s.offsets ? 0 : b * o.batch) + tick * o.tick + h * o.head;
@@ -467,15 +468,15 @@ __device__ __forceinline__ void subtract(float (&x)[4], const float (&y)[4]) {
     for (int e = 0; e < 4; ++e) x[e] -= y[e];
 }
 
-// blocks of an SM at once: 16 warps with 128 registers a thread, 12 with 168
-template <int DP>
-constexpr int chain_blocks(int warps) { return warps == 8 ? 2 : (DP > 64 ? 12 : 16) / warps; }
+// Blocks of an SM at once: 16 warps with 128 registers a thread as blocks of 8 warps, 12 with 168 as blocks of 4 (at dim 64, 97,500 ticks, 8
+// heads: forward, with what is kept, and back 322, 478, 508 us; with 16 warps 346, 595, 557).
+constexpr int chain_blocks(int warps) { return warps == 8 ? 2 : 3; }
 
 // Forward. kKeep: nothing but what the way back needs is written (S before each slot, W, rows of o dO), and o is made to as many
 // terms as the corrections. kParts: what a part makes of a state of zeros, and (tiles past those of the columns) of the columns of 1.
 enum { kForward, kKeep, kParts };
 template <class T, int DP, int WARPS, int MODE>
-__global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<DP>(WARPS) : DP > 64 ? 2 : 3)
+__global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(WARPS) : DP > 64 ? 2 : 3)
     k_delta_chain(const __grid_constant__ Delta s) {
     constexpr bool KEEP = MODE == kKeep, PARTS = MODE == kParts;
     constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX, NO = KEEP ? NX : Terms<T>::out_s, NP = KEEP ? NX : Terms<T>::out_p;
@@ -668,7 +669,7 @@ __device__ __forceinline__ void prefetch(const char* p) { asm volatile("prefetch
 
 // Back. s.last is the state after the recording's last tick. PARTS: what a part leaves of a gradient of zeros, and nothing else.
 template <class T, int DP, int WARPS, bool PARTS>
-__global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks<DP>(WARPS) : DP > 64 ? 2 : 3)
+__global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(WARPS) : DP > 64 ? 2 : 3)
     k_delta_back(const __grid_constant__ Delta s) {
     constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX;
     using Lay = ChainLayout<T, DP, WARPS, NX, true>;

@@ -37,6 +37,8 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     const Slot c = ticks_of(s, slot);
     if (c.n == 0) return;
     const long long tick = (s.offsets ? span_of(s, c.b).start : 0) + c.first;
+    const T* go_rows = row_of<const T>(s, s.go, c.b, h, tick);
+    const char* dn_rows = s.dn.p + ((s.offsets ? 0 : c.b * s.dn.batch) + tick * s.dn.tick + h * s.dn.head) * (s.dn_f32 ? 4 : (int)sizeof(T));
     const int wt = warp >> 1, wd = warp & 1;                 // ticks 16 wt .., columns (of d, or ticks s) 32 wd ..
 
     load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::q, row_of<const T>(s, s.q, c.b, h, tick) + d_block, s.q.tick, c.n, s.D - d_block, s.q.fast, tid);
@@ -80,12 +82,12 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
 #pragma unroll 1
     for (int e0 = 0; e0 < s.E; e0 += 64) {
         if (e0) __syncthreads();
-        load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::go, row_of<const T>(s, s.go, c.b, h, tick) + e0, s.go.tick, c.n, s.E - e0, s.go.fast, tid);
+        load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::go, go_rows + e0, s.go.tick, c.n, s.E - e0, s.go.fast, tid);
         if (s.dn_f32)
-            load_tile<float, NN, 64, kSquare, 256>(tiles + Lay::dn, row_of<const float>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0,
+            load_tile<float, NN, 64, kSquare, 256>(tiles + Lay::dn, reinterpret_cast<const float*>(dn_rows) + e0, s.dn.tick, c.n, s.E - e0,
                                                    s.dn.fast, tid);
         else if constexpr (sizeof(T) == 2)
-            load_tile<T, NN, 64, kSquare, 256>(tiles + Lay::dn, row_of<const T>(s, s.dn, c.b, h, tick) + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast,
+            load_tile<T, NN, 64, kSquare, 256>(tiles + Lay::dn, reinterpret_cast<const T*>(dn_rows) + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast,
                                                tid);
         async_commit();
         if (e0 + 64 < s.E) {                                  // the next columns on their way to L2
@@ -94,11 +96,9 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                 prefetch(reinterpret_cast<const char*>((warp & 1 ? s.gstates : s.states) + ((place * tiles_e + e) * padded_d + d_block / 8) * 32) + lane * 128);
                 if (lane < 16) prefetch(reinterpret_cast<const char*>(s.w + ((2 * place + (warp & 1)) * tiles_e + e) * 4 * 32) + lane * 128);
             }
-            const int row = tid & 63;
-            if (tid < 64 && row < c.n) prefetch(reinterpret_cast<const char*>(row_of<const T>(s, s.go, c.b, h, tick + row) + e0 + 64));
-            else if (tid < 128 && tid >= 64 && row < c.n)
-                prefetch(s.dn_f32 ? reinterpret_cast<const char*>(row_of<const float>(s, s.dn, c.b, h, tick + row) + e0 + 64)
-                                  : reinterpret_cast<const char*>(row_of<const T>(s, s.dn, c.b, h, tick + row) + e0 + 64));
+            const int row = tid & 63, size = s.dn_f32 ? 4 : (int)sizeof(T);
+            if (tid < 128 && row < c.n)
+                prefetch(tid < 64 ? reinterpret_cast<const char*>(go_rows + row * s.go.tick + e0 + 64) : dn_rows + (row * s.dn.tick + e0 + 64) * size);
         }
         // S and R, accumulators of 16 columns x 8 values -> terms in rows of columns; a warp: 16 columns of one of them
         {
@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                 *reinterpret_cast<float2*>(stage + (16 * wt + g + 8 * i) * kRow + 32 * wd + 8 * j + 2 * t4) = make_float2(x[j][2 * i], x[j][2 * i + 1]);
         __syncthreads();
         const int r0 = tid >> 3, col = (tid & 7) * 8, d = d_block + col;
+        const long long at = (s.offsets ? 0 : c.b * o.batch) + tick * o.tick + h * o.head + d;   // (gradients of each head by itself)
         if (d < s.D) {
 #pragma unroll
             for (int r = r0; r < kTicks; r += 32) {
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                 *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stage + r * kRow + col);
                 *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(stage + r * kRow + col + 4);
                 if (f32) {
-                    float* to = row_of<float>(s, o, c.b, h, tick + r) + d;
+                    float* to = reinterpret_cast<float*>(o.p) + at + r * o.tick;
                     if (o.fast) {
                         reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
                         reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                         for (int j = 0; j < 8 && d + j < s.D; ++j) to[j] = v[j];
                     }
                 } else if constexpr (sizeof(T) == 2) {
-                    T* to = row_of<T>(s, o, c.b, h, tick + r) + d;
+                    T* to = reinterpret_cast<T*>(o.p) + at + r * o.tick;
                     T w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) w[j] = from_f<T>(v[j]);
