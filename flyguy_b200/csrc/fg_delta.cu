@@ -344,6 +344,9 @@ void check_heads(const std::string& who, long long heads, std::initializer_list<
     for (long long n : shared) ok = ok && n >= 1 && heads % n == 0;
     if (!ok) throw MemErr{who + ": heads must be a multiple of query_heads, key_heads and value_heads, 1 to 65535"};
 }
+long long slots_of(const fg_delta_args* g) {
+    return g->offsets ? g->ticks / kTicks + g->batch : g->batch * ((g->ticks + kTicks - 1) / kTicks);
+}
 void check_sizes(const fg_delta_args* g, const std::string& who) {
     if (!g) throw MemErr{who + ": no arguments"};
     if (g->batch < 0 || g->ticks < 0) throw MemErr{who + ": a negative size"};
@@ -351,10 +354,10 @@ void check_sizes(const fg_delta_args* g, const std::string& who) {
     if (g->dim < 1 || g->dim > kMaxDim || g->value_dim < 1 || g->value_dim > kMaxValue)
         throw MemErr{who + ": dim must be 1 to 128, value_dim 1 to 256"};
     if (g->type < FG_F32 || g->type > FG_F16) throw MemErr{who + ": unknown type"};
-    if (g->batch * g->heads > (1ll << 27) || g->ticks > (1ll << 36) || g->batch > (1ll << 27)) throw MemErr{who + ": too many recordings or ticks"};
-}
-long long slots_of(const fg_delta_args* g) {
-    return g->offsets ? g->ticks / kTicks + g->batch : g->batch * ((g->ticks + kTicks - 1) / kTicks);
+    // (each in turn, so that no product overflows)
+    const bool few = g->batch <= (1ll << 27) && g->ticks <= (1ll << 36) && g->batch * g->heads <= (1ll << 27) && slots_of(g) <= (1ll << 30) &&
+                     slots_of(g) * g->heads <= (1ll << 38);
+    if (!few) throw MemErr{who + ": too many recordings or ticks"};
 }
 long long all_ticks(const fg_delta_args* g) { return g->offsets ? g->ticks : g->batch * g->ticks; }
 
@@ -429,7 +432,6 @@ void check(const fg_delta_args* g, bool backward) {
     const long long bytes = lay_out(g, backward, s, wide);
     want(!bytes || (g->work && g->work_bytes >= bytes), "the workspace is too small");
     want(reinterpret_cast<uintptr_t>(g->work) % 16 == 0, "the workspace is not 16-byte aligned");
-    want(slots_of(g) < (1ll << 31) && g->batch * g->heads * ((g->value_dim + 31) / 32) < (1ll << 31), "too many recordings or ticks");
 }
 
 Delta delta_of(const fg_delta_args* g) {

@@ -149,7 +149,7 @@ class _DeltaFn(torch.autograd.Function):
         state = _state(state)
         out = job.forward(q, k, v, log_decay, beta, state)
         ctx.job = job
-        ctx.save_for_backward(q, k, v, log_decay, beta, state, job.let_go())
+        ctx.save_for_backward(*map(_kept, (q, k, v, log_decay, beta, state)), job.let_go())
         return out
 
     @staticmethod

@@ -9,6 +9,7 @@ are rounded to the type once."""
 from __future__ import annotations
 
 import struct
+from functools import lru_cache
 
 import torch
 
@@ -61,10 +62,6 @@ class _Norm:
         self.dim, self.eps, self.type, self.device = x.shape[-1], eps, TYPES[x.dtype], x.get_device()
         self.rows = x.numel() // self.dim if self.dim else 0
 
-    def pack(self, x, y=0, gy=0, gx=0, w=None, b=None, gw=None, gb=None, x_row=0, gy_row=0, work=(0, 0)) -> bytes:
-        return _NORM.pack(x, y, gy, gx, _ptr(w), _ptr(b), _ptr(gw), _ptr(gb), self.rows, self.dim, x_row, gy_row, self.type, self.eps,
-                          *work)
-
     def forward(self, x, w, b):
         x, step = _rows(x)
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -74,15 +71,24 @@ class _Norm:
 
     def backward(self, x, w, b, gy, want_w, want_b):
         (x, x_row), (gy, gy_row) = _rows(x), _rows(gy if gy.dtype is x.dtype else gy.to(x.dtype))
-        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        gx = torch.empty_like(x, memory_format=torch.contiguous_format)
         gw = torch.empty_like(w) if want_w else None
         gb = torch.empty_like(b) if want_b else None
-        a = dict(gy=gy.data_ptr(), gx=gx.data_ptr(), w=w, gw=gw, gb=gb, x_row=x_row, gy_row=gy_row)
         room, work = None, (0, 0)
         if want_w or want_b:
-            room, work = _room(lib().fg_layer_norm_work(self.pack(x.data_ptr(), **a)), x.device)
-        _call(lib().fg_layer_norm_bwd, self.pack(x.data_ptr(), **a, work=work), self.device)
+            room, work = _room(_norm_room(self.rows, self.dim), x.device)
+        _call(lib().fg_layer_norm_bwd, _NORM.pack(x.data_ptr(), 0, gy.data_ptr(), gx.data_ptr(), _ptr(w), 0, _ptr(gw), _ptr(gb), self.rows, self.dim,
+                                                  x_row, gy_row, self.type, self.eps, *work), self.device)
         return gx, gw, gb
+
+
+@lru_cache(maxsize=256)
+def _norm_room(rows: int, dim: int) -> int:
+    """Bytes of workspace for the sums of so many rows (fg_layer_norm_work; the same for all types)."""
+    size = lib().fg_layer_norm_work(_NORM.pack(0, 0, 0, 0, 0, 0, 1, 1, rows, dim, dim, dim, 0, 1.0, 0, 0))
+    if size < 0:                                          # (raised here: an error is not kept)
+        raise FlyguyError(lib().fg_mem_last_error().decode())
+    return size
 
 
 class _NormFn(torch.autograd.Function):
@@ -90,7 +96,7 @@ class _NormFn(torch.autograd.Function):
     def forward(ctx, x, w, b, job):
         y = job.forward(x, w, b)
         ctx.job = job
-        ctx.save_for_backward(x, w, b)
+        ctx.save_for_backward(_kept(x), _kept(w), _kept(b))
         return y
 
     @staticmethod

@@ -340,6 +340,30 @@ def test_only_some_learn(cuda):
         assert all(t.grad is None for m, t in leaves.items() if m != n)
 
 
+def test_inputs_made_in_inference_mode_stay_constants(cuda):
+    x, go, gs = _inputs(22, (1, 40), 1, 2, (2, 2, 2), 32, 32, torch.float32)
+    _, _, want = _run(x, go, gs)
+    with torch.inference_mode():
+        fixed = {n: t.cuda() for n, t in x.items()}
+    v = x["v"].cuda().requires_grad_()
+    o, end = delta.delta_attention(*(fixed | {"v": v}).values())
+    got, = torch.autograd.grad((o, end), v, (go.cuda(), gs.cuda()))
+    assert torch.equal(got, want["v"])
+
+
+def test_broadcast_gates_learn(cuda):
+    """One gate for all ticks and heads, expanded: its gradient is the sum."""
+    x, go, gs = _inputs(23, (2, 40), 2, 2, (2, 2, 2), 32, 32, torch.float32)
+    x["log_decay"][:], x["beta"][:] = -0.1, 0.3
+    _, _, want = _want(x, None, go, gs, 32 ** -0.5)
+    gate = torch.tensor([-0.1, 0.3], device=cuda, requires_grad=True)
+    c = {n: t.cuda() for n, t in x.items()}
+    o, end = delta.delta_attention(c["q"], c["k"], c["v"], gate[0].expand(2, 40, 2), gate[1].expand(2, 40, 2), c["state"])
+    got, = torch.autograd.grad((o, end), gate, (go.cuda(), gs.cuda()))
+    for g, n in zip(got, ("log_decay", "beta")):
+        assert abs(g.item() - want[n].sum().item()) <= 1e-5 * want[n].abs().sum().item()
+
+
 def test_one_output_alone_learns(cuda):
     """The gradient of o alone, and of the states alone."""
     x, go, gs = _inputs(19, (2, 40), 2, 2, (2, 2, 2), 32, 32, torch.float32)

@@ -144,6 +144,14 @@ def test_layer_norm_captured_on_another_stream(cuda):
         assert torch.equal(a, b)
 
 
+def test_layer_norm_of_inputs_made_in_inference_mode(cuda):
+    with torch.inference_mode():
+        x = torch.randn(5, 40, device=cuda)
+    w = torch.ones(40, device=cuda, requires_grad=True)
+    gw, = torch.autograd.grad(layers.layer_norm(x, w).sum(), w)
+    _near(gw, _norm(_np(x), 1.0, 0.0, 1e-5).sum(0), torch.float32, 5e-6)
+
+
 def test_layer_norm_refusals(cuda):
     x = torch.zeros(4, 8, device=cuda)
     for args, words in (((torch.zeros(4, 8),), "CUDA"), ((x.double(),), "float32, bfloat16"), ((x, torch.zeros(7, device=cuda)), "weight must be"),

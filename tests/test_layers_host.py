@@ -61,7 +61,8 @@ def test_no_arguments_are_an_error():
 
 @pytest.mark.parametrize("at, value, words", [
     (0, -1, "negative"), (1, -5, "negative"), (2, 0, "multiple"), (3, 3, "multiple"), (4, 0, "multiple"), (5, 8, "multiple"), (6, 0, "dim must be"),
-    (6, 129, "dim must be"), (7, 257, "value_dim 1 to 256"), (7, 0, "value_dim"), (8, 3, "unknown type"), (0, 1 << 40, "too many"), (1, 1 << 50, "too many")])
+    (6, 129, "dim must be"), (7, 257, "value_dim 1 to 256"), (7, 0, "value_dim"), (8, 3, "unknown type"), (0, 1 << 40, "too many"), (1, 1 << 50, "too many"),
+    (0, (1 << 63) - 1, "too many"), (1, (1 << 63) - 1, "too many"), (1, 1 << 36, "too many")])
 def test_refused_sizes(at, value, words):
     L = native.lib()
     sizes = (*GOOD[:at], value, *GOOD[at + 1:])
