@@ -375,7 +375,8 @@ struct Wide {
     float *q = nullptr, *k = nullptr, *v = nullptr, *last = nullptr;
 };
 // Parts of a recording (k_delta_join): as many as keep the blocks within one round of the SMs, of 512 ticks at least; four at least, or
-// the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: PARTS us in 27 parts, 5,230 in one.
+// the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: 1,300 us in 27 parts
+// (the parts' own 716, put together 78, then 503), as many chunks one after another 5,230.
 int parts_of(const fg_delta_args* g) {
     const long long rows = std::max<long long>(1, g->batch * g->heads), mean = g->offsets ? g->ticks / std::max<long long>(1, g->batch) : g->ticks;
     const long long parts = std::min<long long>(64, std::min(12 * kSms / (rows * ((g->value_dim + 15) / 16)), mean / 512));
@@ -389,6 +390,7 @@ long long lay_out(const fg_delta_args* g, bool backward, Delta& s, Wide& wide) {
     };
     const int kept = of([](auto t) { return t.kept; }), out = of([](auto t) { return t.out_p; });
     const long long places = slots_of(g) * g->heads, tiles = (g->value_dim + 15) / 16, padded = g->dim > 64 ? 128 : 64;
+    if (g->offsets) room.take(s.table, slots_of(g) * (long long)sizeof(Slot));
     room.take(s.x, places * kept * 2 * kChunk * kChunk * 2);
     room.take(s.p, places * (backward ? kept : out) * 2 * kChunk * kChunk * 2);
     room.take(s.gates, places * kGates * kTicks * 4);
@@ -466,6 +468,10 @@ void launch(K* kernel, dim3 grid, int threads, int bytes, OnEachDevice& here, cu
 template <class T, int DP, int NP>
 void prepare(const Delta& s, cudaStream_t st) {
     static OnEachDevice here;
+    if (s.offsets && s.slots) {
+        k_delta_slots<<<(unsigned)((s.slots + 127) / 128), 128, 0, st>>>(s);
+        MCK(cudaGetLastError());
+    }
     if (s.slots) launch(k_delta_prep<T, DP, NP>, dim3((unsigned)s.slots, s.heads), 128, PrepLayout<T, DP>::bytes, here, st, s);
 }
 // WARPS: 16 columns of values each

@@ -15,8 +15,13 @@
 // them for rows: N^T = V^T - S^T K^T, W^T = N^T - (N^T B) X^T, O^T = S^T Q^T + U^T P^T, S^T += U^T K. An accumulator is the next
 // product's left operand as it lies, so states, corrections and outputs never leave the registers, and warps meet only to have tiles of
 // K, Q, V, X, P loaded (mma.sync: 25% of the tensor cores' rate, but the chain from state to state has no trip through shared
-// memory or TMEM in it). Chunks of 32 ticks leave room for 16 warps an SM at dim 128; with 64 ticks, 8 warps, the products were the same
-// and waited twice as long on one another.
+// memory or TMEM in it). Chunks of 32 ticks need 16 registers an accumulator of a tick's row where 64 need 32, which leaves room for 12 to
+// 16 warps an SM instead of 8.
+//
+// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 497 us (298 products a warp and chunk, 273 us of the tensor cores' at 552
+// TFLOP/s of mma.sync), with what is kept 777, back 916. The tensor pipe is 55%, 50% and 40% busy, issue slots 40%, DRAM 14%, 27% and
+// 33%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S and W,
+// too. X, P and the gates take 94 and 102 us: some 1,700 instructions a warp, of them 100 products.
 #pragma once
 #include "fg_delta.cuh"
 
@@ -24,6 +29,10 @@ namespace {
 
 constexpr int kGates = 5;
 
+struct Slot {
+    long long tick;
+    int b, n;
+};
 struct Delta {
     Operand q, k, v, o, go;
     Operand gq, gk, dn;              // gradients of q, k and v (dN), in T or (gq_f32 ..) fp32
@@ -34,6 +43,7 @@ struct Delta {
     long long batch, ticks, slots;
     int heads, D, E, gq_f32, gk_f32, dn_f32;
     float scale;
+    Slot* table;                     // [slot], of recordings end to end
     bf16 *x, *p;                     // [slot][head][chunk][term][32][32]
     float* gates;                    // [slot][head][5][64]: e^G and e^{G_31 - G} of the chunks, beta, G of the slot as two floats
     float4 *states, *gstates;        // [slot][head][tile of 16 columns][DP / 8][32]: S before and R behind, transposed, as accumulators
@@ -55,16 +65,8 @@ __device__ __forceinline__ Span span_of(const Delta& s, long long b) {
 __device__ __forceinline__ long long slot_of(const Delta& s, long long b, long long start) {
     return s.offsets ? start / kTicks + b : b * ((s.ticks + kTicks - 1) / kTicks);
 }
-struct Slot {
-    long long b, first;              // recording, first tick (of the recording's)
-    int n;                           // ticks, 0: this slot is empty
-};
-__device__ __forceinline__ Slot ticks_of(const Delta& s, long long slot) {
-    if (!s.offsets) {
-        const uint32_t per = (uint32_t)((s.ticks + kTicks - 1) / kTicks), b = (uint32_t)slot / per;   // (slots are fewer than 2^31)
-        const long long first = (long long)((uint32_t)slot - b * per) * kTicks;
-        return {b, first, (int)min((long long)kTicks, s.ticks - first)};
-    }
+// What a slot holds: n ticks of recording b from `tick` on (of the buffer's, where recordings lie end to end); n = 0: nothing.
+__device__ __forceinline__ Slot find_slot(const Delta& s, long long slot) {
     long long lo = 0, hi = s.batch - 1;                      // the last recording whose slots begin at or before this one
     while (lo < hi) {
         const long long mid = (lo + hi + 1) / 2;
@@ -73,7 +75,19 @@ __device__ __forceinline__ Slot ticks_of(const Delta& s, long long slot) {
     }
     const Span sp = span_of(s, lo);
     const long long first = (slot - slot_of(s, lo, sp.start)) * kTicks;
-    return {lo, first, first < 0 ? 0 : (int)max(0ll, min((long long)kTicks, sp.n - first))};
+    return {sp.start + first, (int)lo, first < 0 ? 0 : (int)max(0ll, min((long long)kTicks, sp.n - first))};
+}
+// of packed recordings, once for all blocks that ask (a search is some 8 loads that wait for one another: 97,500 ticks of 130 recordings, 8
+// heads, X and P and the gradients of q and k took 908 us with one in each block, now 816)
+__global__ void __launch_bounds__(128) k_delta_slots(const __grid_constant__ Delta s) {
+    const long long slot = blockIdx.x * 128ll + threadIdx.x;
+    if (slot < s.slots) s.table[slot] = find_slot(s, slot);
+}
+__device__ __forceinline__ Slot ticks_of(const Delta& s, long long slot) {
+    if (s.offsets) return s.table[slot];
+    const uint32_t per = (uint32_t)((s.ticks + kTicks - 1) / kTicks), b = (uint32_t)slot / per;   // (slots are fewer than 2^31)
+    const long long first = (long long)((uint32_t)slot - b * per) * kTicks;
+    return {first, (int)b, (int)min((long long)kTicks, s.ticks - first)};
 }
 // the chunks of a part: whole slots, as many in each but the last ones
 struct Part {
@@ -116,7 +130,7 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
     const int h = blockIdx.y;
     const Slot c = ticks_of(s, slot);
     if (c.n == 0) return;
-    const long long tick = (s.offsets ? span_of(s, c.b).start : 0) + c.first;
+    const long long tick = c.tick;
     load_tile<T, NI, DP, kStride, 128>(sk, row_of<const T>(s, s.k, c.b, h, tick), s.k.tick, c.n, s.D, s.k.fast, tid);
     load_tile<T, NI, DP, kStride, 128>(sk + Lay::tile, row_of<const T>(s, s.q, c.b, h, tick), s.q.tick, c.n, s.D, s.q.fast, tid);
     async_commit();

@@ -679,8 +679,9 @@ long long norm_work(const fg_norm_args* g) {
 
 constexpr int kSumThreads = 128;                              // of a backward block whose lanes share rows
 
-// f(V, PER, GROUP, rows at once forward and back) as types, and the threads that share a row. Lanes of a warp share a row where they hold it in
-// 32 values of 16 bits or 20 of fp32 each: no barriers (65,536 rows of 1,024 in bf16 and back: 55 + 160 us, as blocks of 4 warps 87 + 218).
+// What the ring does not take: few rows, short ones, ones whose tensors begin unlike. f(V, PER, GROUP, rows at once forward and back) as types,
+// and the threads that share a row: 8 lanes a short one, a warp up to 64 units, then a block (its barriers cost several rows' sums at once;
+// 65,536 rows of 1,024 in bf16 and back took 87 + 207 us this way, 55 + 160 with a warp a row in registers, 54 + 96 in the ring).
 template <class T, class F>
 void by_shape(int v, int dim, F&& f) {
     const int units = (dim + v - 1) / v;
@@ -823,8 +824,8 @@ struct Drop {
     float by;
 };
 
-// A thread makes one block of the generator, 8 values of 16 bits. 65,536 rows of 1,024 in bf16: with a residual DROPA us, 61% of it DRAM's at
-// the measured rate and the rest the generator's 20 wide products, 40 exclusive ors and 20 key sums for 8 values; without DROPB. Loads asked
+// A thread makes one block of the generator, 8 values of 16 bits. 65,536 rows of 1,024 in bf16: with a residual 63 us, 98% of a plain copy's
+// rate, without 55 (74%: there the generator's 20 wide products, 40 exclusive ors and 20 key sums for 8 values count). Loads asked
 // for before the generator runs, or two blocks at a time, took longer (74 and 81 us).
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256, 8) k_dropout(const __grid_constant__ Drop a) {
