@@ -24,8 +24,7 @@ struct Step {
     float scale;
 };
 // A block takes 32 columns of a row's state of one head, whole in registers: V columns a thread of every (256 V / 32)-th row. One
-// pass over them gives k S and q S, and o = q S + (q k) u needs no second one. State in and out is the cost.
-// V columns and PER rows a thread
+// pass over them gives k S and q S, and o = q S + (q k) u needs no second one: PER values a column. State in and out is the cost.
 template <class T, int V, int PER>
 __global__ void __launch_bounds__(256, PER * V <= 16 ? 5 : 3) k_delta_step(const __grid_constant__ Step s) {
     constexpr int kAcross = 32 / V, kRows = 256 / kAcross, kPer = PER;
@@ -645,7 +644,7 @@ int fg_delta_step(const fg_delta_step_args* g, void* stream) {
             using T = decltype(t);
             const long long items = g->batch * g->heads;
             // whole states through shared memory where each SM has several (2,048 rows, 8 heads of 128 x 128: 476 us by columns)
-            if (by4 && items >= 8 * kSms && s.D * s.E <= 16384 && s.E * 2 <= 4 * kWideThreads && s.D * (s.E / 4) <= kWidePer * (kWideThreads / (s.E / 4)) * (s.E / 4)) {
+            if (by4 && items >= 8 * kSms && s.D * s.E <= 16384 && s.D <= kWidePer * (kWideThreads / (s.E / 4))) {
                 const int bytes = WideLayout(s.D, s.E).bytes;
                 static OnEachDevice here;
                 here.first(current_device(), [] { allow_shared(k_delta_step_wide<T>, WideLayout(128, 128).bytes); });

@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     } else if (s.glast) {
         each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.glast[state0 + at]; });
     }
-    if (!PARTS && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {                               // a slot's second chunk without ticks
+    if (!PARTS && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {   // a slot's second chunk without ticks
         const long long at = ((from.place + (long long)(chunks >> 1) * s.heads) * tiles_e + e0 / 16) * kTicks + kChunk + lane;
         s.vdn[at] = s.db[at] = 0.f;
     }

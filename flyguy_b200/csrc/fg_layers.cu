@@ -669,7 +669,7 @@ void check(const fg_norm_args* g, const char* who) {
     if (g->rows < 0 || g->rows > (1ll << 40)) throw MemErr{w + ": rows must be 0 to 2^40"};
     if (g->dim < 1 || g->dim > (1ll << 24)) throw MemErr{w + ": dim must be 1 to 2^24"};
     if (g->type < FG_F32 || g->type > FG_F16) throw MemErr{w + ": unknown type"};
-    if (!(g->eps > 0)) throw MemErr{w + ": eps must be positive"};
+    if (!((float)g->eps > 0)) throw MemErr{w + ": eps must be positive in fp32"};
 }
 bool any_length(const fg_norm_args* g) { return g->dim > kLongest; }
 long long norm_work(const fg_norm_args* g) {

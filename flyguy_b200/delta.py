@@ -194,7 +194,7 @@ def _step_sizes(q, k, v, log_decay, beta, state, *types) -> tuple[tuple, bytes]:
         raise FlyguyError
     (batch, heads), (slots, *of_state), dim, value_dim = log_decay, state, q[2], v[2]
     if not (q[0] == k[0] == v[0] == batch and k[2] == dim and of_state == [heads, dim, value_dim] and heads and q[1] and k[1] and v[1]
-            and not heads % q[1] and not heads % k[1] and not heads % v[1] and (slots >= batch or not own_slots)):
+            and dim and value_dim and not heads % q[1] and not heads % k[1] and not heads % v[1] and (slots >= batch or not own_slots)):
         raise FlyguyError
     return (batch, heads, value_dim), struct.pack("=9q", slots, batch, heads, q[1], k[1], v[1], dim, value_dim, TYPES[types[0]])
 
@@ -204,6 +204,8 @@ def _step_inputs(q, k, v, log_decay, beta, state, slots) -> tuple:
     q, k, v = _values("q", q, (3,)), _values("k", k, (3,), q), _values("v", v, (3,), q)
     batch, _, dim = q.shape
     value_dim = v.shape[-1]
+    if not dim or not value_dim:
+        raise FlyguyError("dim and value dim must be at least 1")
     if k.shape[0] != batch or k.shape[-1] != dim or v.shape[0] != batch:
         raise FlyguyError(f"k and v must be {(batch, 'key heads', dim)} and {(batch, 'value heads', 'value dim')}, not "
                           f"{tuple(k.shape)} and {tuple(v.shape)}")
@@ -261,7 +263,8 @@ class DeltaMemory(memory.TickMemory):
     The observations are normed (layer_norm) and projected in `dtype` to key_heads queries and keys of unit length (norm_rotate), heads
     values, and each head's gates: beta = sigmoid(b) and log_decay = -softplus(a) / span, the heads' spans spread from ticks[0] to
     ticks[1]. delta_attention carries the states, each head's output is normed, some of it dropped while learning (in training mode:
-    dropout with `seed`, one call of the generator a forward), and a last projection, zero at first, gives the logits."""
+    dropout with `seed`, one call of the generator a forward; in a captured forward `seed` has to be an int64 tensor on the device,
+    changed between replays), and a last projection, zero at first, gives the logits."""
 
     def __init__(self, obs_dim: int, n_actions: int, heads: int = 8, key_heads: int = 2, dim: int = 64,
                  ticks: tuple[float, float] = (16.0, 4096.0), base: float = 10000.0, dropout: float = 0.0, seed: int = 0,
@@ -295,6 +298,8 @@ class DeltaMemory(memory.TickMemory):
         o, end = delta_attention(*self._inputs(obs, positions), state, offsets=offsets)
         o = self._normed(o)
         if self.training and self.dropout:
+            if not isinstance(self.seed, torch.Tensor) and torch.cuda.is_current_stream_capturing():
+                raise FlyguyError("each replay of a captured forward would drop the same values: seed must be an int64 tensor")
             o = layers.dropout(o, self.dropout, self.seed, call=self.calls)
             self.calls += 1
         return self._logits(o), end

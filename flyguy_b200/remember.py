@@ -93,6 +93,8 @@ def main() -> None:
     ap.add_argument("--rule", choices=("decay", "delta"), default="decay")
     ap.add_argument("--dropout", type=float, default=0.0, help="of the delta rule's outputs, while learning")
     a = ap.parse_args()
+    if a.dropout and a.rule != "delta":
+        ap.error("--dropout goes with --rule delta")
     game = Game(max_batch=-(-max(a.recordings * a.ticks, a.cars) // 32) * 32, rule=a.rule, dropout=a.dropout)
     game.learn(a.steps, a.recordings, a.ticks, a.ago, a.lr, log=print)
     obs, right = recordings(a.cars, a.ticks, a.ago, game.obs_dim, game.n_act, torch.Generator().manual_seed(99), game.device)

@@ -510,3 +510,12 @@ def test_refusals(cuda):
     with pytest.raises(FlyguyError, match="slots"):
         delta.delta_step(*tick.values(), slots=torch.zeros(3, dtype=torch.int64, device=cuda))
     assert np.isfinite(delta.delta_step(*tick.values()).cpu().numpy()).all()
+
+
+def test_heads_of_no_values_are_refused(cuda):
+    for dim, value_dim in ((0, 4), (4, 0)):
+        q, v, gate = torch.zeros(2, 1, dim, device=cuda), torch.zeros(2, 1, value_dim, device=cuda), torch.zeros(2, 1, device=cuda)
+        with pytest.raises(FlyguyError, match="dim"):
+            delta.delta_step(q, q, v, gate, gate, torch.zeros(2, 1, dim, value_dim, device=cuda))
+        with pytest.raises(FlyguyError, match="dim"):
+            delta.delta_attention(q, q, v, gate, gate, offsets=torch.tensor([0, 2], device=cuda))

@@ -121,6 +121,37 @@ def test_dropout_is_for_learning_alone(game, cuda):
     memory.sync()
 
 
+def test_a_captured_forward_drops_by_a_seed_on_the_device(game, monkeypatch, cuda):
+    m, obs = game.memory, _obs(game, 2, 32, 7, cuda)
+    with monkeypatch.context() as patch:
+        patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with torch.no_grad(), pytest.raises(FlyguyError, match="seed must be"):
+            m(obs)
+    monkeypatch.setattr(m, "seed", torch.tensor(3, device=cuda))
+    graph, side, at = torch.cuda.CUDAGraph(), torch.cuda.Stream(), m.calls
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        m(obs)
+        m.calls = at
+        with torch.cuda.graph(graph, stream=side):
+            got = m(obs)[0]
+    torch.cuda.current_stream().wait_stream(side)
+    for seed in (3, 4):
+        m.seed.fill_(seed)
+        graph.replay()
+        m.calls = at
+        with torch.no_grad():
+            assert torch.equal(got, m(obs)[0])
+    memory.sync()
+
+
+def test_dropout_goes_with_the_delta_rule(monkeypatch, capsys):
+    monkeypatch.setattr(sys, "argv", "remember --dropout 0.1".split())
+    with pytest.raises(SystemExit):
+        remember.main()
+    assert "--rule delta" in capsys.readouterr().err
+
+
 def test_the_command_runs_with_the_delta_rule(monkeypatch, capsys, cuda):
     monkeypatch.setattr(sys, "argv", "remember --rule delta --dropout 0.1 --steps 2 --recordings 4 --ticks 40 --cars 3".split())
     remember.main()

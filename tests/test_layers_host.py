@@ -113,6 +113,13 @@ def test_refused_steps_norms_and_dropouts():
     assert L.fg_dropout(drop(0, 0), None) == 0 and L.fg_layer_norm(norm(0, 8), None) == 0
 
 
+def test_an_eps_that_is_zero_in_fp32_is_refused():
+    L = native.lib()
+    a = layers._NORM.pack(0, 0, 0, 0, 0, 0, 0, 0, 4, 8, 8, 8, 0, 1e-60, 0, 0)
+    for fn in (L.fg_layer_norm, L.fg_layer_norm_bwd):
+        assert fn(a, None) == -1 and "eps" in _error()
+
+
 def test_no_kernel_is_set_up_once_for_all_devices():
     for f in ("fg_delta.cu", "fg_delta_chain.cuh", "fg_delta_grad.cuh", "fg_layers.cu"):
         text = (native.PKG / "csrc" / f).read_text()
