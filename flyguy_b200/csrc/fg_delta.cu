@@ -371,7 +371,7 @@ struct Room {
     }
 };
 struct Wide {
-    float *q = nullptr, *k = nullptr, *v = nullptr, *last = nullptr;
+    float *q = nullptr, *k = nullptr, *v = nullptr;
 };
 // Parts of a recording (k_delta_join): as many as keep the blocks within one round of the SMs, of 512 ticks at least; four at least, or
 // the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: 1,300 us in 27 parts
@@ -381,42 +381,52 @@ int parts_of(const fg_delta_args* g) {
     const long long parts = std::min<long long>(64, std::min(12 * kSms / (rows * ((g->value_dim + 15) / 16)), mean / 512));
     return parts >= 4 ? (int)parts : 1;
 }
-// places s's parts; returns their size
-long long lay_out(const fg_delta_args* g, bool backward, Delta& s, Wide& wide) {
-    Room room{static_cast<char*>(g->work)};
+// What the way back can take over from the way forward, and what only a call itself needs: `held` and the workspace (g->work), or, without
+// a forward that held it, both in the workspace. Returns their sizes.
+struct Sizes {
+    long long work, held;
+};
+Sizes lay_out(const fg_delta_args* g, bool backward, bool holds, void* held, Delta& s, Wide& wide) {
+    Room room{static_cast<char*>(g->work)}, over{static_cast<char*>(held)};
+    Room& kept = holds ? over : room;
     const auto of = [&](auto f) {
         return g->type == FG_F32 ? f(Terms<float>()) : g->type == FG_F16 ? f(Terms<__half>()) : f(Terms<bf16>());
     };
-    const int kept = of([](auto t) { return t.kept; }), out = of([](auto t) { return t.out_p; });
+    const bool all_terms = backward || holds;
+    const int terms = of([](auto t) { return t.kept; }), out = of([](auto t) { return t.out_p; });
     const long long places = slots_of(g) * g->heads, tiles = (g->value_dim + 15) / 16, padded = g->dim > 64 ? 128 : 64;
-    if (g->offsets) room.take(s.table, slots_of(g) * (long long)sizeof(Slot));
-    room.take(s.x, places * kept * 2 * kChunk * kChunk * 2);
-    room.take(s.p, places * (backward ? kept : out) * 2 * kChunk * kChunk * 2);
-    room.take(s.gates, places * kGates * kTicks * 4);
+    if (g->offsets) kept.take(s.table, slots_of(g) * (long long)sizeof(Slot));
+    kept.take(s.x, places * terms * 2 * kChunk * kChunk * 2);
+    kept.take(s.p, places * (all_terms ? terms : out) * 2 * kChunk * kChunk * 2);
+    kept.take(s.gates, places * kGates * kTicks * 4);
     s.parts = parts_of(g);
     if (s.parts > 1) {
         const long long all = g->batch * g->heads * s.parts * 4, dim = padded;
         room.take(s.own, all * 16 * tiles * dim);
-        room.take(s.turn, all * dim * dim);
+        kept.take(s.turn, all * dim * dim);
         room.take(s.start, all * 16 * tiles * dim);
     }
-    if (!backward) return room.used;
-    room.take(s.states, places * tiles * padded * 64);
-    room.take(s.gstates, places * tiles * padded * 64);
-    room.take(s.w, places * tiles * 8 * 512);
-    room.take(s.od, places * tiles * kTicks * 4);
-    room.take(s.vdn, places * tiles * kTicks * 4);
-    room.take(s.db, places * tiles * kTicks * 4);
-    room.take(s.anchor, places * tiles * 4);
-    room.take(wide.last, g->batch * g->heads * g->dim * g->value_dim * 4);
-    const long long rows = all_ticks(g) * g->heads * 4;
-    if (g->query_heads != g->heads) room.take(wide.q, rows * g->dim);
-    if (g->key_heads != g->heads) room.take(wide.k, rows * g->dim);
-    if (g->value_heads != g->heads) room.take(wide.v, rows * g->value_dim);
-    return room.used;
+    if (all_terms) {
+        kept.take(s.states, places * tiles * padded * 64);
+        kept.take(s.w, places * tiles * 8 * 512);
+        kept.take(s.o32, places * tiles * 8 * 512);
+        kept.take(s.kept_last, g->batch * g->heads * g->dim * g->value_dim * 4);
+    }
+    if (backward) {
+        room.take(s.gstates, places * tiles * padded * 64);
+        room.take(s.od, places * tiles * kTicks * 4);
+        room.take(s.vdn, places * tiles * kTicks * 4);
+        room.take(s.db, places * tiles * kTicks * 4);
+        room.take(s.anchor, places * tiles * 4);
+        const long long rows = all_ticks(g) * g->heads * 4;
+        if (g->query_heads != g->heads) room.take(wide.q, rows * g->dim);
+        if (g->key_heads != g->heads) room.take(wide.k, rows * g->dim);
+        if (g->value_heads != g->heads) room.take(wide.v, rows * g->value_dim);
+    }
+    return {room.used, over.used};
 }
 
-void check(const fg_delta_args* g, bool backward) {
+void check(const fg_delta_args* g, bool backward, bool holds, const void* held, long long held_bytes) {
     const std::string who = backward ? "fg_delta_attn_bwd" : "fg_delta_attn";
     check_sizes(g, who);
     const auto want = [&](bool ok, const char* what) {
@@ -430,9 +440,11 @@ void check(const fg_delta_args* g, bool backward) {
     want(!backward || !g->gstate || (g->gstate != g->state && g->gstate != g->gstate_out), "gstate is state or gstate_out");
     Delta s{};
     Wide wide;
-    const long long bytes = lay_out(g, backward, s, wide);
-    want(!bytes || (g->work && g->work_bytes >= bytes), "the workspace is too small");
+    const Sizes bytes = lay_out(g, backward, holds, nullptr, s, wide);
+    want(!bytes.work || (g->work && g->work_bytes >= bytes.work), "the workspace is too small");
     want(reinterpret_cast<uintptr_t>(g->work) % 16 == 0, "the workspace is not 16-byte aligned");
+    want(!holds || !bytes.held || (held && held_bytes >= bytes.held), "what is held is too small");
+    want(reinterpret_cast<uintptr_t>(held) % 16 == 0, "what is held is not 16-byte aligned");
 }
 
 Delta delta_of(const fg_delta_args* g) {
@@ -507,67 +519,58 @@ void parts_forward(const Delta& s, cudaStream_t st) {
     chain<T, DP, 4, kParts>(s, st);
     join<DP, false>(s, st);
 }
+// forward, and all that the way back needs
+// 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 800 and 960 us;
+// before O was kept 777 and 917, where blocks of 4 warps with 168 registers took 1,185 and 1,030)
 template <class T, int DP>
-void forward(const Delta& s, cudaStream_t st) {
+constexpr int wide_block = Terms<T>::in == 1 && DP == 128 ? 8 : 4;
+template <class T, int DP>
+void forward_kept(const Delta& s, cudaStream_t st) {
+    prepare<T, DP, Terms<T>::kept>(s, st);
+    parts_forward<T, DP>(s, st);
+    if (s.E > 64) chain<T, DP, wide_block<T, DP>, kKeep>(s, st);
+    else chain<T, DP, 4, kKeep>(s, st);
+}
+template <class T, int DP>
+void forward(const Delta& s, bool keep, cudaStream_t st) {
+    if (keep) return forward_kept<T, DP>(s, st);
     prepare<T, DP, Terms<T>::out_p>(s, st);
     parts_forward<T, DP>(s, st);
     chain<T, DP, 4, kForward>(s, st);
 }
 template <class T, int DP>
-void backward(Delta s, float* last, cudaStream_t st) {
-    prepare<T, DP, Terms<T>::kept>(s, st);
-    s.last = last;
-    parts_forward<T, DP>(s, st);
-    // 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 777 and 917 us, as
-    // blocks of 4 warps with 168 registers 1,185 and 1,030)
-    constexpr int wide = Terms<T>::in == 1 && DP == 128 ? 8 : 4;
-    if (s.E > 64) chain<T, DP, wide, kKeep>(s, st);
-    else chain<T, DP, 4, kKeep>(s, st);
+void backward(const Delta& s, bool kept, cudaStream_t st) {
+    if (!kept) forward_kept<T, DP>(s, st);
     if (s.parts > 1) {
         chain_back<T, DP, 4, true>(s, st);
         join<DP, true>(s, st);
     }
-    if (s.E > 64) chain_back<T, DP, wide, false>(s, st);
+    if (s.E > 64) chain_back<T, DP, wide_block<T, DP>, false>(s, st);
     else chain_back<T, DP, 4, false>(s, st);
     gradients<T>(s, st);
 }
 
-}  // namespace
-
-extern "C" {
-
-long long fg_delta_work(const fg_delta_args* g, int backward) {
-    return mem_guard([&]() -> long long {
-        check_sizes(g, "fg_delta_work");
-        fg_delta_args sizes = *g;
-        sizes.work = nullptr;
-        Delta s{};
-        Wide wide;
-        return lay_out(&sizes, backward != 0, s, wide);
-    });
-}
-
-int fg_delta_attn(const fg_delta_args* g, void* stream) {
+int attn(const fg_delta_args* g, bool holds, void* held, long long held_bytes, void* stream) {
     return (int)mem_guard([&]() -> long long {
-        check(g, false);
+        check(g, false, holds, held, held_bytes);
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         clear_outside(g->offsets, g->batch, g->ticks, {&g->o}, {g->heads}, {g->value_dim}, 1, size_of(g->type), st);
         if (!g->batch) return 0;
         Delta s = delta_of(g);
         Wide wide;
-        lay_out(g, false, s, wide);
+        lay_out(g, false, holds, held, s, wide);
         by_type(g->type, [&](auto t) {
             using T = decltype(t);
-            if (s.D > 64) forward<T, 128>(s, st);
-            else forward<T, 64>(s, st);
+            if (s.D > 64) forward<T, 128>(s, holds, st);
+            else forward<T, 64>(s, holds, st);
         });
         return 0;
     });
 }
 
-int fg_delta_attn_bwd(const fg_delta_args* g, void* stream) {
+int attn_bwd(const fg_delta_args* g, bool holds, void* held, long long held_bytes, void* stream) {
     return (int)mem_guard([&]() -> long long {
-        check(g, true);
+        check(g, true, holds, held, held_bytes);
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         const auto clear = [&] {                              // (last: sums of shared heads go over all ticks)
             clear_outside(g->offsets, g->batch, g->ticks, {&g->gq, &g->gk, &g->gv}, {g->query_heads, g->key_heads, g->value_heads},
@@ -580,7 +583,9 @@ int fg_delta_attn_bwd(const fg_delta_args* g, void* stream) {
         }
         Delta s = delta_of(g);
         Wide wide;
-        lay_out(g, true, s, wide);
+        lay_out(g, true, holds, held, s, wide);
+        s.o.p = nullptr;
+        s.last = nullptr;
         s.glast = g->gstate_out;
         s.gfirst = g->gstate;
         s.glog_decay = gate(g->glog_decay);
@@ -596,8 +601,8 @@ int fg_delta_attn_bwd(const fg_delta_args* g, void* stream) {
             out(s.gq, s.gq_f32, g->gq, wide.q, g->dim);
             out(s.gk, s.gk_f32, g->gk, wide.k, g->dim);
             out(s.dn, s.dn_f32, g->gv, wide.v, g->value_dim);
-            if (s.D > 64) backward<T, 128>(s, wide.last, st);
-            else backward<T, 64>(s, wide.last, st);
+            if (s.D > 64) backward<T, 128>(s, holds, st);
+            else backward<T, 64>(s, holds, st);
             const auto add = [&](const fg_ticks& to, long long heads, long long dim, const float* room) {
                 if (room && all_ticks(g))
                     share_sum<T>(room, to, g->offsets ? 1 : g->batch, g->ticks, (int)g->heads, (int)heads, (int)dim, st);
@@ -609,6 +614,32 @@ int fg_delta_attn_bwd(const fg_delta_args* g, void* stream) {
         clear();
         return 0;
     });
+}
+
+}  // namespace
+
+extern "C" {
+
+static Sizes delta_sizes(const fg_delta_args* g, const char* who, bool backward, bool holds) {
+    check_sizes(g, who);
+    fg_delta_args sizes = *g;
+    sizes.work = nullptr;
+    Delta s{};
+    Wide wide;
+    return lay_out(&sizes, backward, holds, nullptr, s, wide);
+}
+long long fg_delta_work(const fg_delta_args* g, int backward) {
+    return mem_guard([&]() -> long long { return delta_sizes(g, "fg_delta_work", backward & 1, backward >> 1 & 1).work; });
+}
+long long fg_delta_held(const fg_delta_args* g) {
+    return mem_guard([&]() -> long long { return delta_sizes(g, "fg_delta_held", false, true).held; });
+}
+
+int fg_delta_attn(const fg_delta_args* g, void* stream) { return attn(g, false, nullptr, 0, stream); }
+int fg_delta_attn_hold(const fg_delta_args* g, void* held, long long held_bytes, void* stream) { return attn(g, true, held, held_bytes, stream); }
+int fg_delta_attn_bwd(const fg_delta_args* g, void* stream) { return attn_bwd(g, false, nullptr, 0, stream); }
+int fg_delta_attn_bwd_held(const fg_delta_args* g, void* held, long long held_bytes, void* stream) {
+    return attn_bwd(g, true, held, held_bytes, stream);
 }
 
 int fg_delta_step(const fg_delta_step_args* g, void* stream) {

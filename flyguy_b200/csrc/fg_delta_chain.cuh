@@ -19,9 +19,9 @@
 // 16 warps an SM instead of 8.
 //
 // 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 497 us (298 products a warp and chunk, 273 us of the tensor cores' at 552
-// TFLOP/s of mma.sync), with what is kept 777, back 916. The tensor pipe is 55%, 50% and 40% busy, issue slots 40%, DRAM 14%, 27% and
-// 33%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S and W,
-// too. X, P and the gates take 94 and 102 us: some 1,700 instructions a warp, of them 100 products.
+// TFLOP/s of mma.sync), with what is kept 800, back 960. The tensor pipe is 55%, 50% and 40% busy, issue slots 40%, DRAM 14%, 27% and
+// 33%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S, W and O,
+// too. X, P and the gates take 101 us: some 1,700 instructions a warp, of them 100 products.
 #pragma once
 #include "fg_delta.cuh"
 
@@ -38,7 +38,7 @@ struct Delta {
     Operand gq, gk, dn;              // gradients of q, k and v (dN), in T or (gq_f32 ..) fp32
     Gate log_decay, beta, glog_decay, gbeta;
     const float *first, *glast;      // [batch][heads][D][E], or NULL: zeros
-    float *last, *gfirst;            // or NULL: not wanted
+    float *last, *kept_last, *gfirst;   // or NULL: not wanted
     const long long* offsets;
     long long batch, ticks, slots;
     int heads, D, E, gq_f32, gk_f32, dn_f32;
@@ -47,7 +47,7 @@ struct Delta {
     bf16 *x, *p;                     // [slot][head][chunk][term][32][32]
     float* gates;                    // [slot][head][5][64]: e^G and e^{G_31 - G} of the chunks, beta, G of the slot as two floats
     float4 *states, *gstates;        // [slot][head][tile of 16 columns][DP / 8][32]: S before and R behind, transposed, as accumulators
-    float4* w;                       // [slot][head][chunk][tile][4][32]: W^T as accumulators
+    float4 *w, *o32;                 // [slot][head][chunk][tile][4][32]: W^T and O^T as accumulators
     float *od, *vdn, *db;            // [slot][head][tile][64]: rows of o dO, v dN, dbeta
     float* anchor;                   // [slot][head][tile]: <R, S> behind
     // few long recordings are split into parts, see k_delta_join
@@ -486,7 +486,7 @@ __device__ __forceinline__ void subtract(float (&x)[4], const float (&y)[4]) {
 // heads: forward, with what is kept, and back 322, 478, 508 us; with 16 warps 346, 595, 557).
 constexpr int chain_blocks(int warps) { return warps == 8 ? 2 : 3; }
 
-// Forward. kKeep: nothing but what the way back needs is written (S before each slot, W, rows of o dO), and o is made to as many
+// Forward. kKeep: what the way back needs is written, too (S before each slot, W, O in fp32), o (if wanted) is made to as many
 // terms as the corrections. kParts: what a part makes of a state of zeros, and (tiles past those of the columns) of the columns of 1.
 enum { kForward, kKeep, kParts };
 template <class T, int DP, int WARPS, int MODE>
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: forward with 168 registers 415 and 380 us (64 recordings
     // of 1,024 ticks, 8 heads of 128), with what is kept and 128 registers 675 and 747
     constexpr bool kTogether = WARPS == 8;
-    using Lay = ChainLayout<T, DP, WARPS, NP, KEEP>;
+    using Lay = ChainLayout<T, DP, WARPS, NP, false>;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
@@ -515,9 +515,8 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     const long long state0 = (b * s.heads + h) * s.D * s.E;
     const bool mine = e0 < 16 * all_tiles;
     const Source<T> from{row_of<const T>(s, s.k, b, h, sp.start), row_of<const T>(s, s.q, b, h, sp.start),
-                         row_of<const T>(s, s.v, b, h, sp.start) + e_block, KEEP ? row_of<const T>(s, s.go, b, h, sp.start) + e_block : nullptr,
-                         slot_of(s, b, sp.start) * s.heads + h};
-    T* out = MODE == kForward ? row_of<T>(s, s.o, b, h, sp.start) + e0 : nullptr;
+                         row_of<const T>(s, s.v, b, h, sp.start) + e_block, nullptr, slot_of(s, b, sp.start) * s.heads + h};
+    T* out = MODE == kForward || (KEEP && s.o.p) ? row_of<T>(s, s.o, b, h, sp.start) + e0 : nullptr;
     const auto ticks = [&](int i) { return (int)min((long long)kChunk, sp.n - (long long)i * kChunk); };
 
     float S[DP / 8][4];
@@ -543,7 +542,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
         each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { v = s.first[state0 + at]; });
     }
 
-    const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NP, KEEP, !PARTS>(s, from, to, i, ticks(i), s.E - e_block); };
+    const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NP, false, !PARTS>(s, from, to, i, ticks(i), s.E - e_block); };
     each_chunk<Lay>(tiles, part, false, load, [&](bf16* now, int i) {
         if (!mine) return;
         const uint32_t tile = smem_at(now), rows_n = tile + at_rows_n(lane, Lay::stride), rows_m = tile + at_rows_m(lane, Lay::stride),
@@ -599,8 +598,8 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
 #pragma unroll
             for (int j = 0; j < 4; ++j) subtract(N[j], Y[j]);
         }
+        const long long w_place = (2 * place + (i & 1)) * tiles_e + e0 / 16;
         if constexpr (KEEP) {
-            const long long w_place = (2 * place + (i & 1)) * tiles_e + e0 / 16;
 #pragma unroll
             for (int j = 0; j < 4; ++j) s.w[(w_place * 4 + j) * 32 + lane] = make_float4(N[j][0], N[j][1], N[j][2], N[j][3]);
         }
@@ -629,21 +628,12 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
                 if (k == 0) products<NP, NP, NP, 2, false>(O, a, at);
                 else products<NP, NP, NP, 1, false>(O + 2, a, at);
             }
-            if constexpr (!KEEP) {
-                store_rows<T, Lay::vstride>(O, now + Lay::v + 16 * warp, out + (long long)i * kChunk * s.o.tick, s.o.tick, ticks(i), s.E - e0, s.o.fast, lane);
-            } else {
-                float sums[8];
+            if constexpr (KEEP) {
 #pragma unroll
-                for (int jp = 0; jp < 2; ++jp) {
-                    float v[2][4];
-                    two_columns<NI, Lay::vstride>(columns + 2 * Lay::go, jp, v);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) sums[4 * jp + 2 * j + e] = O[2 * jp + j][e] * v[j][e] + O[2 * jp + j][e + 2] * v[j][e + 2];
-                }
-                s.od[warp_place * kTicks + (i & 1) * kChunk + 8 * (lane >> 3) + 2 * (lane & 3) + (lane >> 2 & 1)] = column_sums(sums, lane);
+                for (int j = 0; j < 4; ++j) s.o32[(w_place * 4 + j) * 32 + lane] = make_float4(O[j][0], O[j][1], O[j][2], O[j][3]);
             }
+            if (!KEEP || out)
+                store_rows<T, Lay::vstride>(O, now + Lay::v + 16 * warp, out + (long long)i * kChunk * s.o.tick, s.o.tick, ticks(i), s.E - e0, s.o.fast, lane);
         }
         // S = e^{G_31} S + (e^{G_31 - G} K)^T U
         uint32_t a[2][NS][4];
@@ -664,29 +654,26 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
             for (int j = 0; j < 4; ++j) scale_add(S[2 * d + j], make_float2(fade, fade), acc[j]);
         }
     });
-    // a slot's second chunk without ticks
-    if (KEEP && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {
-        const long long place = from.place + (long long)(chunks >> 1) * s.heads;
-        s.od[(place * tiles_e + e0 / 16) * kTicks + kChunk + lane] = 0.f;
-    }
     if constexpr (PARTS) {
         if (!mine) return;
         const bool turn = e0 >= 16 * tiles_e;
         float* to = turn ? s.turn + part_place * DP * DP : s.own + part_place * 16 * tiles_e * DP;
         each_pair<DP>(S, turn ? e0 - 16 * tiles_e : e0, lane, [&](int at, float& x, float& y) { *reinterpret_cast<float2*>(to + at) = make_float2(x, y); });
-    } else if (s.last && (chunks ? part.first < chunks && part.end == chunks : blockIdx.y == 0)) {
-        each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { s.last[state0 + at] = v; });
+    } else if (chunks ? part.first < chunks && part.end == chunks : blockIdx.y == 0) {
+        if (s.last) each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { s.last[state0 + at] = v; });
+        if (KEEP) each_value<DP>(S, s.D, s.E, e0, lane, [&](long long at, float& v) { s.kept_last[state0 + at] = v; });
     }
 }
 
 __device__ __forceinline__ void prefetch(const char* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// Back. s.last is the state after the recording's last tick. PARTS: what a part leaves of a gradient of zeros, and nothing else.
+// Back. s.kept_last is the state after the recording's last tick. PARTS: what a part leaves of a gradient of zeros, and nothing else.
 template <class T, int DP, int WARPS, bool PARTS>
 __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(WARPS) : DP > 64 ? 2 : 3)
     k_delta_back(const __grid_constant__ Delta s) {
     constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX;
     using Lay = ChainLayout<T, DP, WARPS, NX, true>;
+    constexpr bool kEarly = DP == 64;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
@@ -725,7 +712,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     }
     if (!PARTS && mine && (chunks & 1) && part.first < chunks && part.end == chunks) {   // a slot's second chunk without ticks
         const long long at = ((from.place + (long long)(chunks >> 1) * s.heads) * tiles_e + e0 / 16) * kTicks + kChunk + lane;
-        s.vdn[at] = s.db[at] = 0.f;
+        s.od[at] = s.vdn[at] = s.db[at] = 0.f;
     }
 
     const auto load = [&](bf16* to, int i) { load_chunk<T, DP, WARPS, NX, true>(s, from, to, i, ticks(i), s.E - e_block); };
@@ -744,7 +731,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
                 for (int at = lane * 128; at < DP / 8 * 512; at += 32 * 128) prefetch(states + at);
             }
             const long long before = (2 * (place - (i & 1 ? 0 : s.heads)) + !(i & 1)) * tiles_e + e0 / 16;
-            if (lane < 16) prefetch(reinterpret_cast<const char*>(s.w + before * 4 * 32) + lane * 128);
+            prefetch(reinterpret_cast<const char*>((lane < 16 ? s.w : s.o32) + before * 4 * 32) + (lane & 15) * 128);
         }
         float N[4][4];
         // R^T K^T, and <R, S> behind the slot
@@ -772,7 +759,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
                 }
             }
         }
-        if (last && !PARTS) each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { anchor = fmaf(v, s.last[state0 + at], anchor); });
+        if (last && !PARTS) each_value<DP>(R, s.D, s.E, e0, lane, [&](long long at, float& v) { anchor = fmaf(v, s.kept_last[state0 + at], anchor); });
         if (slot_end) {
             anchor = warp_sum(anchor);
             if (lane == 0) s.anchor[warp_place] = anchor;
@@ -791,6 +778,12 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
         }
         // dR = dU - X^T B dU
         const int column = (i & 1) * kChunk + 8 * (lane >> 3) + 2 * (lane & 3) + (lane >> 2 & 1);
+        float4 o[4];                                          // (asked for where registers are free)
+        const auto fetch_o = [&]() {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = __ldg(s.o32 + (w_place * 4 + j) * 32 + lane);
+        };
+        if (!PARTS && kEarly) fetch_o();
         {
             float Y[4][4];
             float4 w[4];
@@ -824,6 +817,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
                     sums[2 * j + 1] = N[j][1] * w[j].y + N[j][3] * w[j].w;
                 }
                 s.db[warp_place * kTicks + column] = column_sums(sums, lane);
+                if (!kEarly) fetch_o();
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) scale2(N[j], gate2(beta, j, lane));
@@ -863,10 +857,18 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
         // R = e^{G_31} R + (scale e^G dO)^T Q - (e^G dN)^T K
         const float fade = from0[kChunk - 1];
         uint32_t a[2][NS][4], q[2][NX][4];
+        float dots[8];                                        // rows of o dO
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             float v[2][4];
             two_columns<NI, Lay::vstride>(columns + 2 * Lay::go, k, v);
+            if constexpr (!PARTS) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    dots[4 * k + 2 * j] = fmaf(o[2 * k + j].x, v[j][0], o[2 * k + j].z * v[j][2]);
+                    dots[4 * k + 2 * j + 1] = fmaf(o[2 * k + j].y, v[j][1], o[2 * k + j].w * v[j][3]);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float2 f = gate2(from0, 2 * k + j, lane);
@@ -876,6 +878,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
             left<NS>(N[2 * k], N[2 * k + 1], a[k]);
             left<NX>(v[0], v[1], q[k]);
         }
+        if constexpr (!PARTS) s.od[warp_place * kTicks + column] = column_sums(dots, lane);
 #pragma unroll
         for (int d = 0; d < DP / 16; d += 2) {
             float acc[4][4];

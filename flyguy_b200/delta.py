@@ -63,9 +63,10 @@ def _gate_ticks(t: torch.Tensor) -> tuple[int, int, int, int]:
 
 
 @lru_cache(maxsize=256)
-def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tuple, bytes, int, int]:
-    """Of a call of these shapes and this type: the states' and o's shape, its fields from batch to type, and the bytes of workspace
-    that it and its gradients need (fg_delta_work). recordings: None, or how many the offsets name."""
+def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tuple, bytes, tuple, int]:
+    """Of a call of these shapes and this type: the states' and o's shape, its fields from batch to type, the bytes of workspace
+    that it and its gradients need, by themselves and with what is held between them (fg_delta_work), and the bytes held
+    (fg_delta_held). recordings: None, or how many the offsets name."""
     lead, dim, value_dim = q[:-2], q[-1], v[-1]
     if recordings is None:
         batch, ticks = lead if len(lead) == 2 else (1, lead[0])
@@ -73,14 +74,17 @@ def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tupl
         batch, ticks = recordings, lead[0]
     heads = log_decay[-1]
     sizes = (batch, ticks, heads, q[-2], k[-2], v[-2], dim, value_dim, TYPES[typ])
-    rooms = []
-    for backward in (0, 1):
-        rooms.append(lib().fg_delta_work(_DELTA.pack(*(0,) * 52, int(recordings is not None), *sizes, 1.0, 0, 0), backward))
-        if rooms[-1] < 0:                                 # (raised here: an error is not kept)
-            raise FlyguyError(lib().fg_mem_last_error().decode())
-    return (batch, heads, dim, value_dim), (*lead, heads, value_dim), struct.pack("=9q", *sizes), *rooms
+    packed = _DELTA.pack(*(0,) * 52, int(recordings is not None), *sizes, 1.0, 0, 0)
+    rooms = *(lib().fg_delta_work(packed, which) for which in range(4)), lib().fg_delta_held(packed)
+    if min(rooms) < 0:                                    # (raised here: an error is not kept)
+        raise FlyguyError(lib().fg_mem_last_error().decode())
+    return (batch, heads, dim, value_dim), (*lead, heads, value_dim), struct.pack("=9q", *sizes), rooms[:4], rooms[4]
 
 
+# A forward with gradients holds what its backward needs (states of every 64 ticks, corrections and outputs in float32, X and P: at dim 128 of
+# bfloat16 2.4 KB a tick and head, where q, k, v and o are 1 KB) if that is at most so many bytes; else the backward makes it again. 64
+# recordings of 1,024 ticks, 8 heads of 128: 1.26 GB, 2,755 us for both ways; made again 3,290.
+HELD_AT_MOST = 4 << 30
 _NOTHING = bytes(32)                                      # an fg_ticks of NULL
 _TICKS, _POINTERS, _END = struct.Struct("=4q"), struct.Struct("=5q"), struct.Struct("=d2q")
 
@@ -99,7 +103,7 @@ class _Delta:
             offsets = _offsets(offsets, q)
         _head_counts(q, k, v, log_decay, beta)
         self.device, self.offsets = q.get_device(), offsets
-        self.states, self.o_shape, self.sizes, self.room, self.room_back = _delta_sizes(
+        self.states, self.o_shape, self.sizes, self.rooms, self.held = _delta_sizes(
             q.shape, k.shape, v.shape, log_decay.shape, beta.shape, q.dtype, None if offsets is None else offsets.shape[0] - 1)
         if state is not None:
             _float32("state", state, q, self.states)
@@ -115,21 +119,26 @@ class _Delta:
         again.__dict__.update(self.__dict__, offsets=offsets)
         return again
 
-    def run(self, fn, size: int, ticks: bytes, device, state=0, state_out=0, gstate_out=0, gstate=0) -> None:
-        room, work = _room(size, device)
+    def run(self, backward: int, held, ticks: bytes, device, state=0, state_out=0, gstate_out=0, gstate=0) -> None:
+        room, work = _room(self.rooms[backward if held is None else 2 + backward], device)
+        if held is None:
+            fn = lib().fg_delta_attn_bwd if backward else lib().fg_delta_attn
+        else:
+            holding, at = lib().fg_delta_attn_bwd_held if backward else lib().fg_delta_attn_hold, held.data_ptr()
+            fn = lambda packed, stream: holding(packed, at, self.held, stream)   # noqa: E731
         _call(fn, ticks + _POINTERS.pack(state, state_out, gstate_out, gstate, _ptr(self.offsets)) + self.sizes + _END.pack(self.scale, *work),
               self.device)
 
-    def forward(self, q, k, v, log_decay, beta, state):
+    def forward(self, q, k, v, log_decay, beta, state, held=None):
         o = q.new_empty(self.o_shape)
         end = log_decay.new_empty(self.states)
         pack = _TICKS.pack
         ticks = (pack(*_ticks(q)) + pack(*_ticks(k)) + pack(*_ticks(v)) + pack(*_ticks(o)) + 4 * _NOTHING + pack(*_gate_ticks(log_decay))
                  + pack(*_gate_ticks(beta)) + 2 * _NOTHING)
-        self.run(lib().fg_delta_attn, self.room, ticks, q.device, _ptr(state), end.data_ptr())
+        self.run(0, held, ticks, q.device, _ptr(state), end.data_ptr())
         return o, end
 
-    def backward(self, q, k, v, log_decay, beta, state, go, gend, want_state: bool):
+    def backward(self, q, k, v, log_decay, beta, state, held, go, gend, want_state: bool):
         go = _grad("the gradient of o", go, q, self.o_shape)
         if gend is not None:
             gend = _state(gend.float())
@@ -137,7 +146,7 @@ class _Delta:
         gstate = torch.empty(self.states, dtype=torch.float32, device=q.device) if want_state else None
         ticks = b"".join([_TICKS.pack(*_ticks(t)) for t in (q, k, v)] + [_NOTHING] + [_TICKS.pack(*_ticks(t)) for t in (go, gq, gk, gv)]
                          + [_TICKS.pack(*_gate_ticks(t)) for t in (log_decay, beta, gl, gb)])
-        self.run(lib().fg_delta_attn_bwd, self.room_back, ticks, q.device, _ptr(state), 0, _ptr(gend), _ptr(gstate))
+        self.run(1, held, ticks, q.device, _ptr(state), 0, _ptr(gend), _ptr(gstate))
         return gq, gk, gv, gl, gb, gstate
 
 
@@ -147,9 +156,10 @@ class _DeltaFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         q, k, v = (_values("q", t, (3, 4)) for t in (q, k, v))
         state = _state(state)
-        out = job.forward(q, k, v, log_decay, beta, state)
+        held = _room(job.held, q.device)[0] if job.held <= HELD_AT_MOST else None
+        out = job.forward(q, k, v, log_decay, beta, state, held)
         ctx.job = job
-        ctx.save_for_backward(*map(_kept, (q, k, v, log_decay, beta, state)), job.let_go())
+        ctx.save_for_backward(*map(_kept, (q, k, v, log_decay, beta, state)), held, job.let_go())
         return out
 
     @staticmethod
@@ -170,7 +180,8 @@ def delta_attention(q, k, v, log_decay, beta, state=None, scale: float | None = 
     before the first and after the last get zeros, in o and in the gradients). state float32 [recordings, heads, dim, value
     dim] before the first ticks (None: zeros). scale: dim^-0.5 when None. dim at most 128, value dim at most 256.
     log_decay is at most 0, minus infinity forgets the state (anything below -256 does, in float32).
-    Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v, log_decay, beta and state.
+    Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v, log_decay, beta and state. With
+    gradients, o is made of more terms (the states are the same bits), and up to HELD_AT_MOST bytes are held for the backward.
 
     A recording's ticks are worked on in tiles of 64: a NaN or an infinity stays in its recording and head and out of the tiles
     before it, but reaches all ticks of its own and those after it, and infinities become NaN (delta_step goes tick by tick)."""

@@ -67,6 +67,9 @@ SIGNATURES = {
     "fg_decay_step": (_ci, [_vp, _vp]),
     "fg_delta_attn": (_ci, [_vp, _vp]),
     "fg_delta_attn_bwd": (_ci, [_vp, _vp]),
+    "fg_delta_attn_hold": (_ci, [_vp, _vp, _cll, _vp]),
+    "fg_delta_attn_bwd_held": (_ci, [_vp, _vp, _cll, _vp]),
+    "fg_delta_held": (_cll, [_vp]),
     "fg_delta_work": (_cll, [_vp, _ci]),
     "fg_delta_step": (_ci, [_vp, _vp]),
     "fg_layer_norm": (_ci, [_vp, _vp]),

@@ -318,7 +318,13 @@ typedef struct fg_delta_args {
 int fg_delta_attn(const fg_delta_args* args, void* stream);
 /* Gradients of q, k, v, log_decay, beta and state; o and state_out are unused. */
 int fg_delta_attn_bwd(const fg_delta_args* args, void* stream);
-long long fg_delta_work(const fg_delta_args* args, int backward);
+/* The same two with what the way back needs of the way forward kept between them: `held`, fg_delta_held bytes, 16-byte aligned, written by the
+ * first and read by the second, with the same arguments but the gradients. Saves the second most of a forward. */
+int fg_delta_attn_hold(const fg_delta_args* args, void* held, long long held_bytes, void* stream);
+int fg_delta_attn_bwd_held(const fg_delta_args* args, void* held, long long held_bytes, void* stream);
+long long fg_delta_held(const fg_delta_args* args);
+/* Bytes of workspace: of fg_delta_attn 0, of fg_delta_attn_bwd 1, of fg_delta_attn_hold 2, of fg_delta_attn_bwd_held 3. */
+long long fg_delta_work(const fg_delta_args* args, int which);
 
 typedef struct fg_delta_step_args {
     fg_ticks q, k, v, o;              /* one tick: the tick stride is unused */

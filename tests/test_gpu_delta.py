@@ -99,9 +99,10 @@ def _compare(x, go, gs, typ, spans=None, offsets=None, scale=None):
     for n in got:
         assert got[n].dtype is x[n].dtype
         _near(got[n], want[n], TOL[typ] if n in "qkv" else KEPT[typ], "gradient of " + n)
-    with torch.no_grad():                                        # (forward alone: the same bits)
+    with torch.no_grad():                                        # (forward alone: the same states, o of its own number of terms)
         again = delta.delta_attention(*(t.cuda() for t in x.values()), scale=scale, offsets=offsets)
-    assert torch.equal(again[0], o) and torch.equal(again[1], end)
+    _near(again[0], torch.cat(want_o) if spans is not None else torch.stack(want_o), TOL[typ], "o alone")
+    assert torch.equal(again[1], end)
 
 
 # batch, ticks, heads, query / key / value heads, dim, value dim
@@ -519,3 +520,46 @@ def test_heads_of_no_values_are_refused(cuda):
             delta.delta_step(q, q, v, gate, gate, torch.zeros(2, 1, dim, value_dim, device=cuda))
         with pytest.raises(FlyguyError, match="dim"):
             delta.delta_attention(q, q, v, gate, gate, offsets=torch.tensor([0, 2], device=cuda))
+
+
+@pytest.mark.parametrize("typ", TYPES, ids=names)
+@pytest.mark.parametrize("sizes", [(2, 100, 2, (1, 2, 1), 40, 72), (1, 2304, 2, (2, 1, 1), 72, 20), (2, 64, 1, (1, 1, 1), 128, 128)], ids=["chunks", "parts", "wide"])
+def test_what_is_held_and_what_is_made_again_give_the_same_gradients(sizes, typ, monkeypatch, cuda):
+    """The way back over what the forward held (twice), and over what it makes itself, its workspace full of NaN first."""
+    B, T, H, heads, D, E = sizes
+    x, go, gs = _inputs(50, (B, T), B, H, heads, D, E, typ)
+    leaves = [t.cuda().requires_grad_() for t in x.values()]
+    out = delta.delta_attention(*leaves)
+    want = torch.autograd.grad(out, leaves, (go.cuda(), gs.cuda()), retain_graph=True)
+    twice = torch.autograd.grad(out, leaves, (go.cuda(), gs.cuda()))
+    monkeypatch.setattr(delta, "HELD_AT_MOST", 0)
+
+    def room(size, device):
+        t = torch.full((-(-size // 4),), math.nan, device=device)
+        return t, (t.data_ptr(), size)
+
+    monkeypatch.setattr(delta, "_room", room)
+    again = torch.autograd.grad(delta.delta_attention(*leaves), leaves, (go.cuda(), gs.cuda()))
+    for a, b, c in zip(want, twice, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_packed_recordings_made_again(monkeypatch, cuda):
+    x, go, gs = _inputs(51, (300,), 4, 4, (4, 2, 2), 64, 64, torch.bfloat16)
+    offsets = torch.tensor([3, 3, 100, 131, 290], device=cuda)
+    want = _run(x, go, gs, None, offsets)
+    monkeypatch.setattr(delta, "HELD_AT_MOST", 0)
+    got = _run(x, go, gs, None, offsets)
+    assert torch.equal(got[1], want[1]) and all(torch.equal(got[2][n], want[2][n]) for n in got[2])
+
+
+def test_the_states_that_come_out_may_be_played_on_before_the_backward(cuda):
+    """delta_step changes them in place; the backward has its own."""
+    x, go, _ = _inputs(52, (2, 70), 2, 2, (2, 2, 2), 64, 64, torch.float32)
+    leaves = [t.cuda().requires_grad_() for t in x.values()]
+    want = torch.autograd.grad(delta.delta_attention(*leaves)[0], leaves, go.cuda())
+    o, end = delta.delta_attention(*leaves)
+    with torch.no_grad():
+        delta.delta_step(*(t[:, -1] for t in leaves[:5]), end)
+    for a, b in zip(torch.autograd.grad(o, leaves, go.cuda()), want):
+        assert torch.equal(a, b)

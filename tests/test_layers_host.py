@@ -87,6 +87,22 @@ def test_refused_pointers_and_workspaces():
     assert L.fg_delta_attn_bwd(_delta(GOOD, work=(4096, size), **same), None) == -1 and "gstate is state" in _error()
 
 
+def test_what_is_held():
+    L = native.lib()
+    some = {f"f{4 * i}": 4096 for i in range(12)}
+    held = L.fg_delta_held(_delta(GOOD))
+    assert held > 0 and L.fg_delta_held(None) == -1 and L.fg_delta_held(_delta((-1, *GOOD[1:]))) == -1
+    work = [L.fg_delta_work(_delta(GOOD), which) for which in range(4)]
+    assert work[2] < work[0] and work[3] < work[1] <= work[3] + held
+    for fn, size in ((L.fg_delta_attn_hold, work[2]), (L.fg_delta_attn_bwd_held, work[3])):
+        args = _delta(GOOD, work=(4096, size), **some)
+        assert fn(None, 4096, held, None) == -1 and "no arguments" in _error()
+        assert fn(args, 4096, held - 1, None) == -1 and "held is too small" in _error()
+        assert fn(args, None, held, None) == -1 and "held is too small" in _error()
+        assert fn(args, 4097, held, None) == -1 and "held is not 16-byte aligned" in _error()
+    assert L.fg_delta_attn_bwd_held(_delta(GOOD, work=(4096, work[3] - 1), **some), 4096, held, None) == -1 and "workspace is too small" in _error()
+
+
 def test_a_workspace_is_the_recordings_slots_and_nothing_more():
     """Packed recordings take at most a slot more each than their ticks do; parts only where recordings are few and long."""
     L = native.lib()
