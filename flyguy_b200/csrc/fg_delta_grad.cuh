@@ -48,40 +48,11 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::k, row_of<const T>(s, s.k, c.b, h, tick) + d_block, s.k.tick, c.n, s.D - d_block, s.k.fast, tid);
     for (int i = tid; i < kGates * kTicks; i += 256) gates[i] = s.gates[place * kGates * kTicks + i];
 
-    // the gates' gradients
-    if (blockIdx.z == 0 && warp == 0) {
-        float dot[2] = {}, db[2] = {}, anchor = 0.f;
-        for (int e = 0; e < tiles_e; ++e) {
-            const long long at = (place * tiles_e + e) * kTicks + 2 * lane;
-            const float2 o = *reinterpret_cast<const float2*>(s.od + at), v = *reinterpret_cast<const float2*>(s.vdn + at),
-                         x = *reinterpret_cast<const float2*>(s.db + at);
-            dot[0] += o.x - v.x;
-            dot[1] += o.y - v.y;
-            db[0] += x.x;
-            db[1] += x.y;
-            anchor += s.anchor[place * tiles_e + e];
-        }
-        float after = dot[0] + dot[1];                       // of this lane's ticks and all later ones
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float x = __shfl_down_sync(0xffffffffu, after, o);
-            if (lane + o < 32) after += x;
-        }
-        const float next = __shfl_down_sync(0xffffffffu, after, 1);
-        const float rest = (lane < 31 ? next : 0.f) + anchor;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = 2 * lane + i;
-            if (t >= c.n) continue;
-            *gate_of(s, s.glog_decay, c.b, h, tick + t) = i ? rest + dot[1] : rest + dot[1] + dot[0];
-            *gate_of(s, s.gbeta, c.b, h, tick + t) = db[i];
-        }
-    }
-
-    __syncthreads();                                          // the gates are there
     float dq[4][4] = {}, dk[4][4] = {}, du[4][4] = {}, dp[4][4] = {}, dd[4][4] = {};
     const uint32_t at_m = smem_at(tiles) + at_rows_m(lane, kSquare), at_n = smem_at(tiles) + at_rows_n(lane, kSquare);
     const bool below = 32 * wd <= 16 * wt;                   // this warp's ticks s x t meet the diagonal's lower side
+    const float* beta = s.gates + (place * kGates + 2) * kTicks;
+    if (lane < 16 && (warp >> 1) < tiles_e) prefetch(reinterpret_cast<const char*>(s.w + ((2 * place + (warp & 1)) * tiles_e + (warp >> 1)) * 4 * 32) + lane * 128);
 #pragma unroll 1
     for (int e0 = 0; e0 < s.E; e0 += 64) {
         if (e0) __syncthreads();
@@ -130,13 +101,17 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
             const float4* from = s.w + ((2 * place + half) * tiles_e + e) * 4 * 32 + lane;
             const uint32_t to = smem_at(tiles) + 2 * (Lay::u + 32 * half * kSquare + 16 * te) + at_rows_n(lane, kSquare);
             float4 v[4];
+            float2 by[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = there ? __ldg(from + j * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int j = 0; j < 4; ++j) {
+                v[j] = there ? __ldg(from + j * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                by[j] = __ldg(reinterpret_cast<const float2*>(beta + 32 * half + 8 * j + 2 * t4));
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float x[2][4] = {{v[2 * j].x, v[2 * j].y, v[2 * j].z, v[2 * j].w}, {v[2 * j + 1].x, v[2 * j + 1].y, v[2 * j + 1].z, v[2 * j + 1].w}};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) scale2(x[i], gate2(gates + 2 * kTicks + 32 * half, 2 * j + i, lane));
+                for (int i = 0; i < 2; ++i) scale2(x[i], by[2 * j + i]);
                 uint32_t a[NG][4];
                 left<NG>(x[0], x[1], a);
 #pragma unroll
@@ -275,6 +250,35 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     put(s.gq, s.gq_f32, dq);
     __syncthreads();
     put(s.gk, s.gk_f32, dk);
+    // the gates' gradients
+    if (blockIdx.z == 0 && warp == 0) {
+        float dot[2] = {}, db[2] = {}, anchor = 0.f;
+        for (int e = 0; e < tiles_e; ++e) {
+            const long long at = (place * tiles_e + e) * kTicks + 2 * lane;
+            const float2 o = *reinterpret_cast<const float2*>(s.od + at), v = *reinterpret_cast<const float2*>(s.vdn + at),
+                         x = *reinterpret_cast<const float2*>(s.db + at);
+            dot[0] += o.x - v.x;
+            dot[1] += o.y - v.y;
+            db[0] += x.x;
+            db[1] += x.y;
+            anchor += s.anchor[place * tiles_e + e];
+        }
+        float after = dot[0] + dot[1];                       // of this lane's ticks and all later ones
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float x = __shfl_down_sync(0xffffffffu, after, o);
+            if (lane + o < 32) after += x;
+        }
+        const float next = __shfl_down_sync(0xffffffffu, after, 1);
+        const float rest = (lane < 31 ? next : 0.f) + anchor;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = 2 * lane + i;
+            if (t >= c.n) continue;
+            *gate_of(s, s.glog_decay, c.b, h, tick + t) = i ? rest + dot[1] : rest + dot[1] + dot[0];
+            *gate_of(s, s.gbeta, c.b, h, tick + t) = db[i];
+        }
+    }
 }
 
 }  // namespace
