@@ -86,28 +86,16 @@ def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tupl
 # recordings of 1,024 ticks, 8 heads of 128: 1.26 GB, 2,755 us for both ways; made again 3,290.
 HELD_AT_MOST = 4 << 30
 _NOTHING = bytes(32)                                      # an fg_ticks of NULL
+_FORWARD, _NO_GRADIENTS = struct.Struct("=48q"), (0,) * 16
 _TICKS, _POINTERS, _END = struct.Struct("=4q"), struct.Struct("=5q"), struct.Struct("=d2q")
 
 
 class _Delta:
     """What forward and backward of one call share."""
 
-    def __init__(self, q, k, v, log_decay, beta, state, scale, offsets):
-        lead, dim = q.shape[:-2], q.shape[-1]
-        if k.shape[:-2] != lead or k.shape[-1] != dim or v.shape[:-2] != lead:
-            raise FlyguyError(f"k and v must be {(*lead, 'key heads', dim)} and {(*lead, 'value heads', 'value dim')}, not "
-                              f"{tuple(k.shape)} and {tuple(v.shape)}")
-        if offsets is not None:
-            if len(lead) != 1:
-                raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
-            offsets = _offsets(offsets, q)
-        _head_counts(q, k, v, log_decay, beta)
-        self.device, self.offsets = q.get_device(), offsets
-        self.states, self.o_shape, self.sizes, self.rooms, self.held = _delta_sizes(
-            q.shape, k.shape, v.shape, log_decay.shape, beta.shape, q.dtype, None if offsets is None else offsets.shape[0] - 1)
-        if state is not None:
-            _float32("state", state, q, self.states)
-        self.scale = float(dim ** -0.5 if scale is None else scale)
+    def __init__(self, device: int, sizes: tuple, scale: float, offsets=None):
+        self.device, self.offsets, self.scale = device, offsets, scale
+        self.states, self.o_shape, self.sizes, self.rooms, self.held = sizes
 
     def let_go(self) -> torch.Tensor | None:
         """The offsets, for autograd to keep until the backward."""
@@ -115,9 +103,7 @@ class _Delta:
         return kept
 
     def take_up(self, offsets):
-        again = object.__new__(_Delta)
-        again.__dict__.update(self.__dict__, offsets=offsets)
-        return again
+        return _Delta(self.device, (self.states, self.o_shape, self.sizes, self.rooms, self.held), self.scale, offsets)
 
     def run(self, backward: int, held, ticks: bytes, device, state=0, state_out=0, gstate_out=0, gstate=0) -> None:
         room, work = _room(self.rooms[backward if held is None else 2 + backward], device)
@@ -132,9 +118,8 @@ class _Delta:
     def forward(self, q, k, v, log_decay, beta, state, held=None):
         o = q.new_empty(self.o_shape)
         end = log_decay.new_empty(self.states)
-        pack = _TICKS.pack
-        ticks = (pack(*_ticks(q)) + pack(*_ticks(k)) + pack(*_ticks(v)) + pack(*_ticks(o)) + 4 * _NOTHING + pack(*_gate_ticks(log_decay))
-                 + pack(*_gate_ticks(beta)) + 2 * _NOTHING)
+        ticks = _FORWARD.pack(*_ticks(q), *_ticks(k), *_ticks(v), *_ticks(o), *_NO_GRADIENTS, *_gate_ticks(log_decay), *_gate_ticks(beta),
+                              0, 0, 0, 0, 0, 0, 0, 0)
         self.run(0, held, ticks, q.device, _ptr(state), end.data_ptr())
         return o, end
 
@@ -169,6 +154,41 @@ class _DeltaFn(torch.autograd.Function):
         return *ctx.job.take_up(offsets).backward(*ins, go, gend, ctx.needs_input_grad[5]), None
 
 
+@lru_cache(maxsize=256)
+def _delta_shapes(q, k, v, log_decay, beta, state, *types) -> tuple:
+    """_delta_sizes of a call of these shapes and types without offsets; an error without words."""
+    if not (len(q) == len(k) == len(v) in (3, 4) and q[:-2] == k[:-2] == v[:-2] == log_decay[:-1] and q[-1] == k[-1] and log_decay == beta
+            and types[0] in TYPES and types[0] is types[1] is types[2] and types[3:5] == (torch.float32,) * 2):
+        raise FlyguyError
+    heads = log_decay[-1]
+    if not heads or any(not t[-2] or heads % t[-2] for t in (q, k, v)):
+        raise FlyguyError
+    sizes = _delta_sizes(q, k, v, log_decay, beta, types[0], None)
+    if state is not None and (state != sizes[0] or types[5] is not torch.float32):
+        raise FlyguyError
+    return sizes
+
+
+def _delta_inputs(q, k, v, log_decay, beta, state, offsets) -> tuple:
+    """The inputs as the library takes them and the call's sizes, or what is wrong with them."""
+    q = _values("q", q, (3, 4))
+    k, v = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
+    log_decay, beta = _gate("log_decay", log_decay, q.shape[:-2], q), _gate("beta", beta, q.shape[:-2], q)
+    lead, dim = q.shape[:-2], q.shape[-1]
+    if k.shape[:-2] != lead or k.shape[-1] != dim or v.shape[:-2] != lead:
+        raise FlyguyError(f"k and v must be {(*lead, 'key heads', dim)} and {(*lead, 'value heads', 'value dim')}, not "
+                          f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if offsets is not None:
+        if len(lead) != 1:
+            raise FlyguyError("offsets go with recordings packed end to end: q is [ticks, heads, dim]")
+        offsets = _offsets(offsets, q)
+    _head_counts(q, k, v, log_decay, beta)
+    sizes = _delta_sizes(q.shape, k.shape, v.shape, log_decay.shape, beta.shape, q.dtype, None if offsets is None else offsets.shape[0] - 1)
+    if state is not None:
+        _float32("state", state, q, sizes[0])
+    return q, k, v, log_decay, beta, offsets, sizes
+
+
 def delta_attention(q, k, v, log_decay, beta, state=None, scale: float | None = None,
                     offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
     """The gated delta rule for every recording and head: S_t = exp(log_decay_t) S_{t-1} + k_t u_t^T, u_t = beta_t (v_t -
@@ -185,10 +205,19 @@ def delta_attention(q, k, v, log_decay, beta, state=None, scale: float | None = 
 
     A recording's ticks are worked on in tiles of 64: a NaN or an infinity stays in its recording and head and out of the tiles
     before it, but reaches all ticks of its own and those after it, and infinities become NaN (delta_step goes tick by tick)."""
-    q = _values("q", q, (3, 4))
-    k, v = _values("k", k, (3, 4), q), _values("v", v, (3, 4), q)
-    log_decay, beta = _gate("log_decay", log_decay, q.shape[:-2], q), _gate("beta", beta, q.shape[:-2], q)
-    job = _Delta(q, k, v, log_decay, beta, state, scale, offsets)
+    try:                                                  # (what most calls are, by the sizes alone)
+        if offsets is not None:
+            raise FlyguyError
+        sizes = _delta_shapes(q.shape, k.shape, v.shape, log_decay.shape, beta.shape, None if state is None else state.shape,
+                              q.dtype, k.dtype, v.dtype, log_decay.dtype, beta.dtype, None if state is None else state.dtype)
+        device = q.get_device()
+        if not (q.stride(-1) == k.stride(-1) == v.stride(-1) == 1 and device >= 0 and (state is None or state.get_device() == device)
+                and k.get_device() == v.get_device() == log_decay.get_device() == beta.get_device() == device):
+            raise FlyguyError
+    except (AttributeError, FlyguyError):
+        q, k, v, log_decay, beta, offsets, sizes = _delta_inputs(q, k, v, log_decay, beta, state, offsets)
+        device = q.get_device()
+    job = _Delta(device, sizes, q.shape[-1] ** -0.5 if scale is None else float(scale), offsets)
     _no_tangents(q, k, v, log_decay, beta, state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or beta.requires_grad
                                     or (state is not None and state.requires_grad)):
