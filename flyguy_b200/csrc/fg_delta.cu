@@ -520,7 +520,7 @@ void parts_forward(const Delta& s, cudaStream_t st) {
     join<DP, false>(s, st);
 }
 // forward, and all that the way back needs
-// 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 800 and 960 us;
+// 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 800 and 965 us;
 // before O was kept 777 and 917, where blocks of 4 warps with 168 registers took 1,185 and 1,030)
 template <class T, int DP>
 constexpr int wide_block = Terms<T>::in == 1 && DP == 128 ? 8 : 4;

@@ -8,8 +8,8 @@
 // A block of 8 warps makes 64 columns of one slot of one head: warp = 16 ticks x 32 columns. The products with S and R run over blocks of 64
 // of their columns; S, R and W arrive as the chain's accumulators and go through shared memory, where reading across turns them.
 //
-// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 838 us (1.6 GB, 245 us at a plain copy's rate; the products 150). Bound by what follows one
-// another in a block of which an SM holds two: the loads, their terms, the products, the masks; tensor pipe 31%, issue slots 35%, DRAM 34%.
+// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 807 us (1.6 GB, 245 us at a plain copy's rate; the products 150). Bound by what follows one
+// another in a block of which an SM holds two: the loads, their terms, the products, the masks; tensor pipe 36%, issue slots 36%, DRAM 38%.
 #pragma once
 #include "fg_delta_chain.cuh"
 
