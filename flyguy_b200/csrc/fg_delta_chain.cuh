@@ -483,7 +483,7 @@ __device__ __forceinline__ void subtract(float (&x)[4], const float (&y)[4]) {
 }
 
 // Blocks of an SM at once: 16 warps with 128 registers a thread as blocks of 8 warps, 12 with 168 as blocks of 4 (at dim 64, 97,500 ticks, 8
-// heads: forward, with what is kept, and back 322, 478, 508 us; with 16 warps 346, 595, 557).
+// heads: with what is kept and back 441 and 523 us; before O was kept 478 and 508, with 16 warps 595 and 557).
 constexpr int chain_blocks(int warps) { return warps == 8 ? 2 : 3; }
 
 // Forward. kKeep: what the way back needs is written, too (S before each slot, W, O in fp32), o (if wanted) is made to as many
@@ -494,8 +494,8 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     k_delta_chain(const __grid_constant__ Delta s) {
     constexpr bool KEEP = MODE == kKeep, PARTS = MODE == kParts;
     constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX, NO = KEEP ? NX : Terms<T>::out_s, NP = KEEP ? NX : Terms<T>::out_p;
-    // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: forward with 168 registers 415 and 380 us (64 recordings
-    // of 1,024 ticks, 8 heads of 128), with what is kept and 128 registers 675 and 747
+    // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: with what is kept and 128 registers 800 and 1,083 us (64
+    // recordings of 1,024 ticks, 8 heads of 128), forward with 168 504 and 501, with what is kept at dim 64 497 and 441
     constexpr bool kTogether = WARPS == 8;
     using Lay = ChainLayout<T, DP, WARPS, NP, false>;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
