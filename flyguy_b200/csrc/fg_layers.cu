@@ -430,24 +430,36 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
             for (int i = 0; i < N; ++i) sum = plus(sum, d[i]);
         }
         const P off = same<P>(-warp_sum(both(sum)) / (float)a.dim);   // - mean
-        P squares = same<P>(0.f);
+        P squares = same<P>(0.f), s0 = squares, s1 = squares;
         sum = squares;
-        const auto centred = [&](int j, int c, P(&d)[N]) {
-            const Unit<T, V> x = unit(j);
-#pragma unroll
-            for (int i = 0; i < N; ++i) d[i] = plus(lane_of<T, V>(x, i), off);
-            keep(c, d);
-        };
+        // back: sums of g and g d with them, and g d r = r (g d) + lack g, so that a row is gone over three times
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int c = column(j);
             if (c >= a.dim) break;
+            const Unit<T, V> x = unit(j);
             P d[N];
-            centred(j, c, d);
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = plus(lane_of<T, V>(x, i), off);
+            keep(c, d);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 sum = plus(sum, d[i]);
                 squares = times_plus(d[i], d[i], squares);
+            }
+            if constexpr (BACK) {
+                const Unit<T, V> g = gunit(j);
+                P y[N], v[N];
+                weight(j, v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = lane_of<T, V>(g, i);
+                keep(c, y);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const P z = times(y[i], v[i]);
+                    s0 = plus(s0, z);
+                    s1 = times_plus(z, d[i], s1);
+                }
             }
         }
         float one, other;
@@ -458,38 +470,16 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
             for (int j = 0; j < PER; ++j) {
                 const int c = column(j);
                 if (c >= a.dim) break;
-                P d[N];
-                centred(j, c, d);
+                const Unit<T, V> x = unit(j);
                 float o[V];
 #pragma unroll
-                for (int i = 0; i < N; ++i) values_of<V>(times_plus(times_plus(d[i], inv, lack), w[j][i], b[j][i]), i, o);
+                for (int i = 0; i < N; ++i)
+                    values_of<V>(times_plus(times_plus(plus(lane_of<T, V>(x, i), off), inv, lack), w[j][i], b[j][i]), i, o);
                 put(reinterpret_cast<T*>(a.y) + row * a.dim, c, o);
             }
         } else {
-            P s0 = same<P>(0.f), s1 = s0;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int c = column(j);
-                if (c >= a.dim) break;
-                const Unit<T, V> g = gunit(j);
-                P d[N], y[N], v[N];
-                centred(j, c, d);
-                weight(j, v);
-#pragma unroll
-                for (int i = 0; i < N; ++i) y[i] = lane_of<T, V>(g, i);
-                keep(c, y);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const P h = times_plus(d[i], inv, lack), z = times(y[i], v[i]);
-                    if constexpr (SUMS) {
-                        aw[j][i] = times_plus(y[i], h, aw[j][i]);
-                        ab[j][i] = plus(ab[j][i], y[i]);
-                    }
-                    s0 = plus(s0, z);
-                    s1 = times_plus(z, h, s1);
-                }
-            }
-            const P m = same<P>(-warp_sum(both(s0)) / (float)a.dim), k = same<P>(-warp_sum(both(s1)) / (float)a.dim);
+            const float g = warp_sum(both(s0)), gd = warp_sum(both(s1));
+            const P m = same<P>(-g / (float)a.dim), k = same<P>(-fmaf(gd, one, g * other) / (float)a.dim);
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const int c = column(j);
@@ -500,8 +490,12 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
                 float o[V];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const P d = times_plus(plus(lane_of<T, V>(x, i), off), inv, lack);
-                    values_of<V>(times(times_plus(d, k, times_plus(lane_of<T, V>(g, i), v[i], m)), inv), i, o);
+                    const P h = times_plus(plus(lane_of<T, V>(x, i), off), inv, lack), y = lane_of<T, V>(g, i);
+                    if constexpr (SUMS) {                     // (of values outside the row: never used)
+                        aw[j][i] = times_plus(y, h, aw[j][i]);
+                        ab[j][i] = plus(ab[j][i], y);
+                    }
+                    values_of<V>(times(times_plus(h, k, times_plus(y, v[i], m)), inv), i, o);
                 }
                 put(reinterpret_cast<T*>(a.gx) + row * a.dim, c, o);
             }
@@ -681,7 +675,7 @@ constexpr int kSumThreads = 128;                              // of a backward b
 
 // What the ring does not take: few rows, short ones, ones whose tensors begin unlike. f(V, PER, GROUP, rows at once forward and back) as types,
 // and the threads that share a row: 8 lanes a short one, a warp up to 64 units, then a block (its barriers cost several rows' sums at once;
-// 65,536 rows of 1,024 in bf16 and back took 87 + 207 us this way, 55 + 160 with a warp a row in registers, 54 + 96 in the ring).
+// 65,536 rows of 1,024 in bf16 and back took 87 + 207 us this way, 55 + 160 with a warp a row in registers, 54 + 85 in the ring).
 template <class T, class F>
 void by_shape(int v, int dim, F&& f) {
     const int units = (dim + v - 1) / v;
