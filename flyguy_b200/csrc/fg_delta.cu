@@ -374,8 +374,8 @@ struct Wide {
     float *q = nullptr, *k = nullptr, *v = nullptr;
 };
 // Parts of a recording (k_delta_join): as many as keep the blocks within one round of the SMs, of 512 ticks at least; four at least, or
-// the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: 1,300 us in 27 parts
-// (the parts' own 716, put together 78, then 503), as many chunks one after another 5,230.
+// the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: 1,310 us in 27 parts
+// (the parts' own 709, put together 78, then 522), as many chunks one after another 5,230.
 int parts_of(const fg_delta_args* g) {
     const long long rows = std::max<long long>(1, g->batch * g->heads), mean = g->offsets ? g->ticks / std::max<long long>(1, g->batch) : g->ticks;
     const long long parts = std::min<long long>(64, std::min(12 * kSms / (rows * ((g->value_dim + 15) / 16)), mean / 512));

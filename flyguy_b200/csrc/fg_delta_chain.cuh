@@ -18,7 +18,7 @@
 // memory or TMEM in it). Chunks of 32 ticks need 16 registers an accumulator of a tick's row where 64 need 32, which leaves room for 12 to
 // 16 warps an SM instead of 8.
 //
-// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 497 us (298 products a warp and chunk, 273 us of the tensor cores' at 552
+// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 522 us (310 products a warp and chunk, 284 us of the tensor cores' at 552
 // TFLOP/s of mma.sync), with what is kept 800, back 965. The tensor pipe is 55%, 49% and 36% busy, issue slots 40%, DRAM 14%, 33% and
 // 39%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S, W and O,
 // too. X, P and the gates take 101 us: some 1,700 instructions a warp, of them 100 products.
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     constexpr bool KEEP = MODE == kKeep, PARTS = MODE == kParts;
     constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX, NO = KEEP ? NX : Terms<T>::out_s, NP = KEEP ? NX : Terms<T>::out_p;
     // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: with what is kept and 128 registers 800 and 1,083 us (64
-    // recordings of 1,024 ticks, 8 heads of 128), forward with 168 504 and 501, with what is kept at dim 64 497 and 441
+    // recordings of 1,024 ticks, 8 heads of 128), forward with 168 504 and 501 (P of one term), with what is kept at dim 64 497 and 441
     constexpr bool kTogether = WARPS == 8;
     using Lay = ChainLayout<T, DP, WARPS, NP, false>;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;

@@ -8,7 +8,7 @@
 // A block of 8 warps makes 64 columns of one slot of one head: warp = 16 ticks x 32 columns. The products with S and R run over blocks of 64
 // of their columns; S, R and W arrive as the chain's accumulators and go through shared memory, where reading across turns them.
 //
-// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 807 us (1.6 GB, 245 us at a plain copy's rate; the products 150). Bound by what follows one
+// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 893 us (1.6 GB, 245 us at a plain copy's rate; the products 180). Bound by what follows one
 // another in a block of which an SM holds two: the loads, their terms, the products, the masks; tensor pipe 36%, issue slots 36%, DRAM 38%.
 #pragma once
 #include "fg_delta_chain.cuh"
@@ -17,19 +17,19 @@ namespace {
 
 template <class T>
 struct GradLayout {
-    static constexpr int in = Terms<T>::in, terms_n = Terms<T>::grad_n, terms_s = Terms<T>::grad_s, terms = Terms<T>::grad, plane = kTicks * kSquare;
+    static constexpr int in = Terms<T>::in, terms_n = Terms<T>::grad_n, terms_s = Terms<T>::grad_s, terms_r = Terms<T>::grad_r, terms = Terms<T>::grad, plane = kTicks * kSquare;
     static constexpr int q = 0, k = q + in * plane, go = k + in * plane, dn = go + in * plane, u = dn + terms_n * plane, s = u + terms * plane,
-                         r = s + terms_s * plane, values = r + terms_s * plane;
+                         r = s + terms_s * plane, values = r + terms_r * plane;
     static constexpr int dp = go, d = dp + terms * plane;     // later, over dO, dN and U
     static constexpr int out = s;                             // and at last, fp32 rows over S and R
     static constexpr int bytes = 2 * values + 4 * kGates * kTicks;
-    static_assert(in + terms_n >= terms && 2 * terms_s * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
+    static_assert(in + terms_n >= terms && (terms_s + terms_r) * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
 };
 
 template <class T>
 __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(const __grid_constant__ Delta s) {
     using Lay = GradLayout<T>;
-    constexpr int NI = Lay::in, NN = Lay::terms_n, NS = Lay::terms_s, NG = Lay::terms, kPlane = Lay::plane;
+    constexpr int NI = Lay::in, NN = Lay::terms_n, NS = Lay::terms_s, NR = Lay::terms_r, NG = Lay::terms, kPlane = Lay::plane;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* tiles = reinterpret_cast<bf16*>(smem);
     float* gates = reinterpret_cast<float*>(smem + 2 * Lay::values);
@@ -88,10 +88,12 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                 const float x[2][4] = {{v[2 * j].x, v[2 * j].y, v[2 * j].z, v[2 * j].w}, {v[2 * j + 1].x, v[2 * j + 1].y, v[2 * j + 1].z, v[2 * j + 1].w}};
                 left<NS>(x[0], x[1], a);
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
+                for (int n = 0; n < NS; ++n) {
+                    if (which && n >= NR) break;
                     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to + 2 * (n * kPlane + 16 * j)), "r"(a[n][0]),
                                  "r"(a[n][1]), "r"(a[n][2]), "r"(a[n][3])
                                  : "memory");
+                }
             }
         }
         // U = B W; a warp: 16 columns of one chunk (without ticks: zeros)
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
             const auto state = [&](int j, int p) { return at_m + 2 * (Lay::s + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * p); };
             products<NI, NS, NG, 2, true>(dq, go, state);
             products<NN, NS, NG, 2, true>(dk, dn, state);
-            products<NG, NS, NG, 2, true>(du, u, [&](int j, int p) { return at_m + 2 * (Lay::r + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * p); });
+            products<NG, NR, NG, 2, true>(du, u, [&](int j, int p) { return at_m + 2 * (Lay::r + j * kPlane + 16 * e * kSquare + 32 * wd + 16 * p); });
             if (below) {
                 const auto at = [&](int j, int p) { return at_n + 2 * (Lay::u + j * kPlane + (32 * wd + 16 * p) * kSquare + 16 * e); };
                 products<NI, NG, NG, 2, false>(dp, go, at);

@@ -12,8 +12,8 @@ Queries, keys and values are float32, bfloat16 or float16 of one type, any strid
 first); gates and states are float32. Gradients are of the first order. DeltaMemory puts the operators together.
 
 Products run on the tensor cores in bfloat16 terms: what is carried from chunk to chunk (states, corrections and their gradients)
-has two terms, 2^-17 of each value, three and 2^-24 where the inputs are float32, and sums are float32. Outputs and the gradients of q, k
-and v of bfloat16 are made of once rounded operands, each of the size of the result's own rounding."""
+and the gates' gradients have three, 2^-24 of each value; outputs and the gradients of q and k of bfloat16 two, where one would
+be of the size of the result's own rounding (gv alone goes into them once rounded). Sums are float32."""
 from __future__ import annotations
 
 import struct
