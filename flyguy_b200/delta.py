@@ -83,7 +83,7 @@ def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tupl
 
 # A forward with gradients holds what its backward needs (states of every 64 ticks, corrections and outputs in float32, X and P: at dim 128 of
 # bfloat16 2.4 KB a tick and head, where q, k, v and o are 1 KB) if that is at most so many bytes; else the backward makes it again. 64
-# recordings of 1,024 ticks, 8 heads of 128: 1.26 GB, 2,755 us for both ways; made again 3,290.
+# recordings of 1,024 ticks, 8 heads of 128: 1.32 GB, 2,755 us for both ways; made again 3,290.
 HELD_AT_MOST = 4 << 30
 _NOTHING = bytes(32)                                      # an fg_ticks of NULL
 _FORWARD, _NO_GRADIENTS = struct.Struct("=48q"), (0,) * 16
