@@ -53,15 +53,18 @@ struct Norm {
     float eps;
 };
 
-// sums over the threads that share a row: GROUP lanes, or (0) the block
-template <int GROUP, int N>
+// sums over the threads that share a row: GROUP lanes, or (0) the block, which hands them over in two places of `room` in turn, each of WIDEST
+// sums of 16 warps, the most that the kernel asks for at once. (One barrier a sum: a place is written again only after the barrier of the sum
+// between, and that holds for sums of unequal numbers because the places are the kernel's and not the sum's.)
+template <int GROUP, int WIDEST, int N>
 __device__ __forceinline__ void row_sums(float (&s)[N], float* room, int& turn) {
+    static_assert(N <= WIDEST, "a place holds the sums");
 #pragma unroll
     for (int o = (GROUP ? GROUP : 32) / 2; o; o >>= 1)
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
     if constexpr (GROUP == 0) {
-        float* at = room + (turn ^= 1) * 16 * N;              // (two places in turn: one barrier a sum)
+        float* at = room + (turn ^= 1) * 16 * WIDEST;
         const int warps = blockDim.x >> 5;
         if ((threadIdx.x & 31) == 0) {
 #pragma unroll
@@ -108,7 +111,7 @@ struct Rows {
                     for (int i = 0; i < V; ++i) mean[r] += to_f(u[r][j].v[i]);
                 }
         }
-        row_sums<GROUP, ROWS>(mean, room, turn);
+        row_sums<GROUP, 2 * ROWS>(mean, room, turn);
         float s[2 * ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -555,13 +558,13 @@ __global__ void __launch_bounds__(128, 4) k_norm_ring(const __grid_constant__ No
 // Rows of any length: read three times, the second and third from the caches.
 template <class T>
 __global__ void __launch_bounds__(512) k_norm_any(const __grid_constant__ Norm a, float* stats) {
-    __shared__ float room[128];
+    __shared__ float room[64];
     int turn = 0;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_row;
         float s[1] = {0.f};
         for (int c = threadIdx.x; c < a.dim; c += 512) s[0] += to_f(x[c]);
-        row_sums<0, 1>(s, room, turn);
+        row_sums<0, 2>(s, room, turn);
         const float mean = s[0] / (float)a.dim;
         float q[2] = {0.f, 0.f}, r, lack;
         for (int c = threadIdx.x; c < a.dim; c += 512) {
