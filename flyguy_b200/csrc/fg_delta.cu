@@ -371,7 +371,8 @@ struct Room {
     }
 };
 struct Wide {
-    float *q = nullptr, *k = nullptr, *v = nullptr;
+    float *q = nullptr, *k = nullptr, *v = nullptr;   // gradients of each head in fp32, of shared ones
+    bf16 *high = nullptr, *low = nullptr;             // dN as two terms, of 16-bit values that are not shared
 };
 // Parts of a recording (k_delta_join): as many as keep the blocks within one round of the SMs, of 512 ticks at least; four at least, or
 // the work is not worth it. 1 recording of 65,536 ticks, 8 heads of 128 in bf16: 1,310 us in 27 parts
@@ -421,7 +422,12 @@ Sizes lay_out(const fg_delta_args* g, bool backward, bool holds, void* held, Del
         const long long rows = all_ticks(g) * g->heads * 4;
         if (g->query_heads != g->heads) room.take(wide.q, rows * g->dim);
         if (g->key_heads != g->heads) room.take(wide.k, rows * g->dim);
-        if (g->value_heads != g->heads) room.take(wide.v, rows * g->value_dim);
+        if (g->value_heads != g->heads) {
+            room.take(wide.v, rows * g->value_dim);
+        } else if (g->type != FG_F32) {
+            if (g->type == FG_F16) room.take(wide.high, rows / 2 * padded_values((int)g->value_dim));
+            room.take(wide.low, rows / 2 * padded_values((int)g->value_dim));
+        }
     }
     return {room.used, over.used};
 }
@@ -520,7 +526,7 @@ void parts_forward(const Delta& s, cudaStream_t st) {
     join<DP, false>(s, st);
 }
 // forward, and all that the way back needs
-// 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 800 and 965 us;
+// 64 or 128 columns of values a block: 16 warps an SM with 128 registers a thread where dim is over 64 (forward and back 800 and 1,015 us;
 // before O was kept 777 and 917, where blocks of 4 warps with 168 registers took 1,185 and 1,030)
 template <class T, int DP>
 constexpr int wide_block = Terms<T>::in == 1 && DP == 128 ? 8 : 4;
@@ -601,6 +607,13 @@ int attn_bwd(const fg_delta_args* g, bool holds, void* held, long long held_byte
             out(s.gq, s.gq_f32, g->gq, wide.q, g->dim);
             out(s.gk, s.gk_f32, g->gk, wide.k, g->dim);
             out(s.dn, s.dn_f32, g->gv, wide.v, g->value_dim);
+            const auto term = [&](Operand& to, bf16* room) {
+                const long long row = padded_values(s.E);
+                to = operand({room, g->ticks * g->heads * row, g->heads * row, row}, g->heads, g->heads, row, 2);
+            };
+            term(s.dn_low, wide.low);
+            if (std::is_same<T, bf16>::value) s.dn_high = s.dn;
+            else term(s.dn_high, wide.high);
             if (s.D > 64) backward<T, 128>(s, holds, st);
             else backward<T, 64>(s, holds, st);
             const auto add = [&](const fg_ticks& to, long long heads, long long dim, const float* room) {

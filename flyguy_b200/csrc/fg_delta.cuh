@@ -178,15 +178,14 @@ __device__ __forceinline__ float column_sums(float (&v)[8], int lane) {
 }
 
 // Terms by type: of inputs; of all that is carried from chunk to chunk and what corrects it (states, X, their gradients); of S and of P
-// and U where they make o; for the gradients of q and k of U, dP and D, of S, of R, and of dN (gv in the type of v, where no heads
-// share it).
+// and U where they make o; for the gradients of q and k of U, dP and D, of S, of R, and of dN.
 // Three terms keep states, their gradients and the gates' as good as fp32 products and sums would (64 recordings of 1,024 ticks, 8 heads of
 // 128 in bf16: 3e-7 to 7e-7 off; with two terms 4e-6 to 1e-5, in 360 instead of 497 us for the chain forward). o and the gradients of
 // q and k are rounded to 16 bits in the end, 1.65e-3 of their norm. With P, U and S of one term they were up to 3.1e-3 off (o of short
-// recordings, nearly all P U), with these terms o and gq are as good as their rounding and gk, for dN's, 1.9e-3 to 2.3e-3 (o 522 instead of
-// 501 us, gradients 893 instead of 807).
+// recordings, nearly all P U), with R and dN of one gk 2.3e-3; with these terms o, gq and gk are as good as their rounding (o 522 instead of
+// 501 us; gradients with R and dN of one term 893 instead of 1,032, the way back to them 965 instead of 1,015).
 template <class T> struct Terms;
-template <> struct Terms<bf16> { static constexpr int in = 1, kept = 3, out_s = 2, out_p = 2, grad = 2, grad_s = 2, grad_r = 1, grad_n = 1; };
+template <> struct Terms<bf16> { static constexpr int in = 1, kept = 3, out_s = 2, out_p = 2, grad = 2, grad_s = 2, grad_r = 2, grad_n = 2; };
 template <> struct Terms<__half> { static constexpr int in = 2, kept = 3, out_s = 2, out_p = 2, grad = 2, grad_s = 2, grad_r = 2, grad_n = 2; };
 template <> struct Terms<float> { static constexpr int in = 3, kept = 3, out_s = 3, out_p = 3, grad = 3, grad_s = 3, grad_r = 3, grad_n = 3; };
 

@@ -18,8 +18,8 @@
 // memory or TMEM in it). Chunks of 32 ticks need 16 registers an accumulator of a tick's row where 64 need 32, which leaves room for 12 to
 // 16 warps an SM instead of 8.
 //
-// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 522 us (310 products a warp and chunk, 284 us of the tensor cores' at 552
-// TFLOP/s of mma.sync), with what is kept 800, back 965. The tensor pipe is 55%, 49% and 36% busy, issue slots 40%, DRAM 14%, 33% and
+// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 522 us (310 products a warp and chunk, 301 us of the tensor cores' at 552
+// TFLOP/s of mma.sync), with what is kept 800, back 1,015. The tensor pipe is 55%, 49% and 36% busy, issue slots 40%, DRAM 14%, 33% and
 // 39%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S, W and O,
 // too. X, P and the gates take 101 us: some 1,700 instructions a warp, of them 100 products.
 #pragma once
@@ -36,6 +36,7 @@ struct Slot {
 struct Delta {
     Operand q, k, v, o, go;
     Operand gq, gk, dn;              // gradients of q, k and v (dN), in T or (gq_f32 ..) fp32
+    Operand dn_high, dn_low;         // dN in T of 16 bits as two terms for the gradients of k: of bf16 the first is gv itself
     Gate log_decay, beta, glog_decay, gbeta;
     const float *first, *glast;      // [batch][heads][D][E], or NULL: zeros
     float *last, *kept_last, *gfirst;   // or NULL: not wanted
@@ -89,6 +90,8 @@ __device__ __forceinline__ Slot ticks_of(const Delta& s, long long slot) {
     const long long first = (long long)((uint32_t)slot - b * per) * kTicks;
     return {first, (int)b, (int)min((long long)kTicks, s.ticks - first)};
 }
+// values of a row of dn_high or dn_low
+__host__ __device__ constexpr int padded_values(int E) { return (E + 7) / 8 * 8; }
 // the chunks of a part: whole slots, as many in each but the last ones
 struct Part {
     int first, end;
@@ -495,7 +498,7 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
     constexpr bool KEEP = MODE == kKeep, PARTS = MODE == kParts;
     constexpr int NI = Terms<T>::in, NX = Terms<T>::kept, NS = NX, NO = KEEP ? NX : Terms<T>::out_s, NP = KEEP ? NX : Terms<T>::out_p;
     // Q S beside K S, S's terms made once, or after W, with 16 fewer registers held: with what is kept and 128 registers 800 and 1,083 us (64
-    // recordings of 1,024 ticks, 8 heads of 128), forward with 168 504 and 501 (P of one term), with what is kept at dim 64 497 and 441
+    // recordings of 1,024 ticks, 8 heads of 128), forward with 168 504 and 501 (P of one term; 522 with two), with what is kept at dim 64 497 and 441
     constexpr bool kTogether = WARPS == 8;
     using Lay = ChainLayout<T, DP, WARPS, NP, false>;
     constexpr int kPlane = kChunk * Lay::stride, kSm = kChunk * kSmall;
@@ -839,9 +842,18 @@ __global__ void __launch_bounds__(32 * WARPS, Terms<T>::in == 1 ? chain_blocks(W
             const long long tick = sp.start + (long long)i * kChunk;
             const int n = ticks(i);
             bf16* room = now + Lay::v + 16 * warp;
-            if (sizeof(T) == 2 && !s.dn_f32)
+            if (sizeof(T) == 2 && !s.dn_f32) {
                 store_rows<T, Lay::vstride>(N, room, row_of<T>(s, s.dn, b, h, tick) + e0, s.dn.tick, n, s.E - e0, s.dn.fast, lane);
-            else if constexpr (NI > 1)
+                const int whole = padded_values(s.E) - e0;    // (columns past E are zeros)
+                if constexpr (!std::is_same<T, bf16>::value)
+                    store_rows<bf16, Lay::vstride>(N, room, row_of<bf16>(s, s.dn_high, b, h, tick) + e0, s.dn_high.tick, n, whole, true, lane);
+                float rest[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rest[j][e] = N[j][e] - to_f(from_f<bf16>(N[j][e]));
+                store_rows<bf16, Lay::vstride>(rest, room, row_of<bf16>(s, s.dn_low, b, h, tick) + e0, s.dn_low.tick, n, whole, true, lane);
+            } else if constexpr (NI > 1)
                 store_rows<float, Lay::vstride>(N, room, row_of<float>(s, s.dn, b, h, tick) + e0, s.dn.tick, n, s.E - e0, s.dn.fast, lane);
             else {                                            // (one plane: fp32 straight from the registers)
                 float* to = row_of<float>(s, s.dn, b, h, tick) + e0;

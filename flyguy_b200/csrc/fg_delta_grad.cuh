@@ -8,7 +8,7 @@
 // A block of 8 warps makes 64 columns of one slot of one head: warp = 16 ticks x 32 columns. The products with S and R run over blocks of 64
 // of their columns; S, R and W arrive as the chain's accumulators and go through shared memory, where reading across turns them.
 //
-// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 893 us (1.6 GB, 245 us at a plain copy's rate; the products 180). Bound by what follows one
+// 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 1,032 us (2.3 GB, 350 us at a plain copy's rate; the products 440). Bound by what follows one
 // another in a block of which an SM holds two: the loads, their terms, the products, the masks; tensor pipe 36%, issue slots 36%, DRAM 38%.
 #pragma once
 #include "fg_delta_chain.cuh"
@@ -23,7 +23,7 @@ struct GradLayout {
     static constexpr int dp = go, d = dp + terms * plane;     // later, over dO, dN and U
     static constexpr int out = s;                             // and at last, fp32 rows over S and R
     static constexpr int bytes = 2 * values + 4 * kGates * kTicks;
-    static_assert(in + terms_n >= terms && (terms_s + terms_r) * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
+    static_assert(terms_s >= terms_r && in + terms_n >= terms && (terms_s + terms_r) * plane >= 2 * kTicks * 68 && bytes <= 227 * 1024, "room");
 };
 
 template <class T>
@@ -41,7 +41,9 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
     if (c.n == 0) return;
     const long long tick = c.tick;
     const T* go_rows = row_of<const T>(s, s.go, c.b, h, tick);
-    const char* dn_rows = s.dn.p + ((s.offsets ? 0 : (long long)c.b * s.dn.batch) + tick * s.dn.tick + h * s.dn.head) * (s.dn_f32 ? 4 : (int)sizeof(T));
+    const float* dn_rows = s.dn_f32 ? row_of<const float>(s, s.dn, c.b, h, tick) : nullptr;
+    const bf16 *dn_high = s.dn_f32 ? nullptr : row_of<const bf16>(s, s.dn_high, c.b, h, tick),
+               *dn_low = s.dn_f32 ? nullptr : row_of<const bf16>(s, s.dn_low, c.b, h, tick);
     const int wt = warp >> 1, wd = warp & 1;                 // ticks 16 wt .., columns (of d, or ticks s) 32 wd ..
 
     load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::q, row_of<const T>(s, s.q, c.b, h, tick) + d_block, s.q.tick, c.n, s.D - d_block, s.q.fast, tid);
@@ -58,11 +60,14 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
         if (e0) __syncthreads();
         load_tile<T, NI, 64, kSquare, 256>(tiles + Lay::go, go_rows + e0, s.go.tick, c.n, s.E - e0, s.go.fast, tid);
         if (s.dn_f32)
-            load_tile<float, NN, 64, kSquare, 256>(tiles + Lay::dn, reinterpret_cast<const float*>(dn_rows) + e0, s.dn.tick, c.n, s.E - e0,
-                                                   s.dn.fast, tid);
-        else if constexpr (sizeof(T) == 2)
-            load_tile<T, NN, 64, kSquare, 256>(tiles + Lay::dn, reinterpret_cast<const T*>(dn_rows) + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast,
-                                               tid);
+            load_tile<float, NN, 64, kSquare, 256>(tiles + Lay::dn, dn_rows + e0, s.dn.tick, c.n, s.E - e0, s.dn.fast, tid);
+        else if constexpr (sizeof(T) == 2) {
+            static_assert(NN == 2, "dN's terms");
+            const int whole = padded_values(s.E) - e0;
+            load_tile<bf16, 1, 64, kSquare, 256>(tiles + Lay::dn, dn_high + e0, s.dn_high.tick, c.n, std::is_same<T, bf16>::value ? s.E - e0 : whole,
+                                                 s.dn_high.fast, tid);
+            load_tile<bf16, 1, 64, kSquare, 256>(tiles + Lay::dn + kPlane, dn_low + e0, s.dn_low.tick, c.n, whole, s.dn_low.fast, tid);
+        }
         async_commit();
         if (e0 + 64 < s.E) {                                  // the next columns on their way to L2
             const int e = e0 / 16 + 4 + (warp >> 1);
@@ -70,9 +75,10 @@ __global__ void __launch_bounds__(256, Terms<T>::in == 1 ? 2 : 1) k_delta_grads(
                 prefetch(reinterpret_cast<const char*>((warp & 1 ? s.gstates : s.states) + ((place * tiles_e + e) * padded_d + d_block / 8) * 32) + lane * 128);
                 if (lane < 16) prefetch(reinterpret_cast<const char*>(s.w + ((2 * place + (warp & 1)) * tiles_e + e) * 4 * 32) + lane * 128);
             }
-            const int row = tid & 63, size = s.dn_f32 ? 4 : (int)sizeof(T);
-            if (tid < 128 && row < c.n)
-                prefetch(tid < 64 ? reinterpret_cast<const char*>(go_rows + row * s.go.tick + e0 + 64) : dn_rows + (row * s.dn.tick + e0 + 64) * size);
+            const int row = tid & 63, which = tid >> 6;
+            const void* rows[3] = {go_rows + row * s.go.tick + e0 + 64, dn_high + row * s.dn_high.tick + e0 + 64, dn_low + row * s.dn_low.tick + e0 + 64};
+            if (s.dn_f32) rows[1] = rows[2] = dn_rows + row * s.dn.tick + e0 + 64;
+            if (which < (s.dn_f32 ? 2 : 3) && row < c.n) prefetch(static_cast<const char*>(rows[which]));
         }
         // S and R, accumulators of 16 columns x 8 values -> terms in rows of columns; a warp: 16 columns of one of them
         {

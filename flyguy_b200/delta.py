@@ -12,8 +12,8 @@ Queries, keys and values are float32, bfloat16 or float16 of one type, any strid
 first); gates and states are float32. Gradients are of the first order. DeltaMemory puts the operators together.
 
 Products run on the tensor cores in bfloat16 terms: what is carried from chunk to chunk (states, corrections and their gradients)
-and the gates' gradients have three, 2^-24 of each value; outputs and the gradients of q and k of bfloat16 two, where one would
-be of the size of the result's own rounding (gv alone goes into them once rounded). Sums are float32."""
+and the gates' gradients have three, 2^-24 of each value; outputs and the gradients of q and k of 16-bit types two, where one would
+be of the size of the result's own rounding. Sums are float32."""
 from __future__ import annotations
 
 import struct
@@ -83,7 +83,7 @@ def _delta_sizes(q, k, v, log_decay, beta, typ, recordings) -> tuple[tuple, tupl
 
 # A forward with gradients holds what its backward needs (states of every 64 ticks, corrections and outputs in float32, X and P: at dim 128 of
 # bfloat16 2.4 KB a tick and head, where q, k, v and o are 1 KB) if that is at most so many bytes; else the backward makes it again. 64
-# recordings of 1,024 ticks, 8 heads of 128: 1.32 GB, 2,755 us for both ways; made again 3,290.
+# recordings of 1,024 ticks, 8 heads of 128: 1.32 GB, 2,953 us for both ways; made again 3,518.
 HELD_AT_MOST = 4 << 30
 _NOTHING = bytes(32)                                      # an fg_ticks of NULL
 _FORWARD, _NO_GRADIENTS = struct.Struct("=48q"), (0,) * 16
