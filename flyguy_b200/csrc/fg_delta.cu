@@ -137,10 +137,10 @@ struct WideLayout {
     int state, bytes;                // of a place, of the block
     __host__ __device__ WideLayout(int D, int E) : state(D * E * 4), bytes(kWidePlaces * D * E * 4 + kWideSums + 4 * 5 * kMaxStep + 64) {}
 };
-// a phase of a barrier, given up after about 2 s
-__device__ __forceinline__ bool phase_of(uint32_t bar, uint32_t parity) {
+// a phase of a barrier, given up after about 2 s (or so many times that)
+__device__ __forceinline__ bool phase_of(uint32_t bar, uint32_t parity, int times = 1) {
     uint32_t done = 0;
-    for (int tries = 0; !done && tries < 20000; ++tries)
+    for (int tries = 0; !done && tries < 20000 * times; ++tries)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n\t"
@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(kWideThreads + 32, 1) k_delta_step_wide(const 
         for (uint32_t i = 0; nth(i) < items; ++i) {
             const uint32_t place = i % kWidePlaces;
             if (slots[place] >= 0) {
-                if (!phase_of(done + 8 * place, (phases >> place) & 1)) {
+                // (longer than the workers wait for this state: whatever they worked on is sent off)
+                if (!phase_of(done + 8 * place, (phases >> place) & 1, 2)) {
                     atomicExch(&g_step_error, 1);
                     break;
                 }
@@ -244,12 +245,14 @@ __global__ void __launch_bounds__(kWideThreads + 32, 1) k_delta_step_wide(const 
         ndecay = s.log_decay[b * s.log_batch + h * s.log_head];
         nbeta = s.beta[b * s.beta_batch + h * s.beta_head];
     };
+    const auto out_of = [&](uint32_t item) {
+        return reinterpret_cast<T*>(s.o.p) + (long long)(item / (uint32_t)s.heads) * s.o.batch + item % (uint32_t)s.heads * s.o.head;
+    };
     ahead(0);
     uint32_t phases = 0;
     for (uint32_t i = 0; nth(i) < items; ++i) {
-        const uint32_t item = nth(i), place = i % kWidePlaces;
-        const long long b = item / (uint32_t)s.heads, slot = nslot;
-        const int h = (int)(item - (uint32_t)b * (uint32_t)s.heads);
+        const uint32_t place = i % kWidePlaces;
+        const long long slot = nslot;
         float *sk = row + (i & 1) * 2 * kMaxStep, *sq = sk + kMaxStep;
         if (tid < s.D) {
             sk[tid] = to_f(nk);
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kWideThreads + 32, 1) k_delta_step_wide(const 
         }
         const float v = to_f(nv), decay = expf(ndecay), beta = nbeta;
         ahead(i + 1);
-        T* o = reinterpret_cast<T*>(s.o.p) + b * s.o.batch + h * s.o.head;
+        T* o = out_of(nth(i));
         workers(true);                                        // k and q are there
         if (slot < 0 || slot >= s.n_slots) {                  // (the same for all threads)
             for (int e = tid; e < s.E; e += kWideThreads) o[e] = from_f<T>(0.f);
@@ -289,8 +292,9 @@ __global__ void __launch_bounds__(kWideThreads + 32, 1) k_delta_step_wide(const 
         float qk = 0.f;
         for (int d = tid & 31; d < s.D; d += 32) qk = fmaf(sk[d], sq[d], qk);
         qk = warp_sum(qk);
-        if (!workers(there)) {                                // (for all threads, if for one: the state stays as it was)
-            for (int e = tid; e < s.E; e += kWideThreads) o[e] = from_f<T>(__int_as_float(0x7fffffff));
+        if (!workers(there)) {                                // (for all threads, if for one: this state and the block's later ones stay as they were)
+            for (uint32_t k = i; nth(k) < items; ++k)
+                for (int e = tid; e < s.E; e += kWideThreads) out_of(nth(k))[e] = from_f<T>(__int_as_float(0x7fffffff));
             if (tid == 0) atomicExch(&g_step_error, 1);
             break;
         }

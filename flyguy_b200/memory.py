@@ -501,7 +501,8 @@ def decay_step(q, k, v, log_decay, state, scale: float | None = None, slots=None
 
 def sync(device=None) -> None:
     """Waits for the current stream of `device` (None: the current one). An error if a wait inside a kernel of these operators has
-    run out on it, now or earlier in this process; what that call left holds NaN."""
+    run out on it, now or earlier in this process; what that call left holds NaN (of delta.delta_step: outputs alone, the states of those
+    rows are as they were)."""
     with torch.cuda.device(device):
         if lib().fg_mem_sync(_raw_stream(_device())):
             raise FlyguyError(lib().fg_mem_last_error().decode())

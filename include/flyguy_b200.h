@@ -339,8 +339,9 @@ typedef struct fg_delta_step_args {
 /* One tick of fg_delta_attn for each row, its state updated in place; dim and value_dim to 256. */
 int fg_delta_step(const fg_delta_step_args* args, void* stream);
 
-/* Waits for the stream; -1 if a call of these on the current device gave up a wait on the tensor cores (about 2 s; the outputs,
- * gradients and states of its recording and head then hold NaN), now or earlier in this process. */
+/* Waits for the stream; -1 if a call of these on the current device gave up a wait (about 2 s), now or earlier in this process: in
+ * fg_decay_attn one on the tensor cores (the outputs, gradients and states of its recording and head then hold NaN), in fg_delta_step one for
+ * a state (the outputs of its row and head and of those that its block had left hold NaN, their states are as they were). */
 int fg_mem_sync(void* stream);
 /* Why the calling thread's last call of these failed ("" after a success). */
 const char* fg_mem_last_error(void);
