@@ -16,6 +16,7 @@ and the gates' gradients have three, 2^-24 of each value; outputs and the gradie
 be of the size of the result's own rounding. Sums are float32."""
 from __future__ import annotations
 
+import math
 import struct
 from functools import lru_cache
 
@@ -300,10 +301,11 @@ def delta_step(q, k, v, log_decay, beta, state, scale: float | None = None, slot
 class DeltaMemory(memory.TickMemory):
     """TickMemory with the gated delta rule: a memory that can replace what it holds, with gates that the observations set.
 
-    The observations are normed (layer_norm) and projected in `dtype` to key_heads queries and keys of unit length (norm_rotate), heads
-    values, and each head's gates: beta = sigmoid(b) and log_decay = -softplus(a) / span, the heads' spans spread from ticks[0] to
-    ticks[1]. delta_attention carries the states, each head's output is normed, some of it dropped while learning (in training mode:
-    dropout with `seed`, one call of the generator a forward; in a captured forward `seed` has to be an int64 tensor on the device,
+    The observations are normed (layer_norm) and projected in `dtype` to key_heads queries and keys (norm_rotate), heads values, and each
+    head's gates: beta = sigmoid(b) and log_decay = -softplus(a) / span, the heads' spans spread from ticks[0] to ticks[1]. Keys are of
+    unit length at first and no longer whatever k_weight learns (its largest value is brought down to dim^-0.5), so that no state grows
+    by what it forgets. delta_attention carries the states, each head's output is normed, some of it dropped while learning (in training
+    mode: dropout with `seed`, one call of the generator a forward; in a captured forward `seed` has to be an int64 tensor on the device,
     changed between replays), and a last projection, zero at first, gives the logits."""
 
     def __init__(self, obs_dim: int, n_actions: int, heads: int = 8, key_heads: int = 2, dim: int = 64,
@@ -311,6 +313,7 @@ class DeltaMemory(memory.TickMemory):
                  dtype: torch.dtype = torch.bfloat16):
         super().__init__(obs_dim, n_actions, heads, key_heads, dim, ticks, base, dtype)
         self.dropout, self.seed, self.calls = dropout, seed, 0
+        self.longest = torch.tensor(dim ** -0.5, dtype=torch.float32, device="cpu").item()   # (as the weight has it)
         self.qkv = nn.Linear(obs_dim, (2 * key_heads + heads) * dim, bias=False)
         self.gates = nn.Linear(obs_dim, 2 * heads)
         nn.init.zeros_(self.gates.weight)
@@ -320,13 +323,17 @@ class DeltaMemory(memory.TickMemory):
         self.obs_weight, self.obs_bias = nn.Parameter(torch.ones(obs_dim)), nn.Parameter(torch.zeros(obs_dim))
         self.o_weight, self.o_bias = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.zeros(dim))
 
+    def _key_weight(self) -> torch.Tensor:
+        """k_weight, or where a value of it is over dim^-0.5 as much of it as leaves none: a normed key's square is dim at most."""
+        return torch.renorm(self.k_weight.unsqueeze(0), math.inf, 0, self.longest).squeeze(0)
+
     def _inputs(self, obs: torch.Tensor, positions):
         obs = layers.layer_norm(obs.float(), self.obs_weight, self.obs_bias)
         x = nn.functional.linear(obs.to(self.dtype), self.qkv.weight.to(self.dtype))
         x = x.unflatten(-1, (2 * self.key_heads + self.heads, self.dim))
         q, k, v = x.split((self.key_heads, self.key_heads, self.heads), -2)
         a, b = nn.functional.linear(obs, self.gates.weight, self.gates.bias).chunk(2, -1)
-        q, k = memory.norm_rotate(q, k, self.turns, self.q_weight, self.k_weight, positions)
+        q, k = memory.norm_rotate(q, k, self.turns, self.q_weight, self._key_weight(), positions)
         return q, k, v, nn.functional.softplus(a) * self.log_decay, torch.sigmoid(b)
 
     def _normed(self, o: torch.Tensor) -> torch.Tensor:
