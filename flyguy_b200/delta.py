@@ -339,16 +339,20 @@ class DeltaMemory(memory.TickMemory):
     def _normed(self, o: torch.Tensor) -> torch.Tensor:
         return layers.layer_norm(o, self.o_weight, self.o_bias)
 
-    def forward(self, obs: torch.Tensor, state=None, positions=None, offsets=None) -> tuple[torch.Tensor, torch.Tensor]:
-        """As TickMemory.forward."""
+    def forward(self, obs: torch.Tensor, state=None, positions=None, offsets=None, call: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """As TickMemory.forward. call: the generator's, where values are dropped; None: `calls`, which counts such forwards. A forward that
+        is run again for its backward (activation checkpointing) has to be given it, or it would drop other values: it is refused."""
         offsets, positions = self._places(obs, state, positions, offsets)
         o, end = delta_attention(*self._inputs(obs, positions), state, offsets=offsets)
         o = self._normed(o)
         if self.training and self.dropout:
             if not isinstance(self.seed, torch.Tensor) and torch.cuda.is_current_stream_capturing():
                 raise FlyguyError("each replay of a captured forward would drop the same values: seed must be an int64 tensor")
-            o = layers.dropout(o, self.dropout, self.seed, call=self.calls)
-            self.calls += 1
+            if call is None:
+                if torch._C._current_graph_task_id() != -1:    # (inside a backward)
+                    raise FlyguyError("a forward that is run again for its backward would drop other values: give it its call, as the first time")
+                call, self.calls = self.calls, self.calls + 1
+            o = layers.dropout(o, self.dropout, self.seed, call=call)
         return self._logits(o), end
 
     @torch.no_grad()
