@@ -306,7 +306,8 @@ class DeltaMemory(memory.TickMemory):
     unit length at first and no longer whatever k_weight learns (its largest value is brought down to dim^-0.5), so that no state grows
     by what it forgets. delta_attention carries the states, each head's output is normed, some of it dropped while learning (in training
     mode: dropout with `seed`, one call of the generator a forward; in a captured forward `seed` has to be an int64 tensor on the device,
-    changed between replays), and a last projection, zero at first, gives the logits."""
+    changed between replays), and a last projection, zero at first, gives the logits. state_dict has the count of calls, `seed` is the
+    caller's to give again; memories, and ranks, of one seed drop alike."""
 
     def __init__(self, obs_dim: int, n_actions: int, heads: int = 8, key_heads: int = 2, dim: int = 64,
                  ticks: tuple[float, float] = (16.0, 4096.0), base: float = 10000.0, dropout: float = 0.0, seed: int = 0,
@@ -322,6 +323,17 @@ class DeltaMemory(memory.TickMemory):
             self.k_weight.fill_(dim ** -0.5)               # keys of unit length
         self.obs_weight, self.obs_bias = nn.Parameter(torch.ones(obs_dim)), nn.Parameter(torch.zeros(obs_dim))
         self.o_weight, self.o_bias = nn.Parameter(torch.ones(dim)), nn.Parameter(torch.zeros(dim))
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "calls"] = torch.tensor(self.calls, device="cpu")
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if prefix + "calls" in state_dict:                 # (dictionaries without it are loaded as before)
+            self.calls = int(state_dict[prefix + "calls"])
+            if prefix + "calls" in unexpected_keys:
+                unexpected_keys.remove(prefix + "calls")
 
     def _key_weight(self) -> torch.Tensor:
         """k_weight, or where a value of it is over dim^-0.5 as much of it as leaves none: a normed key's square is dim at most."""

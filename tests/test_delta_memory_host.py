@@ -40,3 +40,21 @@ def test_keys_are_no_longer_than_one_whatever_is_learned(dim):
         assert abs((ends[0] - ends[1]) / 2e-6 - got[i]) <= 1e-6 * g.sum()
         with torch.no_grad():
             m.k_weight[i] += 1e-6
+
+
+def test_a_saved_memory_goes_on_counting_its_calls():
+    """Loaded, by itself and inside another module, it drops where it had come to; a dictionary of before the count loads, too."""
+    m, other = (delta.DeltaMemory(8, 4, heads=2, key_heads=1, dim=16, dropout=0.1) for _ in range(2))
+    m.calls = 41
+    saved = m.state_dict()
+    other.load_state_dict(saved)
+    assert other.calls == 41
+    m.calls = 5
+    inside = torch.nn.Sequential(torch.nn.Linear(8, 8), other)
+    inside.load_state_dict(torch.nn.Sequential(torch.nn.Linear(8, 8), m).state_dict())
+    assert other.calls == 5
+    del saved["calls"]
+    other.load_state_dict(saved)
+    assert other.calls == 5
+    with pytest.raises(RuntimeError, match="Unexpected"):
+        other.load_state_dict(saved | {"cells": torch.tensor(1)})
