@@ -637,6 +637,7 @@ __global__ void __launch_bounds__(512) k_norm_sums(const float* __restrict__ par
 }
 
 constexpr int kNormBlocks = 12 * kSms;                         // partial sums of a backward pass at most
+constexpr int kAnyBlocks = 64;                                // the same of rows of any length
 constexpr int kLongest = 8192;                                // values of a row that the registers of a block hold
 
 int vector_of(const fg_norm_args* g, bool backward) {
@@ -669,9 +670,11 @@ void check(const fg_norm_args* g, const char* who) {
     if (!((float)g->eps > 0)) throw MemErr{w + ": eps must be positive in fp32"};
 }
 bool any_length(const fg_norm_args* g) { return g->dim > kLongest; }
+// blocks that leave sums for gw and gb, at most
+long long norm_blocks(const fg_norm_args* g) { return std::min<long long>(g->rows, any_length(g) ? kAnyBlocks : kNormBlocks); }
 long long norm_work(const fg_norm_args* g) {
     if (!g->gw && !g->gb) return 0;
-    return (kNormBlocks * 2 * g->dim + (any_length(g) ? 3 * g->rows : 0)) * 4;
+    return (norm_blocks(g) * 2 * g->dim + (any_length(g) ? 3 * g->rows : 0)) * 4;
 }
 
 constexpr int kSumThreads = 128;                              // of a backward block whose lanes share rows
@@ -771,11 +774,11 @@ void norm_backward(const fg_norm_args* g, cudaStream_t st) {
     const bool sums = g->gw || g->gb;
     int blocks = 0;
     if (any_length(g)) {
-        float* stats = sums ? a.part + 2ll * kNormBlocks * a.dim : nullptr;
+        float* stats = sums ? a.part + 2 * norm_blocks(g) * a.dim : nullptr;
         k_norm_any<T><<<(unsigned)std::min<long long>(a.rows, kSms * 4), 512, 0, st>>>(a, stats);
         MCK(cudaGetLastError());
         if (sums) {
-            blocks = (int)std::min<long long>(a.rows, 64);
+            blocks = (int)norm_blocks(g);
             k_norm_columns<T><<<dim3((unsigned)((a.dim + 255) / 256), blocks), 256, 0, st>>>(a, stats);
         }
     } else if (by_ring<T>(g, true, [&](auto per, auto shift) {

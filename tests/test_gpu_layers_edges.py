@@ -27,3 +27,21 @@ def test_rows_of_many_warps_are_the_same_bits_each_time(typ, rows, dim, cuda):
     want = h * w.double() + b.double()
     # (half a step of the type, and 1e-6 of the largest for sums of up to 9,000 values)
     assert ((first[0].double() - want).abs() <= torch.finfo(typ).eps / 2 * want.abs() * 1.001 + 1e-6 * want.abs().max()).all()
+
+
+def test_one_row_of_a_million_values_learns(cuda):
+    """Its sums' workspace is of the row's size, not of as many rows as there are blocks."""
+    n = 1 << 20
+    x = torch.randn(1, n, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_()
+    w, b = torch.ones(n, device=cuda, requires_grad=True), torch.zeros(n, device=cuda, requires_grad=True)
+    gy = torch.randn(1, n, generator=torch.Generator().manual_seed(4)).cuda()
+    y = layers.layer_norm(x, w, b)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    gw, gb = torch.autograd.grad(y, (w, b), gy)
+    assert torch.cuda.max_memory_allocated() - before <= 8 * 4 * n
+    assert torch.equal(gb, gy[0])
+    d = x.detach().double()
+    want = gy.double() * (d - d.mean()) / (d.var(correction=0) + 1e-5).sqrt()
+    assert (gw.double() - want[0]).abs().max() <= 5e-6 * want.abs().max()
