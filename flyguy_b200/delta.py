@@ -201,8 +201,9 @@ def delta_attention(q, k, v, log_decay, beta, state=None, scale: float | None = 
     before the first and after the last get zeros, in o and in the gradients). state float32 [recordings, heads, dim, value
     dim] before the first ticks (None: zeros). scale: dim^-0.5 when None. dim at most 128, value dim at most 256.
     log_decay is at most 0, minus infinity forgets the state (anything below -256 does, in float32).
-    Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v, log_decay, beta and state. With
-    gradients, o is made of more terms (the states are the same bits), and up to HELD_AT_MOST bytes are held for the backward.
+    Returns o [.., heads, value dim] and the states after the last ticks; gradients of q, k, v, log_decay, beta and state. A
+    forward with gradients holds what its backward needs, up to HELD_AT_MOST bytes; o of one that does is made of more terms than o alone or
+    above that (the states are the same bits).
 
     A recording's ticks are worked on in tiles of 64: a NaN or an infinity stays in its recording and head and out of the tiles
     before it, but reaches all ticks of its own and those after it, and infinities become NaN (delta_step goes tick by tick)."""
