@@ -19,8 +19,8 @@
 // 16 warps an SM instead of 8.
 //
 // 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: forward 522 us (310 products a warp and chunk, 301 us of the tensor cores' at 552
-// TFLOP/s of mma.sync), with what is kept 800, back 1,015. The tensor pipe is 55%, 49% and 36% busy, issue slots 40%, DRAM 14%, 33% and
-// 39%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S, W and O,
+// TFLOP/s of mma.sync), with what is kept 800, back 1,015. The tensor pipe is 54%, 49% and 36% busy, issue slots 39%, DRAM 14%, 33% and
+// 38%: products of a warp wait for its own splits into terms and the other way round, more than the warps beside it fill; back for S, W and O,
 // too. X, P and the gates take 101 us: some 1,700 instructions a warp, of them 100 products.
 #pragma once
 #include "fg_delta.cuh"

@@ -9,7 +9,7 @@
 // of their columns; S, R and W arrive as the chain's accumulators and go through shared memory, where reading across turns them.
 //
 // 64 recordings of 1,024 ticks, 8 heads of 128 in bf16: 1,032 us (2.3 GB, 350 us at a plain copy's rate; the products 440). Bound by what follows one
-// another in a block of which an SM holds two: the loads, their terms, the products, the masks; tensor pipe 36%, issue slots 36%, DRAM 38%.
+// another in a block of which an SM holds two: the loads, their terms, the products, the masks; tensor pipe 42%, issue slots 36%, DRAM 33%.
 #pragma once
 #include "fg_delta_chain.cuh"
 
