@@ -34,7 +34,7 @@ _DELTA = struct.Struct("=48q5q9qd2q")
 # fg_delta_step_args: q, k, v, o, log_decay, beta (fg_ticks), state, slots, n_slots, batch, heads, query_heads, key_heads, value_heads, dim,
 # value_dim, type, scale
 _STEP = struct.Struct("=24q11qd")
-_STEP_HEAD, _DOUBLE = struct.Struct("=26q"), struct.Struct("=d")
+_STEP_HEAD, _DOUBLE, _FLOAT = struct.Struct("=26q"), struct.Struct("=d"), struct.Struct("=f")
 
 
 def _gate(name: str, t, lead: tuple, like: torch.Tensor) -> torch.Tensor:
@@ -315,7 +315,6 @@ class DeltaMemory(memory.TickMemory):
                  dtype: torch.dtype = torch.bfloat16):
         super().__init__(obs_dim, n_actions, heads, key_heads, dim, ticks, base, dtype)
         self.dropout, self.seed, self.calls = dropout, seed, 0
-        self.longest = torch.tensor(dim ** -0.5, dtype=torch.float32, device="cpu").item()   # (as the weight has it)
         self.qkv = nn.Linear(obs_dim, (2 * key_heads + heads) * dim, bias=False)
         self.gates = nn.Linear(obs_dim, 2 * heads)
         nn.init.zeros_(self.gates.weight)
@@ -338,7 +337,8 @@ class DeltaMemory(memory.TickMemory):
 
     def _key_weight(self) -> torch.Tensor:
         """k_weight, or where a value of it is over dim^-0.5 as much of it as leaves none: a normed key's square is dim at most."""
-        return torch.renorm(self.k_weight.unsqueeze(0), math.inf, 0, self.longest).squeeze(0)
+        most, = _FLOAT.unpack(_FLOAT.pack(self.dim ** -0.5))   # (as a weight of float32 has it: its first values are not over it)
+        return torch.renorm(self.k_weight.unsqueeze(0), math.inf, 0, most).squeeze(0)
 
     def _inputs(self, obs: torch.Tensor, positions):
         obs = layers.layer_norm(obs.float(), self.obs_weight, self.obs_bias)

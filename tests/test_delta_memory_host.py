@@ -7,7 +7,7 @@ import torch
 from flyguy_b200 import delta
 
 
-@pytest.mark.parametrize("dim", [16, 32, 40, 64, 128])
+@pytest.mark.parametrize("dim", [9, 16, 32, 40, 64, 81, 96, 128])
 def test_keys_are_no_longer_than_one_whatever_is_learned(dim):
     """A normed key x has |x|^2 <= dim, so that |x w|^2 <= dim max(w)^2. At first, and below, the weight is taken as it is, its
     gradient too; beyond, as much of it as keeps the bound, and its gradient is that of differences."""
@@ -58,3 +58,9 @@ def test_a_saved_memory_goes_on_counting_its_calls():
     assert other.calls == 5
     with pytest.raises(RuntimeError, match="Unexpected"):
         other.load_state_dict(saved | {"cells": torch.tensor(1)})
+
+
+def test_a_memory_pickled_whole_has_all_that_it_needs():
+    """Its own attributes are those that a memory pickled before had."""
+    own = set(vars(delta.DeltaMemory(8, 4, heads=2, key_heads=1, dim=16))) - set(vars(torch.nn.Module()))
+    assert own == {"heads", "key_heads", "dim", "dtype", "dropout", "seed", "calls"}
